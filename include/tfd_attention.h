@@ -11,7 +11,9 @@
  *        (eager entry EagerSessionJeffAttentionExt::jeff_full_attention, 214-275)
  *
  * plus entries that extend the same arithmetic without changing the drop-in
- * path (structured Laya masks, batched Jeff rows with native GQA, bf16 Jeff).
+ * path (structured Laya masks, batched Jeff rows with native GQA, bf16 Jeff),
+ * and what a hybrid Jeff model needs around them: linear attention over rows
+ * (prompts and single tokens) and token log probabilities.
  *
  * Conventions
  *   - Every tensor is column-major exactly as the reference passes it:
@@ -263,6 +265,82 @@ int tfd_jeff_full_attention_layer_rows_f32(tfd_ctx *ctx, size_t rows, size_t len
                                            const float *q_norm, const float *k_norm,
                                            const float *mask, uint32_t theta_bits,
                                            uint32_t eps_bits, float *out, unsigned flags);
+
+/*
+ * Linear attention over `rows` independent rows (no counterpart among the
+ * reference's attention ops: its Jeff layers between the full-attention ones):
+ * a state S (key_dim x value_dim) per row and value head that decays with every
+ * token, and is written by a plain or a delta rule. For each active token t:
+ *   S  <- exp(log_decay_t) S
+ *   u   = v_t                                (beta NULL)
+ *       = beta_t (v_t - S^T k_t)             (beta given)
+ *   S  <- S + k_t u^T
+ *   out_t = scale S^T q_t
+ *   q, k:      rows x (length, key_heads*key_dim); value head h uses key head
+ *              h / (heads / key_heads), so key_heads must divide heads.
+ *   v, out:    rows x (length, heads*value_dim).
+ *   log_decay, beta: rows x (length, heads), head h's tokens contiguous; log_decay
+ *              finite or -inf (which forgets the whole state), beta may be NULL.
+ *   mask:      rows x (length), a token is active when mask != 0, or NULL (all are).
+ *              An inactive token leaves the state as it is and its out is 0;
+ *              nothing that q, k, v, log_decay or beta hold there is used.
+ *   state_in:  rows x heads x (key_dim, value_dim), value features contiguous
+ *              (element j + value_dim*i); NULL starts from zeros.
+ *   state_out: the state after the last token, same layout; NULL when not
+ *              wanted; may be state_in itself (the update is then in place; no
+ *              other overlap of the buffers is allowed).
+ *   scale_bits: f32 bits of the factor on the output.
+ * length 1 is the single-token form. key_dim is at most 256 (else
+ * TFD_EUNSUPPORTED). A NaN or inf that an active token holds reaches this head's
+ * later outputs, and may reach those up to 63 tokens before it.
+ */
+int tfd_jeff_linear_attention_rows_f32(tfd_ctx *ctx, size_t rows, size_t length, size_t heads,
+                                       size_t key_heads, size_t key_dim, size_t value_dim,
+                                       const float *q, const float *k, const float *v,
+                                       const float *log_decay, const float *beta,
+                                       const float *mask, uint32_t scale_bits,
+                                       const float *state_in, float *state_out, float *out,
+                                       unsigned flags);
+
+/* As tfd_jeff_linear_attention_rows_f32 with q, k and v given as bf16 bits;
+ * the rest, the states and out stay f32, and no product is rounded to bf16. */
+int tfd_jeff_linear_attention_rows_bf16(tfd_ctx *ctx, size_t rows, size_t length, size_t heads,
+                                        size_t key_heads, size_t key_dim, size_t value_dim,
+                                        const uint16_t *q, const uint16_t *k, const uint16_t *v,
+                                        const float *log_decay, const float *beta,
+                                        const float *mask, uint32_t scale_bits,
+                                        const float *state_in, float *state_out, float *out,
+                                        unsigned flags);
+
+/*
+ * Log probabilities of given tokens under softmax(logits), the entropy (nats)
+ * and the most likely tokens of every position: the readout of an engine that
+ * compares label tokens (JeffEngine::logits' rows, jeff-infer engine.rs:307-329),
+ * as pool_host does it over a Laya prompt's markers (laya-infer model.rs:773-837).
+ *   logits:        (vocab, positions) column-major with leading dimension ld >=
+ *                  vocab: logit i of position p at i + ld*p.
+ *   tokens:        (per_position, positions); a negative token is an unused slot
+ *                  (log probability 0), one past the vocabulary gives NaN. May be
+ *                  NULL with per_position 0.
+ *   log_probs:     (per_position, positions), or NULL with per_position 0.
+ *   entropy:       (positions), or NULL when not wanted.
+ *   top_tokens, top_log_probs: (top, positions), the `top` largest logits in
+ *                  falling order, the lower token first among equal ones (a NaN
+ *                  ranks below every number). NULL with top 0. top is at most
+ *                  vocab (TFD_EINVAL) and 64 (TFD_EUNSUPPORTED).
+ * A logit of -inf has probability 0. A position that holds a NaN or +inf, or
+ * nothing but -inf, has NaN for every log probability of it and the entropy.
+ */
+int tfd_token_log_probs_f32(tfd_ctx *ctx, const float *logits, size_t vocab, size_t ld,
+                            size_t positions, const int64_t *tokens, size_t per_position,
+                            size_t top, float *log_probs, float *entropy, int64_t *top_tokens,
+                            float *top_log_probs, unsigned flags);
+
+/* As tfd_token_log_probs_f32 with the logits given as bf16 bits; every sum is f32. */
+int tfd_token_log_probs_bf16(tfd_ctx *ctx, const uint16_t *logits, size_t vocab, size_t ld,
+                             size_t positions, const int64_t *tokens, size_t per_position,
+                             size_t top, float *log_probs, float *entropy, int64_t *top_tokens,
+                             float *top_log_probs, unsigned flags);
 
 #ifdef __cplusplus
 }

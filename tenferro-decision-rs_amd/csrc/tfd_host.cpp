@@ -36,6 +36,7 @@ constexpr size_t kRopeCacheEntries = 8;
 struct DevBuf {
   void *ptr = nullptr;
   size_t cap = 0;
+  bool captured = false;  // a captured graph holds ptr (reserve_capturable)
 };
 
 struct RopeEntry {
@@ -63,6 +64,10 @@ struct tfd_ctx {
   DevBuf layer;       // intermediates of the layer entries (projections, attention output)
   DevBuf model;       // activations and token inputs of the model forward
   DevBuf planes;      // bf16 planes of the linears' operands
+  DevBuf readout;     // partial statistics of the token log probabilities
+  // Workspaces that a captured graph may still use, outgrown since.
+  std::vector<void *> retired;
+  size_t retired_bytes = 0;
   std::vector<uint8_t> model_host;  // packed token inputs of the last model forward
   bool model_inflight = false;      // an asynchronous forward may still read model_host
   rocblas_handle blas = nullptr;  // the layer entries' GEMMs, on `stream`
@@ -138,6 +143,42 @@ int reserve(tfd_ctx *c, DevBuf &b, size_t bytes) {
   size_t cap = bytes < 256 ? 256 : bytes;
   TFD_HIP(c, hipMalloc(&b.ptr, cap), "hipMalloc");
   b.cap = cap;
+  return TFD_OK;
+}
+
+// Workspace of an entry that may run under stream capture. A capture cannot
+// allocate, so the workspace has to be large enough from an eager call before
+// it; from then on the graph holds the address, and a larger workspace retires
+// the old one (until the context ends) instead of freeing it.
+int reserve_capturable(tfd_ctx *c, const char *op, DevBuf &b, size_t bytes, bool capturing) {
+  if (bytes <= b.cap) {
+    b.captured = b.captured || capturing;
+    return TFD_OK;
+  }
+  if (capturing)
+    return fail(c, TFD_EUNSUPPORTED,
+                "%s: the workspace cannot grow under stream capture; make one call of the same "
+                "sizes before capturing", op);
+  if (b.captured) {
+    try {
+      c->retired.push_back(b.ptr);
+    } catch (const std::bad_alloc &) {
+      return fail(c, TFD_EHIP, "%s: out of host memory", op);
+    }
+    c->retired_bytes += b.cap;
+    b = DevBuf{};
+  }
+  return reserve(c, b, bytes);
+}
+
+// Whether the context's stream is being captured; a call under capture has to
+// be asynchronous.
+int capture_state(tfd_ctx *c, const char *op, unsigned flags, bool *capturing) {
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  TFD_HIP(c, hipStreamIsCapturing(c->stream, &cap), "hipStreamIsCapturing");
+  *capturing = cap != hipStreamCaptureStatusNone;
+  if (*capturing && !(flags & TFD_ASYNC))
+    return invalid(c, op, "flags", "a call under stream capture needs TFD_ASYNC");
   return TFD_OK;
 }
 
@@ -1439,6 +1480,160 @@ int laya_forward(tfd_ctx *c, const tfd_laya_model *m, const int64_t *ids, const 
   return TFD_OK;
 }
 
+// ------------------------------------------------------- linear attention
+
+int linear_run(tfd_ctx *c, bool bf16, size_t rows, size_t length, size_t heads, size_t key_heads,
+               size_t key_dim, size_t value_dim, const void *q, const void *k, const void *v,
+               const float *log_decay, const float *beta, const float *mask, uint32_t scale_bits,
+               const float *state_in, float *state_out, float *out, unsigned flags) {
+  const char *op = bf16 ? "tfd_jeff_linear_attention_rows_bf16"
+                        : "tfd_jeff_linear_attention_rows_f32";
+  if (!c) return TFD_EINVAL;
+  c->err.clear();
+  int rc = check_flags(c, op, flags, TFD_DEVICE_PTRS | TFD_ASYNC);
+  if (rc) return rc;
+  if (key_heads == 0 || heads % key_heads != 0)
+    return invalid(c, op, "key_heads", "heads must be a multiple of key_heads");
+  size_t kn = 0, vn = 0, gn = 0, mn = 0, sn = 0;
+  if (!mul_ok(rows, length, &mn) || !mul_ok(mn, heads, &gn) || !mul_ok(gn, value_dim, &vn) ||
+      !mul_ok(mn, key_heads, &kn) || !mul_ok(kn, key_dim, &kn) || !mul_ok(rows, heads, &sn) ||
+      !mul_ok(sn, key_dim, &sn) || !mul_ok(sn, value_dim, &sn) || vn > SIZE_MAX / 64 ||
+      kn > SIZE_MAX / 64 || sn > SIZE_MAX / 64)
+    return invalid(c, op, "shape", "attention dimensions overflow");
+  if (rows == 0 || heads == 0 || value_dim == 0) return TFD_OK;
+  if (key_dim == 0) return invalid(c, op, "key_dim", "key_dim must not be 0");
+  if (key_dim > (size_t)tfd::kLinearMaxKeyDim)
+    return fail(c, TFD_EUNSUPPORTED, "%s: key_dim %zu exceeds %d", op, key_dim,
+                tfd::kLinearMaxKeyDim);
+  if (length > (size_t)INT32_MAX / 4 || value_dim > (size_t)1 << 20 || heads > 65535 ||
+      rows > 65535)
+    return fail(c, TFD_EUNSUPPORTED, "%s: length/value_dim/heads/rows exceed the launch grid", op);
+  if ((length && (!q || !k || !v || !log_decay || !out)))
+    return invalid(c, op, "inputs", "null buffer");
+  if (length == 0 && !state_out) return TFD_OK;
+  if ((rc = ensure_ready(c))) return rc;
+  bool capturing = false;
+  if ((rc = capture_state(c, op, flags, &capturing))) return rc;
+  const size_t es = bf16 ? 2 : 4;
+  const void *q_d = nullptr, *k_d = nullptr, *v_d = nullptr, *g_d = nullptr, *b_d = nullptr,
+             *m_d = nullptr, *si_d = nullptr;
+  void *so_d = nullptr, *out_d = nullptr;
+  if ((rc = operand(c, flags, 1, q, es * kn, &q_d))) return rc;
+  if ((rc = operand(c, flags, 2, k, es * kn, &k_d))) return rc;
+  if ((rc = operand(c, flags, 3, v, es * vn, &v_d))) return rc;
+  if ((rc = operand(c, flags, 4, log_decay, sizeof(float) * gn, &g_d))) return rc;
+  if (beta && (rc = operand(c, flags, 5, beta, sizeof(float) * gn, &b_d))) return rc;
+  if (mask && (rc = operand(c, flags, 6, mask, sizeof(float) * mn, &m_d))) return rc;
+  if (state_in && (rc = operand(c, flags, 7, state_in, sizeof(float) * sn, &si_d))) return rc;
+  if (state_out && (rc = output(c, flags, 8, state_out, sizeof(float) * sn, &so_d))) return rc;
+  if ((rc = output(c, flags, 0, out, sizeof(float) * vn, &out_d))) return rc;
+  tfd::LinearArgs a{};
+  a.q = q_d;
+  a.k = k_d;
+  a.v = v_d;
+  a.log_decay = static_cast<const float *>(g_d);
+  a.beta = static_cast<const float *>(b_d);
+  a.mask = static_cast<const float *>(m_d);
+  a.state_in = static_cast<const float *>(si_d);
+  a.state_out = static_cast<float *>(so_d);
+  a.out = static_cast<float *>(out_d);
+  a.rows = (int)rows;
+  a.L = (int)length;
+  a.heads = (int)heads;
+  a.key_heads = (int)key_heads;
+  a.group = (int)(heads / key_heads);
+  a.dk = (int)key_dim;
+  a.dv = (int)value_dim;
+  a.scale = bits_to_f32(scale_bits);
+  a.bf16 = bf16;
+  a.state_vec = value_dim % 4 == 0 && aligned16(si_d) && aligned16(so_d);
+  tfd::KernelEvents ev;
+  if (!capturing && (rc = timing_events(c, &ev))) return rc;
+  TFD_HIP(c, tfd::launch_linear_attention(a, c->stream, ev), "linear_attention launch");
+  if (!(flags & TFD_DEVICE_PTRS) && state_out)
+    TFD_HIP(c, hipMemcpyAsync(state_out, so_d, sizeof(float) * sn, hipMemcpyDeviceToHost, c->stream),
+            "hipMemcpyAsync D2H");
+  return finish(c, flags, out, out_d, sizeof(float) * vn);
+}
+
+// ------------------------------------------------ token log probabilities
+
+int log_probs_run(tfd_ctx *c, bool bf16, const void *logits, size_t vocab, size_t ld,
+                  size_t positions, const int64_t *tokens, size_t per, size_t top,
+                  float *log_probs, float *entropy, int64_t *top_tokens, float *top_log_probs,
+                  unsigned flags) {
+  const char *op = bf16 ? "tfd_token_log_probs_bf16" : "tfd_token_log_probs_f32";
+  if (!c) return TFD_EINVAL;
+  c->err.clear();
+  int rc = check_flags(c, op, flags, TFD_DEVICE_PTRS | TFD_ASYNC);
+  if (rc) return rc;
+  size_t n = 0, pn = 0, tn = 0;
+  if (!mul_ok(ld, positions, &n) || !mul_ok(per, positions, &pn) ||
+      !mul_ok(top, positions, &tn) || n > SIZE_MAX / 64 || pn > SIZE_MAX / 64 ||
+      tn > SIZE_MAX / 64)
+    return invalid(c, op, "shape", "logits dimensions overflow");
+  if (ld < vocab) return invalid(c, op, "ld", "the leading dimension must be at least vocab");
+  if (top > vocab) return invalid(c, op, "top", "top must not exceed vocab");
+  if (positions == 0) return TFD_OK;
+  if (vocab == 0) return invalid(c, op, "vocab", "vocab must not be 0");
+  if (top > tfd::kLogProbMaxTop)
+    return fail(c, TFD_EUNSUPPORTED, "%s: top %zu exceeds %zu", op, top, tfd::kLogProbMaxTop);
+  if (vocab > (size_t)1 << 30 || positions > (size_t)1 << 30 || per > (size_t)INT32_MAX / 4)
+    return fail(c, TFD_EUNSUPPORTED, "%s: vocab/positions/per_position exceed the launch grid",
+                op);
+  if (!logits || (per && (!tokens || !log_probs)) || (top && (!top_tokens || !top_log_probs)))
+    return invalid(c, op, "inputs", "null buffer");
+  if ((rc = ensure_ready(c))) return rc;
+  bool capturing = false;
+  if ((rc = capture_state(c, op, flags, &capturing))) return rc;
+  const size_t es = bf16 ? 2 : 4;
+  // The last position may end at its vocab-th logit.
+  const size_t used = n - (ld - vocab);
+  const void *x_d = nullptr, *t_d = nullptr;
+  void *lp_d = nullptr, *e_d = nullptr, *tt_d = nullptr, *tl_d = nullptr;
+  if ((rc = operand(c, flags, 1, logits, es * used, &x_d))) return rc;
+  if (per && (rc = operand(c, flags, 2, tokens, sizeof(int64_t) * pn, &t_d))) return rc;
+  if (per && (rc = output(c, flags, 0, log_probs, sizeof(float) * pn, &lp_d))) return rc;
+  if (entropy && (rc = output(c, flags, 3, entropy, sizeof(float) * positions, &e_d))) return rc;
+  if (top && (rc = output(c, flags, 4, top_tokens, sizeof(int64_t) * tn, &tt_d))) return rc;
+  if (top && (rc = output(c, flags, 5, top_log_probs, sizeof(float) * tn, &tl_d))) return rc;
+  tfd::LogProbArgs a{};
+  a.logits = x_d;
+  a.tokens = static_cast<const int64_t *>(t_d);
+  a.log_probs = static_cast<float *>(lp_d);
+  a.entropy = static_cast<float *>(e_d);
+  a.top_tokens = static_cast<int64_t *>(tt_d);
+  a.top_log_probs = static_cast<float *>(tl_d);
+  a.vocab = vocab;
+  a.ld = ld;
+  a.positions = positions;
+  a.per = (int)per;
+  a.top = (int)top;
+  a.bf16 = bf16;
+  tfd::log_probs_plan(a, c->cus);
+  if (a.parts > 1) {
+    const size_t parts = positions * (size_t)a.parts;
+    const size_t stats = (4 * sizeof(float) * parts + 255) & ~(size_t)255;
+    if ((rc = reserve_capturable(c, op, c->readout, stats + 8 * parts * top, capturing))) return rc;
+    a.part_stats = static_cast<float *>(c->readout.ptr);
+    a.part_keys = reinterpret_cast<unsigned long long *>(static_cast<char *>(c->readout.ptr) + stats);
+  }
+  tfd::KernelEvents ev;
+  if (!capturing && (rc = timing_events(c, &ev))) return rc;
+  TFD_HIP(c, tfd::launch_log_probs(a, c->stream, ev), "log_probs launch");
+  if (!(flags & TFD_DEVICE_PTRS)) {
+    const struct { void *host, *dev; size_t bytes; } back[3] = {
+        {entropy, e_d, sizeof(float) * positions},
+        {top ? top_tokens : nullptr, tt_d, sizeof(int64_t) * tn},
+        {top ? top_log_probs : nullptr, tl_d, sizeof(float) * tn}};
+    for (const auto &b : back)
+      if (b.host)
+        TFD_HIP(c, hipMemcpyAsync(b.host, b.dev, b.bytes, hipMemcpyDeviceToHost, c->stream),
+                "hipMemcpyAsync D2H");
+  }
+  return finish(c, flags, log_probs, lp_d, sizeof(float) * pn);
+}
+
 }  // namespace
 
 // ---------------------------------------------------------------- C ABI
@@ -1478,6 +1673,8 @@ void tfd_ctx_destroy(tfd_ctx *c) {
     if (c->layer.ptr) (void)hipFree(c->layer.ptr);
     if (c->planes.ptr) (void)hipFree(c->planes.ptr);
     if (c->model.ptr) (void)hipFree(c->model.ptr);
+    if (c->readout.ptr) (void)hipFree(c->readout.ptr);
+    for (void *p : c->retired) (void)hipFree(p);
     if (c->blas) (void)rocblas_destroy_handle(c->blas);
     for (auto &e : c->rope) {
       (void)hipFree(e.cos_d);
@@ -1508,7 +1705,7 @@ void *tfd_ctx_stream(tfd_ctx *c) {
 size_t tfd_ctx_retained_bytes(const tfd_ctx *c) {
   if (!c) return 0;
   size_t total = sizeof(tfd_ctx) + c->bits.cap + c->kp.cap + c->layer.cap + c->model.cap + c->planes.cap +
-                 c->model_host.capacity();
+                 c->model_host.capacity() + c->readout.cap + c->retired_bytes;
   for (const auto &b : c->staging) total += b.cap;
   for (const auto &e : c->rope) total += e.bytes;
   return total;
@@ -1707,6 +1904,44 @@ int tfd_jeff_full_attention_layer_rows_f32(tfd_ctx *c, size_t rows, size_t lengt
   if (rc) return rc;
   return jeff_layer(c, rows, length, hidden, heads, kv_heads, head_dim, rotary_dim, x, w_q,
                     w_gate, w_k, w_v, w_o, q_norm, k_norm, mask, theta_bits, eps_bits, out, flags);
+}
+
+int tfd_jeff_linear_attention_rows_f32(tfd_ctx *c, size_t rows, size_t length, size_t heads,
+                                       size_t key_heads, size_t key_dim, size_t value_dim,
+                                       const float *q, const float *k, const float *v,
+                                       const float *log_decay, const float *beta,
+                                       const float *mask, uint32_t scale_bits,
+                                       const float *state_in, float *state_out, float *out,
+                                       unsigned flags) {
+  return linear_run(c, false, rows, length, heads, key_heads, key_dim, value_dim, q, k, v,
+                    log_decay, beta, mask, scale_bits, state_in, state_out, out, flags);
+}
+
+int tfd_jeff_linear_attention_rows_bf16(tfd_ctx *c, size_t rows, size_t length, size_t heads,
+                                        size_t key_heads, size_t key_dim, size_t value_dim,
+                                        const uint16_t *q, const uint16_t *k, const uint16_t *v,
+                                        const float *log_decay, const float *beta,
+                                        const float *mask, uint32_t scale_bits,
+                                        const float *state_in, float *state_out, float *out,
+                                        unsigned flags) {
+  return linear_run(c, true, rows, length, heads, key_heads, key_dim, value_dim, q, k, v,
+                    log_decay, beta, mask, scale_bits, state_in, state_out, out, flags);
+}
+
+int tfd_token_log_probs_f32(tfd_ctx *c, const float *logits, size_t vocab, size_t ld,
+                            size_t positions, const int64_t *tokens, size_t per_position,
+                            size_t top, float *log_probs, float *entropy, int64_t *top_tokens,
+                            float *top_log_probs, unsigned flags) {
+  return log_probs_run(c, false, logits, vocab, ld, positions, tokens, per_position, top, log_probs,
+                       entropy, top_tokens, top_log_probs, flags);
+}
+
+int tfd_token_log_probs_bf16(tfd_ctx *c, const uint16_t *logits, size_t vocab, size_t ld,
+                             size_t positions, const int64_t *tokens, size_t per_position,
+                             size_t top, float *log_probs, float *entropy, int64_t *top_tokens,
+                             float *top_log_probs, unsigned flags) {
+  return log_probs_run(c, true, logits, vocab, ld, positions, tokens, per_position, top, log_probs,
+                       entropy, top_tokens, top_log_probs, flags);
 }
 
 int tfd_laya_forward_f32(tfd_ctx *c, const tfd_laya_model *model, const int64_t *ids,

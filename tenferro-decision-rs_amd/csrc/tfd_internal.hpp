@@ -326,4 +326,50 @@ struct SkinnyArgs {
 };
 hipError_t launch_skinny(const SkinnyArgs &g, int cus, hipStream_t stream);
 
+// ------------------------------------------------ linear attention
+
+// Key features the state of the linear attention may have.
+constexpr int kLinearMaxKeyDim = 256;
+// q, k: rows x (L, key_heads * dk), v, out: rows x (L, heads * dv), token
+// contiguous; log_decay, beta: rows x (L, heads); mask: rows x (L) or null;
+// states: rows x heads x (dk, dv), value feature contiguous, or null (zero /
+// not wanted; state_out may be state_in). beta null: plain decayed writes.
+struct LinearArgs {
+  const void *q, *k, *v;
+  const float *log_decay, *beta, *mask;
+  const float *state_in;
+  float *state_out, *out;
+  int rows, L, heads, key_heads, group, dk, dv;
+  float scale;
+  bool bf16;       // q, k and v
+  bool state_vec;  // 16-byte access to the states' rows: dv % 4 == 0, aligned
+};
+hipError_t launch_linear_attention(const LinearArgs &a, hipStream_t stream,
+                                   const KernelEvents &ev);
+
+// ------------------------------------------------ token log probabilities
+
+// Up to this many logits a position is one wavefront's.
+constexpr size_t kLogProbWaveVocab = 2048;
+// Alternatives a position may return: one wavefront's lanes.
+constexpr size_t kLogProbMaxTop = 64;
+struct LogProbArgs {
+  const void *logits;  // f32 or bf16, logit i of position p at i + ld * p
+  const int64_t *tokens;     // per x positions
+  float *log_probs;          // per x positions
+  float *entropy;            // positions, or null
+  int64_t *top_tokens;       // top x positions
+  float *top_log_probs;
+  size_t vocab, ld, positions;
+  int per, top;
+  bool bf16;
+  // Set by log_probs_plan: parts per position of part_pieces 16-byte pieces,
+  // and their statistics (4 floats a part) and keys (top a part).
+  int parts, part_pieces;
+  float *part_stats;
+  unsigned long long *part_keys;
+};
+void log_probs_plan(LogProbArgs &a, int cus);
+hipError_t launch_log_probs(const LogProbArgs &a, hipStream_t stream, const KernelEvents &ev);
+
 }  // namespace tfd

@@ -1,0 +1,341 @@
+// Log probabilities of given tokens, the entropy and the largest logits of
+// every position of a (vocab, positions) matrix of logits, in one pass.
+//
+// With m = max x, z = sum e^(x - m), a = sum e^(x - m) (x - m):
+//   log p(i) = (x_i - m) - log z,   entropy = log z - a / z.
+// Each lane keeps its own (m, z, a) and moves m by
+//   z' = f z,  a' = f (a + (m - m') z),  f = e^(m - m'),
+// so a position is read once, 16 bytes a lane, and the lanes, waves and parts
+// of a position are joined in a fixed order (the same bits on every run). A
+// NaN or +inf logit makes z NaN, no finite logit makes it 0: both end as NaN.
+//
+// The `top` largest logits: every wave keeps its best 64 so far sorted across
+// its lanes, as unique 64-bit keys (value order, then the lower index first),
+// and compares the 16 bytes' maximum, which the softmax needs anyway, with
+// the top-th of them. What passes is collected in LDS and merged 64 at a time
+// by a bitonic network; for logits in random order that is a few merges in a
+// row of 10^5.
+//
+// Bound by reading the logits. A position goes to one wave up to 2048 logits,
+// to one workgroup of four waves past that, and to several workgroups (joined
+// by a second kernel) when there are too few positions to fill the chip.
+#include <hip/hip_ext.h>
+#include <math.h>
+
+#include "tfd_device.hpp"
+#include "tfd_internal.hpp"
+
+namespace tfd {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3.402823466e38f;
+// Exponents are clamped here: e^-1e30 is 0, and 0 * -1e30 is 0, not NaN.
+constexpr float kFar = -1.0e30f;
+
+typedef unsigned long long u64;
+
+// Value order of a logit: larger numbers have larger codes, -0 equals 0, a NaN
+// ranks below every number.
+__device__ __forceinline__ uint32_t value_code(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return x != x ? 0u : (b & 0x80000000u ? ~b : b | 0x80000000u);
+}
+__device__ __forceinline__ float code_value(uint32_t c) {
+  if (c == 0u) return NAN;
+  return __uint_as_float(c & 0x80000000u ? c & 0x7fffffffu : ~c);
+}
+__device__ __forceinline__ u64 key_of(float x, uint32_t index) {
+  return ((u64)value_code(x) << 32) | (uint32_t)~index;
+}
+
+// One stage of a bitonic network over the wave's lanes: lanes whose bit
+// `keep_max` is set keep the larger of the pair (l, l ^ o).
+__device__ __forceinline__ u64 exchange(u64 v, int o, bool keep_max) {
+  const u64 w = __shfl_xor(v, o);
+  return (v > w) == keep_max ? v : w;
+}
+// Sorts one key a lane, largest in lane 0.
+__device__ __forceinline__ u64 sort64(u64 v, int lane) {
+#pragma unroll
+  for (int n = 2; n <= 64; n <<= 1)
+#pragma unroll
+    for (int o = n >> 1; o > 0; o >>= 1)
+      v = exchange(v, o, ((lane & o) == 0) == ((lane & n) == 0));
+  return v;
+}
+// The 64 largest of two sorted lists, sorted.
+__device__ __forceinline__ u64 merge64(u64 a, u64 b, int lane) {
+  const u64 r = __shfl(b, 63 - lane);
+  u64 v = a > r ? a : r;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = exchange(v, o, (lane & o) == 0);
+  return v;
+}
+
+// Softmax statistics of part of a position.
+struct Stats {
+  float m, z, a;
+};
+__device__ __forceinline__ void move_reference(Stats &s, float m) {
+  const float d = fmaxf(s.m - m, kFar);
+  const float f = s.m == m ? 1.0f : fast_exp2(d * kLog2e);
+  s.a = f * (s.a + d * s.z);
+  s.z = f * s.z;
+  s.m = m;
+}
+// e^(x - m) and its product with x - m for one logit.
+__device__ __forceinline__ void add_logit(Stats &s, float x) {
+  float d = x - s.m;
+  d = d < kFar ? kFar : d;  // keeps a NaN
+  const float e = fast_exp2(d * kLog2e);
+  s.z += e;
+  s.a = fmaf(e, d, s.a);
+}
+__device__ __forceinline__ Stats wave_join(Stats s) {
+  move_reference(s, wave_max_f(s.m));
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    s.z += __shfl_xor(s.z, o);
+    s.a += __shfl_xor(s.a, o);
+  }
+  return s;
+}
+
+// What is left once a position's statistics and list are known (one wave).
+__device__ __forceinline__ void write_position(const LogProbArgs &a, long pos, const Stats &s,
+                                               u64 best, int lane) {
+  const float logz = logf(s.z);
+  if (lane == 0 && a.entropy) a.entropy[pos] = logz - s.a / s.z;
+  if (lane < a.top) {
+    a.top_tokens[pos * a.top + lane] = (int64_t)(uint32_t)~(uint32_t)best;
+    a.top_log_probs[pos * a.top + lane] = (code_value((uint32_t)(best >> 32)) - s.m) - logz;
+  }
+  for (int j = lane; j < a.per; j += 64) {
+    const int64_t t = a.tokens[pos * a.per + j];
+    float lp = 0.0f;
+    if (t >= 0) {
+      float x = NAN;
+      if (t < (int64_t)a.vocab) {
+        const size_t at = (size_t)pos * a.ld + (size_t)t;
+        x = a.bf16 ? bf16_to_f32(static_cast<const unsigned short *>(a.logits)[at])
+                   : static_cast<const float *>(a.logits)[at];
+      }
+      lp = (x - s.m) - logz;
+    }
+    a.log_probs[pos * a.per + j] = lp;
+  }
+}
+
+// Workgroup = one part of one position; NW waves. Parts are whole numbers of
+// 16-byte pieces of the position, counted from the 16-byte boundary at or
+// before its first logit.
+template <bool BF16, bool TOP, int NW>
+__global__ __launch_bounds__(64 * NW) void log_probs_kernel(LogProbArgs a) {
+  constexpr int E = BF16 ? 8 : 4;  // logits per 16 bytes
+  constexpr int U = 4;             // 16-byte pieces in flight per lane
+  __shared__ u64 buf[NW][64];
+  __shared__ float stats[NW][3];
+  const int lane = threadIdx.x & 63, wave = NW == 1 ? 0 : threadIdx.x >> 6;
+  const long pos = blockIdx.x / (unsigned)a.parts;
+  const int part = (int)(blockIdx.x - (unsigned)pos * (unsigned)a.parts);
+  const char *row = static_cast<const char *>(a.logits) + (size_t)pos * a.ld * (16 / E);
+  const int skew = (int)((reinterpret_cast<uintptr_t>(row) & 15) / (16 / E));
+  const char *base = row - skew * (16 / E);
+  const int vocab = (int)a.vocab;
+  // Pieces of this part: piece p holds logits E p - skew .. E p - skew + E - 1.
+  const int pieces = (vocab + skew + E - 1) / E;
+  const int p0 = min(part * a.part_pieces, pieces), p1 = min(p0 + a.part_pieces, pieces);
+
+  Stats s{kLowest, 0.0f, 0.0f};
+  u64 best = 0, bar = 0;  // the wave's sorted list, its top-th key
+  float bar_value = NAN;  // the top-th value, NaN while there is none
+  int held = 0;           // keys in buf
+  auto flush = [&] {
+    const u64 fresh = lane < held ? buf[wave][lane] : 0;
+    best = merge64(best, sort64(fresh, lane), lane);
+    bar = __shfl(best, a.top - 1);
+    bar_value = bar ? code_value((uint32_t)(bar >> 32)) : NAN;
+    held = 0;
+    __builtin_amdgcn_wave_barrier();
+  };
+
+  for (int p = p0 + wave * 64 + lane; p - lane < p1; p += 64 * NW * U) {
+    float x[U][E];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int q = p + u * 64 * NW;
+      const int first = q * E - skew;
+      if (q < p1 && first >= 0 && first + E <= vocab) {
+        if constexpr (BF16) {
+          const u16x8 h = *reinterpret_cast<const u16x8 *>(base + (size_t)q * 16);
+#pragma unroll
+          for (int e = 0; e < E; ++e) x[u][e] = bf16_to_f32(h[e]);
+        } else {
+          const f32x4 h = *reinterpret_cast<const f32x4 *>(base + (size_t)q * 16);
+#pragma unroll
+          for (int e = 0; e < E; ++e) x[u][e] = h[e];
+        }
+      } else {
+        // The row's first and last piece, and lanes past the part: -inf adds nothing.
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int i = first + e;
+          x[u][e] = -INFINITY;
+          if (q < p1 && i >= 0 && i < vocab) {
+            if constexpr (BF16)
+              x[u][e] = bf16_to_f32(reinterpret_cast<const unsigned short *>(row)[i]);
+            else
+              x[u][e] = reinterpret_cast<const float *>(row)[i];
+          }
+        }
+      }
+    }
+    float mx[U], m = s.m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      mx[u] = x[u][0];
+#pragma unroll
+      for (int e = 1; e < E; ++e) mx[u] = fmaxf(mx[u], x[u][e]);
+      m = fmaxf(m, mx[u]);
+    }
+    if (m > s.m) move_reference(s, m);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) add_logit(s, x[u][e]);
+    if constexpr (TOP) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int q = p + u * 64 * NW, first = q * E - skew;
+        // Indices grow from piece to piece of a wave, so a value equal to the
+        // bar's comes too late; within the pieces below the whole key decides.
+        if (!__any(q < p1 && !(mx[u] <= bar_value))) continue;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int i = first + e;
+          const u64 key = q < p1 && i >= 0 && i < vocab ? key_of(x[u][e], (uint32_t)i) : 0;
+          u64 pass = __ballot(key > bar);
+          if (!pass) continue;
+          if (held + __popcll(pass) > 64) {
+            flush();
+            pass = __ballot(key > bar);
+          }
+          if (key > bar)
+            buf[wave][held + __popcll(pass & (((u64)1 << lane) - 1))] = key;
+          held += __popcll(pass);
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
+    }
+  }
+  s = wave_join(s);
+  if constexpr (TOP) flush();
+  if constexpr (NW > 1) {
+    if constexpr (TOP) buf[wave][lane] = best;
+    if (lane == 0) {
+      stats[wave][0] = s.m;
+      stats[wave][1] = s.z;
+      stats[wave][2] = s.a;
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    float m = s.m;
+#pragma unroll
+    for (int w = 1; w < NW; ++w) m = fmaxf(m, stats[w][0]);
+    move_reference(s, m);
+#pragma unroll
+    for (int w = 1; w < NW; ++w) {
+      Stats t{stats[w][0], stats[w][1], stats[w][2]};
+      move_reference(t, m);
+      s.z += t.z;
+      s.a += t.a;
+      if constexpr (TOP) best = merge64(best, buf[w][lane], lane);
+    }
+  }
+  if (a.parts == 1) {
+    write_position(a, pos, s, best, lane);
+    return;
+  }
+  if (lane == 0) {
+    float *o = a.part_stats + 4 * (size_t)blockIdx.x;
+    o[0] = s.m;
+    o[1] = s.z;
+    o[2] = s.a;
+  }
+  if (TOP && lane < a.top) a.part_keys[(size_t)blockIdx.x * a.top + lane] = best;
+}
+
+// Joins the parts of a position: lane l takes parts l, l + 64, ... (one wave).
+template <bool TOP>
+__global__ __launch_bounds__(64) void log_probs_join_kernel(LogProbArgs a) {
+  const long pos = blockIdx.x;
+  const int lane = threadIdx.x;
+  Stats s{kLowest, 0.0f, 0.0f};
+  for (int p = lane; p < a.parts; p += 64) {
+    const float *o = a.part_stats + 4 * ((size_t)pos * a.parts + p);
+    Stats t{o[0], o[1], o[2]};
+    const float m = fmaxf(s.m, t.m);
+    move_reference(s, m);
+    move_reference(t, m);
+    s.z += t.z;
+    s.a += t.a;
+  }
+  s = wave_join(s);
+  u64 best = 0;
+  if constexpr (TOP) {
+    // The parts' lists are `top` keys each: 64 keys at a time.
+    const size_t n = (size_t)a.parts * a.top;
+    const u64 *keys = a.part_keys + (size_t)pos * n;
+    for (size_t i = 0; i < n; i += 64)
+      best = merge64(best, sort64(i + lane < n ? keys[i + lane] : 0, lane), lane);
+  }
+  write_position(a, pos, s, best, lane);
+}
+
+template <bool BF16, bool TOP>
+void launch_parts(const LogProbArgs &a, int waves, hipStream_t stream, const KernelEvents &ev) {
+  const dim3 grid((unsigned)(a.positions * (size_t)a.parts));
+  hipEvent_t stop = a.parts == 1 ? ev.stop : nullptr;
+  if (waves == 1)
+    hipExtLaunchKernelGGL((log_probs_kernel<BF16, TOP, 1>), grid, dim3(64), 0, stream, ev.start,
+                          stop, 0, a);
+  else
+    hipExtLaunchKernelGGL((log_probs_kernel<BF16, TOP, 4>), grid, dim3(256), 0, stream, ev.start,
+                          stop, 0, a);
+  if (a.parts == 1) return;
+  hipExtLaunchKernelGGL((log_probs_join_kernel<TOP>), dim3((unsigned)a.positions), dim3(64), 0,
+                        stream, nullptr, ev.stop, 0, a);
+}
+
+}  // namespace
+
+// Pieces are 16 bytes; a wave takes 256 of them a step (U of 64 lanes).
+void log_probs_plan(LogProbArgs &a, int cus) {
+  const size_t per_piece = a.bf16 ? 8 : 4;
+  const size_t pieces = (a.vocab + 2 * (per_piece - 1)) / per_piece;  // at any skew
+  a.parts = 1;
+  a.part_pieces = (int)pieces;
+  if (a.vocab <= kLogProbWaveVocab) return;
+  // Parts of at least two steps of a workgroup, until every CU has two workgroups.
+  const size_t want = a.positions ? (2 * (size_t)cus + a.positions - 1) / a.positions : 1;
+  const size_t most = (pieces + 2047) / 2048;
+  size_t parts = want < most ? want : most;
+  if (parts <= 1) return;
+  const size_t len = (pieces + parts - 1) / parts;
+  a.part_pieces = (int)len;
+  a.parts = (int)((pieces + len - 1) / len);
+}
+
+hipError_t launch_log_probs(const LogProbArgs &a, hipStream_t stream, const KernelEvents &ev) {
+  const int waves = a.vocab <= kLogProbWaveVocab ? 1 : 4;
+  if (a.bf16)
+    a.top ? launch_parts<true, true>(a, waves, stream, ev)
+          : launch_parts<true, false>(a, waves, stream, ev);
+  else
+    a.top ? launch_parts<false, true>(a, waves, stream, ev)
+          : launch_parts<false, false>(a, waves, stream, ev);
+  return hipGetLastError();
+}
+
+}  // namespace tfd

@@ -10,6 +10,8 @@ The reference exposes the two ops as eager-session extension methods:
 
 and as ``ExtensionOp`` descriptors (``LayaAttentionBlockOp``,
 ``JeffFullAttentionOp``) whose payload stores the f64 parameters as f32 bits.
+Beside them stand the operators a hybrid Jeff model needs around its full-attention
+layers: ``jeff_linear_attention_rows`` / ``_step`` and ``token_log_probs``.
 This module keeps those names, argument meanings and error behaviour, and runs
 every call on the GPU through ``libtfd_attention.so``. There is no CPU
 fallback: if the library or a GPU is missing, calls raise.
@@ -26,7 +28,7 @@ import hashlib
 import os
 import struct
 from dataclasses import dataclass
-from typing import Optional, Sequence
+from typing import Any, NamedTuple, Optional, Sequence
 
 import numpy as np
 
@@ -73,6 +75,10 @@ EXPORTED_SYMBOLS = (
     "tfd_jeff_full_attention_rows_bf16",
     "tfd_laya_attention_layer_f32",
     "tfd_jeff_full_attention_layer_rows_f32",
+    "tfd_jeff_linear_attention_rows_f32",
+    "tfd_jeff_linear_attention_rows_bf16",
+    "tfd_token_log_probs_f32",
+    "tfd_token_log_probs_bf16",
     "tfd_laya_forward_f32",
 )
 
@@ -154,6 +160,10 @@ def load_library(path: Optional[str] = None) -> ctypes.CDLL:
             I, [P, S, S, S, S, S, S, S, P, P, P, P, P, P, P, P, P, U32, U32, P, F]),
         "tfd_laya_forward_f32": (I, [P, P, P, P, S, S, P, P, S, P, P, P, F]),
     }
+    for kind in ("f32", "bf16"):
+        sig[f"tfd_jeff_linear_attention_rows_{kind}"] = (
+            I, [P, S, S, S, S, S, S, P, P, P, P, P, P, U32, P, P, P, F])
+        sig[f"tfd_token_log_probs_{kind}"] = (I, [P, P, S, S, S, P, S, S, P, P, P, P, F])
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
         fn.restype = res
@@ -254,6 +264,7 @@ _TORCH_DTYPES = {
     np.dtype(np.float32): ("float32",),
     np.dtype(np.uint8): ("uint8", "bool"),
     np.dtype(np.uint16): ("uint16", "int16", "bfloat16"),
+    np.dtype(np.int64): ("int64",),
 }
 
 
@@ -370,12 +381,12 @@ def _shape_arr(shape):
     return (ctypes.c_size_t * len(shape))(*shape)
 
 
-def _new_out(like: _Arg, n: int):
+def _new_out(like: _Arg, n: int, dtype=np.float32):
     if like.device:
         import torch
 
-        return torch.empty(n, dtype=torch.float32, device=like.obj.device)
-    return np.empty(n, dtype=np.float32)
+        return torch.empty(n, dtype=getattr(torch, np.dtype(dtype).name), device=like.obj.device)
+    return np.empty(n, dtype=dtype)
 
 
 # ------------------------------------------------------------------ op descriptors
@@ -601,6 +612,112 @@ def jeff_full_attention_rows(q, k, v, gate, q_norm, k_norm, mask, rows: int, len
           aq.ptr, ak.ptr, av.ptr, ag.ptr, aqn.ptr, akn.ptr, am.ptr,
           f32_bits(theta), f32_bits(eps), a_out.ptr, flags)
     return a_out.obj
+
+
+# ------------------------------------------------------------------ linear attention
+
+def jeff_linear_attention_rows(q, k, v, log_decay, beta, mask, rows: int, length: int, heads: int,
+                               key_heads: int, key_dim: int, value_dim: int, *,
+                               scale: Optional[float] = None, state=None, state_out=None,
+                               want_state: bool = True, bf16: bool = False,
+                               ctx: Optional[Context] = None, out=None):
+    """Linear attention over rows (include/tfd_attention.h): per row and value
+    head a state S (key_dim x value_dim) with, for every active token,
+    S <- exp(log_decay) S, then S <- S + k u^T with u = v (``beta`` None) or
+    beta (v - S^T k), and out = scale S^T q.
+
+    q, k are rows x (length, key_heads*key_dim), v and out rows x (length,
+    heads*value_dim), log_decay and beta rows x (length, heads), mask rows x
+    (length) or None, states rows x heads x (key_dim, value_dim) with the value
+    features contiguous. ``scale`` is 1/sqrt(key_dim) if None. ``state`` None starts
+    from zeros; ``state_out`` may be ``state`` itself. bf16 takes q, k and v as
+    bf16 bits. Returns (out, state after the last token), the state None unless
+    ``want_state`` or given a ``state_out``."""
+    ctx = ctx or default_context()
+    dt = np.uint16 if bf16 else np.float32
+    nk, nv = rows * length * key_heads * key_dim, rows * length * heads * value_dim
+    ng, ns = rows * length * heads, rows * heads * key_dim * value_dim
+    aq, ak, av = (_Arg(x, dt, nm, c) for x, nm, c in ((q, "q", nk), (k, "k", nk), (v, "v", nv)))
+    ag = _Arg(log_decay, np.float32, "log_decay", ng)
+    ab, am, asi = (_Arg(x, np.float32, nm, c if x is not None else None) for x, nm, c in
+                   ((beta, "beta", ng), (mask, "mask", rows * length), (state, "state", ns)))
+    if out is None:
+        out = _new_out(aq, nv)
+    if state_out is None and want_state:
+        state_out = _new_out(aq, ns)
+    elif state_out is state and state is not None:
+        state_out = asi.obj
+    a_out = _Arg(out, np.float32, "out", nv)
+    aso = _Arg(state_out, np.float32, "state_out", ns if state_out is not None else None)
+    flags = _flags([aq, ak, av, ag, ab, am, asi, aso, a_out], ctx)
+    fn = (ctx._lib.tfd_jeff_linear_attention_rows_bf16 if bf16
+          else ctx._lib.tfd_jeff_linear_attention_rows_f32)
+    _call(ctx, flags, fn, ctx.handle, rows, length, heads, key_heads, key_dim, value_dim, aq.ptr,
+          ak.ptr, av.ptr, ag.ptr, ab.ptr, am.ptr,
+          f32_bits(max(key_dim, 1) ** -0.5 if scale is None else scale), asi.ptr, aso.ptr, a_out.ptr, flags)
+    return a_out.obj, aso.obj
+
+
+def jeff_linear_attention_step(q, k, v, log_decay, beta, state, rows: int, heads: int,
+                               key_heads: int, key_dim: int, value_dim: int, *, mask=None,
+                               scale: Optional[float] = None, bf16: bool = False,
+                               ctx: Optional[Context] = None, out=None):
+    """``jeff_linear_attention_rows`` for one token a row: ``state`` (f32, contiguous)
+    is updated in place, also that of rows past a ``mask`` of zeros, which keep
+    theirs. Returns out, rows x (heads*value_dim)."""
+    if not _is_torch(state) and not (
+            isinstance(state, np.ndarray) and state.dtype == np.float32
+            and state.flags.c_contiguous and state.flags.writeable):
+        raise InvalidArgument(TFD_EINVAL, "state: expected a contiguous float32 array to update")
+    return jeff_linear_attention_rows(q, k, v, log_decay, beta, mask, rows, 1, heads, key_heads,
+                                      key_dim, value_dim, scale=scale, state=state,
+                                      state_out=state, bf16=bf16, ctx=ctx, out=out)[0]
+
+
+# ------------------------------------------------------------------ readout
+
+class TokenLogProbs(NamedTuple):
+    """What ``token_log_probs`` returns, flat column-major: log_probs
+    (per_position, positions), entropy (positions), top_tokens and top_log_probs
+    (top, positions), the last two None without ``top``, log_probs without tokens."""
+
+    log_probs: Any
+    entropy: Any
+    top_tokens: Any
+    top_log_probs: Any
+
+
+def token_log_probs(logits, tokens, positions: int, vocab: int, *, top: int = 0,
+                    leading_dim: Optional[int] = None, bf16: bool = False,
+                    ctx: Optional[Context] = None) -> TokenLogProbs:
+    """Log probabilities of given tokens under softmax(logits), the entropy and the
+    ``top`` most likely tokens at every position (include/tfd_attention.h).
+
+    logits: (vocab, positions) column-major, a position's logits contiguous and
+    positions ``leading_dim`` (vocab if None) apart. tokens: int64 (per_position,
+    positions), a negative one an unused slot (log probability 0), or None.
+    bf16 takes the logits as bf16 bits."""
+    ctx = ctx or default_context()
+    ld = vocab if leading_dim is None else leading_dim
+    ax = _Arg(logits, np.uint16 if bf16 else np.float32, "logits")
+    need = ld * (positions - 1) + vocab if positions else 0
+    if not need <= ax.n <= max(need, ld * positions):
+        raise InvalidArgument(TFD_EINVAL, f"logits: {ax.n} elements, the shape needs {need}")
+    at = _Arg(tokens, np.int64, "tokens")
+    per = at.n // positions if positions else 0
+    if at.n != per * positions:
+        raise InvalidArgument(TFD_EINVAL, f"tokens: {at.n} elements, not a whole number of "
+                              f"tokens for each of {positions} positions")
+    new = [_Arg(_new_out(ax, n, dt) if n is not None else None, dt, nm) for n, dt, nm in (
+        (per * positions if tokens is not None else None, np.float32, "log_probs"),
+        (positions, np.float32, "entropy"),
+        (top * positions if top > 0 else None, np.int64, "top_tokens"),
+        (top * positions if top > 0 else None, np.float32, "top_log_probs"))]
+    flags = _flags([ax, at, *new], ctx)
+    fn = ctx._lib.tfd_token_log_probs_bf16 if bf16 else ctx._lib.tfd_token_log_probs_f32
+    _call(ctx, flags, fn, ctx.handle, ax.ptr, vocab, ld, positions, at.ptr, per, top,
+          *[a.ptr for a in new], flags)
+    return TokenLogProbs(*[a.obj for a in new])
 
 
 def to_bf16_bits(x: np.ndarray) -> np.ndarray:

@@ -1,0 +1,371 @@
+"""Linear attention over rows, prompts and single tokens, against its recurrence
+in 64 bits, token by token.
+
+Tolerance. Without the delta rule every output and state element is a sum of
+products whose terms carry at most n = key_dim + 64 + length roundings of 2^-24
+each, taken on the sum of the terms' absolute values (`size`, the same recurrence
+on absolute values). Roundings to nearest are independent and unbiased to first
+order, so six standard deviations are 6 sqrt(n) 2^-24 of it; 8 more cover the
+decays' exponentials and the scale. With the delta rule and keys of unit length the
+step S -> e^g (I - beta k k^T) S does not lengthen any vector for beta in [0, 1], so
+errors add up over the tokens without growing: the same count holds for a head's
+errors against the largest norm its state (and with it the output) has had, plus its
+largest write.
+"""
+import numpy as np
+import pytest
+
+import tenferro_ext as te
+from tenferro_ext.workloads import Lcg
+
+
+def reference(q, k, v, g, beta, mask, scale, state):
+    """q, k (R, HK, dk, L), v (R, H, dv, L), g, beta (R, H, L), mask (R, L),
+    state (R, H, dk, dv): out (R, H, dv, L), state, and their `size`s."""
+    R, H, dv, L = v.shape
+    HK, dk = q.shape[1:3]
+    idx = np.arange(H) // (H // HK)
+    S = np.zeros((R, H, dk, dv)) if state is None else state.astype(np.float64)
+    A = np.abs(S)
+    out, size = np.zeros((2, R, H, dv, L))
+    norm = np.sqrt((S ** 2).sum((2, 3)))
+    for t in range(L):
+        on = np.ones(R, bool) if mask is None else mask[:, t] != 0
+        if not on.any():
+            continue
+        kt, qt = k[on][..., t][:, idx].astype(np.float64), q[on][..., t][:, idx].astype(np.float64)
+        f = np.exp(g[on, :, t].astype(np.float64))[..., None, None]
+        D = S[on] * f
+        u = v[on, :, :, t].astype(np.float64)
+        if beta is not None:
+            u = beta[on, :, t].astype(np.float64)[..., None] * (u - np.einsum("rhij,rhi->rhj", D, kt))
+        S[on] = D + kt[..., None] * u[:, :, None]
+        out[on, :, :, t] = scale * np.einsum("rhij,rhi->rhj", S[on], qt)
+        if beta is None:
+            A[on] = A[on] * f + np.abs(kt)[..., None] * np.abs(u)[:, :, None]
+            size[on, :, :, t] = abs(scale) * np.einsum("rhij,rhi->rhj", A[on], np.abs(qt))
+        else:
+            norm[on] = np.maximum(norm[on], np.sqrt((S[on] ** 2).sum((2, 3))))
+            norm[on] = np.maximum(norm[on], np.sqrt((u ** 2).sum(2)))
+    if beta is not None:
+        A = np.broadcast_to(norm[..., None, None], S.shape)
+        size = abs(scale) * norm[..., None, None] * np.sqrt(
+            (q.astype(np.float64) ** 2).sum(2)).max(-1, initial=0.0)[:, idx][..., None, None] * np.ones_like(out)
+    return out, S, size, A
+
+
+class Problem:
+    def __init__(self, R, L, H, HK, dk, dv, *, bf16=False, delta=True, mask=None, state=False,
+                 decay=1.0, seed=1):
+        rng = Lcg(seed * 7919 + R * 1000003 + L * 1009 + H * 101 + dk * 11 + dv)
+
+        def normal(*shape):
+            return rng.normal(int(np.prod(shape))).astype(np.float32).reshape(shape)
+
+        def unit(x):
+            return x / np.sqrt((x * x).sum(2, keepdims=True))
+
+        self.dims = (R, L, H, HK, dk, dv)
+        self.q, self.k = unit(normal(R, HK, dk, L)), unit(normal(R, HK, dk, L))
+        self.v = normal(R, H, dv, L)
+        self.g = -np.abs(normal(R, H, L)) * np.float32(decay)
+        self.beta = (1 / (1 + np.exp(-normal(R, H, L)))).astype(np.float32) if delta else None
+        self.state = normal(R, H, dk, dv) if state else None
+        self.bf16, self.mask = bf16, None
+        if bf16:
+            self.q, self.k, self.v = (te.bf16_bits_to_f32(te.to_bf16_bits(x))
+                                      for x in (self.q, self.k, self.v))
+        if mask == "left":  # one row of them without any active token
+            self.mask = np.zeros((R, L), np.float32)
+            for r in range(R):
+                self.mask[r, (L * r + R - 1) // R:] = 1.0
+            self.mask[-1] = 0.0
+        elif mask == "holes":
+            self.mask = (rng.uniform(R * L) < 0.7).astype(np.float32).reshape(R, L)
+
+    def args(self, to=lambda x: x):
+        bits = te.to_bf16_bits if self.bf16 else lambda x: x
+        ops = [bits(self.q), bits(self.k), bits(self.v), self.g, self.beta, self.mask]
+        return [to(np.ascontiguousarray(x).reshape(-1)) if x is not None else None for x in ops]
+
+    def run(self, ctx, to=lambda x: x, **kw):
+        R, L, H, HK, dk, dv = self.dims
+        state = to(self.state.reshape(-1)) if self.state is not None else None
+        return te.jeff_linear_attention_rows(*self.args(to), R, L, H, HK, dk, dv, state=state,
+                                             bf16=self.bf16, ctx=ctx, **kw)
+
+    def check(self, out, state, scale=None):
+        R, L, H, HK, dk, dv = self.dims
+        scale = float(np.float32(dk ** -0.5 if scale is None else scale))
+        want, S, size, A = reference(self.q, self.k, self.v, self.g, self.beta, self.mask, scale,
+                                     self.state)
+        tol = 2.0 ** -24 * (8 + 6 * np.sqrt(dk + 64 + L))
+        out = np.asarray(out, np.float64).reshape(want.shape)
+        assert (np.abs(out - want) <= tol * size + 1e-37).all(), np.nanmax(
+            np.abs(out - want) / (size + 1e-30))
+        if state is not None:
+            state = np.asarray(state, np.float64).reshape(S.shape)
+            assert (np.abs(state - S) <= tol * A + 1e-37).all(), np.nanmax(
+                np.abs(state - S) / (A + 1e-30))
+
+
+def cuda(x):
+    import torch
+
+    return torch.from_numpy(np.ascontiguousarray(x).copy()).cuda()
+
+
+def host(x):
+    return x.cpu().numpy()
+
+
+# ------------------------------------------------------------------ refusals (no GPU)
+
+
+@pytest.fixture()
+def ctx():
+    c = te.Context(0)
+    yield c
+    c.close()
+
+
+def test_refusals_before_any_device_call(ctx):
+    R, L, H, HK, dk, dv = 2, 3, 4, 2, 8, 5
+    f = lambda n: np.zeros(n, np.float32)
+    good = dict(q=f(R * L * HK * dk), k=f(R * L * HK * dk), v=f(R * L * H * dv),
+                log_decay=f(R * L * H), beta=f(R * L * H), mask=f(R * L))
+    call = lambda dims=(R, L, H, HK, dk, dv), **kw: te.jeff_linear_attention_rows(
+        *[kw.get(n, x) for n, x in good.items()], *dims, ctx=ctx,
+        **{n: x for n, x in kw.items() if n not in good})
+    for name, x in good.items():
+        with pytest.raises(te.InvalidArgument, match=f"{name}: {x.size - 1} elements"):
+            call(**{name: x[:-1]})
+    with pytest.raises(te.InvalidArgument, match="state: 3 elements"):
+        call(state=f(3))
+    with pytest.raises(te.InvalidArgument, match="state_out: 3 elements"):
+        call(state_out=f(3))
+    with pytest.raises(te.InvalidArgument, match="multiple of key_heads"):
+        call((R, L, 3, 2, dk, dv), v=f(R * L * 3 * dv), log_decay=f(R * L * 3), beta=f(R * L * 3))
+    big = 257
+    with pytest.raises(te.Unsupported, match="key_dim 257 exceeds 256"):
+        call((R, L, H, HK, big, dv), q=f(R * L * HK * big), k=f(R * L * HK * big))
+    rc = ctx._lib.tfd_jeff_linear_attention_rows_f32(
+        ctx.handle, R, L, H, 0, dk, dv, *[None] * 6, 0, None, None, None, 0)
+    assert rc == te.TFD_EINVAL
+    rc = ctx._lib.tfd_jeff_linear_attention_rows_f32(
+        ctx.handle, R, L, H, HK, dk, dv, *[None] * 6, 0, None, None, None, 0)
+    assert rc == te.TFD_EINVAL and "null buffer" in ctx._lib.tfd_last_error(ctx.handle).decode()
+    rc = ctx._lib.tfd_jeff_linear_attention_rows_f32(
+        ctx.handle, 1 << 40, 1 << 40, H, HK, dk, dv, *[None] * 6, 0, None, None, None, 0)
+    assert rc == te.TFD_EINVAL and "overflow" in ctx._lib.tfd_last_error(ctx.handle).decode()
+    rc = ctx._lib.tfd_jeff_linear_attention_rows_bf16(
+        ctx.handle, R, L, H, HK, dk, dv, *[None] * 6, 0, None, None, None, te.TFD_ASYNC)
+    assert rc == te.TFD_EINVAL and "TFD_ASYNC" in ctx._lib.tfd_last_error(ctx.handle).decode()
+    with pytest.raises(te.InvalidArgument, match="state: expected a contiguous float32 array"):
+        te.jeff_linear_attention_step(f(dk), f(dk), f(dv), f(1), None, np.zeros(dk * dv), 1, 1, 1,
+                                      dk, dv, ctx=ctx)
+
+
+def test_empty_problems_need_no_gpu(ctx):
+    z = np.zeros(0, np.float32)
+    out, state = te.jeff_linear_attention_rows(z, z, z, z, None, None, 0, 5, 2, 1, 4, 4, ctx=ctx)
+    assert out.size == 0 and state.size == 0
+    out, state = te.jeff_linear_attention_rows(z, z, z, z, None, None, 3, 0, 2, 1, 4, 4,
+                                               want_state=False, ctx=ctx)
+    assert out.size == 0 and state is None
+
+
+# ------------------------------------------------------------------ on the GPU
+
+SHAPES = [  # rows, length, heads, key_heads, key_dim, value_dim
+    (1, 1, 1, 1, 1, 1), (2, 2, 2, 1, 5, 3), (3, 17, 4, 2, 20, 33), (2, 63, 2, 2, 32, 32),
+    (1, 64, 3, 1, 64, 48), (2, 65, 2, 1, 16, 130), (3, 127, 2, 2, 128, 128), (1, 128, 2, 1, 96, 80),
+    (2, 129, 4, 4, 72, 20), (1, 200, 2, 1, 256, 72), (2, 257, 3, 3, 130, 257), (1, 600, 2, 1, 64, 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("delta", [True, False], ids=["delta", "plain"])
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_against_the_recurrence(gpu_ctx, shape, bf16, delta):
+    for i, mask in enumerate((None, "left", "holes")):
+        p = Problem(*shape, bf16=bf16, delta=delta, mask=mask, state=i != 1, seed=i,
+                    decay=(0.02, 1.0, 5.0)[i])
+        out, state = p.run(gpu_ctx, cuda)
+        p.check(host(out), host(state))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("length", [1, 30, 150])
+@pytest.mark.parametrize("delta", [True, False], ids=["delta", "plain"])
+def test_decays_that_forget(gpu_ctx, length, delta):
+    """log_decay -inf, very negative and very small magnitudes side by side: a sum
+    of such decays over the tokens in 32 bits would lose the small ones."""
+    p = Problem(2, length, 2, 1, 64, 40, delta=delta, state=True, decay=0.01)
+    p.g[:, :, ::7] = -1000.0
+    p.g[0, :, 3::11] = -np.inf
+    p.g[1, 1, 5::9] = -100.0
+    p.g[:, 0, 2::13] = 0.0
+    out, state = p.run(gpu_ctx, cuda)
+    p.check(host(out), host(state))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("length", [2, 150])
+def test_inactive_tokens_hold_anything(gpu_ctx, length):
+    for bf16 in (False, True):
+        p = Problem(2, length, 4, 2, 40, 24, bf16=bf16, mask="holes", state=True)
+        p.mask[0, 0], p.mask[1, -1] = 0.0, 0.0
+        want = [host(x) for x in p.run(gpu_ctx, cuda)]
+        off = p.mask == 0
+        for x in (p.q, p.k, p.v, p.g, p.beta):
+            y = np.moveaxis(x, -1, 1)  # (R, L, ...)
+            y[off] = np.nan
+        p.v[0, 0, 0][off[0]] = np.inf
+        got = [host(x) for x in p.run(gpu_ctx, cuda)]
+        for a, b in zip(got, want):
+            assert np.array_equal(a, b)
+        out = got[0].reshape(2, -1, length)
+        assert (np.moveaxis(out, 1, 2)[off] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("delta", [True, False], ids=["delta", "plain"])
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_a_prompt_in_pieces_and_single_tokens(gpu_ctx, bf16, delta):
+    """The state carries over from call to call: 100 + 75 tokens as prompts, then 5
+    single tokens with the state updated in place, are the 180 tokens at once."""
+    p = Problem(3, 180, 4, 2, 64, 48, bf16=bf16, delta=delta, mask="holes")
+    R, L, H, HK, dk, dv = p.dims
+    outs, state = [], None
+
+    def part(a, b):
+        w = Problem(R, b - a, H, HK, dk, dv, bf16=bf16, delta=delta)
+        w.q, w.k, w.v, w.g, w.mask = (x[..., a:b] for x in (p.q, p.k, p.v, p.g, p.mask))
+        w.beta = p.beta[..., a:b] if delta else None
+        return w
+
+    for a, b in ((0, 100), (100, 175)):
+        w = part(a, b)
+        out, state = te.jeff_linear_attention_rows(*w.args(cuda), *w.dims, state=state, bf16=bf16,
+                                                   ctx=gpu_ctx)
+        outs.append(host(out).reshape(R, H, dv, b - a))
+    for t in range(175, 180):
+        q, k, v, g, beta, mask = part(t, t + 1).args(cuda)
+        out = te.jeff_linear_attention_step(q, k, v, g, beta, state, R, H, HK, dk, dv, mask=mask,
+                                            bf16=bf16, ctx=gpu_ctx)
+        outs.append(host(out).reshape(R, H, dv, 1))
+    p.check(np.concatenate(outs, -1), host(state))
+
+
+@pytest.mark.gpu
+def test_state_in_place_zero_length_and_host_arrays(gpu_ctx):
+    for L in (0, 1, 90):
+        p = Problem(2, L, 2, 2, 33, 18, state=True)
+        state = cuda(p.state.reshape(-1))
+        dims = p.dims
+        out, same = te.jeff_linear_attention_rows(*p.args(cuda), *dims, state=state,
+                                                  state_out=state, ctx=gpu_ctx)
+        assert same is state
+        p.check(host(out), host(state))
+        out, s = p.run(gpu_ctx)  # host arrays: uploaded, run, downloaded
+        assert isinstance(out, np.ndarray)
+        assert np.array_equal(s, host(state))
+        p.check(out, s)
+        out2, none = p.run(gpu_ctx, cuda, want_state=False)
+        assert none is None and np.array_equal(host(out2), out)
+        p.state = None
+        out, s = p.run(gpu_ctx, cuda, scale=0.7)
+        p.check(host(out), host(s), scale=0.7)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("length", [1, 8, 77, 256])
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_unaligned_buffers_and_their_surroundings(gpu_ctx, length, bf16):
+    """Operands one element off a 16-byte boundary, outputs inside larger buffers
+    that keep what is around them: the same bits as with whole buffers."""
+    import torch
+
+    p = Problem(2, length, 4, 2, 64, 36, bf16=bf16, mask="holes", state=True)
+    want = [host(x) for x in p.run(gpu_ctx, cuda)]
+
+    def shifted(x):
+        y = cuda(np.concatenate((x[:1], x.reshape(-1), x[:1])))
+        return y[1:-1]
+
+    buf = [torch.full((w.size + 2,), 7.0, device="cuda") for w in want]
+    p.run(gpu_ctx, shifted, out=buf[0][1:-1], state_out=buf[1][1:-1])
+    for b, w in zip(buf, want):
+        b = host(b)
+        assert b[0] == 7.0 and b[-1] == 7.0 and np.array_equal(b[1:-1], w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 1, 16, 16, 128, 128), (2, 300, 4, 2, 128, 64)], ids=str)
+def test_repeats_streams_and_graphs(shape):
+    """The same bits on every run, on another stream, and on every replay of a graph,
+    also after a larger call of the same context."""
+    import torch
+
+    stream = torch.cuda.Stream()
+    with te.Context(0, stream=stream.cuda_stream) as ctx, torch.cuda.stream(stream):
+        p = Problem(*shape, state=True, mask="holes")
+        R, L, H, HK, dk, dv = shape
+        want = [host(x) for x in p.run(ctx, cuda)]
+        ops = p.args(cuda)
+        state, out, new = cuda(p.state.reshape(-1)), cuda(want[0] * 0), cuda(want[1] * 0)
+        call = lambda: te.jeff_linear_attention_rows(*ops, *p.dims, state=state, state_out=new,
+                                                     ctx=ctx, out=out)
+        with te.asynchronous():
+            call()
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                call()
+        for i in range(4):
+            out.fill_(-1.0), new.fill_(-1.0)
+            graph.replay()
+            stream.synchronize()
+            assert np.array_equal(host(out), want[0]) and np.array_equal(host(new), want[1])
+            if i == 1:  # a larger call in between, eager
+                b = Problem(2 * R, L + 200, H, HK, dk, dv)
+                b.check(*[host(x) for x in b.run(ctx, cuda)])
+        with te.asynchronous(), pytest.raises(te.TenferroExtError):
+            big = Problem(9, 1500, H, HK, dk, 256)
+            args = big.args(cuda)
+            o, s = torch.empty(9 * 1500 * H * 256, device="cuda"), torch.empty(
+                9 * H * dk * 256, device="cuda")
+            stream.synchronize()
+            graph2 = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph2, stream=stream):
+                te.jeff_linear_attention_rows(*args, *big.dims, state_out=s, out=o, ctx=ctx)
+                raise te.TenferroExtError(0, "captured without growing")
+    with te.Context(0) as own:  # the context's own stream, ordered against torch's
+        got = [host(x) for x in p.run(own, cuda)]
+        assert all(np.array_equal(a, b) for a, b in zip(got, want))
+        assert own.retained_bytes() > 0
+
+
+@pytest.mark.gpu
+def test_states_past_four_gigabytes(gpu_ctx):
+    """Single tokens of so many rows that the states' offsets pass 32 bits."""
+    import torch
+
+    R, H, dk, dv = 4200, 16, 128, 128
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    new = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    q, k = (torch.nn.functional.normalize(new(R, H, dk), dim=2) for _ in range(2))
+    v, g, beta = new(R, H, dv), -new(R, H).abs(), torch.rand(R, H, generator=gen, device="cuda")
+    state = new(R, H, dk, dv)
+    rows = torch.tensor([0, 2047, 2048, 4095, 4096, R - 1])
+    before = state[rows.cuda()].cpu().numpy()
+    out = te.jeff_linear_attention_step(q.view(-1), k.view(-1), v.view(-1), g.view(-1),
+                                        beta.view(-1), state.view(-1), R, H, H, dk, dv,
+                                        ctx=gpu_ctx)
+    part = lambda x: x[rows.cuda()].cpu().numpy()
+    p = Problem(len(rows), 1, H, H, dk, dv)
+    p.q, p.k, p.v, p.g, p.beta = part(q)[..., None], part(k)[..., None], part(v)[..., None], \
+        part(g)[..., None], part(beta)[..., None]
+    p.state = before
+    p.check(part(out.view(R, -1)), part(state))
