@@ -153,7 +153,7 @@ hipError_t launch_recurrent(const LinearArgs &a, hipStream_t stream, const Kerne
 
 }  // namespace
 
-hipError_t launch_linear_attention(const LinearArgs &a, hipStream_t stream,
+hipError_t launch_linear_recurrent(const LinearArgs &a, hipStream_t stream,
                                    const KernelEvents &ev) {
   if (a.bf16)
     return a.beta ? launch_recurrent<unsigned short, true>(a, stream, ev)

@@ -64,6 +64,7 @@ struct tfd_ctx {
   DevBuf layer;       // intermediates of the layer entries (projections, attention output)
   DevBuf model;       // activations and token inputs of the model forward
   DevBuf planes;      // bf16 planes of the linears' operands
+  DevBuf linear;      // chunk states, writes and solves of the linear attention
   DevBuf readout;     // partial statistics of the token log probabilities
   // Workspaces that a captured graph may still use, outgrown since.
   std::vector<void *> retired;
@@ -1482,6 +1483,11 @@ int laya_forward(tfd_ctx *c, const tfd_laya_model *m, const int64_t *ids, const 
 
 // ------------------------------------------------------- linear attention
 
+// Tokens up to which the recurrence runs token by token.
+constexpr size_t kLinearRecurrentTokens = 12;
+// Workspace of the chunked form that is not passed while one row fits it.
+constexpr size_t kLinearWorkspace = (size_t)2 << 30;
+
 int linear_run(tfd_ctx *c, bool bf16, size_t rows, size_t length, size_t heads, size_t key_heads,
                size_t key_dim, size_t value_dim, const void *q, const void *k, const void *v,
                const float *log_decay, const float *beta, const float *mask, uint32_t scale_bits,
@@ -1547,9 +1553,43 @@ int linear_run(tfd_ctx *c, bool bf16, size_t rows, size_t length, size_t heads, 
   a.scale = bits_to_f32(scale_bits);
   a.bf16 = bf16;
   a.state_vec = value_dim % 4 == 0 && aligned16(si_d) && aligned16(so_d);
+  a.vec_k = length % 4 == 0 && (reinterpret_cast<uintptr_t>(k_d) & (4 * es - 1)) == 0;
+  a.vec_v = length % 4 == 0 && (reinterpret_cast<uintptr_t>(v_d) & (4 * es - 1)) == 0;
   tfd::KernelEvents ev;
-  if (!capturing && (rc = timing_events(c, &ev))) return rc;
-  TFD_HIP(c, tfd::launch_linear_attention(a, c->stream, ev), "linear_attention launch");
+  if (length <= kLinearRecurrentTokens) {
+    if (!capturing && (rc = timing_events(c, &ev))) return rc;
+    TFD_HIP(c, tfd::launch_linear_recurrent(a, c->stream, ev), "linear_recurrent launch");
+  } else {
+    // As many rows at once as the workspace limit allows, at least one.
+    a.rows = 1;
+    const size_t row = tfd::linear_space(a).total();
+    size_t at_once = std::max<size_t>(1, kLinearWorkspace / row);
+    at_once = std::min(rows, at_once);
+    if ((rc = reserve_capturable(c, op, c->linear, row * at_once, capturing))) return rc;
+    if (!capturing && (rc = timing_events(c, &ev))) return rc;
+    auto from = [](const void *p, size_t bytes) {
+      return p ? static_cast<const char *>(p) + bytes : nullptr;
+    };
+    for (size_t r0 = 0; r0 < rows; r0 += at_once) {
+      tfd::LinearArgs b = a;
+      b.rows = (int)std::min(at_once, rows - r0);
+      b.q = from(q_d, es * (kn / rows) * r0);
+      b.k = from(k_d, es * (kn / rows) * r0);
+      b.v = from(v_d, es * (vn / rows) * r0);
+      const size_t f = sizeof(float);
+      b.log_decay = reinterpret_cast<const float *>(from(g_d, f * (gn / rows) * r0));
+      b.beta = reinterpret_cast<const float *>(from(b_d, f * (gn / rows) * r0));
+      b.mask = reinterpret_cast<const float *>(from(m_d, f * length * r0));
+      b.state_in = reinterpret_cast<const float *>(from(si_d, f * (sn / rows) * r0));
+      if (so_d) b.state_out = static_cast<float *>(so_d) + sn / rows * r0;
+      b.out = static_cast<float *>(out_d) + vn / rows * r0;
+      TFD_HIP(c,
+              tfd::launch_linear_chunks(b, c->linear.ptr, c->stream,
+                                        tfd::KernelEvents{r0 ? nullptr : ev.start,
+                                                          r0 + at_once < rows ? nullptr : ev.stop}),
+              "linear_chunks launch");
+    }
+  }
   if (!(flags & TFD_DEVICE_PTRS) && state_out)
     TFD_HIP(c, hipMemcpyAsync(state_out, so_d, sizeof(float) * sn, hipMemcpyDeviceToHost, c->stream),
             "hipMemcpyAsync D2H");
@@ -1673,6 +1713,7 @@ void tfd_ctx_destroy(tfd_ctx *c) {
     if (c->layer.ptr) (void)hipFree(c->layer.ptr);
     if (c->planes.ptr) (void)hipFree(c->planes.ptr);
     if (c->model.ptr) (void)hipFree(c->model.ptr);
+    if (c->linear.ptr) (void)hipFree(c->linear.ptr);
     if (c->readout.ptr) (void)hipFree(c->readout.ptr);
     for (void *p : c->retired) (void)hipFree(p);
     if (c->blas) (void)rocblas_destroy_handle(c->blas);
@@ -1705,7 +1746,8 @@ void *tfd_ctx_stream(tfd_ctx *c) {
 size_t tfd_ctx_retained_bytes(const tfd_ctx *c) {
   if (!c) return 0;
   size_t total = sizeof(tfd_ctx) + c->bits.cap + c->kp.cap + c->layer.cap + c->model.cap + c->planes.cap +
-                 c->model_host.capacity() + c->readout.cap + c->retired_bytes;
+                 c->model_host.capacity() + c->linear.cap + c->readout.cap +
+                 c->retired_bytes;
   for (const auto &b : c->staging) total += b.cap;
   for (const auto &e : c->rope) total += e.bytes;
   return total;

@@ -343,9 +343,32 @@ struct LinearArgs {
   float scale;
   bool bf16;       // q, k and v
   bool state_vec;  // 16-byte access to the states' rows: dv % 4 == 0, aligned
+  bool vec_k, vec_v;  // access to four tokens of k, v at once: L % 4 == 0, aligned
 };
-hipError_t launch_linear_attention(const LinearArgs &a, hipStream_t stream,
+// Token by token.
+hipError_t launch_linear_recurrent(const LinearArgs &a, hipStream_t stream,
                                    const KernelEvents &ev);
+
+// By chunks of this many tokens (linear_chunks.hip).
+constexpr int kLinearChunk = 64;
+// One chunk's solve operand: six blocks of three pieces.
+constexpr int kLinearSolveBytes = 6 * 3 * 1024;
+// Contraction steps of 32 key features, a power of two.
+inline int linear_steps(int dk) { return dk <= 32 ? 1 : dk <= 64 ? 2 : dk <= 128 ? 4 : 8; }
+// Bytes of the workspace of launch_linear_chunks: the states before and the
+// writes of every chunk (f32), and the solve operands.
+struct LinearSpace {
+  size_t states, writes, solve;
+  size_t total() const { return states + writes + solve; }
+};
+inline LinearSpace linear_space(const LinearArgs &a) {
+  const size_t chunks = (size_t)a.rows * a.heads * ((a.L + kLinearChunk - 1) / kLinearChunk);
+  const size_t tiles = (size_t)((a.dv + 15) / 16);
+  return LinearSpace{chunks * tiles * linear_steps(a.dk) * 2048, a.beta ? chunks * tiles * 4096 : 0,
+                     a.beta ? chunks * kLinearSolveBytes : 0};
+}
+hipError_t launch_linear_chunks(const LinearArgs &a, void *ws, hipStream_t stream,
+                                const KernelEvents &ev);
 
 // ------------------------------------------------ token log probabilities
 
