@@ -5,10 +5,11 @@
 //   U    = T (beta (V - d K S0))                 (plain: U = V)
 //   O    = scale (d Q S0 + (D . Q K^T) U)
 //   S0  <- e^G S0 + K^T (e U)
-// Three kernels, the last and the first parallel over the chunks:
-//   linear_solve_kernel   T of every chunk (delta rule only)
-//   linear_walk_kernel    along each (row, head): U and the states S0
-//   linear_output_kernel  O of every chunk
+// Two kernels:
+//   linear_pairs_kernel  over all chunks at once: the decays, D . Q K^T and T
+//   linear_walk_kernel   along each (row, head): U, O and the state, which stays in
+//                        the accumulators from the first chunk to the last
+// Chunks without an active token are skipped by both.
 //
 // Products run on the bf16 matrix cores with f32 accumulation, f32 operands as
 // three bf16 pieces (six products, tfd_device.hpp), bf16 operands as they are:
@@ -67,6 +68,19 @@ __device__ __forceinline__ f32x4 mma(const frag (&a)[NA], const frag (&b)[NB], f
   return mfma_16x16x32_bf16(a[0], b[0], c);
 }
 
+// The pieces (of a, of b) of product number x of the NA x NB that count, small first.
+template <int NA, int NB>
+struct Products {
+  static constexpr int n = NA == 3 && NB == 3 ? 6 : (NA == 3 || NB == 3 ? 3 : 1);
+  static constexpr int a(int x) {
+    constexpr int six[6] = {0, 2, 1, 0, 1, 0};
+    return NA == 1 ? 0 : (NB == 1 ? 2 - x : six[x]);
+  }
+  static constexpr int b(int x) {
+    constexpr int six[6] = {2, 0, 1, 1, 0, 0};
+    return NB == 1 ? 0 : (NA == 1 ? 2 - x : six[x]);
+  }
+};
 template <int NP>
 __device__ __forceinline__ void load_frag(const unsigned char *block, int lane, frag (&p)[NP]) {
 #pragma unroll
@@ -85,42 +99,76 @@ struct Pieces {
   static constexpr int n = sizeof(T) == 4 ? 3 : 1;
 };
 
+// Loads go through a buffer resource of the head's (feature, token) matrix: one
+// 32-bit offset, no branch; past its end they give 0 (offsets stay below 2^31, so a
+// feature past key_dim is past the end, never wrapped). Rows before
+// the end run into the next one (tokens behind the sequence), and inactive tokens
+// hold anything: both are dropped where the values are used, so that nothing
+// waits for a load before that.
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+constexpr int kNowhere = (int)0x80000000u;  // past every resource's end
+
+// What a lane holds of an operand: eight f32, four pairs of bf16 (packed), or
+// eight single bf16.
+struct Raw {
+  uint32_t d[8];
+};
+
 template <typename T>
-__device__ __forceinline__ float as_f32(T x) {
-  if constexpr (sizeof(T) == 2)
-    return bf16_to_f32(x);
+__device__ __forceinline__ uint32_t load_one(Rsrc m, int off) {
+  if constexpr (sizeof(T) == 4)
+    return __builtin_amdgcn_raw_buffer_load_b32(m, off, 0, 0);
   else
-    return x;
+    return __builtin_amdgcn_raw_buffer_load_b16(m, off, 0, 0);
+}
+// Four consecutive tokens into d[0..3] (f32, single bf16) or d[0..1] (packed).
+// 16-byte f32 loads need 4-byte alignment only, 8-byte bf16 ones are taken with
+// `packed` alone (length % 4 == 0, aligned).
+template <typename T>
+__device__ __forceinline__ void load_four(Rsrc m, int off, bool packed, uint32_t *d) {
+  if constexpr (sizeof(T) == 4) {
+    const auto x = __builtin_amdgcn_raw_buffer_load_b128(m, off, 0, 0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) d[e] = x[e];
+  } else if (packed) {
+    const auto x = __builtin_amdgcn_raw_buffer_load_b64(m, off, 0, 0);
+    d[0] = x[0], d[1] = x[1];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) d[e] = load_one<T>(m, off + 2 * e);
+  }
 }
 
+// Eight values as operand pieces, those whose bit of `on` is not set as 0.
 template <typename T>
-__device__ __forceinline__ void to_frag(const T (&v)[8], frag (&p)[Pieces<T>::n]) {
+__device__ __forceinline__ void to_frag(const Raw &v, bool packed, unsigned on,
+                                        frag (&p)[Pieces<T>::n]) {
   if constexpr (sizeof(T) == 2) {
-    u16x8 h;
+    uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = v[e];
-    p[0] = __builtin_bit_cast(frag, h);
+    for (int i = 0; i < 4; ++i) {
+      w[i] = packed ? v.d[i] : (v.d[2 * i] & 0xffffu) | (v.d[2 * i + 1] << 16);
+      const unsigned pair = on >> (2 * i);
+      w[i] &= (pair & 1u ? 0xffffu : 0u) | (pair & 2u ? 0xffff0000u : 0u);
+    }
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    p[0] = __builtin_bit_cast(frag, u32x4{w[0], w[1], w[2], w[3]});
   } else {
-    split8(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]}, p);
+    f32x4 lo, hi;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      lo[e] = (on >> e) & 1u ? __uint_as_float(v.d[e]) : 0.0f;
+      hi[e] = (on >> (4 + e)) & 1u ? __uint_as_float(v.d[4 + e]) : 0.0f;
+    }
+    split8(lo, hi, p);
   }
 }
-
-// Four consecutive tokens of a feature row, 0 where `act` (bit = token of the
-// chunk) is not set; at = chunk token of the first one. Inactive tokens are
-// only read inside the row (vec: 16 or 8 byte pieces, length % 4 == 0).
+// Value e of four loaded by load_four, as f32.
 template <typename T>
-__device__ __forceinline__ void load4(const T *row, int at, uint64_t act, int n, bool vec, T (&v)[4]) {
-  const unsigned on = (unsigned)(act >> at) & 15u;
-  if (vec) {
-    typedef T vec4 __attribute__((ext_vector_type(4)));
-    vec4 x = {};
-    if (at < n) x = *reinterpret_cast<const vec4 *>(row + at);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = (on >> e) & 1u ? x[e] : T(0);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = (on >> e) & 1u ? row[at + e] : T(0);
-  }
+__device__ __forceinline__ float value_of(const uint32_t *d, bool packed, int e) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(d[e]);
+  if (packed) return __uint_as_float(e & 1 ? d[e >> 1] & 0xffff0000u : d[e >> 1] << 16);
+  return __uint_as_float(d[e] << 16);
 }
 
 // ------------------------------------------------------------------ a chunk
@@ -157,10 +205,6 @@ __device__ __forceinline__ void scan_chunk(const LinearArgs &a, size_t rh, int t
   c.beta[lane] = on && a.beta ? a.beta[rh * a.L + t0 + lane] : 0.0f;
 }
 
-__device__ __forceinline__ float decay_between(const ChunkScan &c, int t, int s) {
-  return c.forget[t] > s ? 0.0f : fast_exp2((float)(c.cum[t] - c.cum[s]));
-}
-
 // Bit t: token t0 + t is there and active (one wavefront's lanes).
 __device__ __forceinline__ uint64_t active_tokens(const LinearArgs &a, int r, int t0, int lane) {
   const int t = t0 + lane;
@@ -168,468 +212,543 @@ __device__ __forceinline__ uint64_t active_tokens(const LinearArgs &a, int r, in
 }
 
 // Token-major operand (rows = tokens, contraction = features f0 ..): blocks
-// [token tile 4][step][piece] of `steps` steps, by the whole workgroup. Lanes
-// read along the tokens, eight features each.
+// [token tile 4][step][piece] of `steps` steps. Lanes read along the tokens, eight
+// features each; octet o of the slab is step o / 4, lane group o % 4.
 template <typename T>
-__device__ __forceinline__ void stage_tokens(unsigned char *dst, const T *src, int L, int f0, int dk,
-                                             int steps, uint64_t act, int thread, int threads) {
-  constexpr int NP = Pieces<T>::n;
-  const int t = thread & 63, tile = t >> 4;
-  const bool on = (act >> t) & 1u;
-  for (int o = thread >> 6; o < 4 * steps; o += threads >> 6) {
-    const int kk = o >> 2, g = o & 3;
-    T v[8];
+__device__ __forceinline__ void load_octet(Rsrc m, int L, int t0, int f0, int o, int t, Raw &v) {
+  const int es = sizeof(T);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int f = f0 + 32 * kk + slot_index(g, e);
-      v[e] = on && f < dk ? src[(size_t)f * L + t] : T(0);
-    }
-    frag p[NP];
-    to_frag<T>(v, p);
-    store_frag<NP>(dst + 1024 * NP * (tile * steps + kk), 16 * g + (t & 15), p);
+  for (int e = 0; e < 8; ++e) {
+    const int f = f0 + 32 * (o >> 2) + slot_index(o & 3, e);
+    v.d[e] = load_one<T>(m, (t0 + t) * es + f * L * es);
+  }
+}
+template <int NP>
+__device__ __forceinline__ void put_octet(unsigned char *dst, int steps, int o, int t,
+                                          const frag (&p)[NP]) {
+  store_frag<NP>(dst + 1024 * NP * ((t >> 4) * steps + (o >> 2)), 16 * (o & 3) + (t & 15), p);
+}
+
+// Feature-major fragments (rows = features of tile i, contraction = tokens of step
+// ks) out of the token-major blocks: ds_read_b64_tr_b16 hands element e of lane j of
+// a group of 16 lanes the value 16 e + j of their 16 x 8 bytes, so lane c of the
+// group reads the four features 4 (c % 4) .. of token 4 g + c / 4.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ s16x4 read_transposed(const unsigned char *p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s16x4 *)(uintptr_t)(__attribute__((address_space(3))) void *)p);
+}
+template <int NP>
+__device__ __forceinline__ void load_frag_t(const unsigned char *blocks, int steps, int i, int ks,
+                                            int lane, frag (&p)[NP]) {
+  const int g = lane >> 4, c = lane & 15;
+  const unsigned char *at = blocks + 1024 * NP * (2 * ks * steps + (i >> 1)) +
+                            16 * (16 * (c & 3) + 4 * g + (c >> 2)) + 8 * (i & 1);
+#pragma unroll
+  for (int x = 0; x < NP; ++x) {
+    const s16x4 lo = read_transposed(at + 1024 * x);
+    const s16x4 hi = read_transposed(at + 1024 * (NP * steps + x));
+    p[x] = __builtin_bit_cast(frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 }
 
-// Feature-major operand (rows = features f0 .., contraction = tokens): blocks
-// [feature tile][step 2][piece] of `tiles` tiles.
-template <typename T>
-__device__ __forceinline__ void stage_features(unsigned char *dst, const T *src, int L, int f0,
-                                               int dk, int tiles, uint64_t act, int n, bool vec,
-                                               int thread, int threads) {
-  constexpr int NP = Pieces<T>::n;
-  const int lane = thread & 63, g = lane >> 4;
-  for (int b = thread >> 6; b < 2 * tiles; b += threads >> 6) {
-    const int tile = b >> 1, ks = b & 1;
-    const int f = f0 + 16 * tile + (lane & 15);
-    T lo[4] = {}, hi[4] = {};
-    if (f < dk) {
-      load4<T>(src + (size_t)f * L, 32 * ks + 4 * g, act, n, vec, lo);
-      load4<T>(src + (size_t)f * L, 32 * ks + 16 + 4 * g, act, n, vec, hi);
-    }
-    const T v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    frag p[NP];
-    to_frag<T>(v, p);
-    store_frag<NP>(dst + 1024 * NP * (2 * tile + ks), lane, p);
-  }
+// Barrier for LDS only: outstanding global loads and stores stay outstanding.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// ------------------------------------------------------------------ T
+// Six operand blocks of a lower triangular 64 x 64 matrix (row tile tt, step ks):
+// the steps past the diagonal hold nothing.
+constexpr int kTri = kLinearTriBytes;
+__device__ __forceinline__ int tri_block(int tt, int ks) { return tt < 2 ? tt : 2 * tt - 2 + ks; }
 
-// Workgroup = one chunk of one (row, head), four waves. K K^T by row tiles, then
-// (I + M)^-1 by 16 x 16 blocks: the diagonal blocks by substitution (one wave
-// each), the others by T_ij = -T_ii sum_(j <= k < i) M_ik T_kj on the f32 matrix
-// cores, one distance i - j after the other.
-template <typename T>
-__global__ __launch_bounds__(256) void linear_solve_kernel(LinearArgs a, unsigned char *solve) {
+// ------------------------------------------------------------------ pairs
+
+// Workgroup = one chunk of one (row, head), four waves. Wave w forms the scores
+// of token tile w against the tiles up to it, transposed, which is the order the
+// walk reads them in; with the delta rule also K K^T the same way and (I + M)^-1
+// by 16 x 16 blocks: the diagonal blocks by substitution (one wave each), the others
+// by T_ij = -T_ii sum_(j <= k < i) M_ik T_kj on the f32 matrix cores, one distance
+// i - j after the other. The first head of a key head's group also leaves the
+// keys and queries behind as operands: the walk then reads whole lines one after
+// the other, whatever the row length (a chunk's piece of a feature row is 128 or
+// 256 bytes, and rows of 2^n tokens put all of them on the same few channels).
+template <typename T, bool DELTA>
+__global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearWork ws) {
   constexpr int NP = Pieces<T>::n;
   constexpr int kS = 68;  // floats per row: 16-byte rows, rows 4 banks apart
-  __shared__ __attribute__((aligned(16))) unsigned char kpl[8 * NP * 1024];
-  __shared__ __attribute__((aligned(16))) float M[kC * kS], X[kC * kS];
+  constexpr int kOperands = 16 * NP * 1024, kMatrices = DELTA ? 2 * kC * kS * 4 : 0;
+  __shared__ __attribute__((aligned(16))) unsigned char
+      smem[kOperands > kMatrices ? kOperands : kMatrices];
   __shared__ ChunkScan sc;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c16 = lane & 15;
+  unsigned char *qpl = smem, *kpl = smem + 8 * NP * 1024;
+  const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int chunk = blockIdx.x, h = blockIdx.y, r = blockIdx.z, nch = gridDim.x;
-  const size_t rh = (size_t)r * a.heads + h;
+  const size_t rh = (size_t)r * a.heads + h, at = rh * nch + chunk;
   const int t0 = chunk * kC, n = min(kC, a.L - t0);
+  const int steps = linear_steps(a.dk), parts = DELTA ? 3 : 2;
+  const size_t kh = (size_t)r * a.key_heads + h / a.group;
+  const uint32_t bytes = (uint32_t)a.dk * a.L * sizeof(T);
+  const Rsrc q = buffer_rsrc(static_cast<const T *>(a.q) + kh * a.dk * a.L, bytes);
+  const Rsrc k = buffer_rsrc(static_cast<const T *>(a.k) + kh * a.dk * a.L, bytes);
+  Raw x[2], y[2];
+  auto fetch = [&](int f0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      load_octet<T>(q, a.L, t0, f0, wave + 4 * i, lane, x[i]);
+      load_octet<T>(k, a.L, t0, f0, wave + 4 * i, lane, y[i]);
+    }
+  };
+  fetch(0);
   const uint64_t act = active_tokens(a, r, t0, lane);
-  if (wave == 0) scan_chunk(a, rh, t0, n, act, lane, sc);
-  const T *k = static_cast<const T *>(a.k) +
-               ((size_t)r * a.key_heads + h / a.group) * a.dk * a.L + t0;
-  f32x4 acc[4] = {};
-  for (int f0 = 0; f0 < a.dk; f0 += 64) {
-    if (f0) __syncthreads();
-    stage_tokens<T>(kpl, k, a.L, f0, a.dk, 2, act, threadIdx.x, 256);
-    __syncthreads();
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      frag x[NP];
-      load_frag<NP>(kpl + 1024 * NP * (2 * wave + kk), lane, x);
-#pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        if (st > wave) continue;
-        frag y[NP];
-        load_frag<NP>(kpl + 1024 * NP * (2 * st + kk), lane, y);
-        acc[st] = mma<NP, NP>(x, y, acc[st]);
-      }
-    }
+  if (h == 0 && threadIdx.x == 0) ws.active[(size_t)r * nch + chunk] = act;
+  if (act == 0) {
+    for (int j = wave; j < a.dv; j += 4)
+      if (lane < n) a.out[(rh * a.dv + j) * a.L + t0 + lane] = 0.0f;
+    return;
   }
-#pragma unroll
-  for (int st = 0; st < 4; ++st)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int t = 16 * wave + 4 * g + e, s = 16 * st + c16;
-      if (st <= wave) M[t * kS + s] = s < t ? sc.beta[t] * decay_between(sc, t, s) * acc[st][e] : 0.0f;
-      X[t * kS + s] = 0.0f;
-    }
-  __syncthreads();
-  // Diagonal block: lane c holds column c of the inverse.
-  {
-    const float *m = M + 16 * wave * kS + 16 * wave;
-    float x[16];
-#pragma unroll
-    for (int t = 0; t < 16; ++t) {
-      float v = t == c16 ? 1.0f : 0.0f;
-#pragma unroll
-      for (int s = 0; s < t; ++s) v = fmaf(-m[t * kS + s], x[s], v);
-      x[t] = v;
-    }
-    if (lane < 16)
-#pragma unroll
-      for (int t = 0; t < 16; ++t) X[(16 * wave + t) * kS + 16 * wave + c16] = x[t];
+  if (wave == 0) {
+    scan_chunk(a, rh, t0, n, act, lane, sc);
+    float *v = ws.factors + at * 3 * kC;
+    v[lane] = sc.from_start[lane];
+    v[kC + lane] = sc.to_end[lane];
+    v[2 * kC + lane] = sc.beta[lane];
   }
+  const bool first = h % a.group == 0;
+  const size_t part = (size_t)4 * steps * NP * 1024;
+  unsigned char *packed = ws.packed + (kh * nch + chunk) * parts * part;
+  unsigned char *pq = packed, *pt = packed + part, *pk = packed + 2 * part;
+  f32x4 score[4] = {}, keys[4] = {};
+  for (int f0 = 0; f0 < 32 * steps; f0 += 64) {
+    if (f0) lds_barrier();
+    const unsigned on = (act >> lane) & 1u ? 0xffu : 0u;
 #pragma unroll
-  for (int d = 1; d < 4; ++d) {
-    __syncthreads();
-    const int i = wave + d, j = wave;
-    if (i < 4) {
-      f32x4 w = {};
-      for (int b = j; b < i; ++b)
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-          w = mfma_16x16x4(M[(16 * i + c16) * kS + 16 * b + 4 * s + g],
-                           X[(16 * b + 4 * s + g) * kS + 16 * j + c16], w);
-      f32x4 v = {};
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-        v = mfma_16x16x4(-X[(16 * i + c16) * kS + 16 * i + 4 * g + s], w[s], v);
-#pragma unroll
-      for (int s = 0; s < 4; ++s) X[(16 * i + 4 * g + s) * kS + 16 * j + c16] = v[s];
+    for (int i = 0; i < 2; ++i) {
+      const int o = wave + 4 * i, step = f0 / 32 + (o >> 2);
+      frag p[NP];
+      to_frag<T>(x[i], false, on, p);
+      put_octet<NP>(qpl, 2, o, lane, p);
+      if (first && step < steps) put_octet<NP>(pq, steps, 4 * step + (o & 3), lane, p);
+      to_frag<T>(y[i], false, on, p);
+      put_octet<NP>(kpl, 2, o, lane, p);
+      if (DELTA && first && step < steps) put_octet<NP>(pk, steps, 4 * step + (o & 3), lane, p);
     }
-  }
-  __syncthreads();
-  // Six operand blocks: steps past the diagonal hold nothing.
-  unsigned char *dst = solve + (rh * nch + chunk) * kLinearSolveBytes;
-  for (int b = wave; b < 6; b += 4) {
-    const int tt = b < 2 ? b : 2 + ((b - 2) >> 1), ks = b < 2 ? 0 : (b - 2) & 1;
-    const float *x = X + (16 * tt + c16) * kS + 32 * ks + 4 * g;
-    frag p[3];
-    split8(*reinterpret_cast<const f32x4 *>(x), *reinterpret_cast<const f32x4 *>(x + 16), p);
-    store_frag<3>(dst + 3072 * b, lane, p);
-  }
-}
-
-// Operand block of T's row tile tt at step ks.
-__device__ __forceinline__ int solve_block(int tt, int ks) { return tt < 2 ? tt : 2 * tt - 2 + ks; }
-
-// ------------------------------------------------------------------ the walk
-
-// Workgroup = up to 8 waves of one (row, head), a wave = 16 value columns with their
-// whole state in accumulators (feature 16 n + 4 (lane / 16) + e, column lane % 16).
-// The waves share the chunk's keys (both orders) and T in LDS.
-template <typename T, bool DELTA, int NI>
-__global__ __launch_bounds__(512) void linear_walk_kernel(LinearArgs a, const unsigned char *solve,
-                                                          float *states, float *writes) {
-  constexpr int NP = Pieces<T>::n;
-  constexpr int SI = NI < 8 ? NI : 8;      // feature tiles per slab of the keys
-  constexpr int SK = SI / 2, NS = NI / SI;  // contraction steps per slab, slabs
-  __shared__ __attribute__((aligned(16))) unsigned char kt[2 * SI * NP * 1024];
-  __shared__ __attribute__((aligned(16))) unsigned char kpl[DELTA ? 4 * SK * NP * 1024 : 16];
-  __shared__ __attribute__((aligned(16))) unsigned char tpl[DELTA ? kLinearSolveBytes : 16];
-  __shared__ ChunkScan sc;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c16 = lane & 15;
-  const int threads = blockDim.x;
-  const int h = blockIdx.y, r = blockIdx.z;
-  const int jt = blockIdx.x * (threads >> 6) + wave, j = 16 * jt + c16;
-  const bool here = 16 * jt < a.dv, col = j < a.dv;
-  const size_t rh = (size_t)r * a.heads + h;
-  const int nch = (a.L + kC - 1) / kC, jtiles = (a.dv + 15) / 16;
-  const T *k = static_cast<const T *>(a.k) + ((size_t)r * a.key_heads + h / a.group) * a.dk * a.L;
-  const T *v = static_cast<const T *>(a.v) + (rh * a.dv + (col ? j : 0)) * a.L;
-
-  f32x4 S[NI] = {};
-  if (a.state_in && col) {
-    const float *p = a.state_in + rh * a.dk * a.dv + j;
+    lds_barrier();
+    if (f0 + 64 < 32 * steps) fetch(f0 + 64);
+    if (first)
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int f = 16 * i + 4 * g + e;
-        S[i][e] = f < a.dk ? p[(size_t)f * a.dv] : 0.0f;
+      for (int b = 0; b < 2; ++b) {  // feature tile i of the slab at both token steps
+        const int i = wave, tile = f0 / 16 + i;
+        if (tile >= 2 * steps) continue;
+        frag p[NP];
+        load_frag_t<NP>(kpl, 2, i, b, lane, p);
+        store_frag<NP>(pt + 1024 * NP * (2 * tile + b), lane, p);
       }
-  }
-  for (int chunk = 0; chunk < nch; ++chunk) {
-    const int t0 = chunk * kC, n = min(kC, a.L - t0);
-    const uint64_t act = active_tokens(a, r, t0, lane);
-    __syncthreads();  // the last chunk's operands are read
-    if (wave == 0) scan_chunk(a, rh, t0, n, act, lane, sc);
-    stage_features<T>(kt, k + t0, a.L, 0, a.dk, SI, act, n, a.vec_k, threadIdx.x, threads);
-    if constexpr (DELTA) {
-      stage_tokens<T>(kpl, k + t0, a.L, 0, a.dk, SK, act, threadIdx.x, threads);
-      const unsigned char *src = solve + (rh * nch + chunk) * kLinearSolveBytes;
-      for (int i = threadIdx.x * 16; i < kLinearSolveBytes; i += threads * 16)
-        *reinterpret_cast<f32x4 *>(tpl + i) = *reinterpret_cast<const f32x4 *>(src + i);
-    }
-    __syncthreads();
-    if (here) {  // S0 for the outputs, in fragment order
-      float *o = states + ((rh * nch + chunk) * jtiles + jt) * (size_t)(NI / 2) * 512 + 8 * lane;
-#pragma unroll
-      for (int i = 0; i < NI; ++i)
-        *reinterpret_cast<f32x4 *>(o + (i >> 1) * 512 + 4 * (i & 1)) = S[i];
-    }
-    f32x4 U[4];
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt) {
-      T x[4] = {};
-      if (col) load4<T>(v + t0, 16 * tt + 4 * g, act, n, a.vec_v, x);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) U[tt][e] = as_f32<T>(x[e]);
-    }
-    if constexpr (DELTA) {
-      f32x4 X[4] = {};
-#pragma unroll
-      for (int slab = 0; slab < NS; ++slab) {
-        if (slab) {
-          __syncthreads();
-          stage_tokens<T>(kpl, k + t0, a.L, 16 * SI * slab, a.dk, SK, act, threadIdx.x, threads);
-          __syncthreads();
-        }
-#pragma unroll
-        for (int kk = 0; kk < SK; ++kk) {
-          frag s[3];
-          split8(S[SI * slab + 2 * kk], S[SI * slab + 2 * kk + 1], s);
-#pragma unroll
-          for (int tt = 0; tt < 4; ++tt) {
-            frag x[NP];
-            load_frag<NP>(kpl + 1024 * NP * (tt * SK + kk), lane, x);
-            X[tt] = mma<NP, 3>(x, s, X[tt]);
-          }
-        }
-      }
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int t = 16 * tt + 4 * g + e;
-          X[tt][e] = sc.beta[t] * fmaf(-sc.from_start[t], X[tt][e], U[tt][e]);
-        }
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt) U[tt] = f32x4{};
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        frag x[3];
-        split8(X[2 * ks], X[2 * ks + 1], x);
-#pragma unroll
-        for (int tt = 2 * ks; tt < 4; ++tt) {
-          frag s[3];
-          load_frag<3>(tpl + 3072 * solve_block(tt, ks), lane, s);
-          U[tt] = mma<3, 3>(s, x, U[tt]);
-        }
-      }
-      if (here) {
-        float *o = writes + ((rh * nch + chunk) * jtiles + jt) * (size_t)1024 + 8 * lane;
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
-          *reinterpret_cast<f32x4 *>(o + (tt >> 1) * 512 + 4 * (tt & 1)) = U[tt];
-      }
-    }
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) U[tt][e] *= sc.to_end[16 * tt + 4 * g + e];
-    const float whole = sc.from_start[kC - 1];
-    frag u[2][3];
-    split8(U[0], U[1], u[0]);
-    split8(U[2], U[3], u[1]);
-#pragma unroll
-    for (int slab = 0; slab < NS; ++slab) {
-      if (slab) {
-        __syncthreads();
-        stage_features<T>(kt, k + t0, a.L, 16 * SI * slab, a.dk, SI, act, n, a.vec_k, threadIdx.x,
-                          threads);
-        __syncthreads();
-      }
-#pragma unroll
-      for (int i = 0; i < SI; ++i) {
-        f32x4 s = S[SI * slab + i] * whole;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          frag x[NP];
-          load_frag<NP>(kt + 1024 * NP * (2 * i + ks), lane, x);
-          s = mma<NP, 3>(x, u[ks], s);
-        }
-        S[SI * slab + i] = s;
-      }
-    }
-  }
-  if (a.state_out && col) {
-    float *p = a.state_out + rh * a.dk * a.dv + j;
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int f = 16 * i + 4 * g + e;
-        if (f < a.dk) p[(size_t)f * a.dv] = S[i][e];
-      }
-  }
-}
-
-// ------------------------------------------------------------------ outputs
-
-// Workgroup = one chunk of one (row, head), four waves, up to 4 JW column tiles.
-// Wave w forms the scores of token tile w, then the outputs of columns tiles
-// w, w + 4, .. (of the group) for all tokens.
-template <typename T, bool DELTA, int JW>
-__global__ __launch_bounds__(256) void linear_output_kernel(LinearArgs a, const float *states,
-                                                            const float *writes, int steps) {
-  constexpr int NP = Pieces<T>::n;
-  constexpr int NU = DELTA ? 3 : NP;  // pieces of what is written
-  constexpr int kHalf = 8 * 3 * 1024;
-  __shared__ __attribute__((aligned(16))) unsigned char qpl[8 * NP * 1024];
-  __shared__ __attribute__((aligned(16))) unsigned char kpl[kHalf];  // keys, then scores
-  __shared__ ChunkScan sc;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c16 = lane & 15;
-  const int nch = (a.L + kC - 1) / kC, jtiles = (a.dv + 15) / 16;
-  const int chunk = blockIdx.x % nch, group = blockIdx.x / nch, h = blockIdx.y, r = blockIdx.z;
-  const size_t rh = (size_t)r * a.heads + h;
-  const int t0 = chunk * kC, n = min(kC, a.L - t0);
-  const uint64_t act = active_tokens(a, r, t0, lane);
-  if (wave == 0) scan_chunk(a, rh, t0, n, act, lane, sc);
-  const size_t key = ((size_t)r * a.key_heads + h / a.group) * a.dk * a.L + t0;
-  const T *q = static_cast<const T *>(a.q) + key, *k = static_cast<const T *>(a.k) + key;
-  const int jt0 = group * 4 * JW + wave;
-  f32x4 score[4] = {}, O[JW][4] = {};
-  for (int f0 = 0; f0 < a.dk; f0 += 64) {
-    if (f0) __syncthreads();
-    stage_tokens<T>(qpl, q, a.L, f0, a.dk, 2, act, threadIdx.x, 256);
-    stage_tokens<T>(kpl, k, a.L, f0, a.dk, 2, act, threadIdx.x, 256);
-    __syncthreads();
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       if (f0 + 32 * kk >= a.dk) continue;
-      frag y[NP];
-      load_frag<NP>(qpl + 1024 * NP * (2 * wave + kk), lane, y);
+      frag qf[NP], kf[NP];
+      load_frag<NP>(qpl + 1024 * NP * (2 * wave + kk), lane, qf);
+      if (DELTA) load_frag<NP>(kpl + 1024 * NP * (2 * wave + kk), lane, kf);
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
         if (st > wave) continue;
-        frag x[NP];
-        load_frag<NP>(kpl + 1024 * NP * (2 * st + kk), lane, x);
-        score[st] = mma<NP, NP>(x, y, score[st]);
-      }
-#pragma unroll
-      for (int w = 0; w < JW; ++w) {
-        const int jt = jt0 + 4 * w;
-        if (jt >= jtiles) continue;
-        const float *s0 = states + (((rh * nch + chunk) * jtiles + jt) * (size_t)steps +
-                                    (f0 / 32 + kk)) * 512 + 8 * lane;
-        frag s[3];
-        split8(*reinterpret_cast<const f32x4 *>(s0), *reinterpret_cast<const f32x4 *>(s0 + 4), s);
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-          frag x[NP];
-          load_frag<NP>(qpl + 1024 * NP * (2 * tt + kk), lane, x);
-          O[w][tt] = mma<3, NP>(s, x, O[w][tt]);
-        }
+        frag s[NP];
+        load_frag<NP>(kpl + 1024 * NP * (2 * st + kk), lane, s);
+        score[st] = mma<NP, NP>(s, qf, score[st]);
+        if (DELTA) keys[st] = mma<NP, NP>(s, kf, keys[st]);
       }
     }
   }
-  __syncthreads();  // the keys are read: their place takes the scores
-  const int t = 16 * wave + c16;
+  lds_barrier();  // the decays are there, the operands read
+  unsigned char *planes = ws.planes + at * (DELTA ? 2 * kTri : kTri);
+  float *M = reinterpret_cast<float *>(smem), *X = M + kC * kS;
+  {  // lane = token 16 wave + c16, its partners 16 st + 4 g + e
+    const int t = 16 * wave + c16;
+    const double cum_t = sc.cum[t];
+    const int forget_t = sc.forget[t];
+    const float beta_t = sc.beta[t];
 #pragma unroll
-  for (int st = 0; st < 4; ++st)
+    for (int st = 0; st < 4; ++st) {
+      double cum_s[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int s = 16 * st + 4 * g + e;
-      score[st][e] = s <= t ? score[st][e] * decay_between(sc, t, s) : 0.0f;
-    }
-#pragma unroll
-  for (int ks = 0; ks < 2; ++ks) {
-    frag p[3];
-    split8(score[2 * ks], score[2 * ks + 1], p);
-    store_frag<3>(kpl + 3072 * (2 * wave + ks), lane, p);
-  }
-  __syncthreads();
-#pragma unroll
-  for (int tt = 0; tt < 4; ++tt) {
-    const float d = sc.from_start[16 * tt + c16];
-#pragma unroll
-    for (int w = 0; w < JW; ++w) O[w][tt] *= d;
-  }
-#pragma unroll
-  for (int w = 0; w < JW; ++w) {
-    const int jt = jt0 + 4 * w;
-    if (jt >= jtiles) continue;
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      frag u[NU];
-      if constexpr (DELTA) {
-        const float *p = writes + ((rh * nch + chunk) * jtiles + jt) * (size_t)1024 + 512 * ks + 8 * lane;
-        split8(*reinterpret_cast<const f32x4 *>(p), *reinterpret_cast<const f32x4 *>(p + 4), u);
-      } else {
-        const int j = 16 * jt + c16;
-        T lo[4] = {}, hi[4] = {};
-        if (j < a.dv) {
-          const T *row = static_cast<const T *>(a.v) + (rh * a.dv + j) * a.L + t0;
-          load4<T>(row, 32 * ks + 4 * g, act, n, a.vec_v, lo);
-          load4<T>(row, 32 * ks + 16 + 4 * g, act, n, a.vec_v, hi);
-        }
-        const T v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        to_frag<T>(v, u);
-      }
-#pragma unroll
-      for (int tt = 2 * ks; tt < 4; ++tt) {
-        frag x[3];
-        load_frag<3>(kpl + 3072 * (2 * tt + ks), lane, x);
-        O[w][tt] = mma<NU, 3>(u, x, O[w][tt]);
-      }
-    }
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
+      for (int e = 0; e < 4; ++e) cum_s[e] = sc.cum[16 * st + 4 * g + e];
+      f32x4 m;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int j = 16 * jt + 4 * g + e, tok = 16 * tt + c16;
-        if (j < a.dv && tok < n) a.out[(rh * a.dv + j) * a.L + t0 + tok] = a.scale * O[w][tt][e];
+        const int s = 16 * st + 4 * g + e;
+        const float d = forget_t > s || s > t ? 0.0f : fast_exp2((float)(cum_t - cum_s[e]));
+        // Not 0 times a score past the diagonal, which may not be finite.
+        score[st][e] = s <= t ? score[st][e] * d : 0.0f;
+        m[e] = s < t ? beta_t * d * keys[st][e] : 0.0f;
       }
+      if constexpr (DELTA) {
+        *reinterpret_cast<f32x4 *>(M + t * kS + 16 * st + 4 * g) = m;
+        *reinterpret_cast<f32x4 *>(X + t * kS + 16 * st + 4 * g) = f32x4{};
+      }
+    }
+  }
+  if constexpr (DELTA) lds_barrier();
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    if (ks && wave < 2) continue;
+    frag p[3];
+    split8(score[2 * ks], score[2 * ks + 1], p);
+    store_frag<3>(planes + 3072 * tri_block(wave, ks), lane, p);
+  }
+  if constexpr (DELTA) {
+    {  // diagonal block: lane c16 holds that column of the inverse
+      const float *m = M + 16 * wave * kS + 16 * wave;
+      float x[16];
+#pragma unroll
+      for (int t = 0; t < 16; ++t) {
+        float v = t == c16 ? 1.0f : 0.0f;
+#pragma unroll
+        for (int s = 0; s < t; ++s) v = fmaf(-m[t * kS + s], x[s], v);
+        x[t] = v;
+      }
+      if (lane < 16)
+#pragma unroll
+        for (int t = 0; t < 16; ++t) X[(16 * wave + t) * kS + 16 * wave + c16] = x[t];
+    }
+#pragma unroll
+    for (int d = 1; d < 4; ++d) {
+      lds_barrier();
+      const int i = wave + d, j = wave;
+      if (i < 4) {
+        f32x4 w = {};
+        for (int b = j; b < i; ++b)
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            w = mfma_16x16x4(M[(16 * i + c16) * kS + 16 * b + 4 * s + g],
+                             X[(16 * b + 4 * s + g) * kS + 16 * j + c16], w);
+        f32x4 v = {};
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          v = mfma_16x16x4(-X[(16 * i + c16) * kS + 16 * i + 4 * g + s], w[s], v);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) X[(16 * i + 4 * g + s) * kS + 16 * j + c16] = v[s];
+      }
+    }
+    lds_barrier();
+    for (int b = wave; b < 6; b += 4) {
+      const int tt = b < 2 ? b : 2 + ((b - 2) >> 1), ks = b < 2 ? 0 : (b - 2) & 1;
+      const float *x = X + (16 * tt + c16) * kS + 32 * ks + 4 * g;
+      frag p[3];
+      split8(*reinterpret_cast<const f32x4 *>(x), *reinterpret_cast<const f32x4 *>(x + 16), p);
+      store_frag<3>(planes + kTri + 3072 * b, lane, p);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ the walk
+
+// Workgroup = four waves on CT tiles of 16 value columns of one (row, head). The waves
+// share the work of a chunk, which is what every later chunk waits for: wave w has
+// token tile w of U and O, and the feature tiles TI w .. of the state (feature
+// 16 i + 4 (lane / 16) + e, column lane % 16, in accumulators). Three times a chunk
+// (twice without the delta rule) they hand their part to the others as operand
+// pieces in LDS: the state for K S0 and Q S0, V - d K S0 for U, U for O and the
+// state. Keys, queries and triangles come as operands straight from memory into
+// registers, each of its lines to one wave, and are fetched for the next chunk as
+// soon as the present one has been multiplied.
+template <typename T, bool DELTA, int NI, int CT>
+__global__ __launch_bounds__(256) void linear_walk_kernel(LinearArgs a, LinearWork ws) {
+  constexpr int NP = Pieces<T>::n;
+  constexpr int NV = DELTA ? 3 : NP;  // pieces of what is written
+  constexpr int NK = NI / 2, TI = NI >= 4 ? NI / 4 : 1;
+  constexpr int kPart = 4 * NK * NP * 1024, kParts = DELTA ? 3 : 2;
+  constexpr int PB = DELTA ? 2 * kTri : kTri;
+  __shared__ __attribute__((aligned(16))) unsigned char spl[CT][NK * 3 * 1024];
+  __shared__ __attribute__((aligned(16))) unsigned char xpl[DELTA ? CT : 1][DELTA ? 6 * 1024 : 16];
+  __shared__ __attribute__((aligned(16))) unsigned char upl[CT][2 * NV * 1024], epl[CT][6 * 1024];
+  const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nch = (a.L + kC - 1) / kC;
+  // Column groups of a (row, head) go to one XCD (workgroups are dealt to the
+  // eight in turn) and share its L2.
+  const unsigned groups = ((a.dv + 15) / 16 + CT - 1) / CT, heads = (unsigned)(a.rows * a.heads);
+  const unsigned set = blockIdx.x / (8 * groups), in = blockIdx.x - set * 8 * groups;
+  const unsigned width = min(8u, heads - 8 * set), cols = in / width;
+  const size_t rh = 8 * set + (in - cols * width);
+  const int r = (int)(rh / a.heads), h = (int)(rh - (size_t)r * a.heads);
+  const int jw = 16 * CT * cols;
+  const unsigned char *packed = ws.packed + ((size_t)r * a.key_heads + h / a.group) * nch *
+                                                ((size_t)kParts * kPart);
+  // The columns of values, outputs and states.
+  const uint32_t mine = (uint32_t)min(16 * CT, a.dv - jw) * a.L;
+  const size_t col0 = (rh * a.dv + jw) * a.L;
+  const Rsrc v = buffer_rsrc(static_cast<const T *>(a.v) + col0, mine * sizeof(T));
+  const Rsrc out = buffer_rsrc(a.out + col0, mine * 4);
+  const uint32_t state_bytes = (uint32_t)a.dk * a.dv * 4;
+  const int row_off = c16 * a.L + 16 * wave + 4 * g;  // elements: the lane's column and first token
+  const bool owner = TI * wave < NI;
+  f32x4 S[CT][TI] = {};
+  if (a.state_in && owner) {
+    const Rsrc from = buffer_rsrc(a.state_in + rh * a.dk * a.dv, state_bytes);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int j = jw + 16 * ct + c16;
+      const int voff = j < a.dv ? ((16 * TI * wave + 4 * g) * a.dv + j) * 4 : kNowhere;
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          S[ct][i][e] = buffer_load1(from, voff + (16 * i + e) * a.dv * 4, 0);
+    }
+  }
+  // Half of a fragment block: quad x of lanes is half `half` of block `block`.
+  auto put_half = [&](unsigned char *blocks, int half, f32x4 x) {
+    const Bf16x3 p = split_bf16x3(x);
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      *reinterpret_cast<u32x2 *>(blocks + 1024 * i + 16 * lane + 8 * half) = p.p[i];
+  };
+  auto put_state = [&] {
+    if (owner)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int i = 0; i < TI; ++i) {
+          const int tile = TI * wave + i;
+          put_half(spl[ct] + 3072 * (tile >> 1), tile & 1, S[ct][i]);
+        }
+  };
+
+  // The row's chunks with an active token, 64 at a time.
+  const uint64_t *active = ws.active + (size_t)r * nch;
+  uint64_t word = 0, live = 0;
+  int base = -64;
+  struct Chunk {
+    int at;  // -1: none
+    uint64_t act;
+  };
+  auto next_chunk = [&]() -> Chunk {
+    while (!live) {
+      base += 64;
+      if (base >= nch) return Chunk{-1, 0};
+      word = base + lane < nch ? active[base + lane] : 0;
+      live = __ballot(word != 0);
+    }
+    const int b = __ffsll((unsigned long long)live) - 1;
+    live &= live - 1;
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)word, b);
+    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(word >> 32), b);
+    return Chunk{base + b, (uint64_t)hi << 32 | lo};
+  };
+
+  frag qf[NK][NP], kf[DELTA ? NK : 1][NP], tf[TI][2][NP], sf[2][3], xf[2][3];
+  f32x4 start, end, beta;
+  float whole = 0.0f;
+  uint32_t write[CT][4];
+  auto fetch_rows = [&](int at) {  // token tile `wave` of queries and keys
+    const unsigned char *p = packed + (size_t)at * (kParts * kPart) + 1024 * NP * NK * wave;
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) {
+      load_frag<NP>(p + 1024 * NP * kk, lane, qf[kk]);
+      if constexpr (DELTA) load_frag<NP>(p + 2 * kPart + 1024 * NP * kk, lane, kf[kk]);
+    }
+  };
+  auto fetch_values = [&](int at) {
+    const float *f = ws.factors + (rh * nch + at) * 3 * kC + 16 * wave + 4 * g;
+    start = *reinterpret_cast<const f32x4 *>(f);
+    end = *reinterpret_cast<const f32x4 *>(f + kC);
+    if (DELTA) beta = *reinterpret_cast<const f32x4 *>(f + 2 * kC);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+      load_four<T>(v, (row_off + at * kC + 16 * ct * a.L) * (int)sizeof(T), a.vec_v, write[ct]);
+  };
+  auto fetch_tri = [&](int at, int which, frag (&f)[2][3]) {
+    const unsigned char *p = ws.planes + (rh * nch + at) * PB + which * kTri;
+    load_frag<3>(p + 3072 * tri_block(wave, 0), lane, f[0]);
+    if (wave >= 2) load_frag<3>(p + 3072 * tri_block(wave, 1), lane, f[1]);
+  };
+  auto fetch_columns = [&](int at) {  // the owned feature tiles of the keys
+    whole = ws.factors[(rh * nch + at) * 3 * kC + kC - 1];
+    if (!owner) return;
+    const unsigned char *p = packed + (size_t)at * (kParts * kPart) + kPart + 2048 * NP * TI * wave;
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) load_frag<NP>(p + 1024 * NP * (2 * i + ks), lane, tf[i][ks]);
+  };
+
+  Chunk cur = next_chunk();
+  if (cur.at >= 0) {
+    fetch_rows(cur.at);
+    fetch_values(cur.at);
+    if (DELTA) fetch_tri(cur.at, 1, xf);
+    fetch_tri(cur.at, 0, sf);
+    fetch_columns(cur.at);
+    put_state();
+    lds_barrier();
+  }
+  while (cur.at >= 0) {
+    const Chunk nxt = next_chunk();
+    // Q S0 and K S0, even and odd steps in accumulators of their own.
+    f32x4 X[CT][2] = {}, O[CT][2] = {};
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) {
+      frag s[CT][3];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) load_frag<3>(spl[ct] + 3072 * kk, lane, s[ct]);
+      typedef Products<NP, 3> P;
+#pragma unroll
+      for (int x = 0; x < P::n; ++x)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          if constexpr (DELTA)
+            X[ct][kk & 1] = mfma_16x16x32_bf16(kf[kk][P::a(x)], s[ct][P::b(x)], X[ct][kk & 1]);
+          O[ct][kk & 1] = mfma_16x16x32_bf16(qf[kk][P::a(x)], s[ct][P::b(x)], O[ct][kk & 1]);
+        }
+    }
+    if (nxt.at >= 0) fetch_rows(nxt.at);
+    f32x4 U[CT];
+    const unsigned on = (unsigned)(cur.act >> (16 * wave + 4 * g));
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        U[ct][e] = (on >> e) & 1u ? value_of<T>(write[ct], a.vec_v, e) : 0.0f;
+      O[ct][0] = start * (O[ct][0] + O[ct][1]);
+      if constexpr (DELTA)
+        put_half(xpl[ct] + 3072 * (wave >> 1), wave & 1,
+                 beta * (U[ct] - start * (X[ct][0] + X[ct][1])));
+    }
+    if constexpr (DELTA) {
+      lds_barrier();
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) U[ct] = f32x4{};
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        if (ks && wave < 2) continue;
+        frag x[CT][3];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) load_frag<3>(xpl[ct] + 3072 * ks, lane, x[ct]);
+        typedef Products<3, 3> P;
+#pragma unroll
+        for (int i = 0; i < P::n; ++i)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+            U[ct] = mfma_16x16x32_bf16(xf[ks][P::a(i)], x[ct][P::b(i)], U[ct]);
+      }
+      if (nxt.at >= 0) fetch_tri(nxt.at, 1, xf);
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      if constexpr (NV == 3) {
+        put_half(upl[ct] + 3072 * (wave >> 1), wave & 1, U[ct]);
+      } else {  // exact: the values are bf16
+        *reinterpret_cast<u32x2 *>(upl[ct] + 1024 * (wave >> 1) + 16 * lane + 8 * (wave & 1)) =
+            __builtin_bit_cast(u32x2, __builtin_convertvector(U[ct], bf16x4));
+      }
+      put_half(epl[ct] + 3072 * (wave >> 1), wave & 1, U[ct] * end);
+    }
+    const float decay = whole;
+    lds_barrier();
+    if (nxt.at >= 0) fetch_values(nxt.at);
+    // The state first: the next chunk waits for it.
+    if (owner) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        frag e[2][3];
+        load_frag<3>(epl[ct], lane, e[0]);
+        load_frag<3>(epl[ct] + 3072, lane, e[1]);
+        typedef Products<NP, 3> P;
+#pragma unroll
+        for (int i = 0; i < TI; ++i) S[ct][i] *= decay;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int x = 0; x < P::n; ++x)
+#pragma unroll
+            for (int i = 0; i < TI; ++i)
+              S[ct][i] = mfma_16x16x32_bf16(tf[i][ks][P::a(x)], e[ks][P::b(x)], S[ct][i]);
+      }
+    }
+    if (nxt.at >= 0) fetch_columns(nxt.at);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      if (ks && wave < 2) continue;
+      frag u[CT][NV];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) load_frag<NV>(upl[ct] + 1024 * NV * ks, lane, u[ct]);
+      typedef Products<3, NV> P;
+#pragma unroll
+      for (int x = 0; x < P::n; ++x)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+          O[ct][0] = mfma_16x16x32_bf16(sf[ks][P::a(x)], u[ct][P::b(x)], O[ct][0]);
+    }
+    put_state();
+    if (nxt.at >= 0) fetch_tri(nxt.at, 0, sf);
+    const int n = min(kC, a.L - cur.at * kC) - 16 * wave - 4 * g;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int off = (row_off + cur.at * kC + 16 * ct * a.L) * 4;
+      const f32x4 y = O[ct][0] * a.scale;
+      if (cur.at * kC + kC <= a.L) {
+        buffer_store4(y, out, off, 0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) buffer_store1(y[e], out, e < n ? off + 4 * e : kNowhere, 0);
+      }
+    }
+    lds_barrier();
+    cur = nxt;
+  }
+  if (a.state_out && owner) {
+    const Rsrc to = buffer_rsrc(a.state_out + rh * a.dk * a.dv, state_bytes);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int j = jw + 16 * ct + c16;
+      const int voff = j < a.dv ? ((16 * TI * wave + 4 * g) * a.dv + j) * 4 : kNowhere;
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          buffer_store1(S[ct][i][e], to, voff + (16 * i + e) * a.dv * 4, 0);
+    }
   }
 }
 
 template <typename T, bool DELTA, int NI>
-hipError_t launch_walk(const LinearArgs &a, const unsigned char *solve, float *states,
-                       float *writes, hipStream_t stream, hipEvent_t start) {
-  const int jtiles = (a.dv + 15) / 16;
-  int nw = 8;
-  while (nw > 1 && nw / 2 >= jtiles) nw /= 2;
-  const dim3 grid((unsigned)((jtiles + nw - 1) / nw), (unsigned)a.heads, (unsigned)a.rows);
-  hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI>), grid, dim3(64 * nw), 0, stream, start,
-                        nullptr, 0, a, solve, states, writes);
-  return hipGetLastError();
+void launch_walk(const LinearArgs &a, const LinearWork &ws, hipStream_t stream, hipEvent_t stop) {
+  const size_t jtiles = (size_t)((a.dv + 15) / 16), heads = (size_t)a.rows * a.heads;
+  if (heads * jtiles > 2 * (size_t)a.cus) {
+    const dim3 grid((unsigned)(heads * ((jtiles + 1) / 2)));
+    hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI, 2>), grid, dim3(256), 0, stream, nullptr,
+                          stop, 0, a, ws);
+  } else {
+    const dim3 grid((unsigned)(heads * jtiles));
+    hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI, 1>), grid, dim3(256), 0, stream, nullptr,
+                          stop, 0, a, ws);
+  }
 }
 
 template <typename T, bool DELTA>
-hipError_t launch_chunks(const LinearArgs &a, unsigned char *ws, hipStream_t stream,
+hipError_t launch_chunks(const LinearArgs &a, unsigned char *mem, hipStream_t stream,
                          const KernelEvents &ev) {
   const LinearSpace sp = linear_space(a);
-  float *states = reinterpret_cast<float *>(ws);
-  float *writes = reinterpret_cast<float *>(ws + sp.states);
-  unsigned char *solve = ws + sp.states + sp.writes;
-  const unsigned nch = (unsigned)((a.L + kC - 1) / kC);
-  hipError_t e = hipSuccess;
-  hipEvent_t start = ev.start;
-  if (DELTA) {
-    hipExtLaunchKernelGGL((linear_solve_kernel<T>), dim3(nch, a.heads, a.rows), dim3(256), 0,
-                          stream, start, nullptr, 0, a, solve);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-    start = nullptr;
-  }
-  const int steps = linear_steps(a.dk);
-  switch (steps) {
-    case 1: e = launch_walk<T, DELTA, 2>(a, solve, states, writes, stream, start); break;
-    case 2: e = launch_walk<T, DELTA, 4>(a, solve, states, writes, stream, start); break;
-    case 4: e = launch_walk<T, DELTA, 8>(a, solve, states, writes, stream, start); break;
-    default: e = launch_walk<T, DELTA, 16>(a, solve, states, writes, stream, start); break;
-  }
+  LinearWork ws;
+  ws.packed = mem;
+  ws.planes = ws.packed + sp.packed;
+  ws.factors = reinterpret_cast<float *>(ws.planes + sp.planes);
+  ws.active = reinterpret_cast<uint64_t *>(ws.planes + sp.planes + sp.factors);
+  const dim3 grid((unsigned)((a.L + kC - 1) / kC), (unsigned)a.heads, (unsigned)a.rows);
+  hipExtLaunchKernelGGL((linear_pairs_kernel<T, DELTA>), grid, dim3(256), 0, stream, ev.start,
+                        nullptr, 0, a, ws);
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int jtiles = (a.dv + 15) / 16;
-  const int jw = jtiles <= 4 ? 1 : (jtiles <= 8 ? 2 : 4);
-  const dim3 grid(nch * (unsigned)((jtiles + 4 * jw - 1) / (4 * jw)), (unsigned)a.heads,
-                  (unsigned)a.rows);
-  if (jw == 1)
-    hipExtLaunchKernelGGL((linear_output_kernel<T, DELTA, 1>), grid, dim3(256), 0, stream, nullptr,
-                          ev.stop, 0, a, states, writes, steps);
-  else if (jw == 2)
-    hipExtLaunchKernelGGL((linear_output_kernel<T, DELTA, 2>), grid, dim3(256), 0, stream, nullptr,
-                          ev.stop, 0, a, states, writes, steps);
+  if (a.dk <= 32)
+    launch_walk<T, DELTA, 2>(a, ws, stream, ev.stop);
+  else if (a.dk <= 64)
+    launch_walk<T, DELTA, 4>(a, ws, stream, ev.stop);
+  else if (a.dk <= 128)
+    launch_walk<T, DELTA, 8>(a, ws, stream, ev.stop);
   else
-    hipExtLaunchKernelGGL((linear_output_kernel<T, DELTA, 4>), grid, dim3(256), 0, stream, nullptr,
-                          ev.stop, 0, a, states, writes, steps);
+    launch_walk<T, DELTA, 16>(a, ws, stream, ev.stop);
   return hipGetLastError();
 }
 

@@ -64,7 +64,7 @@ struct tfd_ctx {
   DevBuf layer;       // intermediates of the layer entries (projections, attention output)
   DevBuf model;       // activations and token inputs of the model forward
   DevBuf planes;      // bf16 planes of the linears' operands
-  DevBuf linear;      // chunk states, writes and solves of the linear attention
+  DevBuf linear;      // chunk operands of the linear attention
   DevBuf readout;     // partial statistics of the token log probabilities
   // Workspaces that a captured graph may still use, outgrown since.
   std::vector<void *> retired;
@@ -1511,8 +1511,7 @@ int linear_run(tfd_ctx *c, bool bf16, size_t rows, size_t length, size_t heads, 
   if (key_dim > (size_t)tfd::kLinearMaxKeyDim)
     return fail(c, TFD_EUNSUPPORTED, "%s: key_dim %zu exceeds %d", op, key_dim,
                 tfd::kLinearMaxKeyDim);
-  if (length > (size_t)INT32_MAX / 4 || value_dim > (size_t)1 << 20 || heads > 65535 ||
-      rows > 65535)
+  if (length > (size_t)1 << 25 || value_dim > 65536 || heads > 65535 || rows > 65535)
     return fail(c, TFD_EUNSUPPORTED, "%s: length/value_dim/heads/rows exceed the launch grid", op);
   if ((length && (!q || !k || !v || !log_decay || !out)))
     return invalid(c, op, "inputs", "null buffer");
@@ -1553,10 +1552,11 @@ int linear_run(tfd_ctx *c, bool bf16, size_t rows, size_t length, size_t heads, 
   a.scale = bits_to_f32(scale_bits);
   a.bf16 = bf16;
   a.state_vec = value_dim % 4 == 0 && aligned16(si_d) && aligned16(so_d);
-  a.vec_k = length % 4 == 0 && (reinterpret_cast<uintptr_t>(k_d) & (4 * es - 1)) == 0;
-  a.vec_v = length % 4 == 0 && (reinterpret_cast<uintptr_t>(v_d) & (4 * es - 1)) == 0;
+  a.vec_k = length % 4 == 0 && (reinterpret_cast<uintptr_t>(k_d) & 7) == 0;
+  a.vec_v = length % 4 == 0 && (reinterpret_cast<uintptr_t>(v_d) & 7) == 0;
+  a.cus = c->cus;
   tfd::KernelEvents ev;
-  if (length <= kLinearRecurrentTokens) {
+  if (length <= kLinearRecurrentTokens || length > tfd::kLinearChunkedTokens) {
     if (!capturing && (rc = timing_events(c, &ev))) return rc;
     TFD_HIP(c, tfd::launch_linear_recurrent(a, c->stream, ev), "linear_recurrent launch");
   } else {

@@ -343,7 +343,8 @@ struct LinearArgs {
   float scale;
   bool bf16;       // q, k and v
   bool state_vec;  // 16-byte access to the states' rows: dv % 4 == 0, aligned
-  bool vec_k, vec_v;  // access to four tokens of k, v at once: L % 4 == 0, aligned
+  bool vec_k, vec_v;  // bf16: access to four tokens of k, v at once (L % 4 == 0, 8-byte aligned)
+  int cus;
 };
 // Token by token.
 hipError_t launch_linear_recurrent(const LinearArgs &a, hipStream_t stream,
@@ -351,21 +352,32 @@ hipError_t launch_linear_recurrent(const LinearArgs &a, hipStream_t stream,
 
 // By chunks of this many tokens (linear_chunks.hip).
 constexpr int kLinearChunk = 64;
-// One chunk's solve operand: six blocks of three pieces.
-constexpr int kLinearSolveBytes = 6 * 3 * 1024;
+// Longest row of it: a head's matrix is addressed with 31 bits.
+constexpr size_t kLinearChunkedTokens = (size_t)1 << 20;
+// A lower triangular 64 x 64 operand: six blocks of three pieces.
+constexpr int kLinearTriBytes = 6 * 3 * 1024;
 // Contraction steps of 32 key features, a power of two.
-inline int linear_steps(int dk) { return dk <= 32 ? 1 : dk <= 64 ? 2 : dk <= 128 ? 4 : 8; }
-// Bytes of the workspace of launch_linear_chunks: the states before and the
-// writes of every chunk (f32), and the solve operands.
+__host__ __device__ inline int linear_steps(int dk) {
+  return dk <= 32 ? 1 : dk <= 64 ? 2 : dk <= 128 ? 4 : 8;
+}
+// Workspace of launch_linear_chunks: per (row, key head, chunk) the queries by
+// tokens, the keys by features and (delta rule) by tokens as operands, per (row, head, chunk) the decayed scores (with
+// the delta rule also the solve operand after them) and 64 factors each from the
+// chunk's start, to its end and beta; per (row, chunk) the active tokens.
+struct LinearWork {
+  unsigned char *packed, *planes;
+  float *factors;
+  uint64_t *active;
+};
 struct LinearSpace {
-  size_t states, writes, solve;
-  size_t total() const { return states + writes + solve; }
+  size_t packed, planes, factors, active;  // bytes
+  size_t total() const { return packed + planes + factors + active; }
 };
 inline LinearSpace linear_space(const LinearArgs &a) {
-  const size_t chunks = (size_t)a.rows * a.heads * ((a.L + kLinearChunk - 1) / kLinearChunk);
-  const size_t tiles = (size_t)((a.dv + 15) / 16);
-  return LinearSpace{chunks * tiles * linear_steps(a.dk) * 2048, a.beta ? chunks * tiles * 4096 : 0,
-                     a.beta ? chunks * kLinearSolveBytes : 0};
+  const size_t nch = (size_t)((a.L + kLinearChunk - 1) / kLinearChunk) * a.rows;
+  return LinearSpace{nch * a.key_heads * linear_steps(a.dk) * (a.beta ? 12 : 8) * (a.bf16 ? 1 : 3) * 1024,
+                     nch * a.heads * kLinearTriBytes * (a.beta ? 2 : 1),
+                     nch * a.heads * 3 * kLinearChunk * 4, nch * 8};
 }
 hipError_t launch_linear_chunks(const LinearArgs &a, void *ws, hipStream_t stream,
                                 const KernelEvents &ev);
