@@ -49,29 +49,97 @@ __device__ __forceinline__ u64 key_of(float x, uint32_t index) {
   return ((u64)value_code(x) << 32) | (uint32_t)~index;
 }
 
-// One stage of a bitonic network over the wave's lanes: lanes whose bit
-// `keep_max` is set keep the larger of the pair (l, l ^ o).
-__device__ __forceinline__ u64 exchange(u64 v, int o, bool keep_max) {
-  const u64 w = __shfl_xor(v, o);
-  return (v > w) == keep_max ? v : w;
+// The value of lane l ^ O, by DPP within rows of 16 lanes and lane swaps across
+// them: no trip through LDS.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int O>
+__device__ __forceinline__ uint32_t xor_lane(uint32_t v, int lane) {
+  static_assert(O == 1 || O == 2 || O == 4 || O == 8 || O == 16 || O == 32 || O == 63, "");
+  if constexpr (O == 1) return dpp<0xB1>(v);             // quad_perm 1 0 3 2
+  if constexpr (O == 2) return dpp<0x4E>(v);             // quad_perm 2 3 0 1
+  if constexpr (O == 4) return dpp<0x1B>(dpp<0x141>(v));  // 7 - l, then quad_perm 3 2 1 0
+  if constexpr (O == 8) return dpp<0x128>(v);            // row_ror 8
+  if constexpr (O == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return lane & 16 ? r[0] : r[1];
+  }
+  if constexpr (O == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return lane & 32 ? r[0] : r[1];
+  }
+  if constexpr (O == 63) return xor_lane<32>(xor_lane<16>(dpp<0x140>(v), lane), lane);  // 15 - l
+}
+template <int O>
+__device__ __forceinline__ u64 xor_lane(u64 v, int lane) {
+  return (u64)xor_lane<O>((uint32_t)(v >> 32), lane) << 32 | xor_lane<O>((uint32_t)v, lane);
+}
+
+// Bitonic stages O, O / 2, .. 1 over the wave's lanes: blocks of N lanes sort
+// downwards and upwards in turn (N = 128: all downwards).
+template <int N, int O>
+__device__ __forceinline__ u64 stages(u64 v, int lane) {
+  const u64 w = xor_lane<O>(v, lane);
+  v = (v > w) == (((lane & O) == 0) == ((lane & N) == 0)) ? v : w;
+  if constexpr (O > 1)
+    return stages<N, O / 2>(v, lane);
+  else
+    return v;
 }
 // Sorts one key a lane, largest in lane 0.
 __device__ __forceinline__ u64 sort64(u64 v, int lane) {
-#pragma unroll
-  for (int n = 2; n <= 64; n <<= 1)
-#pragma unroll
-    for (int o = n >> 1; o > 0; o >>= 1)
-      v = exchange(v, o, ((lane & o) == 0) == ((lane & n) == 0));
-  return v;
+  v = stages<2, 1>(v, lane);
+  v = stages<4, 2>(v, lane);
+  v = stages<8, 4>(v, lane);
+  v = stages<16, 8>(v, lane);
+  v = stages<32, 16>(v, lane);
+  return stages<64, 32>(v, lane);
 }
 // The 64 largest of two sorted lists, sorted.
 __device__ __forceinline__ u64 merge64(u64 a, u64 b, int lane) {
-  const u64 r = __shfl(b, 63 - lane);
-  u64 v = a > r ? a : r;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = exchange(v, o, (lane & o) == 0);
-  return v;
+  const u64 r = xor_lane<63>(b, lane);
+  return stages<128, 32>(a > r ? a : r, lane);
 }
+__device__ __forceinline__ u64 key_at(u64 v, int lane) {
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, lane);
+}
+
+// A wave's largest keys so far: `best` sorted over the lanes, `bar` a key that
+// at least `top` of the keys seen reach (0: none yet), so that only keys from it on
+// matter, and up to 64 keys waiting in LDS.
+struct TopList {
+  u64 best = 0, bar = 0;
+  int held = 0, top;
+  u64 *buf;
+  __device__ __forceinline__ void flush(int lane) {
+    const u64 fresh = lane < held ? buf[lane] : 0;
+    best = merge64(best, sort64(fresh, lane), lane);
+    const u64 b = key_at(best, top - 1);
+    bar = b > bar ? b : bar;
+    held = 0;
+    __builtin_amdgcn_wave_barrier();
+  }
+  // The first keys: `most` is the largest of each lane's. The top-th of them
+  // bounds the list from below before any key is kept.
+  __device__ __forceinline__ void start(u64 most, int lane) {
+    bar = key_at(sort64(most, lane), top - 1);
+  }
+  // One key a lane (0: none). Keys are unique; the bar itself may still come.
+  __device__ __forceinline__ void push(u64 key, int lane) {
+    u64 pass = __ballot(key >= bar && key != 0);
+    if (!pass) return;
+    if (held + __popcll(pass) > 64) {
+      flush(lane);
+      pass = __ballot(key >= bar && key != 0);
+    }
+    if ((pass >> lane) & 1u) buf[held + __popcll(pass & (((u64)1 << lane) - 1))] = key;
+    held += __popcll(pass);
+    __builtin_amdgcn_wave_barrier();
+  }
+};
 
 // Softmax statistics of part of a position.
 struct Stats {
@@ -148,17 +216,11 @@ __global__ __launch_bounds__(64 * NW) void log_probs_kernel(LogProbArgs a) {
   const int p0 = min(part * a.part_pieces, pieces), p1 = min(p0 + a.part_pieces, pieces);
 
   Stats s{kLowest, 0.0f, 0.0f};
-  u64 best = 0, bar = 0;  // the wave's sorted list, its top-th key
-  float bar_value = NAN;  // the top-th value, NaN while there is none
-  int held = 0;           // keys in buf
-  auto flush = [&] {
-    const u64 fresh = lane < held ? buf[wave][lane] : 0;
-    best = merge64(best, sort64(fresh, lane), lane);
-    bar = __shfl(best, a.top - 1);
-    bar_value = bar ? code_value((uint32_t)(bar >> 32)) : NAN;
-    held = 0;
-    __builtin_amdgcn_wave_barrier();
-  };
+  TopList list;
+  list.top = a.top;
+  list.buf = buf[wave];
+  float bar_value = NAN;  // the bar's value, NaN while there is none
+  bool begun = false;
 
   for (int p = p0 + wave * 64 + lane; p - lane < p1; p += 64 * NW * U) {
     float x[U][E];
@@ -205,32 +267,37 @@ __global__ __launch_bounds__(64 * NW) void log_probs_kernel(LogProbArgs a) {
 #pragma unroll
       for (int e = 0; e < E; ++e) add_logit(s, x[u][e]);
     if constexpr (TOP) {
+      auto key = [&](int u, int e) -> u64 {
+        const int q = p + u * 64 * NW, i = q * E - skew + e;
+        return q < p1 && i >= 0 && i < vocab ? key_of(x[u][e], (uint32_t)i) : 0;
+      };
+      if (!begun) {
+        u64 most = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const u64 k = key(u, e);
+            most = k > most ? k : most;
+          }
+        list.start(most, lane);
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int q = p + u * 64 * NW, first = q * E - skew;
-        // Indices grow from piece to piece of a wave, so a value equal to the
-        // bar's comes too late; within the pieces below the whole key decides.
-        if (!__any(q < p1 && !(mx[u] <= bar_value))) continue;
+        // Indices grow from piece to piece of a wave, so after its first pieces a
+        // value equal to the bar's comes too late; within the pieces the key decides.
+        const bool some = begun ? !(mx[u] <= bar_value) : true;
+        if (!__any(p + u * 64 * NW < p1 && some)) continue;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const int i = first + e;
-          const u64 key = q < p1 && i >= 0 && i < vocab ? key_of(x[u][e], (uint32_t)i) : 0;
-          u64 pass = __ballot(key > bar);
-          if (!pass) continue;
-          if (held + __popcll(pass) > 64) {
-            flush();
-            pass = __ballot(key > bar);
-          }
-          if (key > bar)
-            buf[wave][held + __popcll(pass & (((u64)1 << lane) - 1))] = key;
-          held += __popcll(pass);
-          __builtin_amdgcn_wave_barrier();
-        }
+        for (int e = 0; e < E; ++e) list.push(key(u, e), lane);
       }
+      begun = true;
+      bar_value = list.bar ? code_value((uint32_t)(list.bar >> 32)) : NAN;
     }
   }
   s = wave_join(s);
-  if constexpr (TOP) flush();
+  if constexpr (TOP) list.flush(lane);
+  u64 best = list.best;
   if constexpr (NW > 1) {
     if constexpr (TOP) buf[wave][lane] = best;
     if (lane == 0) {
@@ -282,15 +349,27 @@ __global__ __launch_bounds__(64) void log_probs_join_kernel(LogProbArgs a) {
     s.a += t.a;
   }
   s = wave_join(s);
-  u64 best = 0;
+  TopList list;
   if constexpr (TOP) {
-    // The parts' lists are `top` keys each: 64 keys at a time.
+    __shared__ u64 buf[64];
+    list.top = a.top;
+    list.buf = buf;
     const size_t n = (size_t)a.parts * a.top;
     const u64 *keys = a.part_keys + (size_t)pos * n;
-    for (size_t i = 0; i < n; i += 64)
-      best = merge64(best, sort64(i + lane < n ? keys[i + lane] : 0, lane), lane);
+    constexpr int U = 8;  // loads in flight
+    for (size_t i = 0; i < n; i += 64 * U) {
+      u64 k[U], most = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) k[u] = i + 64 * u + lane < n ? keys[i + 64 * u + lane] : 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) most = k[u] > most ? k[u] : most;
+      if (i == 0) list.start(most, lane);
+#pragma unroll
+      for (int u = 0; u < U; ++u) list.push(k[u], lane);
+    }
+    list.flush(lane);
   }
-  write_position(a, pos, s, best, lane);
+  write_position(a, pos, s, list.best, lane);
 }
 
 template <bool BF16, bool TOP>
@@ -310,16 +389,21 @@ void launch_parts(const LogProbArgs &a, int waves, hipStream_t stream, const Ker
 
 }  // namespace
 
-// Pieces are 16 bytes; a wave takes 256 of them a step (U of 64 lanes).
+// Fewest 16-byte pieces of a part: one step of a workgroup's four waves. Fewer spread
+// a position further, but every wave has to find its first `top` and the joining
+// wave reads them all (bf16, 100003 logits, top 20: 21.0 us with 256 pieces, 19.0 with
+// 512, 19.6 with 1024, 22.5 with 2048; 4 x 151936 f32, top 50: 61, 44, 30, 27).
+constexpr size_t kLogProbPart = 1024;
+
 void log_probs_plan(LogProbArgs &a, int cus) {
   const size_t per_piece = a.bf16 ? 8 : 4;
   const size_t pieces = (a.vocab + 2 * (per_piece - 1)) / per_piece;  // at any skew
   a.parts = 1;
   a.part_pieces = (int)pieces;
   if (a.vocab <= kLogProbWaveVocab) return;
-  // Parts of at least two steps of a workgroup, until every CU has two workgroups.
+  // Parts of kLogProbPart pieces or more, until every CU has two workgroups.
   const size_t want = a.positions ? (2 * (size_t)cus + a.positions - 1) / a.positions : 1;
-  const size_t most = (pieces + 2047) / 2048;
+  const size_t most = (pieces + kLogProbPart - 1) / kLogProbPart;
   size_t parts = want < most ? want : most;
   if (parts <= 1) return;
   const size_t len = (pieces + parts - 1) / parts;

@@ -195,6 +195,7 @@ class Context:
         if rc != TFD_OK:
             raise DeviceError(rc, "tfd_ctx_create failed")
         self._h = handle
+        self._stream = None
         self.device = device
 
     @property
@@ -210,7 +211,9 @@ class Context:
         self.check(self._lib.tfd_ctx_synchronize(self._h))
 
     def stream(self) -> int:
-        return self._lib.tfd_ctx_stream(self._h) or 0
+        if self._stream is None:  # the context keeps the stream of its first use
+            self._stream = self._lib.tfd_ctx_stream(self._h) or 0
+        return self._stream
 
     def retained_bytes(self) -> int:
         return self._lib.tfd_ctx_retained_bytes(self._h)
@@ -254,8 +257,14 @@ def default_context() -> Context:
 
 # ------------------------------------------------------------------ buffers
 
+_torch_types: dict = {}  # type -> whether it is one of torch's
+
+
 def _is_torch(x) -> bool:
-    return type(x).__module__.startswith("torch")
+    kind = _torch_types.get(type(x))
+    if kind is None:
+        kind = _torch_types[type(x)] = type(x).__module__.startswith("torch")
+    return kind
 
 
 # torch dtypes accepted for each host dtype: f32 operands, keep/valid bytes,
@@ -266,6 +275,7 @@ _TORCH_DTYPES = {
     np.dtype(np.uint16): ("uint16", "int16", "bfloat16"),
     np.dtype(np.int64): ("int64",),
 }
+_accepted: set = set()  # (torch dtype, host dtype) pairs that passed the check by name
 
 
 class _Arg:
@@ -277,18 +287,22 @@ class _Arg:
     any device access. A torch tensor must already have the element type the
     entry reads (no silent reinterpretation of a half-width type)."""
 
+    __slots__ = ("obj", "name", "ptr", "n", "device")
+
     def __init__(self, x, dtype, name, count: Optional[int] = None):
         self.obj = x
         self.name = name
         if x is None:
             self.ptr, self.n, self.device = None, 0, None
             return
-        if _is_torch(x):
-            allowed = _TORCH_DTYPES[np.dtype(dtype)]
-            got = str(x.dtype).replace("torch.", "")
-            if got not in allowed:
-                raise InvalidArgument(
-                    TFD_EINVAL, f"{name}: tensor dtype {got}, expected {' or '.join(allowed)}")
+        if _torch_types.get(type(x)) or _is_torch(x):
+            if (x.dtype, dtype) not in _accepted:
+                allowed = _TORCH_DTYPES[np.dtype(dtype)]
+                got = str(x.dtype).replace("torch.", "")
+                if got not in allowed:
+                    raise InvalidArgument(
+                        TFD_EINVAL, f"{name}: tensor dtype {got}, expected {' or '.join(allowed)}")
+                _accepted.add((x.dtype, dtype))
             if not x.is_contiguous():
                 raise InvalidArgument(TFD_EINVAL, f"{name}: tensor must be contiguous")
             self.ptr = x.data_ptr()
@@ -325,12 +339,12 @@ def _flags(args: Sequence[_Arg], ctx: Optional["Context"] = None) -> int:
     kinds = {a.device for a in args if a.obj is not None}
     if len(kinds) > 1:
         raise InvalidArgument(TFD_EINVAL, "mix of host arrays and device tensors")
-    if kinds == {True}:
+    if True in kinds:
         if ctx is not None:
             for a in args:
-                if a.obj is not None and a.obj.device.index not in (None, ctx.device):
+                if a.obj is not None and a.obj.get_device() != ctx.device:
                     raise InvalidArgument(
-                        TFD_EINVAL, f"{a.name}: tensor on cuda:{a.obj.device.index}, "
+                        TFD_EINVAL, f"{a.name}: tensor on cuda:{a.obj.get_device()}, "
                         f"the context runs on device {ctx.device}")
         return TFD_DEVICE_PTRS | (TFD_ASYNC if _async else 0)
     return TFD_HOST_PTRS
@@ -352,12 +366,13 @@ class _StreamOrder:
             return
         import torch
 
-        cur = torch.cuda.current_stream(ctx.device)
-        handle = ctx.stream()
-        if not handle or handle == cur.cuda_stream:
+        handle = ctx._stream if ctx._stream is not None else ctx.stream()
+        if handle == torch._C._cuda_getCurrentRawStream(ctx.device):
             return
+        cur = torch.cuda.current_stream(ctx.device)
         self.torch_stream = cur
-        self.stream = torch.cuda.ExternalStream(handle, device=ctx.device)
+        self.stream = (torch.cuda.ExternalStream(handle, device=ctx.device) if handle
+                       else torch.cuda.default_stream(ctx.device))
         self.stream.wait_stream(cur)
         self.flags = flags
 
@@ -385,8 +400,16 @@ def _new_out(like: _Arg, n: int, dtype=np.float32):
     if like.device:
         import torch
 
-        return torch.empty(n, dtype=getattr(torch, np.dtype(dtype).name), device=like.obj.device)
+        return torch.empty(n, dtype=torch.float32 if dtype is np.float32 else torch.int64,
+                           device=like.obj.device)
     return np.empty(n, dtype=dtype)
+
+
+def _ptr(x):
+    """Address of an array or tensor that was just made."""
+    if x is None:
+        return None
+    return x.data_ptr() if _torch_types.get(type(x)) else x.ctypes.data
 
 
 # ------------------------------------------------------------------ op descriptors
@@ -637,25 +660,35 @@ def jeff_linear_attention_rows(q, k, v, log_decay, beta, mask, rows: int, length
     dt = np.uint16 if bf16 else np.float32
     nk, nv = rows * length * key_heads * key_dim, rows * length * heads * value_dim
     ng, ns = rows * length * heads, rows * heads * key_dim * value_dim
-    aq, ak, av = (_Arg(x, dt, nm, c) for x, nm, c in ((q, "q", nk), (k, "k", nk), (v, "v", nv)))
+    aq, ak, av = _Arg(q, dt, "q", nk), _Arg(k, dt, "k", nk), _Arg(v, dt, "v", nv)
     ag = _Arg(log_decay, np.float32, "log_decay", ng)
-    ab, am, asi = (_Arg(x, np.float32, nm, c if x is not None else None) for x, nm, c in
-                   ((beta, "beta", ng), (mask, "mask", rows * length), (state, "state", ns)))
+    ab = _Arg(beta, np.float32, "beta", ng)
+    am = _Arg(mask, np.float32, "mask", rows * length)
+    asi = _Arg(state, np.float32, "state", ns)
+    args = [aq, ak, av, ag, ab, am, asi]
+    # What is made here needs no checks, what is given does.
     if out is None:
         out = _new_out(aq, nv)
-    if state_out is None and want_state:
-        state_out = _new_out(aq, ns)
-    elif state_out is state and state is not None:
-        state_out = asi.obj
-    a_out = _Arg(out, np.float32, "out", nv)
-    aso = _Arg(state_out, np.float32, "state_out", ns if state_out is not None else None)
-    flags = _flags([aq, ak, av, ag, ab, am, asi, aso, a_out], ctx)
+        out_ptr = _ptr(out)
+    else:
+        args.append(_Arg(out, np.float32, "out", nv))
+        out, out_ptr = args[-1].obj, args[-1].ptr
+    if state_out is None:
+        state_out = _new_out(aq, ns) if want_state else None
+        state_ptr = _ptr(state_out)
+    elif state_out is state:
+        state_out, state_ptr = asi.obj, asi.ptr
+    else:
+        args.append(_Arg(state_out, np.float32, "state_out", ns))
+        state_out, state_ptr = args[-1].obj, args[-1].ptr
+    flags = _flags(args, ctx)
     fn = (ctx._lib.tfd_jeff_linear_attention_rows_bf16 if bf16
           else ctx._lib.tfd_jeff_linear_attention_rows_f32)
     _call(ctx, flags, fn, ctx.handle, rows, length, heads, key_heads, key_dim, value_dim, aq.ptr,
           ak.ptr, av.ptr, ag.ptr, ab.ptr, am.ptr,
-          f32_bits(max(key_dim, 1) ** -0.5 if scale is None else scale), asi.ptr, aso.ptr, a_out.ptr, flags)
-    return a_out.obj, aso.obj
+          f32_bits(max(key_dim, 1) ** -0.5 if scale is None else scale), asi.ptr, state_ptr,
+          out_ptr, flags)
+    return out, state_out
 
 
 def jeff_linear_attention_step(q, k, v, log_decay, beta, state, rows: int, heads: int,
@@ -708,16 +741,15 @@ def token_log_probs(logits, tokens, positions: int, vocab: int, *, top: int = 0,
     if at.n != per * positions:
         raise InvalidArgument(TFD_EINVAL, f"tokens: {at.n} elements, not a whole number of "
                               f"tokens for each of {positions} positions")
-    new = [_Arg(_new_out(ax, n, dt) if n is not None else None, dt, nm) for n, dt, nm in (
-        (per * positions if tokens is not None else None, np.float32, "log_probs"),
-        (positions, np.float32, "entropy"),
-        (top * positions if top > 0 else None, np.int64, "top_tokens"),
-        (top * positions if top > 0 else None, np.float32, "top_log_probs"))]
-    flags = _flags([ax, at, *new], ctx)
+    lp = None if tokens is None else _new_out(ax, per * positions)
+    entropy = _new_out(ax, positions)
+    ids = _new_out(ax, top * positions, np.int64) if top > 0 else None
+    top_lp = _new_out(ax, top * positions) if top > 0 else None
+    flags = _flags([ax, at], ctx)
     fn = ctx._lib.tfd_token_log_probs_bf16 if bf16 else ctx._lib.tfd_token_log_probs_f32
-    _call(ctx, flags, fn, ctx.handle, ax.ptr, vocab, ld, positions, at.ptr, per, top,
-          *[a.ptr for a in new], flags)
-    return TokenLogProbs(*[a.obj for a in new])
+    _call(ctx, flags, fn, ctx.handle, ax.ptr, vocab, ld, positions, at.ptr, per, top, _ptr(lp),
+          _ptr(entropy), _ptr(ids), _ptr(top_lp), flags)
+    return TokenLogProbs(lp, entropy, ids, top_lp)
 
 
 def to_bf16_bits(x: np.ndarray) -> np.ndarray:
