@@ -93,11 +93,30 @@ __device__ __forceinline__ void store_frag(unsigned char *block, int lane, const
   for (int i = 0; i < NP; ++i) *reinterpret_cast<frag *>(block + 1024 * i + 16 * lane) = p[i];
 }
 
-// Operand elements: f32 as three pieces, bf16 as itself.
+// Operand elements: f32 as three pieces, bf16 as itself. In memory the keys and
+// queries lie in fragment order as they are: f32 as two blocks of 1 KB (a lane's first
+// and last four elements), split when they are used, bf16 as one.
 template <typename T>
 struct Pieces {
-  static constexpr int n = sizeof(T) == 4 ? 3 : 1;
+  static constexpr int n = sizeof(T) == 4 ? 3 : 1, blocks = sizeof(T) == 4 ? 2 : 1;
 };
+template <typename T>
+struct Stored {
+  f32x4 b[Pieces<T>::blocks];
+};
+template <typename T>
+__device__ __forceinline__ void load_stored(const unsigned char *block, int lane, Stored<T> &s) {
+#pragma unroll
+  for (int i = 0; i < Pieces<T>::blocks; ++i)
+    s.b[i] = *reinterpret_cast<const f32x4 *>(block + 1024 * i + 16 * lane);
+}
+template <typename T>
+__device__ __forceinline__ void to_frag(const Stored<T> &s, frag (&p)[Pieces<T>::n]) {
+  if constexpr (sizeof(T) == 4)
+    split8(s.b[0], s.b[1], p);
+  else
+    p[0] = __builtin_bit_cast(frag, s.b[0]);
+}
 
 // Loads go through a buffer resource of the head's (feature, token) matrix: one
 // 32-bit offset, no branch; past its end they give 0 (offsets stay below 2^31, so a
@@ -108,8 +127,7 @@ struct Pieces {
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 constexpr int kNowhere = (int)0x80000000u;  // past every resource's end
 
-// What a lane holds of an operand: eight f32, four pairs of bf16 (packed), or
-// eight single bf16.
+// Eight values as loaded: f32, or bf16 in a register each.
 struct Raw {
   uint32_t d[8];
 };
@@ -121,56 +139,62 @@ __device__ __forceinline__ uint32_t load_one(Rsrc m, int off) {
   else
     return __builtin_amdgcn_raw_buffer_load_b16(m, off, 0, 0);
 }
-// Four consecutive tokens into d[0..3] (f32, single bf16) or d[0..1] (packed).
-// 16-byte f32 loads need 4-byte alignment only, 8-byte bf16 ones are taken with
-// `packed` alone (length % 4 == 0, aligned).
+// Four consecutive tokens (16-byte loads need 4-byte alignment only).
 template <typename T>
-__device__ __forceinline__ void load_four(Rsrc m, int off, bool packed, uint32_t *d) {
+struct Four {
+  uint32_t d[4];
+};
+template <>
+struct Four<float> {
+  f32x4 v;
+};
+template <typename T>
+__device__ __forceinline__ void load_four(Rsrc m, int off, Four<T> &x) {
   if constexpr (sizeof(T) == 4) {
-    const auto x = __builtin_amdgcn_raw_buffer_load_b128(m, off, 0, 0);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) d[e] = x[e];
-  } else if (packed) {
-    const auto x = __builtin_amdgcn_raw_buffer_load_b64(m, off, 0, 0);
-    d[0] = x[0], d[1] = x[1];
+    x.v = buffer_load4(m, off, 0);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) d[e] = load_one<T>(m, off + 2 * e);
+    for (int e = 0; e < 4; ++e) x.d[e] = load_one<T>(m, off + 2 * e);
+  }
+}
+template <typename T>
+__device__ __forceinline__ f32x4 values_of(const Four<T> &x) {
+  if constexpr (sizeof(T) == 4) {
+    return x.v;
+  } else {
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(x.d[e] << 16);
+    return v;
   }
 }
 
-// Eight values as operand pieces, those whose bit of `on` is not set as 0.
+// In fragment order, 0 where not `on`.
 template <typename T>
-__device__ __forceinline__ void to_frag(const Raw &v, bool packed, unsigned on,
-                                        frag (&p)[Pieces<T>::n]) {
+__device__ __forceinline__ Stored<T> stored(const Raw &v, bool on) {
+  Stored<T> s;
   if constexpr (sizeof(T) == 2) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[i] = packed ? v.d[i] : (v.d[2 * i] & 0xffffu) | (v.d[2 * i + 1] << 16);
-      const unsigned pair = on >> (2 * i);
-      w[i] &= (pair & 1u ? 0xffffu : 0u) | (pair & 2u ? 0xffff0000u : 0u);
-    }
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    p[0] = __builtin_bit_cast(frag, u32x4{w[0], w[1], w[2], w[3]});
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = on ? __builtin_amdgcn_perm(v.d[2 * i + 1], v.d[2 * i], 0x05040100u) : 0u;
+    s.b[0] = __builtin_bit_cast(f32x4, w);
   } else {
-    f32x4 lo, hi;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      lo[e] = (on >> e) & 1u ? __uint_as_float(v.d[e]) : 0.0f;
-      hi[e] = (on >> (4 + e)) & 1u ? __uint_as_float(v.d[4 + e]) : 0.0f;
+      s.b[0][e] = on ? __uint_as_float(v.d[e]) : 0.0f;
+      s.b[1][e] = on ? __uint_as_float(v.d[4 + e]) : 0.0f;
     }
-    split8(lo, hi, p);
   }
+  return s;
 }
-// Value e of four loaded by load_four, as f32.
 template <typename T>
-__device__ __forceinline__ float value_of(const uint32_t *d, bool packed, int e) {
-  if constexpr (sizeof(T) == 4) return __uint_as_float(d[e]);
-  if (packed) return __uint_as_float(e & 1 ? d[e >> 1] & 0xffff0000u : d[e >> 1] << 16);
-  return __uint_as_float(d[e] << 16);
+__device__ __forceinline__ void store_stored(unsigned char *block, int slot, const Stored<T> &s) {
+#pragma unroll
+  for (int i = 0; i < Pieces<T>::blocks; ++i)
+    *reinterpret_cast<f32x4 *>(block + 1024 * i + 16 * slot) = s.b[i];
 }
-
 // ------------------------------------------------------------------ a chunk
 
 struct ChunkScan {
@@ -182,10 +206,11 @@ struct ChunkScan {
 // The chunk's decays, by one wavefront (lane = token). The sums are held in 64
 // bits: a difference of sums is then good to 2^-24 of the terms between them,
 // whatever came before.
-__device__ __forceinline__ void scan_chunk(const LinearArgs &a, size_t rh, int t0, int n,
-                                           uint64_t act, int lane, ChunkScan &c) {
+// log_decay, beta: of token `lane`, as they are in memory.
+__device__ __forceinline__ void scan_chunk(float log_decay, float beta, uint64_t act, int lane,
+                                           ChunkScan &c) {
   const bool on = (act >> lane) & 1u;
-  const float g = on ? a.log_decay[rh * a.L + t0 + lane] : 0.0f;
+  const float g = on ? log_decay : 0.0f;
   const bool forgets = g < kForget;
   double x = forgets ? 0.0 : (double)g * kLog2eD;
 #pragma unroll
@@ -202,13 +227,7 @@ __device__ __forceinline__ void scan_chunk(const LinearArgs &a, size_t rh, int t
   c.forget[lane] = p;
   c.from_start[lane] = p >= 0 ? 0.0f : fast_exp2((float)x);
   c.to_end[lane] = last > lane ? 0.0f : fast_exp2((float)(all - x));
-  c.beta[lane] = on && a.beta ? a.beta[rh * a.L + t0 + lane] : 0.0f;
-}
-
-// Bit t: token t0 + t is there and active (one wavefront's lanes).
-__device__ __forceinline__ uint64_t active_tokens(const LinearArgs &a, int r, int t0, int lane) {
-  const int t = t0 + lane;
-  return __ballot(t < a.L && (!a.mask || a.mask[(size_t)r * a.L + t] != 0.0f));
+  c.beta[lane] = on ? beta : 0.0f;
 }
 
 // Token-major operand (rows = tokens, contraction = features f0 ..): blocks
@@ -223,33 +242,49 @@ __device__ __forceinline__ void load_octet(Rsrc m, int L, int t0, int f0, int o,
     v.d[e] = load_one<T>(m, (t0 + t) * es + f * L * es);
   }
 }
-template <int NP>
-__device__ __forceinline__ void put_octet(unsigned char *dst, int steps, int o, int t,
-                                          const frag (&p)[NP]) {
-  store_frag<NP>(dst + 1024 * NP * ((t >> 4) * steps + (o >> 2)), 16 * (o & 3) + (t & 15), p);
+// Byte offset of octet o's block of `size` bytes for token t, and the token's slot in it.
+__device__ __forceinline__ int octet_block(int size, int steps, int o, int t) {
+  return size * ((t >> 4) * steps + (o >> 2));
 }
+__device__ __forceinline__ int octet_slot(int o, int t) { return 16 * (o & 3) + (t & 15); }
 
-// Feature-major fragments (rows = features of tile i, contraction = tokens of step
-// ks) out of the token-major blocks: ds_read_b64_tr_b16 hands element e of lane j of
-// a group of 16 lanes the value 16 e + j of their 16 x 8 bytes, so lane c of the
-// group reads the four features 4 (c % 4) .. of token 4 g + c / 4.
+// The keys by features (rows = features of tile i, contraction = tokens of step ks):
+// f32 from the matrix itself, where the lane's feature is its row and its tokens
+// lie side by side, bf16 out of the slab's token-major blocks in LDS, where
+// ds_read_b64_tr_b16 hands element e of lane j of a group of 16 the value 16 e + j
+// of their 16 x 8 bytes: lane c of the group reads the four features 4 (c % 4) .. of
+// token 4 g + c / 4.
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ s16x4 read_transposed(const unsigned char *p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (__attribute__((address_space(3))) s16x4 *)(uintptr_t)(__attribute__((address_space(3))) void *)p);
+__device__ __forceinline__ f32x4 read_transposed(const unsigned char *lo, const unsigned char *hi) {
+  typedef __attribute__((address_space(3))) s16x4 *Lds;
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (Lds)(uintptr_t)(__attribute__((address_space(3))) void *)lo);
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (Lds)(uintptr_t)(__attribute__((address_space(3))) void *)hi);
+  return __builtin_bit_cast(f32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
-template <int NP>
-__device__ __forceinline__ void load_frag_t(const unsigned char *blocks, int steps, int i, int ks,
-                                            int lane, frag (&p)[NP]) {
+template <typename T>
+__device__ __forceinline__ Stored<T> keys_by_feature(Rsrc m, int L, int t0, int f0, uint64_t act,
+                                                     const unsigned char *blocks, int i, int ks,
+                                                     int lane) {
+  Stored<T> s;
   const int g = lane >> 4, c = lane & 15;
-  const unsigned char *at = blocks + 1024 * NP * (2 * ks * steps + (i >> 1)) +
-                            16 * (16 * (c & 3) + 4 * g + (c >> 2)) + 8 * (i & 1);
+  if constexpr (sizeof(T) == 4) {
+    const int off = (c * L + 4 * g) * 4 + ((f0 + 16 * i) * L + t0 + 32 * ks) * 4;
+    s.b[0] = buffer_load4(m, off, 0);
+    s.b[1] = buffer_load4(m, off + 64, 0);
+    const uint32_t on = (uint32_t)(act >> (32 * ks)) >> (4 * g);
 #pragma unroll
-  for (int x = 0; x < NP; ++x) {
-    const s16x4 lo = read_transposed(at + 1024 * x);
-    const s16x4 hi = read_transposed(at + 1024 * (NP * steps + x));
-    p[x] = __builtin_bit_cast(frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    for (int e = 0; e < 4; ++e) {
+      s.b[0][e] = (on >> e) & 1u ? s.b[0][e] : 0.0f;
+      s.b[1][e] = (on >> (16 + e)) & 1u ? s.b[1][e] : 0.0f;
+    }
+  } else {
+    const unsigned char *at = blocks + 1024 * (4 * ks + (i >> 1)) +
+                              16 * (16 * (c & 3) + 4 * g + (c >> 2)) + 8 * (i & 1);
+    s.b[0] = read_transposed(at, at + 2048);
   }
+  return s;
 }
 
 // Barrier for LDS only: outstanding global loads and stores stay outstanding.
@@ -270,9 +305,11 @@ __device__ __forceinline__ int tri_block(int tt, int ks) { return tt < 2 ? tt : 
 // by 16 x 16 blocks: the diagonal blocks by substitution (one wave each), the others
 // by T_ij = -T_ii sum_(j <= k < i) M_ik T_kj on the f32 matrix cores, one distance
 // i - j after the other. The first head of a key head's group also leaves the
-// keys and queries behind as operands: the walk then reads whole lines one after
-// the other, whatever the row length (a chunk's piece of a feature row is 128 or
-// 256 bytes, and rows of 2^n tokens put all of them on the same few channels).
+// keys and queries behind in fragment order, the keys both ways: the walk's column
+// groups then each read whole lines with few loads (in the original order, where a
+// wave's token tile is 32 or 64 bytes of a feature row, 8 x 1024 tokens with 8 heads of
+// 256 x 256 in bf16 took 339 us against 129, 2 x 8192 805 against 556).
+// All loads are issued before anything waits for the first of them.
 template <typename T, bool DELTA>
 __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearWork ws) {
   constexpr int NP = Pieces<T>::n;
@@ -292,16 +329,24 @@ __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearW
   const uint32_t bytes = (uint32_t)a.dk * a.L * sizeof(T);
   const Rsrc q = buffer_rsrc(static_cast<const T *>(a.q) + kh * a.dk * a.L, bytes);
   const Rsrc k = buffer_rsrc(static_cast<const T *>(a.k) + kh * a.dk * a.L, bytes);
-  Raw x[2], y[2];
-  auto fetch = [&](int f0) {
+  const int t = min(t0 + lane, a.L - 1);
+  float mask = 1.0f, log_decay = 0.0f, beta = 0.0f;
+  if (a.mask) mask = a.mask[(size_t)r * a.L + t];
+  if (wave == 0) {
+    log_decay = a.log_decay[rh * a.L + t];
+    if (DELTA) beta = a.beta[rh * a.L + t];
+  }
+  Raw x[2][2], y[2][2];  // two slabs of 64 features
+  auto fetch = [&](int f0, Raw (&x)[2], Raw (&y)[2]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       load_octet<T>(q, a.L, t0, f0, wave + 4 * i, lane, x[i]);
       load_octet<T>(k, a.L, t0, f0, wave + 4 * i, lane, y[i]);
     }
   };
-  fetch(0);
-  const uint64_t act = active_tokens(a, r, t0, lane);
+  fetch(0, x[0], y[0]);
+  if (a.dk > 64) fetch(64, x[1], y[1]);
+  const uint64_t act = __ballot(lane < n && mask != 0.0f);
   if (h == 0 && threadIdx.x == 0) ws.active[(size_t)r * nch + chunk] = act;
   if (act == 0) {
     for (int j = wave; j < a.dv; j += 4)
@@ -309,42 +354,44 @@ __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearW
     return;
   }
   if (wave == 0) {
-    scan_chunk(a, rh, t0, n, act, lane, sc);
+    scan_chunk(log_decay, beta, act, lane, sc);
     float *v = ws.factors + at * 3 * kC;
     v[lane] = sc.from_start[lane];
     v[kC + lane] = sc.to_end[lane];
     v[2 * kC + lane] = sc.beta[lane];
   }
   const bool first = h % a.group == 0;
-  const size_t part = (size_t)4 * steps * NP * 1024;
-  unsigned char *packed = ws.packed + (kh * nch + chunk) * parts * part;
-  unsigned char *pq = packed, *pt = packed + part, *pk = packed + 2 * part;
+  constexpr int SB = Pieces<T>::blocks * 1024;
+  const size_t part = (size_t)4 * steps * SB;
+  unsigned char *pq = ws.packed + (kh * nch + chunk) * parts * part;
+  unsigned char *pt = pq + part, *pk = pq + 2 * part;
   f32x4 score[4] = {}, keys[4] = {};
-  for (int f0 = 0; f0 < 32 * steps; f0 += 64) {
+  auto slab = [&](int f0, Raw (&x)[2], Raw (&y)[2]) {
     if (f0) lds_barrier();
-    const unsigned on = (act >> lane) & 1u ? 0xffu : 0u;
+    const bool on = (act >> lane) & 1u;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int o = wave + 4 * i, step = f0 / 32 + (o >> 2);
+      const int o = wave + 4 * i, whole = 4 * (f0 / 32) + o;  // octet of all features
+      const bool keep = first && whole < 4 * steps;
       frag p[NP];
-      to_frag<T>(x[i], false, on, p);
-      put_octet<NP>(qpl, 2, o, lane, p);
-      if (first && step < steps) put_octet<NP>(pq, steps, 4 * step + (o & 3), lane, p);
-      to_frag<T>(y[i], false, on, p);
-      put_octet<NP>(kpl, 2, o, lane, p);
-      if (DELTA && first && step < steps) put_octet<NP>(pk, steps, 4 * step + (o & 3), lane, p);
+      const Stored<T> qs = stored<T>(x[i], on);
+      to_frag<T>(qs, p);
+      store_frag<NP>(qpl + octet_block(NP * 1024, 2, o, lane), octet_slot(o, lane), p);
+      if (keep) store_stored<T>(pq + octet_block(SB, steps, whole, lane), octet_slot(o, lane), qs);
+      const Stored<T> ks = stored<T>(y[i], on);
+      to_frag<T>(ks, p);
+      store_frag<NP>(kpl + octet_block(NP * 1024, 2, o, lane), octet_slot(o, lane), p);
+      if (DELTA && keep)
+        store_stored<T>(pk + octet_block(SB, steps, whole, lane), octet_slot(o, lane), ks);
     }
     lds_barrier();
-    if (f0 + 64 < 32 * steps) fetch(f0 + 64);
-    if (first)
+    const int tile = f0 / 16 + wave;
+    if (first && tile < 2 * steps)
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {  // feature tile i of the slab at both token steps
-        const int i = wave, tile = f0 / 16 + i;
-        if (tile >= 2 * steps) continue;
-        frag p[NP];
-        load_frag_t<NP>(kpl, 2, i, b, lane, p);
-        store_frag<NP>(pt + 1024 * NP * (2 * tile + b), lane, p);
-      }
+      for (int b = 0; b < 2; ++b)
+        store_stored<T>(pt + SB * (2 * tile + b), lane,
+                        keys_by_feature<T>(k, a.L, t0, f0, act, kpl, wave, b, lane));
+    if (f0 + 128 < 32 * steps) fetch(f0 + 128, x, y);
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       if (f0 + 32 * kk >= a.dk) continue;
@@ -360,6 +407,10 @@ __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearW
         if (DELTA) keys[st] = mma<NP, NP>(s, kf, keys[st]);
       }
     }
+  };
+  for (int f0 = 0; f0 < 32 * steps; f0 += 128) {
+    slab(f0, x[0], y[0]);
+    if (f0 + 64 < 32 * steps) slab(f0 + 64, x[1], y[1]);
   }
   lds_barrier();  // the decays are there, the operands read
   unsigned char *planes = ws.planes + at * (DELTA ? 2 * kTri : kTri);
@@ -453,12 +504,14 @@ __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearW
 // state. Keys, queries and triangles come as operands straight from memory into
 // registers, each of its lines to one wave, and are fetched for the next chunk as
 // soon as the present one has been multiplied.
-template <typename T, bool DELTA, int NI, int CT>
-__global__ __launch_bounds__(256) void linear_walk_kernel(LinearArgs a, LinearWork ws) {
+template <typename T, bool DELTA, int NI, int CT, int DEPTH>
+__global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 ? 2 : 1) void linear_walk_kernel(
+    LinearArgs a, LinearWork ws) {
   constexpr int NP = Pieces<T>::n;
   constexpr int NV = DELTA ? 3 : NP;  // pieces of what is written
   constexpr int NK = NI / 2, TI = NI >= 4 ? NI / 4 : 1;
-  constexpr int kPart = 4 * NK * NP * 1024, kParts = DELTA ? 3 : 2;
+  constexpr int SB = Pieces<T>::blocks * 1024;
+  constexpr int kPart = 4 * NK * SB, kParts = DELTA ? 3 : 2;
   constexpr int PB = DELTA ? 2 * kTri : kTri;
   __shared__ __attribute__((aligned(16))) unsigned char spl[CT][NK * 3 * 1024];
   __shared__ __attribute__((aligned(16))) unsigned char xpl[DELTA ? CT : 1][DELTA ? 6 * 1024 : 16];
@@ -538,83 +591,97 @@ __global__ __launch_bounds__(256) void linear_walk_kernel(LinearArgs a, LinearWo
     return Chunk{base + b, (uint64_t)hi << 32 | lo};
   };
 
-  frag qf[NK][NP], kf[DELTA ? NK : 1][NP], tf[TI][2][NP], sf[2][3], xf[2][3];
-  f32x4 start, end, beta;
-  float whole = 0.0f;
-  uint32_t write[CT][4];
-  auto fetch_rows = [&](int at) {  // token tile `wave` of queries and keys
-    const unsigned char *p = packed + (size_t)at * (kParts * kPart) + 1024 * NP * NK * wave;
+  // What a chunk needs from memory, for DEPTH chunks.
+  struct Operands {
+    Stored<T> q[NK], k[DELTA ? NK : 1], t[TI][2];
+    frag scores[2][3], solve[2][3];
+    f32x4 start, end, beta;
+    float whole;
+    Four<T> values[CT];
+  } even, odd;
+  auto fetch_rows = [&](Operands &o, int at) {  // token tile `wave` of queries and keys
+    const unsigned char *p = packed + (size_t)at * (kParts * kPart) + SB * NK * wave;
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk) {
-      load_frag<NP>(p + 1024 * NP * kk, lane, qf[kk]);
-      if constexpr (DELTA) load_frag<NP>(p + 2 * kPart + 1024 * NP * kk, lane, kf[kk]);
+      load_stored<T>(p + SB * kk, lane, o.q[kk]);
+      if constexpr (DELTA) load_stored<T>(p + 2 * kPart + SB * kk, lane, o.k[kk]);
     }
   };
-  auto fetch_values = [&](int at) {
+  auto fetch_values = [&](Operands &o, int at) {
     const float *f = ws.factors + (rh * nch + at) * 3 * kC + 16 * wave + 4 * g;
-    start = *reinterpret_cast<const f32x4 *>(f);
-    end = *reinterpret_cast<const f32x4 *>(f + kC);
-    if (DELTA) beta = *reinterpret_cast<const f32x4 *>(f + 2 * kC);
+    o.start = *reinterpret_cast<const f32x4 *>(f);
+    o.end = *reinterpret_cast<const f32x4 *>(f + kC);
+    if (DELTA) o.beta = *reinterpret_cast<const f32x4 *>(f + 2 * kC);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
-      load_four<T>(v, (row_off + at * kC + 16 * ct * a.L) * (int)sizeof(T), a.vec_v, write[ct]);
+      load_four<T>(v, (row_off + at * kC + 16 * ct * a.L) * (int)sizeof(T), o.values[ct]);
   };
-  auto fetch_tri = [&](int at, int which, frag (&f)[2][3]) {
+  auto fetch_tri = [&](int at, int which, frag (&f)[2][3]) {  // row tile `wave` of a triangle
     const unsigned char *p = ws.planes + (rh * nch + at) * PB + which * kTri;
     load_frag<3>(p + 3072 * tri_block(wave, 0), lane, f[0]);
     if (wave >= 2) load_frag<3>(p + 3072 * tri_block(wave, 1), lane, f[1]);
   };
-  auto fetch_columns = [&](int at) {  // the owned feature tiles of the keys
-    whole = ws.factors[(rh * nch + at) * 3 * kC + kC - 1];
+  auto fetch_columns = [&](Operands &o, int at) {  // the owned feature tiles of the keys
+    o.whole = ws.factors[(rh * nch + at) * 3 * kC + kC - 1];
     if (!owner) return;
-    const unsigned char *p = packed + (size_t)at * (kParts * kPart) + kPart + 2048 * NP * TI * wave;
+    const unsigned char *p = packed + (size_t)at * (kParts * kPart) + kPart + 2 * SB * TI * wave;
 #pragma unroll
     for (int i = 0; i < TI; ++i)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) load_frag<NP>(p + 1024 * NP * (2 * i + ks), lane, tf[i][ks]);
+      for (int ks = 0; ks < 2; ++ks) load_stored<T>(p + SB * (2 * i + ks), lane, o.t[i][ks]);
   };
 
-  Chunk cur = next_chunk();
-  if (cur.at >= 0) {
-    fetch_rows(cur.at);
-    fetch_values(cur.at);
-    if (DELTA) fetch_tri(cur.at, 1, xf);
-    fetch_tri(cur.at, 0, sf);
-    fetch_columns(cur.at);
-    put_state();
-    lds_barrier();
-  }
-  while (cur.at >= 0) {
-    const Chunk nxt = next_chunk();
+  Chunk next[DEPTH + 1];  // the present chunk and those behind it
+#pragma unroll
+  for (int i = 0; i <= DEPTH; ++i) next[i] = next_chunk();
+  auto fetch = [&](Operands &o, int at) {
+    if (at < 0) return;
+    fetch_rows(o, at);
+    fetch_values(o, at);
+    if (DELTA) fetch_tri(at, 1, o.solve);
+    fetch_tri(at, 0, o.scores);
+    fetch_columns(o, at);
+  };
+  fetch(even, next[0].at);
+  if (DEPTH == 2) fetch(odd, next[1].at);
+  put_state();
+  lds_barrier();
+  auto walk = [&](Operands &o) {
+    const Chunk cur = next[0];
+    // Behind the last chunk the present one's operands come again, for nothing: a
+    // branch around the loads makes the compiler wait for them at its end.
+    const int far = next[DEPTH].at >= 0 ? next[DEPTH].at : cur.at;
     // Q S0 and K S0, even and odd steps in accumulators of their own.
     f32x4 X[CT][2] = {}, O[CT][2] = {};
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk) {
-      frag s[CT][3];
+      frag s[CT][3], qf[NP], kf[NP];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) load_frag<3>(spl[ct] + 3072 * kk, lane, s[ct]);
+      to_frag<T>(o.q[kk], qf);
+      if constexpr (DELTA) to_frag<T>(o.k[kk], kf);
       typedef Products<NP, 3> P;
 #pragma unroll
       for (int x = 0; x < P::n; ++x)
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
           if constexpr (DELTA)
-            X[ct][kk & 1] = mfma_16x16x32_bf16(kf[kk][P::a(x)], s[ct][P::b(x)], X[ct][kk & 1]);
-          O[ct][kk & 1] = mfma_16x16x32_bf16(qf[kk][P::a(x)], s[ct][P::b(x)], O[ct][kk & 1]);
+            X[ct][kk & 1] = mfma_16x16x32_bf16(kf[P::a(x)], s[ct][P::b(x)], X[ct][kk & 1]);
+          O[ct][kk & 1] = mfma_16x16x32_bf16(qf[P::a(x)], s[ct][P::b(x)], O[ct][kk & 1]);
         }
     }
-    if (nxt.at >= 0) fetch_rows(nxt.at);
+    fetch_rows(o, far);
     f32x4 U[CT];
     const unsigned on = (unsigned)(cur.act >> (16 * wave + 4 * g));
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
+      const f32x4 given = values_of<T>(o.values[ct]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        U[ct][e] = (on >> e) & 1u ? value_of<T>(write[ct], a.vec_v, e) : 0.0f;
-      O[ct][0] = start * (O[ct][0] + O[ct][1]);
+      for (int e = 0; e < 4; ++e) U[ct][e] = (on >> e) & 1u ? given[e] : 0.0f;
+      O[ct][0] = o.start * (O[ct][0] + O[ct][1]);
       if constexpr (DELTA)
         put_half(xpl[ct] + 3072 * (wave >> 1), wave & 1,
-                 beta * (U[ct] - start * (X[ct][0] + X[ct][1])));
+                 o.beta * (U[ct] - o.start * (X[ct][0] + X[ct][1])));
     }
     if constexpr (DELTA) {
       lds_barrier();
@@ -631,9 +698,9 @@ __global__ __launch_bounds__(256) void linear_walk_kernel(LinearArgs a, LinearWo
         for (int i = 0; i < P::n; ++i)
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct)
-            U[ct] = mfma_16x16x32_bf16(xf[ks][P::a(i)], x[ct][P::b(i)], U[ct]);
+            U[ct] = mfma_16x16x32_bf16(o.solve[ks][P::a(i)], x[ct][P::b(i)], U[ct]);
       }
-      if (nxt.at >= 0) fetch_tri(nxt.at, 1, xf);
+      fetch_tri(far, 1, o.solve);
     }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
@@ -643,13 +710,18 @@ __global__ __launch_bounds__(256) void linear_walk_kernel(LinearArgs a, LinearWo
         *reinterpret_cast<u32x2 *>(upl[ct] + 1024 * (wave >> 1) + 16 * lane + 8 * (wave & 1)) =
             __builtin_bit_cast(u32x2, __builtin_convertvector(U[ct], bf16x4));
       }
-      put_half(epl[ct] + 3072 * (wave >> 1), wave & 1, U[ct] * end);
+      put_half(epl[ct] + 3072 * (wave >> 1), wave & 1, U[ct] * o.end);
     }
-    const float decay = whole;
+    const float decay = o.whole;
     lds_barrier();
-    if (nxt.at >= 0) fetch_values(nxt.at);
+    fetch_values(o, far);
     // The state first: the next chunk waits for it.
     if (owner) {
+      frag tf[TI][2][NP];
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) to_frag<T>(o.t[i][ks], tf[i][ks]);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
         frag e[2][3];
@@ -667,7 +739,7 @@ __global__ __launch_bounds__(256) void linear_walk_kernel(LinearArgs a, LinearWo
               S[ct][i] = mfma_16x16x32_bf16(tf[i][ks][P::a(x)], e[ks][P::b(x)], S[ct][i]);
       }
     }
-    if (nxt.at >= 0) fetch_columns(nxt.at);
+    fetch_columns(o, far);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       if (ks && wave < 2) continue;
@@ -679,11 +751,11 @@ __global__ __launch_bounds__(256) void linear_walk_kernel(LinearArgs a, LinearWo
       for (int x = 0; x < P::n; ++x)
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct)
-          O[ct][0] = mfma_16x16x32_bf16(sf[ks][P::a(x)], u[ct][P::b(x)], O[ct][0]);
+          O[ct][0] = mfma_16x16x32_bf16(o.scores[ks][P::a(x)], u[ct][P::b(x)], O[ct][0]);
     }
     put_state();
-    if (nxt.at >= 0) fetch_tri(nxt.at, 0, sf);
-    const int n = min(kC, a.L - cur.at * kC) - 16 * wave - 4 * g;
+    fetch_tri(far, 0, o.scores);
+    const int n = a.L - cur.at * kC - 16 * wave - 4 * g;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       const int off = (row_off + cur.at * kC + 16 * ct * a.L) * 4;
@@ -696,7 +768,15 @@ __global__ __launch_bounds__(256) void linear_walk_kernel(LinearArgs a, LinearWo
       }
     }
     lds_barrier();
-    cur = nxt;
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) next[i] = next[i + 1];
+    next[DEPTH] = next_chunk();
+  };
+  while (next[0].at >= 0) {
+    walk(even);
+    if (DEPTH == 1) continue;
+    if (next[0].at < 0) break;
+    walk(odd);
   }
   if (a.state_out && owner) {
     const Rsrc to = buffer_rsrc(a.state_out + rh * a.dk * a.dv, state_bytes);
@@ -716,15 +796,17 @@ __global__ __launch_bounds__(256) void linear_walk_kernel(LinearArgs a, LinearWo
 template <typename T, bool DELTA, int NI>
 void launch_walk(const LinearArgs &a, const LinearWork &ws, hipStream_t stream, hipEvent_t stop) {
   const size_t jtiles = (size_t)((a.dv + 15) / 16), heads = (size_t)a.rows * a.heads;
-  if (heads * jtiles > 2 * (size_t)a.cus) {
-    const dim3 grid((unsigned)(heads * ((jtiles + 1) / 2)));
-    hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI, 2>), grid, dim3(256), 0, stream, nullptr,
-                          stop, 0, a, ws);
-  } else {
-    const dim3 grid((unsigned)(heads * jtiles));
-    hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI, 1>), grid, dim3(256), 0, stream, nullptr,
-                          stop, 0, a, ws);
-  }
+  const dim3 one((unsigned)(heads * jtiles)), two((unsigned)(heads * ((jtiles + 1) / 2)));
+  constexpr int kAhead = sizeof(T) == 4 && NI > 8 ? 1 : 2;  // what 512 registers hold
+  if (heads * jtiles <= (size_t)a.cus)
+    hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI, 1, kAhead>), one, dim3(256), 0, stream,
+                          nullptr, stop, 0, a, ws);
+  else if (heads * jtiles <= 2 * (size_t)a.cus)
+    hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI, 1, 1>), one, dim3(256), 0, stream,
+                          nullptr, stop, 0, a, ws);
+  else
+    hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI, 2, 1>), two, dim3(256), 0, stream,
+                          nullptr, stop, 0, a, ws);
 }
 
 template <typename T, bool DELTA>

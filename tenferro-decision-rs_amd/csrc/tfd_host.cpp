@@ -1552,8 +1552,6 @@ int linear_run(tfd_ctx *c, bool bf16, size_t rows, size_t length, size_t heads, 
   a.scale = bits_to_f32(scale_bits);
   a.bf16 = bf16;
   a.state_vec = value_dim % 4 == 0 && aligned16(si_d) && aligned16(so_d);
-  a.vec_k = length % 4 == 0 && (reinterpret_cast<uintptr_t>(k_d) & 7) == 0;
-  a.vec_v = length % 4 == 0 && (reinterpret_cast<uintptr_t>(v_d) & 7) == 0;
   a.cus = c->cus;
   tfd::KernelEvents ev;
   if (length <= kLinearRecurrentTokens || length > tfd::kLinearChunkedTokens) {

@@ -343,7 +343,6 @@ struct LinearArgs {
   float scale;
   bool bf16;       // q, k and v
   bool state_vec;  // 16-byte access to the states' rows: dv % 4 == 0, aligned
-  bool vec_k, vec_v;  // bf16: access to four tokens of k, v at once (L % 4 == 0, 8-byte aligned)
   int cus;
 };
 // Token by token.
@@ -375,7 +374,7 @@ struct LinearSpace {
 };
 inline LinearSpace linear_space(const LinearArgs &a) {
   const size_t nch = (size_t)((a.L + kLinearChunk - 1) / kLinearChunk) * a.rows;
-  return LinearSpace{nch * a.key_heads * linear_steps(a.dk) * (a.beta ? 12 : 8) * (a.bf16 ? 1 : 3) * 1024,
+  return LinearSpace{nch * a.key_heads * linear_steps(a.dk) * (a.beta ? 12 : 8) * (a.bf16 ? 1 : 2) * 1024,
                      nch * a.heads * kLinearTriBytes * (a.beta ? 2 : 1),
                      nch * a.heads * 3 * kLinearChunk * 4, nch * 8};
 }
