@@ -263,6 +263,15 @@ __device__ __forceinline__ f32x4 read_transposed(const unsigned char *lo, const 
       (Lds)(uintptr_t)(__attribute__((address_space(3))) void *)hi);
   return __builtin_bit_cast(f32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
+// 0 for the inactive among a lane's tokens of step ks.
+__device__ __forceinline__ void drop_inactive(uint64_t act, int ks, int g, f32x4 (&b)[2]) {
+  const uint32_t on = (uint32_t)(act >> (32 * ks)) >> (4 * g);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    b[0][e] = (on >> e) & 1u ? b[0][e] : 0.0f;
+    b[1][e] = (on >> (16 + e)) & 1u ? b[1][e] : 0.0f;
+  }
+}
 template <typename T>
 __device__ __forceinline__ Stored<T> keys_by_feature(Rsrc m, int L, int t0, int f0, uint64_t act,
                                                      const unsigned char *blocks, int i, int ks,
@@ -273,12 +282,7 @@ __device__ __forceinline__ Stored<T> keys_by_feature(Rsrc m, int L, int t0, int 
     const int off = (c * L + 4 * g) * 4 + ((f0 + 16 * i) * L + t0 + 32 * ks) * 4;
     s.b[0] = buffer_load4(m, off, 0);
     s.b[1] = buffer_load4(m, off + 64, 0);
-    const uint32_t on = (uint32_t)(act >> (32 * ks)) >> (4 * g);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      s.b[0][e] = (on >> e) & 1u ? s.b[0][e] : 0.0f;
-      s.b[1][e] = (on >> (16 + e)) & 1u ? s.b[1][e] : 0.0f;
-    }
+    drop_inactive(act, ks, g, s.b);
   } else {
     const unsigned char *at = blocks + 1024 * (4 * ks + (i >> 1)) +
                               16 * (16 * (c & 3) + 4 * g + (c >> 2)) + 8 * (i & 1);
@@ -307,10 +311,11 @@ __device__ __forceinline__ int tri_block(int tt, int ks) { return tt < 2 ? tt : 
 // i - j after the other. The first head of a key head's group also leaves the
 // keys and queries behind in fragment order, the keys both ways: the walk's column
 // groups then each read whole lines with few loads (in the original order, where a
-// wave's token tile is 32 or 64 bytes of a feature row, 8 x 1024 tokens with 8 heads of
-// 256 x 256 in bf16 took 339 us against 129, 2 x 8192 805 against 556).
+// wave's token tile is 32 or 64 bytes of a feature row, this kernel and the walk took 14
+// + 222 us instead of 20 + 94 for 8 x 1024 tokens with 8 heads of 256 x 256 in bf16, 62 +
+// 586 instead of 109 + 424 for 2 x 8192 with 16 heads of 128 x 128).
 // All loads are issued before anything waits for the first of them.
-template <typename T, bool DELTA>
+template <typename T, bool DELTA, bool FEATURES>
 __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearWork ws) {
   constexpr int NP = Pieces<T>::n;
   constexpr int kS = 68;  // floats per row: 16-byte rows, rows 4 banks apart
@@ -386,7 +391,7 @@ __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearW
     }
     lds_barrier();
     const int tile = f0 / 16 + wave;
-    if (first && tile < 2 * steps)
+    if (FEATURES && first && tile < 2 * steps)
 #pragma unroll
       for (int b = 0; b < 2; ++b)
         store_stored<T>(pt + SB * (2 * tile + b), lane,
@@ -504,8 +509,19 @@ __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearW
 // state. Keys, queries and triangles come as operands straight from memory into
 // registers, each of its lines to one wave, and are fetched for the next chunk as
 // soon as the present one has been multiplied.
+// f32 keys of up to 128 features are read by features where they are, whole lines of
+// 32 tokens each (16 rows of 1024 tokens, 16 heads of 128 x 128: 404 us, packed 438; 8 x
+// 2048 with 16 heads of 64 x 64: 235, 256; plain 2 x 8192: 449, 477). The delta rule with
+// a workgroup per CU, which waits for every byte, and keys of more features take packed
+// ones (1 x 4096: 260, in place 263; 4 x 1024 with 8 heads of 256 x 256 on 2 key
+// heads: 169, 179).
+template <typename T, bool DELTA>
+constexpr bool keys_in_place(int NI, int depth) {
+  return sizeof(T) == 4 && NI <= 8 && (depth == 1 || !DELTA);
+}
+
 template <typename T, bool DELTA, int NI, int CT, int DEPTH>
-__global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 ? 2 : 1) void linear_walk_kernel(
+__global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 && CT < 4 ? 2 : 1) void linear_walk_kernel(
     LinearArgs a, LinearWork ws) {
   constexpr int NP = Pieces<T>::n;
   constexpr int NV = DELTA ? 3 : NP;  // pieces of what is written
@@ -513,6 +529,7 @@ __global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 ? 2 : 1) void linear_wal
   constexpr int SB = Pieces<T>::blocks * 1024;
   constexpr int kPart = 4 * NK * SB, kParts = DELTA ? 3 : 2;
   constexpr int PB = DELTA ? 2 * kTri : kTri;
+  constexpr bool kKeysPacked = !keys_in_place<T, DELTA>(NI, DEPTH);
   __shared__ __attribute__((aligned(16))) unsigned char spl[CT][NK * 3 * 1024];
   __shared__ __attribute__((aligned(16))) unsigned char xpl[DELTA ? CT : 1][DELTA ? 6 * 1024 : 16];
   __shared__ __attribute__((aligned(16))) unsigned char upl[CT][2 * NV * 1024], epl[CT][6 * 1024];
@@ -534,6 +551,9 @@ __global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 ? 2 : 1) void linear_wal
   const size_t col0 = (rh * a.dv + jw) * a.L;
   const Rsrc v = buffer_rsrc(static_cast<const T *>(a.v) + col0, mine * sizeof(T));
   const Rsrc out = buffer_rsrc(a.out + col0, mine * 4);
+  const Rsrc keys = buffer_rsrc(
+      static_cast<const T *>(a.k) + ((size_t)r * a.key_heads + h / a.group) * a.dk * a.L,
+      (uint32_t)a.dk * a.L * sizeof(T));
   const uint32_t state_bytes = (uint32_t)a.dk * a.dv * 4;
   const int row_off = c16 * a.L + 16 * wave + 4 * g;  // elements: the lane's column and first token
   const bool owner = TI * wave < NI;
@@ -628,7 +648,15 @@ __global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 ? 2 : 1) void linear_wal
 #pragma unroll
     for (int i = 0; i < TI; ++i)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) load_stored<T>(p + SB * (2 * i + ks), lane, o.t[i][ks]);
+      for (int ks = 0; ks < 2; ++ks) {
+        if constexpr (kKeysPacked) {
+          load_stored<T>(p + SB * (2 * i + ks), lane, o.t[i][ks]);
+        } else {
+          const int off = ((16 * (TI * wave + i) + c16) * a.L + at * kC + 32 * ks + 4 * g) * 4;
+          o.t[i][ks].b[0] = buffer_load4(keys, off, 0);
+          o.t[i][ks].b[1] = buffer_load4(keys, off + 64, 0);
+        }
+      }
   };
 
   Chunk next[DEPTH + 1];  // the present chunk and those behind it
@@ -721,7 +749,10 @@ __global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 ? 2 : 1) void linear_wal
 #pragma unroll
       for (int i = 0; i < TI; ++i)
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) to_frag<T>(o.t[i][ks], tf[i][ks]);
+        for (int ks = 0; ks < 2; ++ks) {
+          if constexpr (!kKeysPacked) drop_inactive(cur.act, ks, g, o.t[i][ks].b);
+          to_frag<T>(o.t[i][ks], tf[i][ks]);
+        }
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
         frag e[2][3];
@@ -793,20 +824,42 @@ __global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 ? 2 : 1) void linear_wal
   }
 }
 
+// Column tiles per workgroup and chunks fetched ahead, by how the grid fills the CUs
+// (us for prompts of 512 tokens, 16 heads of 128 x 128 unless stated, both kernels):
+//   one tile each if every workgroup then has a CU to itself, and two chunks ahead as
+//   far as 512 registers hold them: nothing else hides the latency there;
+//   one tile each while two workgroups per CU hold all (4 rows: 72 us, two tiles 91,
+//   four 84), except f32 keys over 128 wide, whose operands leave room for one
+//   (4 rows, 8 heads of 256 x 256: two tiles 94, one 127);
+//   beyond that every operand is loaded and split for more columns at once: four
+//   tiles for the f32 delta rule with keys of 65 to 128 (8 rows: 119 us, two tiles 154,
+//   which spill, one 147; 16 rows: 231, 343, 304), where the splitting weighs most,
+//   two tiles otherwise (8 rows in bf16: 79 us, four tiles 89, one 91; 32 rows of
+//   32 x 32 f32: 145, 161, 159; 16 rows of 64 x 64 f32: 106, 110, 125).
 template <typename T, bool DELTA, int NI>
-void launch_walk(const LinearArgs &a, const LinearWork &ws, hipStream_t stream, hipEvent_t stop) {
+hipError_t launch(const LinearArgs &a, const LinearWork &ws, hipStream_t stream, const KernelEvents &ev) {
+  constexpr bool wide = sizeof(T) == 4 && NI > 8;
+  constexpr int kAhead = wide ? 1 : 2, kTiles = sizeof(T) == 4 && DELTA && NI == 8 ? 4 : 2;
   const size_t jtiles = (size_t)((a.dv + 15) / 16), heads = (size_t)a.rows * a.heads;
-  const dim3 one((unsigned)(heads * jtiles)), two((unsigned)(heads * ((jtiles + 1) / 2)));
-  constexpr int kAhead = sizeof(T) == 4 && NI > 8 ? 1 : 2;  // what 512 registers hold
-  if (heads * jtiles <= (size_t)a.cus)
-    hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI, 1, kAhead>), one, dim3(256), 0, stream,
-                          nullptr, stop, 0, a, ws);
-  else if (heads * jtiles <= 2 * (size_t)a.cus)
-    hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI, 1, 1>), one, dim3(256), 0, stream,
-                          nullptr, stop, 0, a, ws);
+  const size_t one = heads * jtiles, many = heads * ((jtiles + kTiles - 1) / kTiles);
+  const bool few = one <= (size_t)a.cus;
+  const auto pairs = keys_in_place<T, DELTA>(NI, few ? kAhead : 1)
+                         ? linear_pairs_kernel<T, DELTA, sizeof(T) == 2>
+                         : linear_pairs_kernel<T, DELTA, true>;
+  const dim3 chunks((unsigned)((a.L + kC - 1) / kC), (unsigned)a.heads, (unsigned)a.rows);
+  hipExtLaunchKernelGGL(pairs, chunks, dim3(256), 0, stream, ev.start, nullptr, 0, a, ws);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  if (few)
+    hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI, 1, kAhead>), dim3((unsigned)one),
+                          dim3(256), 0, stream, nullptr, ev.stop, 0, a, ws);
+  else if (!wide && one <= 2 * (size_t)a.cus)
+    hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI, 1, 1>), dim3((unsigned)one), dim3(256),
+                          0, stream, nullptr, ev.stop, 0, a, ws);
   else
-    hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI, 2, 1>), two, dim3(256), 0, stream,
-                          nullptr, stop, 0, a, ws);
+    hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI, kTiles, 1>), dim3((unsigned)many),
+                          dim3(256), 0, stream, nullptr, ev.stop, 0, a, ws);
+  return hipGetLastError();
 }
 
 template <typename T, bool DELTA>
@@ -818,20 +871,10 @@ hipError_t launch_chunks(const LinearArgs &a, unsigned char *mem, hipStream_t st
   ws.planes = ws.packed + sp.packed;
   ws.factors = reinterpret_cast<float *>(ws.planes + sp.planes);
   ws.active = reinterpret_cast<uint64_t *>(ws.planes + sp.planes + sp.factors);
-  const dim3 grid((unsigned)((a.L + kC - 1) / kC), (unsigned)a.heads, (unsigned)a.rows);
-  hipExtLaunchKernelGGL((linear_pairs_kernel<T, DELTA>), grid, dim3(256), 0, stream, ev.start,
-                        nullptr, 0, a, ws);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  if (a.dk <= 32)
-    launch_walk<T, DELTA, 2>(a, ws, stream, ev.stop);
-  else if (a.dk <= 64)
-    launch_walk<T, DELTA, 4>(a, ws, stream, ev.stop);
-  else if (a.dk <= 128)
-    launch_walk<T, DELTA, 8>(a, ws, stream, ev.stop);
-  else
-    launch_walk<T, DELTA, 16>(a, ws, stream, ev.stop);
-  return hipGetLastError();
+  if (a.dk <= 32) return launch<T, DELTA, 2>(a, ws, stream, ev);
+  if (a.dk <= 64) return launch<T, DELTA, 4>(a, ws, stream, ev);
+  if (a.dk <= 128) return launch<T, DELTA, 8>(a, ws, stream, ev);
+  return launch<T, DELTA, 16>(a, ws, stream, ev);
 }
 
 }  // namespace

@@ -1483,8 +1483,12 @@ int laya_forward(tfd_ctx *c, const tfd_laya_model *m, const int64_t *ids, const 
 
 // ------------------------------------------------------- linear attention
 
-// Tokens up to which the recurrence runs token by token.
-constexpr size_t kLinearRecurrentTokens = 12;
+// Tokens up to which the recurrence runs token by token, whose time grows with them
+// while a chunk's does not (f32, 16 heads of 128 x 128, us, recurrence against chunk:
+// one row of 8 tokens 20.1 and 19.9, 12 tokens 27.5 and 19.7; 16 rows of 8 tokens 27 and
+// 40, 12 tokens 40 and 40; bf16, whose chunk costs a third of the products: 64 rows of 4
+// tokens 56 and 79, 8 tokens 100 and 83).
+constexpr size_t kLinearRecurrentF32 = 10, kLinearRecurrentBf16 = 6;
 // Workspace of the chunked form that is not passed while one row fits it.
 constexpr size_t kLinearWorkspace = (size_t)2 << 30;
 
@@ -1554,7 +1558,7 @@ int linear_run(tfd_ctx *c, bool bf16, size_t rows, size_t length, size_t heads, 
   a.state_vec = value_dim % 4 == 0 && aligned16(si_d) && aligned16(so_d);
   a.cus = c->cus;
   tfd::KernelEvents ev;
-  if (length <= kLinearRecurrentTokens || length > tfd::kLinearChunkedTokens) {
+  if (length <= (bf16 ? kLinearRecurrentBf16 : kLinearRecurrentF32) || length > tfd::kLinearChunkedTokens) {
     if (!capturing && (rc = timing_events(c, &ev))) return rc;
     TFD_HIP(c, tfd::launch_linear_recurrent(a, c->stream, ev), "linear_recurrent launch");
   } else {

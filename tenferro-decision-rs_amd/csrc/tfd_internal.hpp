@@ -359,10 +359,11 @@ constexpr int kLinearTriBytes = 6 * 3 * 1024;
 __host__ __device__ inline int linear_steps(int dk) {
   return dk <= 32 ? 1 : dk <= 64 ? 2 : dk <= 128 ? 4 : 8;
 }
-// Workspace of launch_linear_chunks: per (row, key head, chunk) the queries by
-// tokens, the keys by features and (delta rule) by tokens as operands, per (row, head, chunk) the decayed scores (with
-// the delta rule also the solve operand after them) and 64 factors each from the
-// chunk's start, to its end and beta; per (row, chunk) the active tokens.
+// Workspace of launch_linear_chunks: per (row, key head, chunk) the queries by tokens,
+// the keys by features (unless they are read in place) and (delta rule) by tokens as operands; per (row,
+// head, chunk) the decayed scores (with the delta rule also the solve operand after them)
+// and 64 factors each from the chunk's start, to its end and beta; per (row, chunk) the
+// active tokens.
 struct LinearWork {
   unsigned char *packed, *planes;
   float *factors;
@@ -374,7 +375,8 @@ struct LinearSpace {
 };
 inline LinearSpace linear_space(const LinearArgs &a) {
   const size_t nch = (size_t)((a.L + kLinearChunk - 1) / kLinearChunk) * a.rows;
-  return LinearSpace{nch * a.key_heads * linear_steps(a.dk) * (a.beta ? 12 : 8) * (a.bf16 ? 1 : 2) * 1024,
+  const size_t parts = a.beta ? 3 : 2, block = a.bf16 ? 1024 : 2048;
+  return LinearSpace{nch * a.key_heads * parts * 4 * linear_steps(a.dk) * block,
                      nch * a.heads * kLinearTriBytes * (a.beta ? 2 : 1),
                      nch * a.heads * 3 * kLinearChunk * 4, nch * 8};
 }
