@@ -500,6 +500,17 @@ __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearW
 
 // ------------------------------------------------------------------ the walk
 
+// f32 keys of up to 128 features are read by features where they are, whole lines of
+// 32 tokens each (16 rows of 1024 tokens, 16 heads of 128 x 128: 404 us, packed 438; 8 x
+// 2048 with 16 heads of 64 x 64: 235, 256; plain 2 x 8192: 449, 477). The delta rule with
+// a workgroup per CU, which waits for every byte, and keys of more features take packed
+// ones (1 x 4096 on four waves: 260, in place 263; 4 x 1024 with 8 heads of 256 x 256 on 2 key
+// heads: 169, 179).
+template <typename T, bool DELTA>
+constexpr bool keys_in_place(int NI, int depth) {
+  return sizeof(T) == 4 && NI <= 8 && (depth == 1 || !DELTA);
+}
+
 // Workgroup = four waves on CT tiles of 16 value columns of one (row, head). The waves
 // share the work of a chunk, which is what every later chunk waits for: wave w has
 // token tile w of U and O, and the feature tiles TI w .. of the state (feature
@@ -509,23 +520,22 @@ __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearW
 // state. Keys, queries and triangles come as operands straight from memory into
 // registers, each of its lines to one wave, and are fetched for the next chunk as
 // soon as the present one has been multiplied.
-// f32 keys of up to 128 features are read by features where they are, whole lines of
-// 32 tokens each (16 rows of 1024 tokens, 16 heads of 128 x 128: 404 us, packed 438; 8 x
-// 2048 with 16 heads of 64 x 64: 235, 256; plain 2 x 8192: 449, 477). The delta rule with
-// a workgroup per CU, which waits for every byte, and keys of more features take packed
-// ones (1 x 4096: 260, in place 263; 4 x 1024 with 8 heads of 256 x 256 on 2 key
-// heads: 169, 179).
-template <typename T, bool DELTA>
-constexpr bool keys_in_place(int NI, int depth) {
-  return sizeof(T) == 4 && NI <= 8 && (depth == 1 || !DELTA);
-}
-
-template <typename T, bool DELTA, int NI, int CT, int DEPTH>
-__global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 && CT < 4 ? 2 : 1) void linear_walk_kernel(
-    LinearArgs a, LinearWork ws) {
+//
+// On eight waves (delta rule) the first four are on the path from one state to the next
+// (K S0, V - d K S0 and U), the others beside it (Q S0 and O, which nothing waits for);
+// the state's tiles are dealt to all eight. `path` and `side` are both true on four.
+//
+// What bounds it: a chunk's three exchanges follow each other, 5400 cycles in bf16 with
+// 128 x 128 and one tile, of which the products are 960; with two workgroups per CU the
+// operands, 8 TB/s out of L2.
+template <typename T, bool DELTA, int NI, int CT, int DEPTH, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 || (DEPTH == 1 && NI <= 8 && CT < 4) ? 2 : 1)
+void linear_walk_kernel(LinearArgs a, LinearWork ws) {
+  constexpr bool kRoles = WAVES == 8;
+  static_assert(DELTA || !kRoles, "without the solve nothing is on the path but the state");
   constexpr int NP = Pieces<T>::n;
   constexpr int NV = DELTA ? 3 : NP;  // pieces of what is written
-  constexpr int NK = NI / 2, TI = NI >= 4 ? NI / 4 : 1;
+  constexpr int NK = NI / 2, TI = NI >= WAVES ? NI / WAVES : 1;
   constexpr int SB = Pieces<T>::blocks * 1024;
   constexpr int kPart = 4 * NK * SB, kParts = DELTA ? 3 : 2;
   constexpr int PB = DELTA ? 2 * kTri : kTri;
@@ -535,6 +545,8 @@ __global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 && CT < 4 ? 2 : 1) void 
   __shared__ __attribute__((aligned(16))) unsigned char upl[CT][2 * NV * 1024], epl[CT][6 * 1024];
   const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w = wave & 3;  // token tile
+  const bool path = !kRoles || wave < 4, side = !kRoles || wave >= 4;
   const int nch = (a.L + kC - 1) / kC;
   // Column groups of a (row, head) go to one XCD (workgroups are dealt to the
   // eight in turn) and share its L2.
@@ -555,7 +567,7 @@ __global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 && CT < 4 ? 2 : 1) void 
       static_cast<const T *>(a.k) + ((size_t)r * a.key_heads + h / a.group) * a.dk * a.L,
       (uint32_t)a.dk * a.L * sizeof(T));
   const uint32_t state_bytes = (uint32_t)a.dk * a.dv * 4;
-  const int row_off = c16 * a.L + 16 * wave + 4 * g;  // elements: the lane's column and first token
+  const int row_off = c16 * a.L + 16 * w + 4 * g;  // elements: the lane's column and first token
   const bool owner = TI * wave < NI;
   f32x4 S[CT][TI] = {};
   if (a.state_in && owner) {
@@ -612,34 +624,37 @@ __global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 && CT < 4 ? 2 : 1) void 
   };
 
   // What a chunk needs from memory, for DEPTH chunks.
+  constexpr bool kBoth = DELTA && !kRoles;
   struct Operands {
-    Stored<T> q[NK], k[DELTA ? NK : 1], t[TI][2];
-    frag scores[2][3], solve[2][3];
+    Stored<T> q[NK], k[kBoth ? NK : 1], t[TI][2];  // with roles q is the wave's of both,
+    frag scores[2][3], solve[2][3];                // and so are the scores
     f32x4 start, end, beta;
     float whole;
     Four<T> values[CT];
   } even, odd;
   auto fetch_rows = [&](Operands &o, int at) {  // token tile `wave` of queries and keys
-    const unsigned char *p = packed + (size_t)at * (kParts * kPart) + SB * NK * wave;
+    const unsigned char *p = packed + (size_t)at * (kParts * kPart) + SB * NK * w;
+    if (kRoles && path) p += 2 * kPart;
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk) {
       load_stored<T>(p + SB * kk, lane, o.q[kk]);
-      if constexpr (DELTA) load_stored<T>(p + 2 * kPart + SB * kk, lane, o.k[kk]);
+      if constexpr (kBoth) load_stored<T>(p + 2 * kPart + SB * kk, lane, o.k[kk]);
     }
   };
   auto fetch_values = [&](Operands &o, int at) {
-    const float *f = ws.factors + (rh * nch + at) * 3 * kC + 16 * wave + 4 * g;
+    const float *f = ws.factors + (rh * nch + at) * 3 * kC + 16 * w + 4 * g;
     o.start = *reinterpret_cast<const f32x4 *>(f);
     o.end = *reinterpret_cast<const f32x4 *>(f + kC);
     if (DELTA) o.beta = *reinterpret_cast<const f32x4 *>(f + 2 * kC);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
-      load_four<T>(v, (row_off + at * kC + 16 * ct * a.L) * (int)sizeof(T), o.values[ct]);
+      load_four<T>(v, path ? (row_off + at * kC + 16 * ct * a.L) * (int)sizeof(T) : kNowhere,
+                   o.values[ct]);
   };
-  auto fetch_tri = [&](int at, int which, frag (&f)[2][3]) {  // row tile `wave` of a triangle
-    const unsigned char *p = ws.planes + (rh * nch + at) * PB + which * kTri;
-    load_frag<3>(p + 3072 * tri_block(wave, 0), lane, f[0]);
-    if (wave >= 2) load_frag<3>(p + 3072 * tri_block(wave, 1), lane, f[1]);
+  auto fetch_tri = [&](int at, bool solve, frag (&f)[2][3]) {  // row tile w of a triangle
+    const unsigned char *p = ws.planes + (rh * nch + at) * PB + (solve ? kTri : 0);
+    load_frag<3>(p + 3072 * tri_block(w, 0), lane, f[0]);
+    if (w >= 2) load_frag<3>(p + 3072 * tri_block(w, 1), lane, f[1]);
   };
   auto fetch_columns = [&](Operands &o, int at) {  // the owned feature tiles of the keys
     o.whole = ws.factors[(rh * nch + at) * 3 * kC + kC - 1];
@@ -666,8 +681,8 @@ __global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 && CT < 4 ? 2 : 1) void 
     if (at < 0) return;
     fetch_rows(o, at);
     fetch_values(o, at);
-    if (DELTA) fetch_tri(at, 1, o.solve);
-    fetch_tri(at, 0, o.scores);
+    if (kBoth) fetch_tri(at, true, o.solve);
+    fetch_tri(at, kRoles && path, o.scores);
     fetch_columns(o, at);
   };
   fetch(even, next[0].at);
@@ -687,29 +702,30 @@ __global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 && CT < 4 ? 2 : 1) void 
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) load_frag<3>(spl[ct] + 3072 * kk, lane, s[ct]);
       to_frag<T>(o.q[kk], qf);
-      if constexpr (DELTA) to_frag<T>(o.k[kk], kf);
+      if constexpr (kBoth) to_frag<T>(o.k[kk], kf);
       typedef Products<NP, 3> P;
 #pragma unroll
       for (int x = 0; x < P::n; ++x)
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-          if constexpr (DELTA)
+          if constexpr (kBoth)
             X[ct][kk & 1] = mfma_16x16x32_bf16(kf[P::a(x)], s[ct][P::b(x)], X[ct][kk & 1]);
           O[ct][kk & 1] = mfma_16x16x32_bf16(qf[P::a(x)], s[ct][P::b(x)], O[ct][kk & 1]);
         }
     }
     fetch_rows(o, far);
     f32x4 U[CT];
-    const unsigned on = (unsigned)(cur.act >> (16 * wave + 4 * g));
+    const unsigned on = (unsigned)(cur.act >> (16 * w + 4 * g));
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       const f32x4 given = values_of<T>(o.values[ct]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) U[ct][e] = (on >> e) & 1u ? given[e] : 0.0f;
       O[ct][0] = o.start * (O[ct][0] + O[ct][1]);
-      if constexpr (DELTA)
-        put_half(xpl[ct] + 3072 * (wave >> 1), wave & 1,
-                 o.beta * (U[ct] - o.start * (X[ct][0] + X[ct][1])));
+      if constexpr (DELTA) {
+        const f32x4 x = kRoles ? O[ct][0] : o.start * (X[ct][0] + X[ct][1]);
+        if (path) put_half(xpl[ct] + 3072 * (w >> 1), w & 1, o.beta * (U[ct] - x));
+      }
     }
     if constexpr (DELTA) {
       lds_barrier();
@@ -717,7 +733,7 @@ __global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 && CT < 4 ? 2 : 1) void 
       for (int ct = 0; ct < CT; ++ct) U[ct] = f32x4{};
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
-        if (ks && wave < 2) continue;
+        if (!path || (ks && w < 2)) continue;
         frag x[CT][3];
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) load_frag<3>(xpl[ct] + 3072 * ks, lane, x[ct]);
@@ -726,20 +742,22 @@ __global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 && CT < 4 ? 2 : 1) void 
         for (int i = 0; i < P::n; ++i)
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct)
-            U[ct] = mfma_16x16x32_bf16(o.solve[ks][P::a(i)], x[ct][P::b(i)], U[ct]);
+            U[ct] = mfma_16x16x32_bf16((kRoles ? o.scores : o.solve)[ks][P::a(i)], x[ct][P::b(i)],
+                                       U[ct]);
       }
-      fetch_tri(far, 1, o.solve);
+      if constexpr (kBoth) fetch_tri(far, true, o.solve);
     }
+    if (path)
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      if constexpr (NV == 3) {
-        put_half(upl[ct] + 3072 * (wave >> 1), wave & 1, U[ct]);
-      } else {  // exact: the values are bf16
-        *reinterpret_cast<u32x2 *>(upl[ct] + 1024 * (wave >> 1) + 16 * lane + 8 * (wave & 1)) =
-            __builtin_bit_cast(u32x2, __builtin_convertvector(U[ct], bf16x4));
+      for (int ct = 0; ct < CT; ++ct) {
+        if constexpr (NV == 3) {
+          put_half(upl[ct] + 3072 * (w >> 1), w & 1, U[ct]);
+        } else {  // exact: the values are bf16
+          *reinterpret_cast<u32x2 *>(upl[ct] + 1024 * (w >> 1) + 16 * lane + 8 * (w & 1)) =
+              __builtin_bit_cast(u32x2, __builtin_convertvector(U[ct], bf16x4));
+        }
+        put_half(epl[ct] + 3072 * (w >> 1), w & 1, U[ct] * o.end);
       }
-      put_half(epl[ct] + 3072 * (wave >> 1), wave & 1, U[ct] * o.end);
-    }
     const float decay = o.whole;
     lds_barrier();
     fetch_values(o, far);
@@ -771,9 +789,13 @@ __global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 && CT < 4 ? 2 : 1) void 
       }
     }
     fetch_columns(o, far);
+    if (kRoles) {  // only the side waits for what comes next
+      put_state();
+      lds_barrier();
+    }
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      if (ks && wave < 2) continue;
+      if (!side || (ks && w < 2)) continue;
       frag u[CT][NV];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) load_frag<NV>(upl[ct] + 1024 * NV * ks, lane, u[ct]);
@@ -784,11 +806,12 @@ __global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 && CT < 4 ? 2 : 1) void 
         for (int ct = 0; ct < CT; ++ct)
           O[ct][0] = mfma_16x16x32_bf16(o.scores[ks][P::a(x)], u[ct][P::b(x)], O[ct][0]);
     }
-    put_state();
-    fetch_tri(far, 0, o.scores);
-    const int n = a.L - cur.at * kC - 16 * wave - 4 * g;
+    if (!kRoles) put_state();
+    fetch_tri(far, kRoles && path, o.scores);
+    const int n = a.L - cur.at * kC - 16 * w - 4 * g;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
+      if (!side) continue;
       const int off = (row_off + cur.at * kC + 16 * ct * a.L) * 4;
       const f32x4 y = O[ct][0] * a.scale;
       if (cur.at * kC + kC <= a.L) {
@@ -798,7 +821,7 @@ __global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 && CT < 4 ? 2 : 1) void 
         for (int e = 0; e < 4; ++e) buffer_store1(y[e], out, e < n ? off + 4 * e : kNowhere, 0);
       }
     }
-    lds_barrier();
+    if (!kRoles) lds_barrier();
 #pragma unroll
     for (int i = 0; i < DEPTH; ++i) next[i] = next[i + 1];
     next[DEPTH] = next_chunk();
@@ -824,22 +847,27 @@ __global__ __launch_bounds__(256, DEPTH == 1 && NI <= 8 && CT < 4 ? 2 : 1) void 
   }
 }
 
-// Column tiles per workgroup and chunks fetched ahead, by how the grid fills the CUs
-// (us for prompts of 512 tokens, 16 heads of 128 x 128 unless stated, both kernels):
+// Column tiles per workgroup, its waves and chunks fetched ahead, by how the grid fills
+// the CUs (us for prompts of 512 tokens, 16 heads of 128 x 128 unless stated, both
+// kernels):
 //   one tile each if every workgroup then has a CU to itself, and two chunks ahead as
-//   far as 512 registers hold them: nothing else hides the latency there;
+//   far as 512 registers hold them: nothing else hides the latency there. The f32 delta
+//   rule, whose products and splitting are the path, on eight waves (1 x 4096: 215, four
+//   261; in bf16 2 x 8192: 433, four 416, where reading the state twice costs more);
 //   one tile each while two workgroups per CU hold all (4 rows: 72 us, two tiles 91,
-//   four 84), except f32 keys over 128 wide, whose operands leave room for one
-//   (4 rows, 8 heads of 256 x 256: two tiles 94, one 127);
+//   four 84), except f32 keys over 128 wide, whose operands leave room for one;
 //   beyond that every operand is loaded and split for more columns at once: four
 //   tiles for the f32 delta rule with keys of 65 to 128 (8 rows: 119 us, two tiles 154,
 //   which spill, one 147; 16 rows: 231, 343, 304), where the splitting weighs most,
 //   two tiles otherwise (8 rows in bf16: 79 us, four tiles 89, one 91; 32 rows of
-//   32 x 32 f32: 145, 161, 159; 16 rows of 64 x 64 f32: 106, 110, 125).
+//   32 x 32 f32: 145, 161, 159; 16 rows of 64 x 64 f32: 106, 110, 125; 4 x 1024 with 8
+//   heads of 256 x 256 f32: 145 on eight waves, 171 on four).
 template <typename T, bool DELTA, int NI>
-hipError_t launch(const LinearArgs &a, const LinearWork &ws, hipStream_t stream, const KernelEvents &ev) {
-  constexpr bool wide = sizeof(T) == 4 && NI > 8;
-  constexpr int kAhead = wide ? 1 : 2, kTiles = sizeof(T) == 4 && DELTA && NI == 8 ? 4 : 2;
+hipError_t launch(const LinearArgs &a, const LinearWork &ws, hipStream_t stream,
+                  const KernelEvents &ev) {
+  constexpr bool f32 = sizeof(T) == 4, wide = f32 && NI > 8;
+  constexpr int kAhead = wide ? 1 : 2, kTiles = f32 && DELTA && NI == 8 ? 4 : 2;
+  constexpr int kFewWaves = f32 && DELTA ? 8 : 4, kWideWaves = wide && DELTA ? 8 : 4;
   const size_t jtiles = (size_t)((a.dv + 15) / 16), heads = (size_t)a.rows * a.heads;
   const size_t one = heads * jtiles, many = heads * ((jtiles + kTiles - 1) / kTiles);
   const bool few = one <= (size_t)a.cus;
@@ -850,16 +878,16 @@ hipError_t launch(const LinearArgs &a, const LinearWork &ws, hipStream_t stream,
   hipExtLaunchKernelGGL(pairs, chunks, dim3(256), 0, stream, ev.start, nullptr, 0, a, ws);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  if (few)
-    hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI, 1, kAhead>), dim3((unsigned)one),
-                          dim3(256), 0, stream, nullptr, ev.stop, 0, a, ws);
-  else if (!wide && one <= 2 * (size_t)a.cus)
-    hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI, 1, 1>), dim3((unsigned)one), dim3(256),
-                          0, stream, nullptr, ev.stop, 0, a, ws);
-  else
-    hipExtLaunchKernelGGL((linear_walk_kernel<T, DELTA, NI, kTiles, 1>), dim3((unsigned)many),
-                          dim3(256), 0, stream, nullptr, ev.stop, 0, a, ws);
-  return hipGetLastError();
+  auto walk = [&](auto kernel, int waves, size_t grid) {
+    hipExtLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * waves), 0, stream, nullptr,
+                          ev.stop, 0, a, ws);
+    return hipGetLastError();
+  };
+  if (few) return walk(linear_walk_kernel<T, DELTA, NI, 1, kAhead, kFewWaves>, kFewWaves, one);
+  if constexpr (!wide)
+    if (one <= 2 * (size_t)a.cus)
+      return walk(linear_walk_kernel<T, DELTA, NI, 1, 1, 4>, 4, one);
+  return walk(linear_walk_kernel<T, DELTA, NI, kTiles, 1, kWideWaves>, kWideWaves, many);
 }
 
 template <typename T, bool DELTA>
