@@ -293,6 +293,11 @@ int tfd_jeff_full_attention_layer_rows_f32(tfd_ctx *ctx, size_t rows, size_t len
  * length 1 is the single-token form. key_dim is at most 256 (else
  * TFD_EUNSUPPORTED). A NaN or inf that an active token holds reaches this head's
  * later outputs, and may reach those up to 63 tokens before it.
+ * Both this and tfd_token_log_probs may run under stream capture (with TFD_ASYNC)
+ * once the context's workspace fits, that is, after one eager call of the same sizes,
+ * else TFD_EUNSUPPORTED. Later, larger calls leave a captured workspace in
+ * place until the context ends. The graphs of one context share its workspaces, with
+ * each other and with its eager calls: replay them in the order of one stream.
  */
 int tfd_jeff_linear_attention_rows_f32(tfd_ctx *ctx, size_t rows, size_t length, size_t heads,
                                        size_t key_heads, size_t key_dim, size_t value_dim,

@@ -1491,6 +1491,8 @@ int laya_forward(tfd_ctx *c, const tfd_laya_model *m, const int64_t *ids, const 
 constexpr size_t kLinearRecurrentF32 = 10, kLinearRecurrentBf16 = 6;
 // Workspace of the chunked form that is not passed while one row fits it.
 constexpr size_t kLinearWorkspace = (size_t)2 << 30;
+// Workgroups of a launch, likewise: 512 threads each, and a grid may have 2^32.
+constexpr size_t kLinearBlocks = (size_t)1 << 22;
 
 int linear_run(tfd_ctx *c, bool bf16, size_t rows, size_t length, size_t heads, size_t key_heads,
                size_t key_dim, size_t value_dim, const void *q, const void *k, const void *v,
@@ -1558,15 +1560,17 @@ int linear_run(tfd_ctx *c, bool bf16, size_t rows, size_t length, size_t heads, 
   a.state_vec = value_dim % 4 == 0 && aligned16(si_d) && aligned16(so_d);
   a.cus = c->cus;
   tfd::KernelEvents ev;
-  if (length <= (bf16 ? kLinearRecurrentBf16 : kLinearRecurrentF32) || length > tfd::kLinearChunkedTokens) {
+  const size_t recurrent = bf16 ? kLinearRecurrentBf16 : kLinearRecurrentF32;
+  if (length <= recurrent || length > tfd::kLinearChunkedTokens) {
     if (!capturing && (rc = timing_events(c, &ev))) return rc;
     TFD_HIP(c, tfd::launch_linear_recurrent(a, c->stream, ev), "linear_recurrent launch");
   } else {
     // As many rows at once as the workspace limit allows, at least one.
     a.rows = 1;
     const size_t row = tfd::linear_space(a).total();
-    size_t at_once = std::max<size_t>(1, kLinearWorkspace / row);
-    at_once = std::min(rows, at_once);
+    const size_t blocks = heads * ((value_dim + 15) / 16);
+    size_t at_once = std::min(kLinearWorkspace / row, kLinearBlocks / blocks);
+    at_once = std::min(rows, std::max<size_t>(1, at_once));
     if ((rc = reserve_capturable(c, op, c->linear, row * at_once, capturing))) return rc;
     if (!capturing && (rc = timing_events(c, &ev))) return rc;
     auto from = [](const void *p, size_t bytes) {

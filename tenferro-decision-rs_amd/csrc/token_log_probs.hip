@@ -411,15 +411,36 @@ void log_probs_plan(LogProbArgs &a, int cus) {
   a.parts = (int)((pieces + len - 1) / len);
 }
 
+// Positions of one launch: 2^30 threads of the 2^32 that a grid may have.
+constexpr size_t kLogProbLaunch = (size_t)1 << 22;
+
 hipError_t launch_log_probs(const LogProbArgs &a, hipStream_t stream, const KernelEvents &ev) {
   const int waves = a.vocab <= kLogProbWaveVocab ? 1 : 4;
-  if (a.bf16)
-    a.top ? launch_parts<true, true>(a, waves, stream, ev)
-          : launch_parts<true, false>(a, waves, stream, ev);
-  else
-    a.top ? launch_parts<false, true>(a, waves, stream, ev)
-          : launch_parts<false, false>(a, waves, stream, ev);
-  return hipGetLastError();
+  for (size_t p0 = 0; p0 < a.positions; p0 += kLogProbLaunch) {
+    LogProbArgs b = a;
+    b.positions = a.positions - p0 < kLogProbLaunch ? a.positions - p0 : kLogProbLaunch;
+    b.logits = static_cast<const char *>(a.logits) + (a.bf16 ? 2 : 4) * a.ld * p0;
+    if (a.per) {
+      b.tokens = a.tokens + a.per * p0;
+      b.log_probs = a.log_probs + a.per * p0;
+    }
+    if (a.entropy) b.entropy = a.entropy + p0;
+    if (a.top) {
+      b.top_tokens = a.top_tokens + a.top * p0;
+      b.top_log_probs = a.top_log_probs + a.top * p0;
+    }
+    const KernelEvents e{p0 ? nullptr : ev.start,
+                         p0 + b.positions < a.positions ? nullptr : ev.stop};
+    if (a.bf16)
+      a.top ? launch_parts<true, true>(b, waves, stream, e)
+            : launch_parts<true, false>(b, waves, stream, e);
+    else
+      a.top ? launch_parts<false, true>(b, waves, stream, e)
+            : launch_parts<false, false>(b, waves, stream, e);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  return hipSuccess;
 }
 
 }  // namespace tfd

@@ -196,6 +196,19 @@ def test_against_the_recurrence(gpu_ctx, shape, bf16, delta):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("delta", [True, False], ids=["delta", "plain"])
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("value_dim", [100, 213])
+@pytest.mark.parametrize("key_dim,length", [(20, 150), (50, 200), (100, 150), (200, 80)])
+def test_grids_past_the_compute_units(gpu_ctx, key_dim, length, value_dim, bf16, delta):
+    """280 and 560 column tiles, which other forms take than a tile per CU."""
+    p = Problem(5, length, 8, 4, key_dim, value_dim, bf16=bf16, delta=delta, mask="left",
+                state=True, decay=0.3)
+    out, state = p.run(gpu_ctx, cuda)
+    p.check(host(out), host(state))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("length", [1, 30, 150])
 @pytest.mark.parametrize("delta", [True, False], ids=["delta", "plain"])
 def test_decays_that_forget(gpu_ctx, length, delta):
@@ -369,3 +382,57 @@ def test_states_past_four_gigabytes(gpu_ctx):
         part(g)[..., None], part(beta)[..., None]
     p.state = before
     p.check(part(out.view(R, -1)), part(state))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_more_rows_than_one_workspace_holds(gpu_ctx, bf16):
+    """2300 rows of two chunks and 16 heads, over 2 GiB of operands: runs of rows follow
+    each other through the workspace."""
+    import torch
+
+    R, L, H, HK, dk, dv = 2300, 70, 16, 8, 32, 32
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    new = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    q, k = (torch.nn.functional.normalize(new(R, HK, dk, L), dim=2) for _ in range(2))
+    v, g, beta = new(R, H, dv, L), -new(R, H, L).abs(), torch.rand(R, H, L, generator=gen,
+                                                                   device="cuda")
+    state, mask = new(R, H, dk, dv), (torch.rand(R, L, generator=gen, device="cuda") < 0.9).float()
+    if bf16:
+        q, k, v = (x.bfloat16() for x in (q, k, v))
+    flat = [x.reshape(-1) for x in (q, k, v, g, beta, mask)]
+    out, after = te.jeff_linear_attention_rows(*flat, R, L, H, HK, dk, dv, state=state.view(-1),
+                                               bf16=bf16, ctx=gpu_ctx)
+    assert gpu_ctx.retained_bytes() < 3 << 30
+    rows = [0, 500, 1000, 1023, 1500, 2047, 2048, R - 1]
+    part = lambda x: x[rows].float().cpu().numpy()
+    p = Problem(len(rows), L, H, HK, dk, dv)
+    p.q, p.k, p.v, p.g, p.beta, p.mask, p.state = map(part, (q, k, v, g, beta, mask, state))
+    p.check(part(out.view(R, -1)), part(after.view(R, -1)))
+    assert bool((out.view(R, H, dv, L) != 0).any(3).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("length", [1 << 20, (1 << 20) + 5])
+def test_the_longest_chunked_row_and_past_it(gpu_ctx, length):
+    """The last tokens of a row of 2^20 tokens, and of one past what the chunks
+    address. e^(sum of the decays) of 300 tokens is below 2^-200: only those count."""
+    import torch
+
+    H, dk, dv, last = 2, 8, 8, 300
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    new = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    q, k = (torch.nn.functional.normalize(new(1, H, dk, length), dim=2) for _ in range(2))
+    v, g, beta = new(1, H, dv, length), -new(1, H, length).abs(), torch.rand(
+        1, H, length, generator=gen, device="cuda")
+    out, state = te.jeff_linear_attention_rows(*(x.reshape(-1) for x in (q, k, v, g, beta)), None, 1,
+                                               length, H, H, dk, dv, ctx=gpu_ctx)
+    part = lambda x: x[..., length - last:].cpu().numpy()
+    q, k, v, g, beta = map(part, (q, k, v, g, beta))
+    assert (g[..., :200].sum(-1) < -139).all()
+    scale = float(np.float32(dk ** -0.5))
+    want, S, size, A = reference(q, k, v, g, beta, None, scale, None)
+    tol = 2.0 ** -24 * (8 + 6 * np.sqrt(dk + 64 + last))
+    got = part(out.view(1, H, dv, length))
+    assert (np.abs(got - want) <= tol * size)[..., 200:].all()
+    assert (np.abs(state.view(1, H, dk, dv).cpu().numpy() - S) <= tol * A).all()

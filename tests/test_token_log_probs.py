@@ -267,3 +267,23 @@ def test_logits_past_four_gigabytes(gpu_ctx):
     check(te.TokenLogProbs(pick(r.log_probs, 1), pick(r.entropy, 1), pick(r.top_tokens, 2),
                            pick(r.top_log_probs, 2)), data, t[rows], 2)
     assert float((r.entropy[1:1000] - np.log(vocab)).abs().max()) < 1e-5
+
+
+@pytest.mark.gpu
+def test_more_positions_than_one_grid_has_threads_for(gpu_ctx):
+    """2^26 + 3 positions of a wavefront each: past 2^32 threads in all."""
+    import torch
+
+    n, vocab = (1 << 26) + 3, 3
+    x = torch.zeros(n, vocab, device="cuda")
+    rows = [0, (1 << 22) - 1, 1 << 22, (1 << 26) - 1, 1 << 26, n - 1]
+    data = logits(len(rows), vocab, False, seed=6)
+    x[rows] = torch.from_numpy(data).cuda()
+    tokens = torch.full((n,), 2, dtype=torch.int64, device="cuda")
+    r = te.token_log_probs(x.view(-1), tokens, n, vocab, top=1, ctx=gpu_ctx)
+    pick = lambda a: a[rows].cpu().numpy()
+    check(te.TokenLogProbs(*map(pick, r)), data, np.full((len(rows), 1), 2), 1)
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    rest[rows] = False
+    assert float((r.entropy[rest] - np.log(3)).abs().max()) < 1e-6
+    assert int(r.top_tokens[rest].max()) == 0
