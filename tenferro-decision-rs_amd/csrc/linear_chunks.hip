@@ -7,8 +7,9 @@
 //   S0  <- e^G S0 + K^T (e U)
 // Two kernels:
 //   linear_pairs_kernel  over all chunks at once: the decays, D . Q K^T and T
-//   linear_walk_kernel   along each (row, head): U, O and the state, which stays in
-//                        the accumulators from the first chunk to the last
+//   linear_delta_kernel, linear_plain_kernel  along each (row, head): U, O and the
+//                        state, which stays in the accumulators from the first chunk to
+//                        the last
 // Chunks without an active token are skipped by both.
 //
 // Products run on the bf16 matrix cores with f32 accumulation, f32 operands as
@@ -511,51 +512,93 @@ constexpr bool keys_in_place(int NI, int depth) {
   return sizeof(T) == 4 && NI <= 8 && (depth == 1 || !DELTA);
 }
 
+// The (row, head) and first value column of a workgroup with CT column tiles. Column
+// groups of a (row, head) go to one XCD (workgroups are dealt to the eight in turn)
+// and share its L2.
+struct Columns {
+  size_t rh;
+  int r, h, j;
+};
+template <int CT>
+__device__ __forceinline__ Columns columns_of(const LinearArgs &a) {
+  const unsigned groups = ((a.dv + 15) / 16 + CT - 1) / CT, heads = (unsigned)(a.rows * a.heads);
+  const unsigned set = blockIdx.x / (8 * groups), in = blockIdx.x - set * 8 * groups;
+  const unsigned width = min(8u, heads - 8 * set), cols = in / width;
+  const size_t rh = 8 * set + (in - cols * width);
+  const int r = (int)(rh / a.heads);
+  return Columns{rh, r, (int)(rh - (size_t)r * a.heads), (int)(16 * CT * cols)};
+}
+
+// A row's chunks with an active token, 64 at a time.
+struct Chunk {
+  int at;  // -1: none
+  uint64_t act;
+};
+struct ActiveChunks {
+  const uint64_t *active;
+  int nch, lane, base = -64;
+  uint64_t word = 0, live = 0;
+  __device__ __forceinline__ ActiveChunks(const uint64_t *active, int nch, int lane)
+      : active(active), nch(nch), lane(lane) {}
+  __device__ __forceinline__ Chunk next() {
+    while (!live) {
+      base += 64;
+      if (base >= nch) return Chunk{-1, 0};
+      word = base + lane < nch ? active[base + lane] : 0;
+      live = __ballot(word != 0);
+    }
+    const int b = __ffsll((unsigned long long)live) - 1;
+    live &= live - 1;
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)word, b);
+    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(word >> 32), b);
+    return Chunk{base + b, (uint64_t)hi << 32 | lo};
+  }
+};
+
+// Half of a fragment block: quad x of the lanes as pieces, half `half` of the block.
+__device__ __forceinline__ void put_half(unsigned char *block, int lane, int half, f32x4 x) {
+  const Bf16x3 p = split_bf16x3(x);
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    *reinterpret_cast<u32x2 *>(block + 1024 * i + 16 * lane + 8 * half) = p.p[i];
+}
+
 // Workgroup = four waves on CT tiles of 16 value columns of one (row, head). The waves
 // share the work of a chunk, which is what every later chunk waits for: wave w has
 // token tile w of U and O, and the feature tiles TI w .. of the state (feature
 // 16 i + 4 (lane / 16) + e, column lane % 16, in accumulators). Three times a chunk
-// (twice without the delta rule) they hand their part to the others as operand
-// pieces in LDS: the state for K S0 and Q S0, V - d K S0 for U, U for O and the
-// state. Keys, queries and triangles come as operands straight from memory into
+// they hand their part to the others as operand pieces in LDS: the state for K S0 and
+// Q S0, V - d K S0 for U, U for O and the state. Keys, queries and triangles come as operands straight from memory into
 // registers, each of its lines to one wave, and are fetched for the next chunk as
 // soon as the present one has been multiplied.
 //
-// On eight waves (delta rule) the first four are on the path from one state to the next
+// On eight waves the first four are on the path from one state to the next
 // (K S0, V - d K S0 and U), the others beside it (Q S0 and O, which nothing waits for);
 // the state's tiles are dealt to all eight. `path` and `side` are both true on four.
 //
 // What bounds it: a chunk's three exchanges follow each other, 5400 cycles in bf16 with
 // 128 x 128 and one tile, of which the products are 960; with two workgroups per CU the
 // operands, 8 TB/s out of L2.
-template <typename T, bool DELTA, int NI, int CT, int DEPTH, int WAVES>
+template <typename T, int NI, int CT, int DEPTH, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || (DEPTH == 1 && NI <= 8 && CT < 4) ? 2 : 1)
-void linear_walk_kernel(LinearArgs a, LinearWork ws) {
+void linear_delta_kernel(LinearArgs a, LinearWork ws) {
   constexpr bool kRoles = WAVES == 8;
-  static_assert(DELTA || !kRoles, "without the solve nothing is on the path but the state");
   constexpr int NP = Pieces<T>::n;
-  constexpr int NV = DELTA ? 3 : NP;  // pieces of what is written
   constexpr int NK = NI / 2, TI = NI >= WAVES ? NI / WAVES : 1;
   constexpr int SB = Pieces<T>::blocks * 1024;
-  constexpr int kPart = 4 * NK * SB, kParts = DELTA ? 3 : 2;
-  constexpr int PB = DELTA ? 2 * kTri : kTri;
-  constexpr bool kKeysPacked = !keys_in_place<T, DELTA>(NI, DEPTH);
+  constexpr int kPart = 4 * NK * SB, kParts = 3;
+  constexpr bool kKeysPacked = !keys_in_place<T, true>(NI, DEPTH);
   __shared__ __attribute__((aligned(16))) unsigned char spl[CT][NK * 3 * 1024];
-  __shared__ __attribute__((aligned(16))) unsigned char xpl[DELTA ? CT : 1][DELTA ? 6 * 1024 : 16];
-  __shared__ __attribute__((aligned(16))) unsigned char upl[CT][2 * NV * 1024], epl[CT][6 * 1024];
+  __shared__ __attribute__((aligned(16))) unsigned char xpl[CT][6 * 1024];
+  __shared__ __attribute__((aligned(16))) unsigned char upl[CT][6 * 1024], epl[CT][6 * 1024];
   const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int w = wave & 3;  // token tile
   const bool path = !kRoles || wave < 4, side = !kRoles || wave >= 4;
   const int nch = (a.L + kC - 1) / kC;
-  // Column groups of a (row, head) go to one XCD (workgroups are dealt to the
-  // eight in turn) and share its L2.
-  const unsigned groups = ((a.dv + 15) / 16 + CT - 1) / CT, heads = (unsigned)(a.rows * a.heads);
-  const unsigned set = blockIdx.x / (8 * groups), in = blockIdx.x - set * 8 * groups;
-  const unsigned width = min(8u, heads - 8 * set), cols = in / width;
-  const size_t rh = 8 * set + (in - cols * width);
-  const int r = (int)(rh / a.heads), h = (int)(rh - (size_t)r * a.heads);
-  const int jw = 16 * CT * cols;
+  const Columns col = columns_of<CT>(a);
+  const size_t rh = col.rh;
+  const int r = col.r, h = col.h, jw = col.j;
   const unsigned char *packed = ws.packed + ((size_t)r * a.key_heads + h / a.group) * nch *
                                                 ((size_t)kParts * kPart);
   // The columns of values, outputs and states.
@@ -583,13 +626,6 @@ void linear_walk_kernel(LinearArgs a, LinearWork ws) {
           S[ct][i][e] = buffer_load1(from, voff + (16 * i + e) * a.dv * 4, 0);
     }
   }
-  // Half of a fragment block: quad x of lanes is half `half` of block `block`.
-  auto put_half = [&](unsigned char *blocks, int half, f32x4 x) {
-    const Bf16x3 p = split_bf16x3(x);
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      *reinterpret_cast<u32x2 *>(blocks + 1024 * i + 16 * lane + 8 * half) = p.p[i];
-  };
   auto put_state = [&] {
     if (owner)
 #pragma unroll
@@ -597,36 +633,14 @@ void linear_walk_kernel(LinearArgs a, LinearWork ws) {
 #pragma unroll
         for (int i = 0; i < TI; ++i) {
           const int tile = TI * wave + i;
-          put_half(spl[ct] + 3072 * (tile >> 1), tile & 1, S[ct][i]);
+          put_half(spl[ct] + 3072 * (tile >> 1), lane, tile & 1, S[ct][i]);
         }
   };
 
-  // The row's chunks with an active token, 64 at a time.
-  const uint64_t *active = ws.active + (size_t)r * nch;
-  uint64_t word = 0, live = 0;
-  int base = -64;
-  struct Chunk {
-    int at;  // -1: none
-    uint64_t act;
-  };
-  auto next_chunk = [&]() -> Chunk {
-    while (!live) {
-      base += 64;
-      if (base >= nch) return Chunk{-1, 0};
-      word = base + lane < nch ? active[base + lane] : 0;
-      live = __ballot(word != 0);
-    }
-    const int b = __ffsll((unsigned long long)live) - 1;
-    live &= live - 1;
-    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)word, b);
-    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(word >> 32), b);
-    return Chunk{base + b, (uint64_t)hi << 32 | lo};
-  };
-
+  ActiveChunks chunks(ws.active + (size_t)r * nch, nch, lane);
   // What a chunk needs from memory, for DEPTH chunks.
-  constexpr bool kBoth = DELTA && !kRoles;
   struct Operands {
-    Stored<T> q[NK], k[kBoth ? NK : 1], t[TI][2];  // with roles q is the wave's of both,
+    Stored<T> q[NK], k[kRoles ? 1 : NK], t[TI][2];  // with roles q is the wave's of both,
     frag scores[2][3], solve[2][3];                // and so are the scores
     f32x4 start, end, beta;
     float whole;
@@ -638,21 +652,21 @@ void linear_walk_kernel(LinearArgs a, LinearWork ws) {
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk) {
       load_stored<T>(p + SB * kk, lane, o.q[kk]);
-      if constexpr (kBoth) load_stored<T>(p + 2 * kPart + SB * kk, lane, o.k[kk]);
+      if constexpr (!kRoles) load_stored<T>(p + 2 * kPart + SB * kk, lane, o.k[kk]);
     }
   };
   auto fetch_values = [&](Operands &o, int at) {
     const float *f = ws.factors + (rh * nch + at) * 3 * kC + 16 * w + 4 * g;
     o.start = *reinterpret_cast<const f32x4 *>(f);
     o.end = *reinterpret_cast<const f32x4 *>(f + kC);
-    if (DELTA) o.beta = *reinterpret_cast<const f32x4 *>(f + 2 * kC);
+    o.beta = *reinterpret_cast<const f32x4 *>(f + 2 * kC);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
       load_four<T>(v, path ? (row_off + at * kC + 16 * ct * a.L) * (int)sizeof(T) : kNowhere,
                    o.values[ct]);
   };
   auto fetch_tri = [&](int at, bool solve, frag (&f)[2][3]) {  // row tile w of a triangle
-    const unsigned char *p = ws.planes + (rh * nch + at) * PB + (solve ? kTri : 0);
+    const unsigned char *p = ws.planes + (rh * nch + at) * (2 * kTri) + (solve ? kTri : 0);
     load_frag<3>(p + 3072 * tri_block(w, 0), lane, f[0]);
     if (w >= 2) load_frag<3>(p + 3072 * tri_block(w, 1), lane, f[1]);
   };
@@ -676,12 +690,12 @@ void linear_walk_kernel(LinearArgs a, LinearWork ws) {
 
   Chunk next[DEPTH + 1];  // the present chunk and those behind it
 #pragma unroll
-  for (int i = 0; i <= DEPTH; ++i) next[i] = next_chunk();
+  for (int i = 0; i <= DEPTH; ++i) next[i] = chunks.next();
   auto fetch = [&](Operands &o, int at) {
     if (at < 0) return;
     fetch_rows(o, at);
     fetch_values(o, at);
-    if (kBoth) fetch_tri(at, true, o.solve);
+    if (!kRoles) fetch_tri(at, true, o.solve);
     fetch_tri(at, kRoles && path, o.scores);
     fetch_columns(o, at);
   };
@@ -702,13 +716,13 @@ void linear_walk_kernel(LinearArgs a, LinearWork ws) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) load_frag<3>(spl[ct] + 3072 * kk, lane, s[ct]);
       to_frag<T>(o.q[kk], qf);
-      if constexpr (kBoth) to_frag<T>(o.k[kk], kf);
+      if constexpr (!kRoles) to_frag<T>(o.k[kk], kf);
       typedef Products<NP, 3> P;
 #pragma unroll
       for (int x = 0; x < P::n; ++x)
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-          if constexpr (kBoth)
+          if constexpr (!kRoles)
             X[ct][kk & 1] = mfma_16x16x32_bf16(kf[P::a(x)], s[ct][P::b(x)], X[ct][kk & 1]);
           O[ct][kk & 1] = mfma_16x16x32_bf16(qf[P::a(x)], s[ct][P::b(x)], O[ct][kk & 1]);
         }
@@ -722,41 +736,32 @@ void linear_walk_kernel(LinearArgs a, LinearWork ws) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) U[ct][e] = (on >> e) & 1u ? given[e] : 0.0f;
       O[ct][0] = o.start * (O[ct][0] + O[ct][1]);
-      if constexpr (DELTA) {
-        const f32x4 x = kRoles ? O[ct][0] : o.start * (X[ct][0] + X[ct][1]);
-        if (path) put_half(xpl[ct] + 3072 * (w >> 1), w & 1, o.beta * (U[ct] - x));
-      }
+      const f32x4 x = kRoles ? O[ct][0] : o.start * (X[ct][0] + X[ct][1]);
+      if (path) put_half(xpl[ct] + 3072 * (w >> 1), lane, w & 1, o.beta * (U[ct] - x));
     }
-    if constexpr (DELTA) {
-      lds_barrier();
+    lds_barrier();
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) U[ct] = f32x4{};
+    for (int ct = 0; ct < CT; ++ct) U[ct] = f32x4{};
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        if (!path || (ks && w < 2)) continue;
-        frag x[CT][3];
+    for (int ks = 0; ks < 2; ++ks) {
+      if (!path || (ks && w < 2)) continue;
+      frag x[CT][3];
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) load_frag<3>(xpl[ct] + 3072 * ks, lane, x[ct]);
-        typedef Products<3, 3> P;
+      for (int ct = 0; ct < CT; ++ct) load_frag<3>(xpl[ct] + 3072 * ks, lane, x[ct]);
+      typedef Products<3, 3> P;
 #pragma unroll
-        for (int i = 0; i < P::n; ++i)
+      for (int i = 0; i < P::n; ++i)
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
-            U[ct] = mfma_16x16x32_bf16((kRoles ? o.scores : o.solve)[ks][P::a(i)], x[ct][P::b(i)],
-                                       U[ct]);
-      }
-      if constexpr (kBoth) fetch_tri(far, true, o.solve);
+        for (int ct = 0; ct < CT; ++ct)
+          U[ct] = mfma_16x16x32_bf16((kRoles ? o.scores : o.solve)[ks][P::a(i)], x[ct][P::b(i)],
+                                     U[ct]);
     }
+    if constexpr (!kRoles) fetch_tri(far, true, o.solve);
     if (path)
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        if constexpr (NV == 3) {
-          put_half(upl[ct] + 3072 * (w >> 1), w & 1, U[ct]);
-        } else {  // exact: the values are bf16
-          *reinterpret_cast<u32x2 *>(upl[ct] + 1024 * (w >> 1) + 16 * lane + 8 * (w & 1)) =
-              __builtin_bit_cast(u32x2, __builtin_convertvector(U[ct], bf16x4));
-        }
-        put_half(epl[ct] + 3072 * (w >> 1), w & 1, U[ct] * o.end);
+        put_half(upl[ct] + 3072 * (w >> 1), lane, w & 1, U[ct]);
+        put_half(epl[ct] + 3072 * (w >> 1), lane, w & 1, U[ct] * o.end);
       }
     const float decay = o.whole;
     lds_barrier();
@@ -796,10 +801,10 @@ void linear_walk_kernel(LinearArgs a, LinearWork ws) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       if (!side || (ks && w < 2)) continue;
-      frag u[CT][NV];
+      frag u[CT][3];
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) load_frag<NV>(upl[ct] + 1024 * NV * ks, lane, u[ct]);
-      typedef Products<3, NV> P;
+      for (int ct = 0; ct < CT; ++ct) load_frag<3>(upl[ct] + 3072 * ks, lane, u[ct]);
+      typedef Products<3, 3> P;
 #pragma unroll
       for (int x = 0; x < P::n; ++x)
 #pragma unroll
@@ -824,7 +829,7 @@ void linear_walk_kernel(LinearArgs a, LinearWork ws) {
     if (!kRoles) lds_barrier();
 #pragma unroll
     for (int i = 0; i < DEPTH; ++i) next[i] = next[i + 1];
-    next[DEPTH] = next_chunk();
+    next[DEPTH] = chunks.next();
   };
   while (next[0].at >= 0) {
     walk(even);
@@ -847,27 +852,270 @@ void linear_walk_kernel(LinearArgs a, LinearWork ws) {
   }
 }
 
+// Without the delta rule the state needs no product with itself: S <- e^G S + K^T (e U)
+// with U = V is a chain of products in the accumulators, and only Q S0 reads it from LDS.
+// Workgroup = eight waves on CT column tiles, one barrier a chunk, what they hand over
+// in two buffers. Waves 0 to 3 have the feature tiles TI w .. of the state, and put it and
+// token tile w of U and e U of the next chunk into LDS; waves 4 to 7 have token tile w
+// of Q S0 and of O. (On four waves that did both, with two barriers: 3 x 777 tokens with 6
+// heads of 96 x 80 48 us, now 38; 2 x 8192 with 16 heads of 128 x 128 442, now 400, in bf16
+// 307, now 269; 8 x 1024 with 8 heads of 256 x 256 231, now 194.)
+// Bound by the operands' way through L2 and LDS: 2 x 8192 in bf16 move 540 MB in and
+// out of both kernels, 2 TB/s.
+template <typename T, int NI, int CT>
+__global__ __launch_bounds__(512, 2) void linear_plain_kernel(LinearArgs a, LinearWork ws) {
+  constexpr int NP = Pieces<T>::n, NK = NI / 2, TI = NI >= 4 ? NI / 4 : 1;
+  constexpr int SB = Pieces<T>::blocks * 1024, kPart = 4 * NK * SB, kParts = 2;
+  constexpr bool kKeysPacked = !keys_in_place<T, false>(NI, 1);
+  __shared__ __attribute__((aligned(16))) unsigned char spl[2][CT][NK * 3 * 1024];
+  __shared__ __attribute__((aligned(16))) unsigned char upl[2][CT][2 * NP * 1024];
+  __shared__ __attribute__((aligned(16))) unsigned char epl[2][CT][6 * 1024];
+  const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
+  const int nch = (a.L + kC - 1) / kC;
+  const Columns col = columns_of<CT>(a);
+  const size_t rh = col.rh, kh = (size_t)col.r * a.key_heads + col.h / a.group;
+  const unsigned char *packed = ws.packed + kh * nch * ((size_t)kParts * kPart);
+  const float *factors = ws.factors + rh * nch * 3 * kC;
+  const uint32_t mine = (uint32_t)min(16 * CT, a.dv - col.j) * a.L;
+  const size_t col0 = (rh * a.dv + col.j) * a.L;
+  const int row_off = c16 * a.L + 16 * w + 4 * g;  // elements: the lane's column and first token
+  ActiveChunks chunks(ws.active + (size_t)col.r * nch, nch, lane);
+  Chunk cur = chunks.next(), next = chunks.next();
+  // Behind the last chunk its operands come again, for nothing: a branch around the
+  // loads makes the compiler wait for them at its end.
+  int ahead = next.at >= 0 ? next.at : cur.at;
+  auto advance = [&] {
+    cur = next;
+    next = chunks.next();
+    if (next.at >= 0) ahead = next.at;
+  };
+
+  if (wave < 4) {
+    const Rsrc v = buffer_rsrc(static_cast<const T *>(a.v) + col0, mine * sizeof(T));
+    const Rsrc keys = buffer_rsrc(static_cast<const T *>(a.k) + kh * a.dk * a.L,
+                                  (uint32_t)a.dk * a.L * sizeof(T));
+    const uint32_t state_bytes = (uint32_t)a.dk * a.dv * 4;
+    const bool owner = TI * w < NI;
+    const int tile0 = TI * w;
+    f32x4 S[CT][TI] = {};
+    auto state_off = [&](int ct) {
+      const int j = col.j + 16 * ct + c16;
+      return j < a.dv ? ((16 * tile0 + 4 * g) * a.dv + j) * 4 : kNowhere;
+    };
+    if (a.state_in && owner) {
+      const Rsrc from = buffer_rsrc(a.state_in + rh * a.dk * a.dv, state_bytes);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int i = 0; i < TI; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            S[ct][i][e] = buffer_load1(from, state_off(ct) + (16 * i + e) * a.dv * 4, 0);
+    }
+    struct Keys {
+      Stored<T> t[TI][2];
+      float whole;
+    } o;
+    struct Values {
+      f32x4 end;
+      Four<T> v[CT];
+    } x;
+    auto fetch_keys = [&](int at) {
+      o.whole = factors[(size_t)at * 3 * kC + kC - 1];
+      if (!owner) return;
+      const unsigned char *p = packed + (size_t)at * (kParts * kPart) + kPart + 2 * SB * tile0;
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          if constexpr (kKeysPacked) {
+            load_stored<T>(p + SB * (2 * i + ks), lane, o.t[i][ks]);
+          } else {
+            const int off = ((16 * (tile0 + i) + c16) * a.L + at * kC + 32 * ks + 4 * g) * 4;
+            o.t[i][ks].b[0] = buffer_load4(keys, off, 0);
+            o.t[i][ks].b[1] = buffer_load4(keys, off + 64, 0);
+          }
+        }
+    };
+    auto fetch_values = [&](int at) {
+      x.end = *reinterpret_cast<const f32x4 *>(factors + (size_t)at * 3 * kC + kC + 16 * w + 4 * g);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+        load_four<T>(v, (row_off + at * kC + 16 * ct * a.L) * (int)sizeof(T), x.v[ct]);
+    };
+    auto put_state = [&](int b) {
+      if (owner)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int i = 0; i < TI; ++i)
+            put_half(spl[b][ct] + 3072 * ((tile0 + i) >> 1), lane, (tile0 + i) & 1, S[ct][i]);
+    };
+    auto put_values = [&](int b, uint64_t act) {
+      const unsigned on = (unsigned)(act >> (16 * w + 4 * g));
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        f32x4 u = values_of<T>(x.v[ct]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] = (on >> e) & 1u ? u[e] : 0.0f;
+        if constexpr (NP == 3)
+          put_half(upl[b][ct] + 3072 * (w >> 1), lane, w & 1, u);
+        else  // exact: the values are bf16
+          *reinterpret_cast<u32x2 *>(upl[b][ct] + 1024 * (w >> 1) + 16 * lane + 8 * (w & 1)) =
+              __builtin_bit_cast(u32x2, __builtin_convertvector(u, bf16x4));
+        put_half(epl[b][ct] + 3072 * (w >> 1), lane, w & 1, u * x.end);
+      }
+    };
+    auto walk = [&](int b) {
+      frag tf[TI][2][NP];
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          if constexpr (!kKeysPacked) drop_inactive(cur.act, ks, g, o.t[i][ks].b);
+          to_frag<T>(o.t[i][ks], tf[i][ks]);
+        }
+      const float decay = o.whole;
+      fetch_keys(ahead);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        frag e[2][3];
+        load_frag<3>(epl[b][ct], lane, e[0]);
+        load_frag<3>(epl[b][ct] + 3072, lane, e[1]);
+        typedef Products<NP, 3> P;
+#pragma unroll
+        for (int i = 0; i < TI; ++i) S[ct][i] *= decay;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int p = 0; p < P::n; ++p)
+#pragma unroll
+            for (int i = 0; i < TI; ++i)
+              S[ct][i] = mfma_16x16x32_bf16(tf[i][ks][P::a(p)], e[ks][P::b(p)], S[ct][i]);
+      }
+      put_values(b ^ 1, next.act);
+      advance();
+      fetch_values(ahead);
+      put_state(b ^ 1);
+      lds_barrier();
+    };
+    if (cur.at >= 0) {
+      fetch_values(cur.at);
+      fetch_keys(cur.at);
+      put_values(0, cur.act);
+      fetch_values(ahead);
+    }
+    put_state(0);
+    lds_barrier();
+    for (int b = 0; cur.at >= 0; b ^= 1) walk(b);
+    if (a.state_out && owner) {
+      const Rsrc to = buffer_rsrc(a.state_out + rh * a.dk * a.dv, state_bytes);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int i = 0; i < TI; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            buffer_store1(S[ct][i][e], to, state_off(ct) + (16 * i + e) * a.dv * 4, 0);
+    }
+  } else {
+    const Rsrc out = buffer_rsrc(a.out + col0, mine * 4);
+    struct Queries {
+      Stored<T> q[NK];
+      frag scores[2][3];
+      f32x4 start;
+    } o;
+    auto fetch_rows = [&](int at) {
+      const unsigned char *p = packed + (size_t)at * (kParts * kPart) + SB * NK * w;
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) load_stored<T>(p + SB * kk, lane, o.q[kk]);
+      o.start = *reinterpret_cast<const f32x4 *>(factors + (size_t)at * 3 * kC + 16 * w + 4 * g);
+    };
+    auto fetch_scores = [&](int at) {
+      const unsigned char *p = ws.planes + (rh * nch + at) * kTri;
+      load_frag<3>(p + 3072 * tri_block(w, 0), lane, o.scores[0]);
+      if (w >= 2) load_frag<3>(p + 3072 * tri_block(w, 1), lane, o.scores[1]);
+    };
+    auto walk = [&](int b) {
+      f32x4 O[CT][2] = {};  // even and odd steps in accumulators of their own
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) {
+        frag s[CT][3], f[NP];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) load_frag<3>(spl[b][ct] + 3072 * kk, lane, s[ct]);
+        to_frag<T>(o.q[kk], f);
+        typedef Products<NP, 3> P;
+#pragma unroll
+        for (int p = 0; p < P::n; ++p)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+            O[ct][kk & 1] = mfma_16x16x32_bf16(f[P::a(p)], s[ct][P::b(p)], O[ct][kk & 1]);
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) O[ct][0] = o.start * (O[ct][0] + O[ct][1]);
+      fetch_rows(ahead);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        if (ks && w < 2) continue;
+        frag u[CT][NP];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) load_frag<NP>(upl[b][ct] + 1024 * NP * ks, lane, u[ct]);
+        typedef Products<3, NP> P;
+#pragma unroll
+        for (int p = 0; p < P::n; ++p)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+            O[ct][0] = mfma_16x16x32_bf16(o.scores[ks][P::a(p)], u[ct][P::b(p)], O[ct][0]);
+      }
+      fetch_scores(ahead);
+      const int t0 = cur.at * kC, n = a.L - t0 - 16 * w - 4 * g;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const int off = (row_off + t0 + 16 * ct * a.L) * 4;
+        const f32x4 y = O[ct][0] * a.scale;
+        if (t0 + kC <= a.L) {
+          buffer_store4(y, out, off, 0);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) buffer_store1(y[e], out, e < n ? off + 4 * e : kNowhere, 0);
+        }
+      }
+      lds_barrier();
+      advance();
+    };
+    if (cur.at >= 0) {
+      fetch_rows(cur.at);
+      fetch_scores(cur.at);
+    }
+    lds_barrier();
+    for (int b = 0; cur.at >= 0; b ^= 1) walk(b);
+  }
+}
+
 // Column tiles per workgroup, its waves and chunks fetched ahead, by how the grid fills
 // the CUs (us for prompts of 512 tokens, 16 heads of 128 x 128 unless stated, both
-// kernels):
+// kernels). With the delta rule
 //   one tile each if every workgroup then has a CU to itself, and two chunks ahead as
-//   far as 512 registers hold them: nothing else hides the latency there. The f32 delta
-//   rule, whose products and splitting are the path, on eight waves (1 x 4096: 215, four
-//   261; in bf16 2 x 8192: 433, four 416, where reading the state twice costs more);
+//   far as 512 registers hold them: nothing else hides the latency there. f32, whose
+//   products and splitting are the path, on eight waves (1 x 4096: 215, four 261; in
+//   bf16 2 x 8192: 433, four 416, where reading the state twice costs more);
 //   one tile each while two workgroups per CU hold all (4 rows: 72 us, two tiles 91,
 //   four 84), except f32 keys over 128 wide, whose operands leave room for one;
 //   beyond that every operand is loaded and split for more columns at once: four
-//   tiles for the f32 delta rule with keys of 65 to 128 (8 rows: 119 us, two tiles 154,
-//   which spill, one 147; 16 rows: 231, 343, 304), where the splitting weighs most,
-//   two tiles otherwise (8 rows in bf16: 79 us, four tiles 89, one 91; 32 rows of
-//   32 x 32 f32: 145, 161, 159; 16 rows of 64 x 64 f32: 106, 110, 125; 4 x 1024 with 8
-//   heads of 256 x 256 f32: 145 on eight waves, 171 on four).
+//   tiles for f32 keys of 65 to 128 (8 rows: 119 us, two tiles 154, which spill, one
+//   147; 16 rows: 231, 343, 304), where the splitting weighs most, two tiles otherwise
+//   (8 rows in bf16: 79 us, four tiles 89, one 91; 32 rows of 32 x 32 f32: 145, 161,
+//   159; 16 rows of 64 x 64 f32: 106, 110, 125; 4 x 1024 with 8 heads of 256 x 256 f32:
+//   145 on eight waves, 171 on four).
+// Without it one tile each if every workgroup has a CU to itself (2 x 8192: 404 us, two
+// tiles 448; bf16 275 and 355), else two (4 rows: 43, one 51; 16 rows: 167, 195; 8 x 1024
+// with 8 heads of 256 x 256 bf16: 111, 124); two chunks ahead brought nothing.
 template <typename T, bool DELTA, int NI>
 hipError_t launch(const LinearArgs &a, const LinearWork &ws, hipStream_t stream,
                   const KernelEvents &ev) {
   constexpr bool f32 = sizeof(T) == 4, wide = f32 && NI > 8;
-  constexpr int kAhead = wide ? 1 : 2, kTiles = f32 && DELTA && NI == 8 ? 4 : 2;
-  constexpr int kFewWaves = f32 && DELTA ? 8 : 4, kWideWaves = wide && DELTA ? 8 : 4;
+  constexpr int kAhead = DELTA && !wide ? 2 : 1, kTiles = f32 && DELTA && NI == 8 ? 4 : 2;
   const size_t jtiles = (size_t)((a.dv + 15) / 16), heads = (size_t)a.rows * a.heads;
   const size_t one = heads * jtiles, many = heads * ((jtiles + kTiles - 1) / kTiles);
   const bool few = one <= (size_t)a.cus;
@@ -883,11 +1131,16 @@ hipError_t launch(const LinearArgs &a, const LinearWork &ws, hipStream_t stream,
                           ev.stop, 0, a, ws);
     return hipGetLastError();
   };
-  if (few) return walk(linear_walk_kernel<T, DELTA, NI, 1, kAhead, kFewWaves>, kFewWaves, one);
-  if constexpr (!wide)
-    if (one <= 2 * (size_t)a.cus)
-      return walk(linear_walk_kernel<T, DELTA, NI, 1, 1, 4>, 4, one);
-  return walk(linear_walk_kernel<T, DELTA, NI, kTiles, 1, kWideWaves>, kWideWaves, many);
+  if constexpr (DELTA) {
+    constexpr int kFewWaves = f32 ? 8 : 4, kManyWaves = wide ? 8 : 4;
+    if (few) return walk(linear_delta_kernel<T, NI, 1, kAhead, kFewWaves>, kFewWaves, one);
+    if constexpr (!wide)
+      if (one <= 2 * (size_t)a.cus) return walk(linear_delta_kernel<T, NI, 1, 1, 4>, 4, one);
+    return walk(linear_delta_kernel<T, NI, kTiles, 1, kManyWaves>, kManyWaves, many);
+  } else {
+    if (few) return walk(linear_plain_kernel<T, NI, 1>, 8, one);
+    return walk(linear_plain_kernel<T, NI, kTiles>, 8, many);
+  }
 }
 
 template <typename T, bool DELTA>
