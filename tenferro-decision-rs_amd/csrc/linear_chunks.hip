@@ -503,13 +503,13 @@ __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearW
 
 // f32 keys of up to 128 features are read by features where they are, whole lines of
 // 32 tokens each (16 rows of 1024 tokens, 16 heads of 128 x 128: 404 us, packed 438; 8 x
-// 2048 with 16 heads of 64 x 64: 235, 256; plain 2 x 8192: 449, 477). The delta rule with
-// a workgroup per CU, which waits for every byte, and keys of more features take packed
-// ones (1 x 4096 on four waves: 260, in place 263; 4 x 1024 with 8 heads of 256 x 256 on 2 key
-// heads: 169, 179).
-template <typename T, bool DELTA>
-constexpr bool keys_in_place(int NI, int depth) {
-  return sizeof(T) == 4 && NI <= 8 && (depth == 1 || !DELTA);
+// 2048 with 16 heads of 64 x 64: 235, 256; plain 2 x 8192: 449, 477; only the delta rule
+// on a small grid, 3 x 777 with 6 heads of 96 x 80, prefers packed ones, 56 against 59).
+// Keys of more features take packed ones (4 x 1024 with 8 heads of 256 x 256 on 2 key
+// heads: 169, in place 179).
+template <typename T>
+constexpr bool keys_in_place(int NI) {
+  return sizeof(T) == 4 && NI <= 8;
 }
 
 // The (row, head) and first value column of a workgroup with CT column tiles. Column
@@ -579,15 +579,15 @@ __device__ __forceinline__ void put_half(unsigned char *block, int lane, int hal
 // What bounds it: a chunk's three exchanges follow each other, 5400 cycles in bf16 with
 // 128 x 128 and one tile, of which the products are 960; with two workgroups per CU the
 // operands, 8 TB/s out of L2.
-template <typename T, int NI, int CT, int DEPTH, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 8 || (DEPTH == 1 && NI <= 8 && CT < 4) ? 2 : 1)
+template <typename T, int NI, int CT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 || (NI <= 8 && CT < 4) ? 2 : 1)
 void linear_delta_kernel(LinearArgs a, LinearWork ws) {
   constexpr bool kRoles = WAVES == 8;
   constexpr int NP = Pieces<T>::n;
   constexpr int NK = NI / 2, TI = NI >= WAVES ? NI / WAVES : 1;
   constexpr int SB = Pieces<T>::blocks * 1024;
   constexpr int kPart = 4 * NK * SB, kParts = 3;
-  constexpr bool kKeysPacked = !keys_in_place<T, true>(NI, DEPTH);
+  constexpr bool kKeysPacked = !keys_in_place<T>(NI);
   __shared__ __attribute__((aligned(16))) unsigned char spl[CT][NK * 3 * 1024];
   __shared__ __attribute__((aligned(16))) unsigned char xpl[CT][6 * 1024];
   __shared__ __attribute__((aligned(16))) unsigned char upl[CT][6 * 1024], epl[CT][6 * 1024];
@@ -638,15 +638,15 @@ void linear_delta_kernel(LinearArgs a, LinearWork ws) {
   };
 
   ActiveChunks chunks(ws.active + (size_t)r * nch, nch, lane);
-  // What a chunk needs from memory, for DEPTH chunks.
+  // What a chunk needs from memory.
   struct Operands {
     Stored<T> q[NK], k[kRoles ? 1 : NK], t[TI][2];  // with roles q is the wave's of both,
     frag scores[2][3], solve[2][3];                // and so are the scores
     f32x4 start, end, beta;
     float whole;
     Four<T> values[CT];
-  } even, odd;
-  auto fetch_rows = [&](Operands &o, int at) {  // token tile `wave` of queries and keys
+  } o;
+  auto fetch_rows = [&](int at) {  // token tile `wave` of queries and keys
     const unsigned char *p = packed + (size_t)at * (kParts * kPart) + SB * NK * w;
     if (kRoles && path) p += 2 * kPart;
 #pragma unroll
@@ -655,7 +655,7 @@ void linear_delta_kernel(LinearArgs a, LinearWork ws) {
       if constexpr (!kRoles) load_stored<T>(p + 2 * kPart + SB * kk, lane, o.k[kk]);
     }
   };
-  auto fetch_values = [&](Operands &o, int at) {
+  auto fetch_values = [&](int at) {
     const float *f = ws.factors + (rh * nch + at) * 3 * kC + 16 * w + 4 * g;
     o.start = *reinterpret_cast<const f32x4 *>(f);
     o.end = *reinterpret_cast<const f32x4 *>(f + kC);
@@ -670,7 +670,7 @@ void linear_delta_kernel(LinearArgs a, LinearWork ws) {
     load_frag<3>(p + 3072 * tri_block(w, 0), lane, f[0]);
     if (w >= 2) load_frag<3>(p + 3072 * tri_block(w, 1), lane, f[1]);
   };
-  auto fetch_columns = [&](Operands &o, int at) {  // the owned feature tiles of the keys
+  auto fetch_columns = [&](int at) {  // the owned feature tiles of the keys
     o.whole = ws.factors[(rh * nch + at) * 3 * kC + kC - 1];
     if (!owner) return;
     const unsigned char *p = packed + (size_t)at * (kParts * kPart) + kPart + 2 * SB * TI * wave;
@@ -688,26 +688,20 @@ void linear_delta_kernel(LinearArgs a, LinearWork ws) {
       }
   };
 
-  Chunk next[DEPTH + 1];  // the present chunk and those behind it
-#pragma unroll
-  for (int i = 0; i <= DEPTH; ++i) next[i] = chunks.next();
-  auto fetch = [&](Operands &o, int at) {
-    if (at < 0) return;
-    fetch_rows(o, at);
-    fetch_values(o, at);
-    if (!kRoles) fetch_tri(at, true, o.solve);
-    fetch_tri(at, kRoles && path, o.scores);
-    fetch_columns(o, at);
-  };
-  fetch(even, next[0].at);
-  if (DEPTH == 2) fetch(odd, next[1].at);
+  Chunk cur = chunks.next(), next = chunks.next();
+  if (cur.at >= 0) {
+    fetch_rows(cur.at);
+    fetch_values(cur.at);
+    if (!kRoles) fetch_tri(cur.at, true, o.solve);
+    fetch_tri(cur.at, kRoles && path, o.scores);
+    fetch_columns(cur.at);
+  }
   put_state();
   lds_barrier();
-  auto walk = [&](Operands &o) {
-    const Chunk cur = next[0];
-    // Behind the last chunk the present one's operands come again, for nothing: a
-    // branch around the loads makes the compiler wait for them at its end.
-    const int far = next[DEPTH].at >= 0 ? next[DEPTH].at : cur.at;
+  while (cur.at >= 0) {
+    // Behind the last chunk its operands come again, for nothing: a branch around the
+    // loads makes the compiler wait for them at its end.
+    const int far = next.at >= 0 ? next.at : cur.at;
     // Q S0 and K S0, even and odd steps in accumulators of their own.
     f32x4 X[CT][2] = {}, O[CT][2] = {};
 #pragma unroll
@@ -727,7 +721,7 @@ void linear_delta_kernel(LinearArgs a, LinearWork ws) {
           O[ct][kk & 1] = mfma_16x16x32_bf16(qf[P::a(x)], s[ct][P::b(x)], O[ct][kk & 1]);
         }
     }
-    fetch_rows(o, far);
+    fetch_rows(far);
     f32x4 U[CT];
     const unsigned on = (unsigned)(cur.act >> (16 * w + 4 * g));
 #pragma unroll
@@ -765,7 +759,7 @@ void linear_delta_kernel(LinearArgs a, LinearWork ws) {
       }
     const float decay = o.whole;
     lds_barrier();
-    fetch_values(o, far);
+    fetch_values(far);
     // The state first: the next chunk waits for it.
     if (owner) {
       frag tf[TI][2][NP];
@@ -793,7 +787,7 @@ void linear_delta_kernel(LinearArgs a, LinearWork ws) {
               S[ct][i] = mfma_16x16x32_bf16(tf[i][ks][P::a(x)], e[ks][P::b(x)], S[ct][i]);
       }
     }
-    fetch_columns(o, far);
+    fetch_columns(far);
     if (kRoles) {  // only the side waits for what comes next
       put_state();
       lds_barrier();
@@ -827,15 +821,8 @@ void linear_delta_kernel(LinearArgs a, LinearWork ws) {
       }
     }
     if (!kRoles) lds_barrier();
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i) next[i] = next[i + 1];
-    next[DEPTH] = chunks.next();
-  };
-  while (next[0].at >= 0) {
-    walk(even);
-    if (DEPTH == 1) continue;
-    if (next[0].at < 0) break;
-    walk(odd);
+    cur = next;
+    next = chunks.next();
   }
   if (a.state_out && owner) {
     const Rsrc to = buffer_rsrc(a.state_out + rh * a.dk * a.dv, state_bytes);
@@ -849,6 +836,280 @@ void linear_delta_kernel(LinearArgs a, LinearWork ws) {
         for (int e = 0; e < 4; ++e)
           buffer_store1(S[ct][i][e], to, voff + (16 * i + e) * a.dv * 4, 0);
     }
+  }
+}
+
+// The delta rule with every wave at one kind of work, for grids that leave a CU to one
+// workgroup: waves 0 to 3 are on the path from one state to the next (token tile w of
+// K S0, of V - d K S0 and of U, feature tiles TI w .. of the state), waves 4 to 7 are a
+// chunk behind them with token tile w of Q S0 and O, between the barriers of the path.
+// The state and U are in two buffers for that. Sums on the path run in several
+// accumulators, whose latency nothing else hides.
+// Against four waves that do both, two chunks ahead (us): bf16, 16 heads of 128 x 128, 2 x
+// 8192 tokens 394 and 417, 1 x 4096 153 and 165; f32 4 x 512 on two tiles 59 and 73.
+template <typename T, int NI, int CT>
+__global__ __launch_bounds__(512, 2) void linear_delta_path_kernel(LinearArgs a, LinearWork ws) {
+  constexpr int NP = Pieces<T>::n, NK = NI / 2, TI = NI >= 4 ? NI / 4 : 1;
+  constexpr int SB = Pieces<T>::blocks * 1024, kPart = 4 * NK * SB, kParts = 3;
+  constexpr bool kKeysPacked = !keys_in_place<T>(NI);
+  __shared__ __attribute__((aligned(16))) unsigned char spl[2][CT][NK * 3 * 1024];
+  __shared__ __attribute__((aligned(16))) unsigned char xpl[CT][6 * 1024], epl[CT][6 * 1024];
+  __shared__ __attribute__((aligned(16))) unsigned char upl[2][CT][6 * 1024];
+  const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
+  const int nch = (a.L + kC - 1) / kC;
+  const Columns col = columns_of<CT>(a);
+  const size_t rh = col.rh, kh = (size_t)col.r * a.key_heads + col.h / a.group;
+  const unsigned char *packed = ws.packed + kh * nch * ((size_t)kParts * kPart);
+  const unsigned char *planes = ws.planes + rh * nch * (2 * kTri);
+  const float *factors = ws.factors + rh * nch * 3 * kC + 16 * w + 4 * g;
+  const uint32_t mine = (uint32_t)min(16 * CT, a.dv - col.j) * a.L;
+  const size_t col0 = (rh * a.dv + col.j) * a.L;
+  const int row_off = c16 * a.L + 16 * w + 4 * g;  // elements: the lane's column and first token
+  ActiveChunks chunks(ws.active + (size_t)col.r * nch, nch, lane);
+  Chunk cur = chunks.next(), next = chunks.next();
+  // Behind the last chunk its operands come again, for nothing: a branch around the
+  // loads makes the compiler wait for them at its end.
+  int ahead = next.at >= 0 ? next.at : cur.at;
+  auto advance = [&] {
+    cur = next;
+    next = chunks.next();
+    if (next.at >= 0) ahead = next.at;
+  };
+  // The wave's token tile of keys or queries, and of the solve operand or the scores.
+  Stored<T> rows[NK];
+  frag tri[2][3];
+  f32x4 start;
+  auto fetch_rows = [&](int at, int part) {
+    const unsigned char *p = packed + (size_t)at * (kParts * kPart) + part * kPart + SB * NK * w;
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) load_stored<T>(p + SB * kk, lane, rows[kk]);
+  };
+  auto fetch_tri = [&](int at, int which) {
+    const unsigned char *p = planes + (size_t)at * (2 * kTri) + which * kTri;
+    load_frag<3>(p + 3072 * tri_block(w, 0), lane, tri[0]);
+    if (w >= 2) load_frag<3>(p + 3072 * tri_block(w, 1), lane, tri[1]);
+  };
+  constexpr int XA = CT == 1 && NK >= 4 ? 4 : 2;
+  auto times_state = [&](int b, f32x4 (&Y)[CT]) {
+    f32x4 X[CT][XA] = {};
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) {
+      frag s[CT][3], f[NP];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) load_frag<3>(spl[b][ct] + 3072 * kk, lane, s[ct]);
+      to_frag<T>(rows[kk], f);
+      typedef Products<NP, 3> P;
+#pragma unroll
+      for (int p = 0; p < P::n; ++p)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+          X[ct][kk % XA] = mfma_16x16x32_bf16(f[P::a(p)], s[ct][P::b(p)], X[ct][kk % XA]);
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      Y[ct] = X[ct][0] + X[ct][1];
+      if constexpr (XA == 4) Y[ct] += X[ct][2] + X[ct][3];
+    }
+  };
+  auto add_times_tri = [&](const unsigned char (*from)[6 * 1024], f32x4 (&U)[CT]) {
+    f32x4 A[2][CT] = {};
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      if (ks && w < 2) continue;
+      frag x[CT][3];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) load_frag<3>(from[ct] + 3072 * ks, lane, x[ct]);
+      typedef Products<3, 3> P;
+#pragma unroll
+      for (int p = 0; p < P::n; ++p)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+          A[ks][ct] = mfma_16x16x32_bf16(tri[ks][P::a(p)], x[ct][P::b(p)], A[ks][ct]);
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) U[ct] += A[0][ct] + A[1][ct];
+  };
+
+  if (wave < 4) {
+    const Rsrc v = buffer_rsrc(static_cast<const T *>(a.v) + col0, mine * sizeof(T));
+    const Rsrc keys = buffer_rsrc(static_cast<const T *>(a.k) + kh * a.dk * a.L,
+                                  (uint32_t)a.dk * a.L * sizeof(T));
+    const uint32_t state_bytes = (uint32_t)a.dk * a.dv * 4;
+    const bool owner = TI * w < NI;
+    const int tile0 = TI * w;
+    f32x4 S[CT][TI] = {};
+    auto state_off = [&](int ct) {
+      const int j = col.j + 16 * ct + c16;
+      return j < a.dv ? ((16 * tile0 + 4 * g) * a.dv + j) * 4 : kNowhere;
+    };
+    if (a.state_in && owner) {
+      const Rsrc from = buffer_rsrc(a.state_in + rh * a.dk * a.dv, state_bytes);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int i = 0; i < TI; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            S[ct][i][e] = buffer_load1(from, state_off(ct) + (16 * i + e) * a.dv * 4, 0);
+    }
+    Stored<T> t[TI][2];
+    Four<T> values[CT];
+    f32x4 end, beta;
+    float whole;
+    auto fetch_keys = [&](int at) {
+      whole = ws.factors[(rh * nch + at) * 3 * kC + kC - 1];
+      if (!owner) return;
+      const unsigned char *p = packed + (size_t)at * (kParts * kPart) + kPart + 2 * SB * tile0;
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          if constexpr (kKeysPacked) {
+            load_stored<T>(p + SB * (2 * i + ks), lane, t[i][ks]);
+          } else {
+            const int off = ((16 * (tile0 + i) + c16) * a.L + at * kC + 32 * ks + 4 * g) * 4;
+            t[i][ks].b[0] = buffer_load4(keys, off, 0);
+            t[i][ks].b[1] = buffer_load4(keys, off + 64, 0);
+          }
+        }
+    };
+    auto fetch_values = [&](int at) {
+      start = *reinterpret_cast<const f32x4 *>(factors + (size_t)at * 3 * kC);
+      beta = *reinterpret_cast<const f32x4 *>(factors + (size_t)at * 3 * kC + 2 * kC);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+        load_four<T>(v, (row_off + at * kC + 16 * ct * a.L) * (int)sizeof(T), values[ct]);
+    };
+    auto fetch_end = [&](int at) {
+      end = *reinterpret_cast<const f32x4 *>(factors + (size_t)at * 3 * kC + kC);
+    };
+    auto put_state = [&](int b) {
+      if (owner)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int i = 0; i < TI; ++i)
+            put_half(spl[b][ct] + 3072 * ((tile0 + i) >> 1), lane, (tile0 + i) & 1, S[ct][i]);
+    };
+    if (cur.at >= 0) {
+      fetch_rows(cur.at, 2);
+      fetch_values(cur.at);
+      fetch_tri(cur.at, 1);
+      fetch_end(cur.at);
+      fetch_keys(cur.at);
+    }
+    put_state(0);
+    lds_barrier();
+    for (int b = 0; cur.at >= 0; b ^= 1) {
+      f32x4 X[CT], U[CT] = {};
+      times_state(b, X);
+      fetch_rows(ahead, 2);
+      const unsigned on = (unsigned)(cur.act >> (16 * w + 4 * g));
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        f32x4 u = values_of<T>(values[ct]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] = (on >> e) & 1u ? u[e] : 0.0f;
+        put_half(xpl[ct] + 3072 * (w >> 1), lane, w & 1, beta * (u - start * X[ct]));
+      }
+      lds_barrier();
+      fetch_values(ahead);
+      add_times_tri(xpl, U);
+      fetch_tri(ahead, 1);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        put_half(epl[ct] + 3072 * (w >> 1), lane, w & 1, U[ct] * end);
+        put_half(upl[b][ct] + 3072 * (w >> 1), lane, w & 1, U[ct]);
+      }
+      lds_barrier();
+      fetch_end(ahead);
+      frag tf[TI][2][NP];
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          if constexpr (!kKeysPacked) drop_inactive(cur.act, ks, g, t[i][ks].b);
+          to_frag<T>(t[i][ks], tf[i][ks]);
+        }
+      const float decay = whole;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        frag e[2][3];
+        load_frag<3>(epl[ct], lane, e[0]);
+        load_frag<3>(epl[ct] + 3072, lane, e[1]);
+        typedef Products<NP, 3> P;
+#pragma unroll
+        for (int i = 0; i < TI; ++i) S[ct][i] *= decay;
+        f32x4 D[TI] = {};
+#pragma unroll
+        for (int p = 0; p < P::n; ++p)
+#pragma unroll
+          for (int i = 0; i < TI; ++i) {
+            S[ct][i] = mfma_16x16x32_bf16(tf[i][0][P::a(p)], e[0][P::b(p)], S[ct][i]);
+            D[i] = mfma_16x16x32_bf16(tf[i][1][P::a(p)], e[1][P::b(p)], D[i]);
+          }
+#pragma unroll
+        for (int i = 0; i < TI; ++i) S[ct][i] += D[i];
+      }
+      fetch_keys(ahead);
+      put_state(b ^ 1);
+      lds_barrier();
+      advance();
+    }
+    if (a.state_out && owner) {
+      const Rsrc to = buffer_rsrc(a.state_out + rh * a.dk * a.dv, state_bytes);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int i = 0; i < TI; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            buffer_store1(S[ct][i][e], to, state_off(ct) + (16 * i + e) * a.dv * 4, 0);
+    }
+  } else {
+    const Rsrc out = buffer_rsrc(a.out + col0, mine * 4);
+    auto fetch_start = [&](int at) {
+      start = *reinterpret_cast<const f32x4 *>(factors + (size_t)at * 3 * kC);
+    };
+    // A chunk's outputs, between the barriers of the next one.
+    auto outputs = [&](int b, auto between) {
+      f32x4 X[CT], O[CT];
+      times_state(b, X);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) O[ct] = start * X[ct];
+      fetch_rows(ahead, 0);
+      fetch_start(ahead);
+      between();
+      add_times_tri(upl[b], O);
+      fetch_tri(ahead, 0);
+      between();
+      const int t0 = cur.at * kC, n = a.L - t0 - 16 * w - 4 * g;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const int off = (row_off + t0 + 16 * ct * a.L) * 4;
+        const f32x4 y = O[ct] * a.scale;
+        if (t0 + kC <= a.L) {
+          buffer_store4(y, out, off, 0);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) buffer_store1(y[e], out, e < n ? off + 4 * e : kNowhere, 0);
+        }
+      }
+      between();
+      advance();
+    };
+    if (cur.at >= 0) {
+      fetch_rows(cur.at, 0);
+      fetch_start(cur.at);
+      fetch_tri(cur.at, 0);
+    }
+    lds_barrier();
+    if (cur.at < 0) return;
+    for (int i = 0; i < 3; ++i) lds_barrier();  // the first chunk's
+    int b = 0;
+    for (; next.at >= 0; b ^= 1) outputs(b, [] { lds_barrier(); });
+    outputs(b, [] {});
   }
 }
 
@@ -866,7 +1127,7 @@ template <typename T, int NI, int CT>
 __global__ __launch_bounds__(512, 2) void linear_plain_kernel(LinearArgs a, LinearWork ws) {
   constexpr int NP = Pieces<T>::n, NK = NI / 2, TI = NI >= 4 ? NI / 4 : 1;
   constexpr int SB = Pieces<T>::blocks * 1024, kPart = 4 * NK * SB, kParts = 2;
-  constexpr bool kKeysPacked = !keys_in_place<T, false>(NI, 1);
+  constexpr bool kKeysPacked = !keys_in_place<T>(NI);
   __shared__ __attribute__((aligned(16))) unsigned char spl[2][CT][NK * 3 * 1024];
   __shared__ __attribute__((aligned(16))) unsigned char upl[2][CT][2 * NP * 1024];
   __shared__ __attribute__((aligned(16))) unsigned char epl[2][CT][6 * 1024];
@@ -1093,53 +1354,52 @@ __global__ __launch_bounds__(512, 2) void linear_plain_kernel(LinearArgs a, Line
   }
 }
 
-// Column tiles per workgroup, its waves and chunks fetched ahead, by how the grid fills
-// the CUs (us for prompts of 512 tokens, 16 heads of 128 x 128 unless stated, both
-// kernels). With the delta rule
-//   one tile each if every workgroup then has a CU to itself, and two chunks ahead as
-//   far as 512 registers hold them: nothing else hides the latency there. f32, whose
-//   products and splitting are the path, on eight waves (1 x 4096: 215, four 261; in
-//   bf16 2 x 8192: 433, four 416, where reading the state twice costs more);
-//   one tile each while two workgroups per CU hold all (4 rows: 72 us, two tiles 91,
-//   four 84), except f32 keys over 128 wide, whose operands leave room for one;
-//   beyond that every operand is loaded and split for more columns at once: four
-//   tiles for f32 keys of 65 to 128 (8 rows: 119 us, two tiles 154, which spill, one
-//   147; 16 rows: 231, 343, 304), where the splitting weighs most, two tiles otherwise
-//   (8 rows in bf16: 79 us, four tiles 89, one 91; 32 rows of 32 x 32 f32: 145, 161,
-//   159; 16 rows of 64 x 64 f32: 106, 110, 125; 4 x 1024 with 8 heads of 256 x 256 f32:
-//   145 on eight waves, 171 on four).
+// Kernel and column tiles per workgroup by how the grid fills the CUs (us for prompts of
+// 512 tokens, 16 heads of 128 x 128 unless stated, both kernels). With the delta rule
+//   the path kernel with one tile if every workgroup then has a CU to itself (2 x 8192 in
+//   bf16: 394, two tiles 511), with two while one tile would put two on a CU (4 rows: 59,
+//   one 75, four waves 73) and for bf16 keys over 128 wide (8 x 1024 with 8 heads of 256 x
+//   256: 177, four waves 195);
+//   beyond that four waves, two or more workgroups a CU: every operand is loaded and
+//   split for four tiles at once with f32 keys of 65 to 128, where the splitting weighs
+//   most (16 rows: 215, two tiles 343, which spill, the path kernel 238), for two
+//   otherwise (16 rows in bf16: 156, four tiles 171, the path kernel 173; 32 rows of 64 x
+//   64 f32: 208, 210, 213);
+//   f32 keys over 128 wide, whose state is half the work, on eight waves that share it
+//   (8 x 1024 with 8 heads of 256 x 256: 275, the path kernel 311; 1 x 4096 301 and 318).
 // Without it one tile each if every workgroup has a CU to itself (2 x 8192: 404 us, two
 // tiles 448; bf16 275 and 355), else two (4 rows: 43, one 51; 16 rows: 167, 195; 8 x 1024
 // with 8 heads of 256 x 256 bf16: 111, 124); two chunks ahead brought nothing.
 template <typename T, bool DELTA, int NI>
 hipError_t launch(const LinearArgs &a, const LinearWork &ws, hipStream_t stream,
                   const KernelEvents &ev) {
-  constexpr bool f32 = sizeof(T) == 4, wide = f32 && NI > 8;
-  constexpr int kAhead = DELTA && !wide ? 2 : 1, kTiles = f32 && DELTA && NI == 8 ? 4 : 2;
+  constexpr bool f32 = sizeof(T) == 4;
   const size_t jtiles = (size_t)((a.dv + 15) / 16), heads = (size_t)a.rows * a.heads;
-  const size_t one = heads * jtiles, many = heads * ((jtiles + kTiles - 1) / kTiles);
-  const bool few = one <= (size_t)a.cus;
-  const auto pairs = keys_in_place<T, DELTA>(NI, few ? kAhead : 1)
-                         ? linear_pairs_kernel<T, DELTA, sizeof(T) == 2>
-                         : linear_pairs_kernel<T, DELTA, true>;
+  auto grid = [&](int tiles) { return dim3((unsigned)(heads * ((jtiles + tiles - 1) / tiles))); };
+  const bool few = heads * jtiles <= (size_t)a.cus, some = heads * jtiles <= 2 * (size_t)a.cus;
   const dim3 chunks((unsigned)((a.L + kC - 1) / kC), (unsigned)a.heads, (unsigned)a.rows);
-  hipExtLaunchKernelGGL(pairs, chunks, dim3(256), 0, stream, ev.start, nullptr, 0, a, ws);
+  hipExtLaunchKernelGGL((linear_pairs_kernel<T, DELTA, !keys_in_place<T>(NI)>), chunks, dim3(256),
+                        0, stream, ev.start, nullptr, 0, a, ws);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  auto walk = [&](auto kernel, int waves, size_t grid) {
-    hipExtLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * waves), 0, stream, nullptr,
-                          ev.stop, 0, a, ws);
+  auto walk = [&](auto kernel, int waves, int tiles) {
+    hipExtLaunchKernelGGL(kernel, grid(tiles), dim3(64 * waves), 0, stream, nullptr, ev.stop, 0, a,
+                          ws);
     return hipGetLastError();
   };
-  if constexpr (DELTA) {
-    constexpr int kFewWaves = f32 ? 8 : 4, kManyWaves = wide ? 8 : 4;
-    if (few) return walk(linear_delta_kernel<T, NI, 1, kAhead, kFewWaves>, kFewWaves, one);
-    if constexpr (!wide)
-      if (one <= 2 * (size_t)a.cus) return walk(linear_delta_kernel<T, NI, 1, 1, 4>, 4, one);
-    return walk(linear_delta_kernel<T, NI, kTiles, 1, kManyWaves>, kManyWaves, many);
+  if constexpr (!DELTA) {
+    if (few) return walk(linear_plain_kernel<T, NI, 1>, 8, 1);
+    return walk(linear_plain_kernel<T, NI, 2>, 8, 2);
+  } else if constexpr (f32 && NI > 8) {
+    if (few) return walk(linear_delta_kernel<T, NI, 1, 8>, 8, 1);
+    return walk(linear_delta_kernel<T, NI, 2, 8>, 8, 2);
   } else {
-    if (few) return walk(linear_plain_kernel<T, NI, 1>, 8, one);
-    return walk(linear_plain_kernel<T, NI, kTiles>, 8, many);
+    if (few) return walk(linear_delta_path_kernel<T, NI, 1>, 8, 1);
+    if (some || NI > 8) return walk(linear_delta_path_kernel<T, NI, 2>, 8, 2);
+    if constexpr (NI <= 8) {
+      constexpr int kTiles = f32 && NI == 8 ? 4 : 2;
+      return walk(linear_delta_kernel<T, NI, kTiles, 4>, 4, kTiles);
+    }
   }
 }
 
