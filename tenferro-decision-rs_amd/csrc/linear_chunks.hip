@@ -5,11 +5,11 @@
 //   U    = T (beta (V - d K S0))                 (plain: U = V)
 //   O    = scale (d Q S0 + (D . Q K^T) U)
 //   S0  <- e^G S0 + K^T (e U)
-// Two kernels:
-//   linear_pairs_kernel  over all chunks at once: the decays, D . Q K^T and T
-//   linear_delta_kernel, linear_plain_kernel  along each (row, head): U, O and the
-//                        state, which stays in the accumulators from the first chunk to
-//                        the last
+// Two kernels follow each other:
+//   linear_pairs_kernel, over all chunks at once: the decays, D . Q K^T and T
+//   one that walks along each (row, head): U, O and the state, which stays in the
+//   accumulators from the first chunk to the last (linear_delta_kernel,
+//   linear_delta_path_kernel, linear_plain_kernel)
 // Chunks without an active token are skipped by both.
 //
 // Products run on the bf16 matrix cores with f32 accumulation, f32 operands as
@@ -140,10 +140,11 @@ __device__ __forceinline__ uint32_t load_one(Rsrc m, int off) {
   else
     return __builtin_amdgcn_raw_buffer_load_b16(m, off, 0, 0);
 }
-// Four consecutive tokens (16-byte loads need 4-byte alignment only).
+// Four consecutive tokens (16-byte loads need 4-byte alignment only). bf16 stays 16 bits
+// until it is used: a value widened across a loop's edge is waited for there.
 template <typename T>
 struct Four {
-  uint32_t d[4];
+  unsigned short d[4];
 };
 template <>
 struct Four<float> {
@@ -155,7 +156,7 @@ __device__ __forceinline__ void load_four(Rsrc m, int off, Four<T> &x) {
     x.v = buffer_load4(m, off, 0);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x.d[e] = load_one<T>(m, off + 2 * e);
+    for (int e = 0; e < 4; ++e) x.d[e] = (unsigned short)load_one<T>(m, off + 2 * e);
   }
 }
 template <typename T>
@@ -165,7 +166,7 @@ __device__ __forceinline__ f32x4 values_of(const Four<T> &x) {
   } else {
     f32x4 v;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(x.d[e] << 16);
+    for (int e = 0; e < 4; ++e) v[e] = __uint_as_float((uint32_t)x.d[e] << 16);
     return v;
   }
 }
@@ -512,23 +513,6 @@ constexpr bool keys_in_place(int NI) {
   return sizeof(T) == 4 && NI <= 8;
 }
 
-// The (row, head) and first value column of a workgroup with CT column tiles. Column
-// groups of a (row, head) go to one XCD (workgroups are dealt to the eight in turn)
-// and share its L2.
-struct Columns {
-  size_t rh;
-  int r, h, j;
-};
-template <int CT>
-__device__ __forceinline__ Columns columns_of(const LinearArgs &a) {
-  const unsigned groups = ((a.dv + 15) / 16 + CT - 1) / CT, heads = (unsigned)(a.rows * a.heads);
-  const unsigned set = blockIdx.x / (8 * groups), in = blockIdx.x - set * 8 * groups;
-  const unsigned width = min(8u, heads - 8 * set), cols = in / width;
-  const size_t rh = 8 * set + (in - cols * width);
-  const int r = (int)(rh / a.heads);
-  return Columns{rh, r, (int)(rh - (size_t)r * a.heads), (int)(16 * CT * cols)};
-}
-
 // A row's chunks with an active token, 64 at a time.
 struct Chunk {
   int at;  // -1: none
@@ -563,280 +547,374 @@ __device__ __forceinline__ void put_half(unsigned char *block, int lane, int hal
     *reinterpret_cast<u32x2 *>(block + 1024 * i + 16 * lane + 8 * half) = p.p[i];
 }
 
-// Workgroup = four waves on CT tiles of 16 value columns of one (row, head). The waves
-// share the work of a chunk, which is what every later chunk waits for: wave w has
-// token tile w of U and O, and the feature tiles TI w .. of the state (feature
-// 16 i + 4 (lane / 16) + e, column lane % 16, in accumulators). Three times a chunk
-// they hand their part to the others as operand pieces in LDS: the state for K S0 and
-// Q S0, V - d K S0 for U, U for O and the state. Keys, queries and triangles come as operands straight from memory into
-// registers, each of its lines to one wave, and are fetched for the next chunk as
-// soon as the present one has been multiplied.
-//
-// On eight waves the first four are on the path from one state to the next
-// (K S0, V - d K S0 and U), the others beside it (Q S0 and O, which nothing waits for);
-// the state's tiles are dealt to all eight. `path` and `side` are both true on four.
-//
-// What bounds it: a chunk's three exchanges follow each other, 5400 cycles in bf16 with
-// 128 x 128 and one tile, of which the products are 960; with two workgroups per CU the
-// operands, 8 TB/s out of L2.
-template <typename T, int NI, int CT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 8 || (NI <= 8 && CT < 4) ? 2 : 1)
-void linear_delta_kernel(LinearArgs a, LinearWork ws) {
-  constexpr bool kRoles = WAVES == 8;
-  constexpr int NP = Pieces<T>::n;
-  constexpr int NK = NI / 2, TI = NI >= WAVES ? NI / WAVES : 1;
-  constexpr int SB = Pieces<T>::blocks * 1024;
-  constexpr int kPart = 4 * NK * SB, kParts = 3;
-  constexpr bool kKeysPacked = !keys_in_place<T>(NI);
-  __shared__ __attribute__((aligned(16))) unsigned char spl[CT][NK * 3 * 1024];
-  __shared__ __attribute__((aligned(16))) unsigned char xpl[CT][6 * 1024];
-  __shared__ __attribute__((aligned(16))) unsigned char upl[CT][6 * 1024], epl[CT][6 * 1024];
-  const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int w = wave & 3;  // token tile
-  const bool path = !kRoles || wave < 4, side = !kRoles || wave >= 4;
-  const int nch = (a.L + kC - 1) / kC;
-  const Columns col = columns_of<CT>(a);
-  const size_t rh = col.rh;
-  const int r = col.r, h = col.h, jw = col.j;
-  const unsigned char *packed = ws.packed + ((size_t)r * a.key_heads + h / a.group) * nch *
-                                                ((size_t)kParts * kPart);
-  // The columns of values, outputs and states.
-  const uint32_t mine = (uint32_t)min(16 * CT, a.dv - jw) * a.L;
-  const size_t col0 = (rh * a.dv + jw) * a.L;
-  const Rsrc v = buffer_rsrc(static_cast<const T *>(a.v) + col0, mine * sizeof(T));
-  const Rsrc out = buffer_rsrc(a.out + col0, mine * 4);
-  const Rsrc keys = buffer_rsrc(
-      static_cast<const T *>(a.k) + ((size_t)r * a.key_heads + h / a.group) * a.dk * a.L,
-      (uint32_t)a.dk * a.L * sizeof(T));
-  const uint32_t state_bytes = (uint32_t)a.dk * a.dv * 4;
-  const int row_off = c16 * a.L + 16 * w + 4 * g;  // elements: the lane's column and first token
-  const bool owner = TI * wave < NI;
-  f32x4 S[CT][TI] = {};
-  if (a.state_in && owner) {
-    const Rsrc from = buffer_rsrc(a.state_in + rh * a.dk * a.dv, state_bytes);
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      const int j = jw + 16 * ct + c16;
-      const int voff = j < a.dv ? ((16 * TI * wave + 4 * g) * a.dv + j) * 4 : kNowhere;
-#pragma unroll
-      for (int i = 0; i < TI; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          S[ct][i][e] = buffer_load1(from, voff + (16 * i + e) * a.dv * 4, 0);
-    }
-  }
-  auto put_state = [&] {
-    if (owner)
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int i = 0; i < TI; ++i) {
-          const int tile = TI * wave + i;
-          put_half(spl[ct] + 3072 * (tile >> 1), lane, tile & 1, S[ct][i]);
-        }
-  };
+// A wave of a workgroup on CT tiles of 16 value columns of one (row, head), its token
+// tile w of the chunks' operands and outputs.
+template <typename T, bool DELTA, int NI, int CT>
+struct Walk {
+  static constexpr int NP = Pieces<T>::n, NK = NI / 2, SB = Pieces<T>::blocks * 1024;
+  static constexpr int kPart = 4 * NK * SB, kParts = DELTA ? 3 : 2;
+  static constexpr int kPlanes = DELTA ? 2 * kTri : kTri;
+  enum { kQueries, kByFeature, kKeys };  // parts of `packed`
+  enum { kScores, kSolve };              // of `planes`
+  typedef unsigned char State[NK * 3 * 1024], Tokens[6 * 1024];  // LDS, a column tile's
 
-  ActiveChunks chunks(ws.active + (size_t)r * nch, nch, lane);
-  // What a chunk needs from memory.
-  struct Operands {
-    Stored<T> q[NK], k[kRoles ? 1 : NK], t[TI][2];  // with roles q is the wave's of both,
-    frag scores[2][3], solve[2][3];                // and so are the scores
-    f32x4 start, end, beta;
-    float whole;
-    Four<T> values[CT];
-  } o;
-  auto fetch_rows = [&](int at) {  // token tile `wave` of queries and keys
-    const unsigned char *p = packed + (size_t)at * (kParts * kPart) + SB * NK * w;
-    if (kRoles && path) p += 2 * kPart;
+  int lane, g, c16, wave, w, nch, L;
+  int r, h, j;  // row, head, first value column
+  size_t rh, kh;
+  const unsigned char *packed, *planes;
+  const float *factors;  // the lane's four tokens'
+  int row_off;           // elements: the lane's column and first token
+  uint32_t mine;         // of the columns
+  size_t col0;
+
+  __device__ __forceinline__ Walk(const LinearArgs &a, const LinearWork &ws) {
+    lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
+    L = a.L, nch = (L + kC - 1) / kC;
+    // Column groups of a (row, head) go to one XCD (workgroups are dealt to the eight
+    // in turn) and share its L2.
+    const unsigned groups = ((a.dv + 15) / 16 + CT - 1) / CT, heads = (unsigned)(a.rows * a.heads);
+    const unsigned set = blockIdx.x / (8 * groups), in = blockIdx.x - set * 8 * groups;
+    const unsigned width = min(8u, heads - 8 * set), cols = in / width;
+    rh = 8 * set + (in - cols * width);
+    r = (int)(rh / a.heads), h = (int)(rh - (size_t)r * a.heads), j = (int)(16 * CT * cols);
+    kh = (size_t)r * a.key_heads + h / a.group;
+    packed = ws.packed + kh * nch * ((size_t)kParts * kPart);
+    planes = ws.planes + rh * nch * kPlanes;
+    factors = ws.factors + rh * nch * 3 * kC + 16 * w + 4 * g;
+    row_off = c16 * L + 16 * w + 4 * g;
+    mine = (uint32_t)min(16 * CT, a.dv - j) * L;
+    col0 = (rh * a.dv + j) * L;
+  }
+  __device__ __forceinline__ ActiveChunks chunks(const LinearWork &ws) const {
+    return ActiveChunks(ws.active + (size_t)r * nch, nch, lane);
+  }
+  __device__ __forceinline__ Rsrc values(const LinearArgs &a) const {
+    return buffer_rsrc(static_cast<const T *>(a.v) + col0, mine * sizeof(T));
+  }
+  __device__ __forceinline__ Rsrc outputs(const LinearArgs &a) const {
+    return buffer_rsrc(a.out + col0, mine * 4);
+  }
+  __device__ __forceinline__ void fetch_rows(int at, int part, Stored<T> (&rows)[NK]) const {
+    const unsigned char *p = packed + (size_t)at * (kParts * kPart) + part * kPart + SB * NK * w;
 #pragma unroll
-    for (int kk = 0; kk < NK; ++kk) {
-      load_stored<T>(p + SB * kk, lane, o.q[kk]);
-      if constexpr (!kRoles) load_stored<T>(p + 2 * kPart + SB * kk, lane, o.k[kk]);
-    }
-  };
-  auto fetch_values = [&](int at) {
-    const float *f = ws.factors + (rh * nch + at) * 3 * kC + 16 * w + 4 * g;
-    o.start = *reinterpret_cast<const f32x4 *>(f);
-    o.end = *reinterpret_cast<const f32x4 *>(f + kC);
-    o.beta = *reinterpret_cast<const f32x4 *>(f + 2 * kC);
+    for (int kk = 0; kk < NK; ++kk) load_stored<T>(p + SB * kk, lane, rows[kk]);
+  }
+  __device__ __forceinline__ void fetch_tri(int at, int which, frag (&f)[2][3]) const {
+    const unsigned char *p = planes + (size_t)at * kPlanes + which * kTri;
+    frag first[3];  // stored behind the branch, which would else wait for it
+    load_frag<3>(p + 3072 * tri_block(w, 0), lane, first);
+    if (w >= 2) load_frag<3>(p + 3072 * tri_block(w, 1), lane, f[1]);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) f[0][i] = first[i];
+  }
+  // Factor 0: from the chunk's start, 1: to its end, 2: beta.
+  __device__ __forceinline__ f32x4 factor(int at, int which) const {
+    return *reinterpret_cast<const f32x4 *>(factors + (size_t)at * 3 * kC + which * kC);
+  }
+  __device__ __forceinline__ void fetch_values(Rsrc v, int at, bool on, Four<T> (&x)[CT]) const {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
-      load_four<T>(v, path ? (row_off + at * kC + 16 * ct * a.L) * (int)sizeof(T) : kNowhere,
-                   o.values[ct]);
-  };
-  auto fetch_tri = [&](int at, bool solve, frag (&f)[2][3]) {  // row tile w of a triangle
-    const unsigned char *p = ws.planes + (rh * nch + at) * (2 * kTri) + (solve ? kTri : 0);
-    load_frag<3>(p + 3072 * tri_block(w, 0), lane, f[0]);
-    if (w >= 2) load_frag<3>(p + 3072 * tri_block(w, 1), lane, f[1]);
-  };
-  auto fetch_columns = [&](int at) {  // the owned feature tiles of the keys
-    o.whole = ws.factors[(rh * nch + at) * 3 * kC + kC - 1];
-    if (!owner) return;
-    const unsigned char *p = packed + (size_t)at * (kParts * kPart) + kPart + 2 * SB * TI * wave;
-#pragma unroll
-    for (int i = 0; i < TI; ++i)
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        if constexpr (kKeysPacked) {
-          load_stored<T>(p + SB * (2 * i + ks), lane, o.t[i][ks]);
-        } else {
-          const int off = ((16 * (TI * wave + i) + c16) * a.L + at * kC + 32 * ks + 4 * g) * 4;
-          o.t[i][ks].b[0] = buffer_load4(keys, off, 0);
-          o.t[i][ks].b[1] = buffer_load4(keys, off + 64, 0);
-        }
-      }
-  };
-
-  Chunk cur = chunks.next(), next = chunks.next();
-  if (cur.at >= 0) {
-    fetch_rows(cur.at);
-    fetch_values(cur.at);
-    if (!kRoles) fetch_tri(cur.at, true, o.solve);
-    fetch_tri(cur.at, kRoles && path, o.scores);
-    fetch_columns(cur.at);
+      load_four<T>(v, on ? (row_off + at * kC + 16 * ct * L) * (int)sizeof(T) : kNowhere, x[ct]);
   }
-  put_state();
-  lds_barrier();
-  while (cur.at >= 0) {
-    // Behind the last chunk its operands come again, for nothing: a branch around the
-    // loads makes the compiler wait for them at its end.
-    const int far = next.at >= 0 ? next.at : cur.at;
-    // Q S0 and K S0, even and odd steps in accumulators of their own.
-    f32x4 X[CT][2] = {}, O[CT][2] = {};
+  // The values of the lane's active tokens.
+  __device__ __forceinline__ f32x4 active_values(const Four<T> &x, uint64_t act) const {
+    const unsigned on = (unsigned)(act >> (16 * w + 4 * g));
+    f32x4 v = values_of<T>(x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (on >> e) & 1u ? v[e] : 0.0f;
+    return v;
+  }
+  __device__ __forceinline__ void put_tokens(Tokens *to, int ct, f32x4 x) const {
+    put_half(to[ct] + 3072 * (w >> 1), lane, w & 1, x);
+  }
+  // rows S0, the steps in XA accumulators.
+  __device__ __forceinline__ void times_state(const Stored<T> (&rows)[NK], const State *spl,
+                                              f32x4 (&Y)[CT]) const {
+    constexpr int XA = CT == 1 && NK >= 4 ? 4 : (NK >= 2 ? 2 : 1);
+    f32x4 X[XA][CT] = {};
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk) {
-      frag s[CT][3], qf[NP], kf[NP];
+      frag s[CT][3], f[NP];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) load_frag<3>(spl[ct] + 3072 * kk, lane, s[ct]);
-      to_frag<T>(o.q[kk], qf);
-      if constexpr (!kRoles) to_frag<T>(o.k[kk], kf);
+      to_frag<T>(rows[kk], f);
       typedef Products<NP, 3> P;
 #pragma unroll
-      for (int x = 0; x < P::n; ++x)
+      for (int p = 0; p < P::n; ++p)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+          X[kk % XA][ct] = mfma_16x16x32_bf16(f[P::a(p)], s[ct][P::b(p)], X[kk % XA][ct]);
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      Y[ct] = X[0][ct];
+#pragma unroll
+      for (int i = 1; i < XA; ++i) Y[ct] += X[i][ct];
+    }
+  }
+  // U += tri x, x of NB pieces in LDS; with one column tile each step in accumulators of
+  // its own.
+  template <int NB>
+  __device__ __forceinline__ void add_tri(const frag (&tri)[2][3], const unsigned char *from,
+                                          int stride, f32x4 (&U)[CT]) const {
+    f32x4 A[CT] = {};
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      if (ks && w < 2) continue;
+      frag x[CT][NB];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+        load_frag<NB>(from + ct * stride + 1024 * NB * ks, lane, x[ct]);
+      typedef Products<3, NB> P;
+#pragma unroll
+      for (int p = 0; p < P::n; ++p)
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-          if constexpr (!kRoles)
-            X[ct][kk & 1] = mfma_16x16x32_bf16(kf[P::a(x)], s[ct][P::b(x)], X[ct][kk & 1]);
-          O[ct][kk & 1] = mfma_16x16x32_bf16(qf[P::a(x)], s[ct][P::b(x)], O[ct][kk & 1]);
+          f32x4 &to = ks && CT == 1 ? A[ct] : U[ct];
+          to = mfma_16x16x32_bf16(tri[ks][P::a(p)], x[ct][P::b(p)], to);
         }
     }
-    fetch_rows(far);
-    f32x4 U[CT];
-    const unsigned on = (unsigned)(cur.act >> (16 * w + 4 * g));
+    if constexpr (CT == 1) U[0] += A[0];
+  }
+  __device__ __forceinline__ void store(Rsrc out, int at, float scale, const f32x4 (&O)[CT]) const {
+    const int t0 = at * kC, n = L - t0 - 16 * w - 4 * g;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const f32x4 given = values_of<T>(o.values[ct]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) U[ct][e] = (on >> e) & 1u ? given[e] : 0.0f;
-      O[ct][0] = o.start * (O[ct][0] + O[ct][1]);
-      const f32x4 x = kRoles ? O[ct][0] : o.start * (X[ct][0] + X[ct][1]);
-      if (path) put_half(xpl[ct] + 3072 * (w >> 1), lane, w & 1, o.beta * (U[ct] - x));
-    }
-    lds_barrier();
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) U[ct] = f32x4{};
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      if (!path || (ks && w < 2)) continue;
-      frag x[CT][3];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) load_frag<3>(xpl[ct] + 3072 * ks, lane, x[ct]);
-      typedef Products<3, 3> P;
-#pragma unroll
-      for (int i = 0; i < P::n; ++i)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-          U[ct] = mfma_16x16x32_bf16((kRoles ? o.scores : o.solve)[ks][P::a(i)], x[ct][P::b(i)],
-                                     U[ct]);
-    }
-    if constexpr (!kRoles) fetch_tri(far, true, o.solve);
-    if (path)
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        put_half(upl[ct] + 3072 * (w >> 1), lane, w & 1, U[ct]);
-        put_half(epl[ct] + 3072 * (w >> 1), lane, w & 1, U[ct] * o.end);
-      }
-    const float decay = o.whole;
-    lds_barrier();
-    fetch_values(far);
-    // The state first: the next chunk waits for it.
-    if (owner) {
-      frag tf[TI][2][NP];
-#pragma unroll
-      for (int i = 0; i < TI; ++i)
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          if constexpr (!kKeysPacked) drop_inactive(cur.act, ks, g, o.t[i][ks].b);
-          to_frag<T>(o.t[i][ks], tf[i][ks]);
-        }
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        frag e[2][3];
-        load_frag<3>(epl[ct], lane, e[0]);
-        load_frag<3>(epl[ct] + 3072, lane, e[1]);
-        typedef Products<NP, 3> P;
-#pragma unroll
-        for (int i = 0; i < TI; ++i) S[ct][i] *= decay;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int x = 0; x < P::n; ++x)
-#pragma unroll
-            for (int i = 0; i < TI; ++i)
-              S[ct][i] = mfma_16x16x32_bf16(tf[i][ks][P::a(x)], e[ks][P::b(x)], S[ct][i]);
-      }
-    }
-    fetch_columns(far);
-    if (kRoles) {  // only the side waits for what comes next
-      put_state();
-      lds_barrier();
-    }
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      if (!side || (ks && w < 2)) continue;
-      frag u[CT][3];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) load_frag<3>(upl[ct] + 3072 * ks, lane, u[ct]);
-      typedef Products<3, 3> P;
-#pragma unroll
-      for (int x = 0; x < P::n; ++x)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-          O[ct][0] = mfma_16x16x32_bf16(o.scores[ks][P::a(x)], u[ct][P::b(x)], O[ct][0]);
-    }
-    if (!kRoles) put_state();
-    fetch_tri(far, kRoles && path, o.scores);
-    const int n = a.L - cur.at * kC - 16 * w - 4 * g;
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      if (!side) continue;
-      const int off = (row_off + cur.at * kC + 16 * ct * a.L) * 4;
-      const f32x4 y = O[ct][0] * a.scale;
-      if (cur.at * kC + kC <= a.L) {
+      const int off = (row_off + t0 + 16 * ct * L) * 4;
+      const f32x4 y = O[ct] * scale;
+      if (t0 + kC <= L) {
         buffer_store4(y, out, off, 0);
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) buffer_store1(y[e], out, e < n ? off + 4 * e : kNowhere, 0);
       }
     }
-    if (!kRoles) lds_barrier();
-    cur = next;
-    next = chunks.next();
   }
-  if (a.state_out && owner) {
-    const Rsrc to = buffer_rsrc(a.state_out + rh * a.dk * a.dv, state_bytes);
+};
+
+// A wave's feature tiles tile0 .. tile0 + TI - 1 of the state (feature 16 i + 4 (lane / 16)
+// + e, column lane % 16, in accumulators), with what the next chunk multiplies in.
+template <typename T, bool DELTA, int NI, int CT, int WAVES>
+struct StateTiles {
+  typedef Walk<T, DELTA, NI, CT> W;
+  static constexpr int TI = NI >= WAVES ? NI / WAVES : 1, NP = W::NP;
+  static constexpr bool kKeysPacked = !keys_in_place<T>(NI);
+  f32x4 S[CT][TI];
+  Stored<T> t[TI][2];
+  float whole;
+  int tile0, voff[CT], step;
+  Rsrc keys;
+  uint32_t bytes;
+
+  __device__ __forceinline__ bool owner() const { return NI >= WAVES || tile0 < NI; }
+  __device__ __forceinline__ StateTiles(const W &k, const LinearArgs &a) {
+    tile0 = TI * k.wave, step = a.dv * 4;
+    keys = buffer_rsrc(static_cast<const T *>(a.k) + k.kh * a.dk * a.L,
+                       (uint32_t)a.dk * a.L * sizeof(T));
+    bytes = (uint32_t)a.dk * a.dv * 4;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const int j = jw + 16 * ct + c16;
-      const int voff = j < a.dv ? ((16 * TI * wave + 4 * g) * a.dv + j) * 4 : kNowhere;
+      const int j = k.j + 16 * ct + k.c16;
+      voff[ct] = j < a.dv ? ((16 * tile0 + 4 * k.g) * a.dv + j) * 4 : kNowhere;
+#pragma unroll
+      for (int i = 0; i < TI; ++i) S[ct][i] = f32x4{};
+    }
+    if (!a.state_in || !owner()) return;
+    const Rsrc from = buffer_rsrc(a.state_in + k.rh * a.dk * a.dv, bytes);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
       for (int i = 0; i < TI; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          buffer_store1(S[ct][i][e], to, voff + (16 * i + e) * a.dv * 4, 0);
-    }
+          S[ct][i][e] = buffer_load1(from, voff[ct] + (16 * i + e) * step, 0);
   }
+  __device__ __forceinline__ void store(const W &k, const LinearArgs &a) const {
+    if (!a.state_out || !owner()) return;
+    const Rsrc to = buffer_rsrc(a.state_out + k.rh * a.dk * a.dv, bytes);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          buffer_store1(S[ct][i][e], to, voff[ct] + (16 * i + e) * step, 0);
+  }
+  __device__ __forceinline__ void fetch(const W &k, const LinearWork &ws, int at) {
+    whole = ws.factors[(k.rh * k.nch + at) * 3 * kC + kC - 1];
+    if (!owner()) return;
+    const unsigned char *p =
+        k.packed + (size_t)at * (W::kParts * W::kPart) + W::kByFeature * W::kPart + 2 * W::SB * tile0;
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        if constexpr (kKeysPacked) {
+          load_stored<T>(p + W::SB * (2 * i + ks), k.lane, t[i][ks]);
+        } else {
+          const int off = ((16 * (tile0 + i) + k.c16) * k.L + at * kC + 32 * ks + 4 * k.g) * 4;
+          t[i][ks].b[0] = buffer_load4(keys, off, 0);
+          t[i][ks].b[1] = buffer_load4(keys, off + 64, 0);
+        }
+      }
+  }
+  // S <- e^G S + K^T (e U), e U in LDS; with one column tile the steps in accumulators
+  // of their own. `taken` runs when the keys have been split.
+  template <typename F>
+  __device__ __forceinline__ void update(const W &k, const typename W::Tokens *epl, uint64_t act,
+                                         F taken) {
+    frag tf[TI][2][NP];
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        if constexpr (!kKeysPacked) drop_inactive(act, ks, k.g, t[i][ks].b);
+        to_frag<T>(t[i][ks], tf[i][ks]);
+      }
+    const float decay = whole;
+    taken();
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      frag e[2][3];
+      load_frag<3>(epl[ct], k.lane, e[0]);
+      load_frag<3>(epl[ct] + 3072, k.lane, e[1]);
+      f32x4 D[TI] = {};
+#pragma unroll
+      for (int i = 0; i < TI; ++i) S[ct][i] *= decay;
+      typedef Products<NP, 3> P;
+#pragma unroll
+      for (int p = 0; p < P::n; ++p)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int i = 0; i < TI; ++i) {
+            f32x4 &to = ks && CT == 1 ? D[i] : S[ct][i];
+            to = mfma_16x16x32_bf16(tf[i][ks][P::a(p)], e[ks][P::b(p)], to);
+          }
+      if constexpr (CT == 1)
+#pragma unroll
+        for (int i = 0; i < TI; ++i) S[ct][i] += D[i];
+    }
+    __builtin_amdgcn_sched_barrier(0);  // loads behind this find the keys' registers free
+  }
+  __device__ __forceinline__ void put(const W &k, typename W::State *spl) const {
+    if (!owner()) return;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+        put_half(spl[ct] + 3072 * ((tile0 + i) >> 1), k.lane, (tile0 + i) & 1, S[ct][i]);
+  }
+};
+
+// In all of the kernels below, operands are fetched for the next chunk as soon as the
+// present one has been multiplied, each line by one wave, straight into registers.
+// Behind the last chunk its operands come again, for nothing: a branch around the loads
+// makes the compiler wait for them at its end.
+
+// The delta rule with the work of a chunk, which is what every later chunk waits for,
+// shared by four waves: wave w has token tile w of U and O, and the feature tiles TI w ..
+// of the state. Three times a chunk they hand their part to the others as operand
+// pieces in LDS: the state for K S0 and Q S0, V - d K S0 for U, U for O and the state.
+// Two or more workgroups a CU hide each other's exchanges; then the operands bound it
+// (8 TB/s out of L2 with bf16 keys).
+// On eight waves the first four are on the path from one state to the next (K S0, V - d
+// K S0 and U), the others beside it (Q S0 and O, which nothing waits for), and the
+// state's tiles are dealt to all eight. `path` and `side` are both true on four.
+template <typename T, int NI, int CT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 || (NI <= 8 && CT < 4) ? 2 : 1)
+void linear_delta_kernel(LinearArgs a, LinearWork ws) {
+  typedef Walk<T, true, NI, CT> W;
+  constexpr bool kRoles = WAVES == 8;
+  constexpr int NP = W::NP, NK = W::NK;
+  __shared__ __attribute__((aligned(16))) typename W::State spl[CT];
+  __shared__ __attribute__((aligned(16))) typename W::Tokens xpl[CT], upl[CT], epl[CT];
+  const W k(a, ws);
+  const bool path = !kRoles || k.wave < 4, side = !kRoles || k.wave >= 4;
+  const Rsrc v = k.values(a), out = k.outputs(a);
+  StateTiles<T, true, NI, CT, WAVES> state(k, a);
+  ActiveChunks chunks = k.chunks(ws);
+  Chunk cur = chunks.next(), next = chunks.next();
+  // With roles `rows` and `tri` are keys and the solve operand, or queries and scores.
+  Stored<T> rows[NK], krows[kRoles ? 1 : NK];
+  frag tri[2][3], solve[2][3];
+  f32x4 start, end, beta;
+  Four<T> values[CT];
+  auto fetch_rows = [&](int at) {
+    k.fetch_rows(at, kRoles && path ? W::kKeys : W::kQueries, rows);
+    if constexpr (!kRoles) k.fetch_rows(at, W::kKeys, krows);
+  };
+  auto fetch_tri = [&](int at) { k.fetch_tri(at, kRoles && path ? W::kSolve : W::kScores, tri); };
+  auto fetch_values = [&](int at) {
+    start = k.factor(at, 0), end = k.factor(at, 1), beta = k.factor(at, 2);
+    k.fetch_values(v, at, path, values);
+  };
+  if (cur.at >= 0) {
+    fetch_rows(cur.at);
+    fetch_values(cur.at);
+    if (!kRoles) k.fetch_tri(cur.at, W::kSolve, solve);
+    fetch_tri(cur.at);
+    state.fetch(k, ws, cur.at);
+  }
+  state.put(k, spl);
+  lds_barrier();
+  while (cur.at >= 0) {
+    const int far = next.at >= 0 ? next.at : cur.at;
+    f32x4 X[2][CT] = {}, O[2][CT] = {};  // K S0 and Q S0, even and odd steps
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) {
+      frag s[CT][3], f[NP], fk[NP];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) load_frag<3>(spl[ct] + 3072 * kk, k.lane, s[ct]);
+      to_frag<T>(rows[kk], f);
+      if constexpr (!kRoles) to_frag<T>(krows[kk], fk);
+      typedef Products<NP, 3> P;
+#pragma unroll
+      for (int p = 0; p < P::n; ++p)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          if constexpr (!kRoles)
+            X[kk & 1][ct] = mfma_16x16x32_bf16(fk[P::a(p)], s[ct][P::b(p)], X[kk & 1][ct]);
+          O[kk & 1][ct] = mfma_16x16x32_bf16(f[P::a(p)], s[ct][P::b(p)], O[kk & 1][ct]);
+        }
+    }
+    fetch_rows(far);
+    f32x4 U[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      O[0][ct] = start * (O[0][ct] + O[1][ct]);
+      const f32x4 x = kRoles ? O[0][ct] : start * (X[0][ct] + X[1][ct]);
+      if (path) k.put_tokens(xpl, ct, beta * (k.active_values(values[ct], cur.act) - x));
+      U[ct] = f32x4{};
+    }
+    lds_barrier();
+    if (path) k.template add_tri<3>(kRoles ? tri : solve, xpl[0], sizeof(xpl[0]), U);
+    if constexpr (!kRoles) k.fetch_tri(far, W::kSolve, solve);
+    if (path)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        k.put_tokens(upl, ct, U[ct]);
+        k.put_tokens(epl, ct, U[ct] * end);
+      }
+    lds_barrier();
+    fetch_values(far);
+    // The state first: the next chunk waits for it.
+    state.update(k, epl, cur.act, [] {});
+    state.fetch(k, ws, far);
+    if (kRoles) {  // only the side waits for what comes next
+      state.put(k, spl);
+      lds_barrier();
+    }
+    if (side) k.template add_tri<3>(tri, upl[0], sizeof(upl[0]), O[0]);
+    if (!kRoles) state.put(k, spl);
+    fetch_tri(far);
+    if (side) k.store(out, cur.at, a.scale, O[0]);
+    if (!kRoles) lds_barrier();
+    cur = next;
+    next = chunks.next();
+  }
+  state.store(k, a);
 }
 
 // The delta rule with every wave at one kind of work, for grids that leave a CU to one
@@ -845,264 +923,92 @@ void linear_delta_kernel(LinearArgs a, LinearWork ws) {
 // chunk behind them with token tile w of Q S0 and O, between the barriers of the path.
 // The state and U are in two buffers for that. Sums on the path run in several
 // accumulators, whose latency nothing else hides.
-// Against four waves that do both, two chunks ahead (us): bf16, 16 heads of 128 x 128, 2 x
-// 8192 tokens 394 and 417, 1 x 4096 153 and 165; f32 4 x 512 on two tiles 59 and 73.
+// Bound by the path: 4700 cycles a chunk in bf16 with 128 x 128 and one tile, of which
+// the products are 580. Against four waves that do both, two chunks ahead (us): bf16, 16
+// heads of 128 x 128, 2 x 8192 tokens 404 and 417, 1 x 4096 158 and 165; f32 4 x 512 on two
+// tiles 58 and 73.
 template <typename T, int NI, int CT>
 __global__ __launch_bounds__(512, 2) void linear_delta_path_kernel(LinearArgs a, LinearWork ws) {
-  constexpr int NP = Pieces<T>::n, NK = NI / 2, TI = NI >= 4 ? NI / 4 : 1;
-  constexpr int SB = Pieces<T>::blocks * 1024, kPart = 4 * NK * SB, kParts = 3;
-  constexpr bool kKeysPacked = !keys_in_place<T>(NI);
-  __shared__ __attribute__((aligned(16))) unsigned char spl[2][CT][NK * 3 * 1024];
-  __shared__ __attribute__((aligned(16))) unsigned char xpl[CT][6 * 1024], epl[CT][6 * 1024];
-  __shared__ __attribute__((aligned(16))) unsigned char upl[2][CT][6 * 1024];
-  const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
-  const int nch = (a.L + kC - 1) / kC;
-  const Columns col = columns_of<CT>(a);
-  const size_t rh = col.rh, kh = (size_t)col.r * a.key_heads + col.h / a.group;
-  const unsigned char *packed = ws.packed + kh * nch * ((size_t)kParts * kPart);
-  const unsigned char *planes = ws.planes + rh * nch * (2 * kTri);
-  const float *factors = ws.factors + rh * nch * 3 * kC + 16 * w + 4 * g;
-  const uint32_t mine = (uint32_t)min(16 * CT, a.dv - col.j) * a.L;
-  const size_t col0 = (rh * a.dv + col.j) * a.L;
-  const int row_off = c16 * a.L + 16 * w + 4 * g;  // elements: the lane's column and first token
-  ActiveChunks chunks(ws.active + (size_t)col.r * nch, nch, lane);
+  typedef Walk<T, true, NI, CT> W;
+  __shared__ __attribute__((aligned(16))) typename W::State spl[2][CT];
+  __shared__ __attribute__((aligned(16))) typename W::Tokens xpl[CT], epl[CT], upl[2][CT];
+  const W k(a, ws);
+  ActiveChunks chunks = k.chunks(ws);
   Chunk cur = chunks.next(), next = chunks.next();
-  // Behind the last chunk its operands come again, for nothing: a branch around the
-  // loads makes the compiler wait for them at its end.
   int ahead = next.at >= 0 ? next.at : cur.at;
   auto advance = [&] {
     cur = next;
     next = chunks.next();
     if (next.at >= 0) ahead = next.at;
   };
-  // The wave's token tile of keys or queries, and of the solve operand or the scores.
-  Stored<T> rows[NK];
+  Stored<T> rows[W::NK];
   frag tri[2][3];
   f32x4 start;
-  auto fetch_rows = [&](int at, int part) {
-    const unsigned char *p = packed + (size_t)at * (kParts * kPart) + part * kPart + SB * NK * w;
-#pragma unroll
-    for (int kk = 0; kk < NK; ++kk) load_stored<T>(p + SB * kk, lane, rows[kk]);
-  };
-  auto fetch_tri = [&](int at, int which) {
-    const unsigned char *p = planes + (size_t)at * (2 * kTri) + which * kTri;
-    load_frag<3>(p + 3072 * tri_block(w, 0), lane, tri[0]);
-    if (w >= 2) load_frag<3>(p + 3072 * tri_block(w, 1), lane, tri[1]);
-  };
-  constexpr int XA = CT == 1 && NK >= 4 ? 4 : 2;
-  auto times_state = [&](int b, f32x4 (&Y)[CT]) {
-    f32x4 X[CT][XA] = {};
-#pragma unroll
-    for (int kk = 0; kk < NK; ++kk) {
-      frag s[CT][3], f[NP];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) load_frag<3>(spl[b][ct] + 3072 * kk, lane, s[ct]);
-      to_frag<T>(rows[kk], f);
-      typedef Products<NP, 3> P;
-#pragma unroll
-      for (int p = 0; p < P::n; ++p)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-          X[ct][kk % XA] = mfma_16x16x32_bf16(f[P::a(p)], s[ct][P::b(p)], X[ct][kk % XA]);
-    }
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      Y[ct] = X[ct][0] + X[ct][1];
-      if constexpr (XA == 4) Y[ct] += X[ct][2] + X[ct][3];
-    }
-  };
-  auto add_times_tri = [&](const unsigned char (*from)[6 * 1024], f32x4 (&U)[CT]) {
-    f32x4 A[2][CT] = {};
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      if (ks && w < 2) continue;
-      frag x[CT][3];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) load_frag<3>(from[ct] + 3072 * ks, lane, x[ct]);
-      typedef Products<3, 3> P;
-#pragma unroll
-      for (int p = 0; p < P::n; ++p)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-          A[ks][ct] = mfma_16x16x32_bf16(tri[ks][P::a(p)], x[ct][P::b(p)], A[ks][ct]);
-    }
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) U[ct] += A[0][ct] + A[1][ct];
-  };
-
-  if (wave < 4) {
-    const Rsrc v = buffer_rsrc(static_cast<const T *>(a.v) + col0, mine * sizeof(T));
-    const Rsrc keys = buffer_rsrc(static_cast<const T *>(a.k) + kh * a.dk * a.L,
-                                  (uint32_t)a.dk * a.L * sizeof(T));
-    const uint32_t state_bytes = (uint32_t)a.dk * a.dv * 4;
-    const bool owner = TI * w < NI;
-    const int tile0 = TI * w;
-    f32x4 S[CT][TI] = {};
-    auto state_off = [&](int ct) {
-      const int j = col.j + 16 * ct + c16;
-      return j < a.dv ? ((16 * tile0 + 4 * g) * a.dv + j) * 4 : kNowhere;
-    };
-    if (a.state_in && owner) {
-      const Rsrc from = buffer_rsrc(a.state_in + rh * a.dk * a.dv, state_bytes);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int i = 0; i < TI; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            S[ct][i][e] = buffer_load1(from, state_off(ct) + (16 * i + e) * a.dv * 4, 0);
-    }
-    Stored<T> t[TI][2];
+  if (k.wave < 4) {
+    const Rsrc v = k.values(a);
+    StateTiles<T, true, NI, CT, 4> state(k, a);
     Four<T> values[CT];
     f32x4 end, beta;
-    float whole;
-    auto fetch_keys = [&](int at) {
-      whole = ws.factors[(rh * nch + at) * 3 * kC + kC - 1];
-      if (!owner) return;
-      const unsigned char *p = packed + (size_t)at * (kParts * kPart) + kPart + 2 * SB * tile0;
-#pragma unroll
-      for (int i = 0; i < TI; ++i)
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          if constexpr (kKeysPacked) {
-            load_stored<T>(p + SB * (2 * i + ks), lane, t[i][ks]);
-          } else {
-            const int off = ((16 * (tile0 + i) + c16) * a.L + at * kC + 32 * ks + 4 * g) * 4;
-            t[i][ks].b[0] = buffer_load4(keys, off, 0);
-            t[i][ks].b[1] = buffer_load4(keys, off + 64, 0);
-          }
-        }
-    };
     auto fetch_values = [&](int at) {
-      start = *reinterpret_cast<const f32x4 *>(factors + (size_t)at * 3 * kC);
-      beta = *reinterpret_cast<const f32x4 *>(factors + (size_t)at * 3 * kC + 2 * kC);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-        load_four<T>(v, (row_off + at * kC + 16 * ct * a.L) * (int)sizeof(T), values[ct]);
-    };
-    auto fetch_end = [&](int at) {
-      end = *reinterpret_cast<const f32x4 *>(factors + (size_t)at * 3 * kC + kC);
-    };
-    auto put_state = [&](int b) {
-      if (owner)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-          for (int i = 0; i < TI; ++i)
-            put_half(spl[b][ct] + 3072 * ((tile0 + i) >> 1), lane, (tile0 + i) & 1, S[ct][i]);
+      start = k.factor(at, 0), beta = k.factor(at, 2);
+      k.fetch_values(v, at, true, values);
     };
     if (cur.at >= 0) {
-      fetch_rows(cur.at, 2);
+      k.fetch_rows(cur.at, W::kKeys, rows);
       fetch_values(cur.at);
-      fetch_tri(cur.at, 1);
-      fetch_end(cur.at);
-      fetch_keys(cur.at);
+      k.fetch_tri(cur.at, W::kSolve, tri);
+      end = k.factor(cur.at, 1);
+      state.fetch(k, ws, cur.at);
     }
-    put_state(0);
+    state.put(k, spl[0]);
     lds_barrier();
     for (int b = 0; cur.at >= 0; b ^= 1) {
       f32x4 X[CT], U[CT] = {};
-      times_state(b, X);
-      fetch_rows(ahead, 2);
-      const unsigned on = (unsigned)(cur.act >> (16 * w + 4 * g));
+      k.times_state(rows, spl[b], X);
+      k.fetch_rows(ahead, W::kKeys, rows);
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        f32x4 u = values_of<T>(values[ct]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) u[e] = (on >> e) & 1u ? u[e] : 0.0f;
-        put_half(xpl[ct] + 3072 * (w >> 1), lane, w & 1, beta * (u - start * X[ct]));
-      }
+      for (int ct = 0; ct < CT; ++ct)
+        k.put_tokens(xpl, ct, beta * (k.active_values(values[ct], cur.act) - start * X[ct]));
       lds_barrier();
       fetch_values(ahead);
-      add_times_tri(xpl, U);
-      fetch_tri(ahead, 1);
+      k.template add_tri<3>(tri, xpl[0], sizeof(xpl[0]), U);
+      k.fetch_tri(ahead, W::kSolve, tri);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        put_half(epl[ct] + 3072 * (w >> 1), lane, w & 1, U[ct] * end);
-        put_half(upl[b][ct] + 3072 * (w >> 1), lane, w & 1, U[ct]);
+        k.put_tokens(epl, ct, U[ct] * end);
+        k.put_tokens(upl[b], ct, U[ct]);
       }
       lds_barrier();
-      fetch_end(ahead);
-      frag tf[TI][2][NP];
-#pragma unroll
-      for (int i = 0; i < TI; ++i)
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          if constexpr (!kKeysPacked) drop_inactive(cur.act, ks, g, t[i][ks].b);
-          to_frag<T>(t[i][ks], tf[i][ks]);
-        }
-      const float decay = whole;
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        frag e[2][3];
-        load_frag<3>(epl[ct], lane, e[0]);
-        load_frag<3>(epl[ct] + 3072, lane, e[1]);
-        typedef Products<NP, 3> P;
-#pragma unroll
-        for (int i = 0; i < TI; ++i) S[ct][i] *= decay;
-        f32x4 D[TI] = {};
-#pragma unroll
-        for (int p = 0; p < P::n; ++p)
-#pragma unroll
-          for (int i = 0; i < TI; ++i) {
-            S[ct][i] = mfma_16x16x32_bf16(tf[i][0][P::a(p)], e[0][P::b(p)], S[ct][i]);
-            D[i] = mfma_16x16x32_bf16(tf[i][1][P::a(p)], e[1][P::b(p)], D[i]);
-          }
-#pragma unroll
-        for (int i = 0; i < TI; ++i) S[ct][i] += D[i];
-      }
-      fetch_keys(ahead);
-      put_state(b ^ 1);
+      end = k.factor(ahead, 1);
+      state.update(k, epl, cur.act, [] {});
+      state.fetch(k, ws, ahead);
+      state.put(k, spl[b ^ 1]);
       lds_barrier();
       advance();
     }
-    if (a.state_out && owner) {
-      const Rsrc to = buffer_rsrc(a.state_out + rh * a.dk * a.dv, state_bytes);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int i = 0; i < TI; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            buffer_store1(S[ct][i][e], to, state_off(ct) + (16 * i + e) * a.dv * 4, 0);
-    }
+    state.store(k, a);
   } else {
-    const Rsrc out = buffer_rsrc(a.out + col0, mine * 4);
-    auto fetch_start = [&](int at) {
-      start = *reinterpret_cast<const f32x4 *>(factors + (size_t)at * 3 * kC);
-    };
+    const Rsrc out = k.outputs(a);
     // A chunk's outputs, between the barriers of the next one.
     auto outputs = [&](int b, auto between) {
-      f32x4 X[CT], O[CT];
-      times_state(b, X);
+      f32x4 O[CT];
+      k.times_state(rows, spl[b], O);
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) O[ct] = start * X[ct];
-      fetch_rows(ahead, 0);
-      fetch_start(ahead);
+      for (int ct = 0; ct < CT; ++ct) O[ct] = start * O[ct];
+      k.fetch_rows(ahead, W::kQueries, rows);
+      start = k.factor(ahead, 0);
       between();
-      add_times_tri(upl[b], O);
-      fetch_tri(ahead, 0);
+      k.template add_tri<3>(tri, upl[b][0], sizeof(upl[b][0]), O);
+      k.fetch_tri(ahead, W::kScores, tri);
       between();
-      const int t0 = cur.at * kC, n = a.L - t0 - 16 * w - 4 * g;
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const int off = (row_off + t0 + 16 * ct * a.L) * 4;
-        const f32x4 y = O[ct] * a.scale;
-        if (t0 + kC <= a.L) {
-          buffer_store4(y, out, off, 0);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) buffer_store1(y[e], out, e < n ? off + 4 * e : kNowhere, 0);
-        }
-      }
+      k.store(out, cur.at, a.scale, O);
       between();
       advance();
     };
     if (cur.at >= 0) {
-      fetch_rows(cur.at, 0);
-      fetch_start(cur.at);
-      fetch_tri(cur.at, 0);
+      k.fetch_rows(cur.at, W::kQueries, rows);
+      start = k.factor(cur.at, 0);
+      k.fetch_tri(cur.at, W::kScores, tri);
     }
     lds_barrier();
     if (cur.at < 0) return;
@@ -1125,248 +1031,99 @@ __global__ __launch_bounds__(512, 2) void linear_delta_path_kernel(LinearArgs a,
 // out of both kernels, 2 TB/s.
 template <typename T, int NI, int CT>
 __global__ __launch_bounds__(512, 2) void linear_plain_kernel(LinearArgs a, LinearWork ws) {
-  constexpr int NP = Pieces<T>::n, NK = NI / 2, TI = NI >= 4 ? NI / 4 : 1;
-  constexpr int SB = Pieces<T>::blocks * 1024, kPart = 4 * NK * SB, kParts = 2;
-  constexpr bool kKeysPacked = !keys_in_place<T>(NI);
-  __shared__ __attribute__((aligned(16))) unsigned char spl[2][CT][NK * 3 * 1024];
+  typedef Walk<T, false, NI, CT> W;
+  constexpr int NP = W::NP;
+  __shared__ __attribute__((aligned(16))) typename W::State spl[2][CT];
   __shared__ __attribute__((aligned(16))) unsigned char upl[2][CT][2 * NP * 1024];
-  __shared__ __attribute__((aligned(16))) unsigned char epl[2][CT][6 * 1024];
-  const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
-  const int nch = (a.L + kC - 1) / kC;
-  const Columns col = columns_of<CT>(a);
-  const size_t rh = col.rh, kh = (size_t)col.r * a.key_heads + col.h / a.group;
-  const unsigned char *packed = ws.packed + kh * nch * ((size_t)kParts * kPart);
-  const float *factors = ws.factors + rh * nch * 3 * kC;
-  const uint32_t mine = (uint32_t)min(16 * CT, a.dv - col.j) * a.L;
-  const size_t col0 = (rh * a.dv + col.j) * a.L;
-  const int row_off = c16 * a.L + 16 * w + 4 * g;  // elements: the lane's column and first token
-  ActiveChunks chunks(ws.active + (size_t)col.r * nch, nch, lane);
+  __shared__ __attribute__((aligned(16))) typename W::Tokens epl[2][CT];
+  const W k(a, ws);
+  ActiveChunks chunks = k.chunks(ws);
   Chunk cur = chunks.next(), next = chunks.next();
-  // Behind the last chunk its operands come again, for nothing: a branch around the
-  // loads makes the compiler wait for them at its end.
   int ahead = next.at >= 0 ? next.at : cur.at;
   auto advance = [&] {
     cur = next;
     next = chunks.next();
     if (next.at >= 0) ahead = next.at;
   };
-
-  if (wave < 4) {
-    const Rsrc v = buffer_rsrc(static_cast<const T *>(a.v) + col0, mine * sizeof(T));
-    const Rsrc keys = buffer_rsrc(static_cast<const T *>(a.k) + kh * a.dk * a.L,
-                                  (uint32_t)a.dk * a.L * sizeof(T));
-    const uint32_t state_bytes = (uint32_t)a.dk * a.dv * 4;
-    const bool owner = TI * w < NI;
-    const int tile0 = TI * w;
-    f32x4 S[CT][TI] = {};
-    auto state_off = [&](int ct) {
-      const int j = col.j + 16 * ct + c16;
-      return j < a.dv ? ((16 * tile0 + 4 * g) * a.dv + j) * 4 : kNowhere;
-    };
-    if (a.state_in && owner) {
-      const Rsrc from = buffer_rsrc(a.state_in + rh * a.dk * a.dv, state_bytes);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int i = 0; i < TI; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            S[ct][i][e] = buffer_load1(from, state_off(ct) + (16 * i + e) * a.dv * 4, 0);
-    }
-    struct Keys {
-      Stored<T> t[TI][2];
-      float whole;
-    } o;
-    struct Values {
-      f32x4 end;
-      Four<T> v[CT];
-    } x;
-    auto fetch_keys = [&](int at) {
-      o.whole = factors[(size_t)at * 3 * kC + kC - 1];
-      if (!owner) return;
-      const unsigned char *p = packed + (size_t)at * (kParts * kPart) + kPart + 2 * SB * tile0;
-#pragma unroll
-      for (int i = 0; i < TI; ++i)
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          if constexpr (kKeysPacked) {
-            load_stored<T>(p + SB * (2 * i + ks), lane, o.t[i][ks]);
-          } else {
-            const int off = ((16 * (tile0 + i) + c16) * a.L + at * kC + 32 * ks + 4 * g) * 4;
-            o.t[i][ks].b[0] = buffer_load4(keys, off, 0);
-            o.t[i][ks].b[1] = buffer_load4(keys, off + 64, 0);
-          }
-        }
-    };
+  if (k.wave < 4) {
+    const Rsrc v = k.values(a);
+    StateTiles<T, false, NI, CT, 4> state(k, a);
+    Four<T> values[CT];
+    f32x4 end;
     auto fetch_values = [&](int at) {
-      x.end = *reinterpret_cast<const f32x4 *>(factors + (size_t)at * 3 * kC + kC + 16 * w + 4 * g);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-        load_four<T>(v, (row_off + at * kC + 16 * ct * a.L) * (int)sizeof(T), x.v[ct]);
-    };
-    auto put_state = [&](int b) {
-      if (owner)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-          for (int i = 0; i < TI; ++i)
-            put_half(spl[b][ct] + 3072 * ((tile0 + i) >> 1), lane, (tile0 + i) & 1, S[ct][i]);
+      end = k.factor(at, 1);
+      k.fetch_values(v, at, true, values);
     };
     auto put_values = [&](int b, uint64_t act) {
-      const unsigned on = (unsigned)(act >> (16 * w + 4 * g));
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        f32x4 u = values_of<T>(x.v[ct]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) u[e] = (on >> e) & 1u ? u[e] : 0.0f;
+        const f32x4 u = k.active_values(values[ct], act);
+        unsigned char *p = upl[b][ct] + 1024 * NP * (k.w >> 1);
         if constexpr (NP == 3)
-          put_half(upl[b][ct] + 3072 * (w >> 1), lane, w & 1, u);
+          put_half(p, k.lane, k.w & 1, u);
         else  // exact: the values are bf16
-          *reinterpret_cast<u32x2 *>(upl[b][ct] + 1024 * (w >> 1) + 16 * lane + 8 * (w & 1)) =
+          *reinterpret_cast<u32x2 *>(p + 16 * k.lane + 8 * (k.w & 1)) =
               __builtin_bit_cast(u32x2, __builtin_convertvector(u, bf16x4));
-        put_half(epl[b][ct] + 3072 * (w >> 1), lane, w & 1, u * x.end);
+        k.put_tokens(epl[b], ct, u * end);
       }
-    };
-    auto walk = [&](int b) {
-      frag tf[TI][2][NP];
-#pragma unroll
-      for (int i = 0; i < TI; ++i)
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          if constexpr (!kKeysPacked) drop_inactive(cur.act, ks, g, o.t[i][ks].b);
-          to_frag<T>(o.t[i][ks], tf[i][ks]);
-        }
-      const float decay = o.whole;
-      fetch_keys(ahead);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        frag e[2][3];
-        load_frag<3>(epl[b][ct], lane, e[0]);
-        load_frag<3>(epl[b][ct] + 3072, lane, e[1]);
-        typedef Products<NP, 3> P;
-#pragma unroll
-        for (int i = 0; i < TI; ++i) S[ct][i] *= decay;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int p = 0; p < P::n; ++p)
-#pragma unroll
-            for (int i = 0; i < TI; ++i)
-              S[ct][i] = mfma_16x16x32_bf16(tf[i][ks][P::a(p)], e[ks][P::b(p)], S[ct][i]);
-      }
-      put_values(b ^ 1, next.act);
-      advance();
-      fetch_values(ahead);
-      put_state(b ^ 1);
-      lds_barrier();
     };
     if (cur.at >= 0) {
       fetch_values(cur.at);
-      fetch_keys(cur.at);
+      state.fetch(k, ws, cur.at);
       put_values(0, cur.act);
       fetch_values(ahead);
     }
-    put_state(0);
+    state.put(k, spl[0]);
     lds_barrier();
-    for (int b = 0; cur.at >= 0; b ^= 1) walk(b);
-    if (a.state_out && owner) {
-      const Rsrc to = buffer_rsrc(a.state_out + rh * a.dk * a.dv, state_bytes);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int i = 0; i < TI; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            buffer_store1(S[ct][i][e], to, state_off(ct) + (16 * i + e) * a.dv * 4, 0);
+    for (int b = 0; cur.at >= 0; b ^= 1) {
+      state.update(k, epl[b], cur.act, [&] { state.fetch(k, ws, ahead); });
+      put_values(b ^ 1, next.act);
+      advance();
+      fetch_values(ahead);
+      state.put(k, spl[b ^ 1]);
+      lds_barrier();
     }
+    state.store(k, a);
   } else {
-    const Rsrc out = buffer_rsrc(a.out + col0, mine * 4);
-    struct Queries {
-      Stored<T> q[NK];
-      frag scores[2][3];
-      f32x4 start;
-    } o;
-    auto fetch_rows = [&](int at) {
-      const unsigned char *p = packed + (size_t)at * (kParts * kPart) + SB * NK * w;
+    const Rsrc out = k.outputs(a);
+    Stored<T> rows[W::NK];
+    frag scores[2][3];
+    f32x4 start;
+    if (cur.at >= 0) {
+      k.fetch_rows(cur.at, W::kQueries, rows);
+      start = k.factor(cur.at, 0);
+      k.fetch_tri(cur.at, W::kScores, scores);
+    }
+    lds_barrier();
+    for (int b = 0; cur.at >= 0; b ^= 1) {
+      f32x4 O[CT];
+      k.times_state(rows, spl[b], O);
 #pragma unroll
-      for (int kk = 0; kk < NK; ++kk) load_stored<T>(p + SB * kk, lane, o.q[kk]);
-      o.start = *reinterpret_cast<const f32x4 *>(factors + (size_t)at * 3 * kC + 16 * w + 4 * g);
-    };
-    auto fetch_scores = [&](int at) {
-      const unsigned char *p = ws.planes + (rh * nch + at) * kTri;
-      load_frag<3>(p + 3072 * tri_block(w, 0), lane, o.scores[0]);
-      if (w >= 2) load_frag<3>(p + 3072 * tri_block(w, 1), lane, o.scores[1]);
-    };
-    auto walk = [&](int b) {
-      f32x4 O[CT][2] = {};  // even and odd steps in accumulators of their own
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk) {
-        frag s[CT][3], f[NP];
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) load_frag<3>(spl[b][ct] + 3072 * kk, lane, s[ct]);
-        to_frag<T>(o.q[kk], f);
-        typedef Products<NP, 3> P;
-#pragma unroll
-        for (int p = 0; p < P::n; ++p)
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
-            O[ct][kk & 1] = mfma_16x16x32_bf16(f[P::a(p)], s[ct][P::b(p)], O[ct][kk & 1]);
-      }
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) O[ct][0] = o.start * (O[ct][0] + O[ct][1]);
-      fetch_rows(ahead);
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        if (ks && w < 2) continue;
-        frag u[CT][NP];
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) load_frag<NP>(upl[b][ct] + 1024 * NP * ks, lane, u[ct]);
-        typedef Products<3, NP> P;
-#pragma unroll
-        for (int p = 0; p < P::n; ++p)
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
-            O[ct][0] = mfma_16x16x32_bf16(o.scores[ks][P::a(p)], u[ct][P::b(p)], O[ct][0]);
-      }
-      fetch_scores(ahead);
-      const int t0 = cur.at * kC, n = a.L - t0 - 16 * w - 4 * g;
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const int off = (row_off + t0 + 16 * ct * a.L) * 4;
-        const f32x4 y = O[ct][0] * a.scale;
-        if (t0 + kC <= a.L) {
-          buffer_store4(y, out, off, 0);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) buffer_store1(y[e], out, e < n ? off + 4 * e : kNowhere, 0);
-        }
-      }
+      for (int ct = 0; ct < CT; ++ct) O[ct] = start * O[ct];
+      k.fetch_rows(ahead, W::kQueries, rows);
+      start = k.factor(ahead, 0);
+      k.template add_tri<NP>(scores, upl[b][0], sizeof(upl[b][0]), O);
+      k.fetch_tri(ahead, W::kScores, scores);
+      k.store(out, cur.at, a.scale, O);
       lds_barrier();
       advance();
-    };
-    if (cur.at >= 0) {
-      fetch_rows(cur.at);
-      fetch_scores(cur.at);
     }
-    lds_barrier();
-    for (int b = 0; cur.at >= 0; b ^= 1) walk(b);
   }
 }
 
 // Kernel and column tiles per workgroup by how the grid fills the CUs (us for prompts of
 // 512 tokens, 16 heads of 128 x 128 unless stated, both kernels). With the delta rule
 //   the path kernel with one tile if every workgroup then has a CU to itself (2 x 8192 in
-//   bf16: 394, two tiles 511), with two while one tile would put two on a CU (4 rows: 59,
+//   bf16: 404, two tiles 511), with two while one tile would put two on a CU (4 rows: 58,
 //   one 75, four waves 73) and for bf16 keys over 128 wide (8 x 1024 with 8 heads of 256 x
-//   256: 177, four waves 195);
+//   256: 181, four waves 195);
 //   beyond that four waves, two or more workgroups a CU: every operand is loaded and
 //   split for four tiles at once with f32 keys of 65 to 128, where the splitting weighs
-//   most (16 rows: 215, two tiles 343, which spill, the path kernel 238), for two
-//   otherwise (16 rows in bf16: 156, four tiles 171, the path kernel 173; 32 rows of 64 x
-//   64 f32: 208, 210, 213);
+//   most (16 rows: 220, two tiles 343, which spill, the path kernel 238), for two
+//   otherwise (16 rows in bf16: 160, four tiles 171, the path kernel 173; 32 rows of 64 x
+//   64 f32: 214, 210, 213);
 //   f32 keys over 128 wide, whose state is half the work, on eight waves that share it
-//   (8 x 1024 with 8 heads of 256 x 256: 275, the path kernel 311; 1 x 4096 301 and 318).
+//   (8 x 1024 with 8 heads of 256 x 256: 279, the path kernel 311; 1 x 4096 306 and 318).
 // Without it one tile each if every workgroup has a CU to itself (2 x 8192: 404 us, two
 // tiles 448; bf16 275 and 355), else two (4 rows: 43, one 51; 16 rows: 167, 195; 8 x 1024
 // with 8 heads of 256 x 256 bf16: 111, 124); two chunks ahead brought nothing.

@@ -1662,7 +1662,8 @@ int log_probs_run(tfd_ctx *c, bool bf16, const void *logits, size_t vocab, size_
     const size_t stats = (4 * sizeof(float) * parts + 255) & ~(size_t)255;
     if ((rc = reserve_capturable(c, op, c->readout, stats + 8 * parts * top, capturing))) return rc;
     a.part_stats = static_cast<float *>(c->readout.ptr);
-    a.part_keys = reinterpret_cast<unsigned long long *>(static_cast<char *>(c->readout.ptr) + stats);
+    a.part_keys =
+        reinterpret_cast<unsigned long long *>(static_cast<char *>(c->readout.ptr) + stats);
   }
   tfd::KernelEvents ev;
   if (!capturing && (rc = timing_events(c, &ev))) return rc;

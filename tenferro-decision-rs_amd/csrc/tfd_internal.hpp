@@ -360,10 +360,10 @@ __host__ __device__ inline int linear_steps(int dk) {
   return dk <= 32 ? 1 : dk <= 64 ? 2 : dk <= 128 ? 4 : 8;
 }
 // Workspace of launch_linear_chunks: per (row, key head, chunk) the queries by tokens,
-// the keys by features (unless they are read in place) and (delta rule) by tokens as operands; per (row,
-// head, chunk) the decayed scores (with the delta rule also the solve operand after them)
-// and 64 factors each from the chunk's start, to its end and beta; per (row, chunk) the
-// active tokens.
+// the keys by features (left out where they are read in place) and (delta rule) by tokens
+// as operands; per (row, head, chunk) the decayed scores (with the delta rule also the
+// solve operand after them) and 64 factors each from the chunk's start, to its end and
+// beta; per (row, chunk) the active tokens.
 struct LinearWork {
   unsigned char *packed, *planes;
   float *factors;
