@@ -796,7 +796,6 @@ struct StateTiles {
 #pragma unroll
         for (int i = 0; i < TI; ++i) S[ct][i] += D[i];
     }
-    __builtin_amdgcn_sched_barrier(0);  // loads behind this find the keys' registers free
   }
   __device__ __forceinline__ void put(const W &k, typename W::State *spl) const {
     if (!owner()) return;
@@ -901,6 +900,7 @@ void linear_delta_kernel(LinearArgs a, LinearWork ws) {
     fetch_values(far);
     // The state first: the next chunk waits for it.
     state.update(k, epl, cur.act, [] {});
+    __builtin_amdgcn_sched_barrier(0);  // the loads find the keys' registers free
     state.fetch(k, ws, far);
     if (kRoles) {  // only the side waits for what comes next
       state.put(k, spl);
@@ -981,6 +981,7 @@ __global__ __launch_bounds__(512, 2) void linear_delta_path_kernel(LinearArgs a,
       lds_barrier();
       end = k.factor(ahead, 1);
       state.update(k, epl, cur.act, [] {});
+      __builtin_amdgcn_sched_barrier(0);  // the loads find the keys' registers free
       state.fetch(k, ws, ahead);
       state.put(k, spl[b ^ 1]);
       lds_barrier();
