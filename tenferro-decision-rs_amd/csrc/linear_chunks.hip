@@ -39,6 +39,7 @@ constexpr double kLog2eD = 1.4426950408889634;
 constexpr float kForget = -104.0f;
 
 typedef bf16x8 frag;
+constexpr int kPieces = 3 * 1024;  // bytes of a block's three pieces
 
 // Contraction index of element e (0..7) of lane group g within a step of 32.
 __device__ __forceinline__ int slot_index(int g, int e) { return 16 * (e >> 2) + 4 * g + (e & 3); }
@@ -453,7 +454,7 @@ __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearW
     if (ks && wave < 2) continue;
     frag p[3];
     split8(score[2 * ks], score[2 * ks + 1], p);
-    store_frag<3>(planes + 3072 * tri_block(wave, ks), lane, p);
+    store_frag<3>(planes + kPieces * tri_block(wave, ks), lane, p);
   }
   if constexpr (DELTA) {
     {  // diagonal block: lane c16 holds that column of the inverse
@@ -495,7 +496,7 @@ __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearW
       const float *x = X + (16 * tt + c16) * kS + 32 * ks + 4 * g;
       frag p[3];
       split8(*reinterpret_cast<const f32x4 *>(x), *reinterpret_cast<const f32x4 *>(x + 16), p);
-      store_frag<3>(planes + kTri + 3072 * b, lane, p);
+      store_frag<3>(planes + kTri + kPieces * b, lane, p);
     }
   }
 }
@@ -556,7 +557,7 @@ struct Walk {
   static constexpr int kPlanes = DELTA ? 2 * kTri : kTri;
   enum { kQueries, kByFeature, kKeys };  // parts of `packed`
   enum { kScores, kSolve };              // of `planes`
-  typedef unsigned char State[NK * 3 * 1024], Tokens[6 * 1024];  // LDS, a column tile's
+  typedef unsigned char State[NK * kPieces], Tokens[2 * kPieces];  // LDS, a column tile's
 
   int lane, g, c16, wave, w, nch, L;
   int r, h, j;  // row, head, first value column
@@ -603,8 +604,8 @@ struct Walk {
   __device__ __forceinline__ void fetch_tri(int at, int which, frag (&f)[2][3]) const {
     const unsigned char *p = planes + (size_t)at * kPlanes + which * kTri;
     frag first[3];  // stored behind the branch, which would else wait for it
-    load_frag<3>(p + 3072 * tri_block(w, 0), lane, first);
-    if (w >= 2) load_frag<3>(p + 3072 * tri_block(w, 1), lane, f[1]);
+    load_frag<3>(p + kPieces * tri_block(w, 0), lane, first);
+    if (w >= 2) load_frag<3>(p + kPieces * tri_block(w, 1), lane, f[1]);
 #pragma unroll
     for (int i = 0; i < 3; ++i) f[0][i] = first[i];
   }
@@ -626,7 +627,7 @@ struct Walk {
     return v;
   }
   __device__ __forceinline__ void put_tokens(Tokens *to, int ct, f32x4 x) const {
-    put_half(to[ct] + 3072 * (w >> 1), lane, w & 1, x);
+    put_half(to[ct] + kPieces * (w >> 1), lane, w & 1, x);
   }
   // rows S0, the steps in XA accumulators.
   __device__ __forceinline__ void times_state(const Stored<T> (&rows)[NK], const State *spl,
@@ -637,7 +638,7 @@ struct Walk {
     for (int kk = 0; kk < NK; ++kk) {
       frag s[CT][3], f[NP];
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) load_frag<3>(spl[ct] + 3072 * kk, lane, s[ct]);
+      for (int ct = 0; ct < CT; ++ct) load_frag<3>(spl[ct] + kPieces * kk, lane, s[ct]);
       to_frag<T>(rows[kk], f);
       typedef Products<NP, 3> P;
 #pragma unroll
@@ -744,8 +745,8 @@ struct StateTiles {
   __device__ __forceinline__ void fetch(const W &k, const LinearWork &ws, int at) {
     whole = ws.factors[(k.rh * k.nch + at) * 3 * kC + kC - 1];
     if (!owner()) return;
-    const unsigned char *p =
-        k.packed + (size_t)at * (W::kParts * W::kPart) + W::kByFeature * W::kPart + 2 * W::SB * tile0;
+    const unsigned char *p = k.packed + (size_t)at * (W::kParts * W::kPart) +
+                             W::kByFeature * W::kPart + 2 * W::SB * tile0;
 #pragma unroll
     for (int i = 0; i < TI; ++i)
 #pragma unroll
@@ -778,7 +779,7 @@ struct StateTiles {
     for (int ct = 0; ct < CT; ++ct) {
       frag e[2][3];
       load_frag<3>(epl[ct], k.lane, e[0]);
-      load_frag<3>(epl[ct] + 3072, k.lane, e[1]);
+      load_frag<3>(epl[ct] + kPieces, k.lane, e[1]);
       f32x4 D[TI] = {};
 #pragma unroll
       for (int i = 0; i < TI; ++i) S[ct][i] *= decay;
@@ -803,7 +804,7 @@ struct StateTiles {
     for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
       for (int i = 0; i < TI; ++i)
-        put_half(spl[ct] + 3072 * ((tile0 + i) >> 1), k.lane, (tile0 + i) & 1, S[ct][i]);
+        put_half(spl[ct] + kPieces * ((tile0 + i) >> 1), k.lane, (tile0 + i) & 1, S[ct][i]);
   }
 };
 
@@ -865,7 +866,7 @@ void linear_delta_kernel(LinearArgs a, LinearWork ws) {
     for (int kk = 0; kk < NK; ++kk) {
       frag s[CT][3], f[NP], fk[NP];
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) load_frag<3>(spl[ct] + 3072 * kk, k.lane, s[ct]);
+      for (int ct = 0; ct < CT; ++ct) load_frag<3>(spl[ct] + kPieces * kk, k.lane, s[ct]);
       to_frag<T>(rows[kk], f);
       if constexpr (!kRoles) to_frag<T>(krows[kk], fk);
       typedef Products<NP, 3> P;

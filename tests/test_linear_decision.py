@@ -136,3 +136,44 @@ def test_prompt_readout_and_steps(bf16):
     # The ended row kept its state, the empty prompt began with a uniform answer.
     np.testing.assert_array_equal(outs[1 + ENDED[1]][ENDED[0]], 0)
     assert np.array_equal(got[0][2].reshape(R, TOP)[3], np.arange(TOP))
+
+
+@pytest.mark.gpu
+def test_two_contexts_at_once():
+    """Prompts and readouts of two contexts on two streams, in flight together: each
+    has its own workspaces, so the results are those of either alone."""
+    import torch
+
+    def problem(seed, rows, length, heads, dk, dv, vocab):
+        rng = Lcg(seed)
+        normal = lambda *s: cuda(rng.normal(int(np.prod(s))).astype(np.float32))
+        dims = (rows, length, heads, heads, dk, dv)
+        kv = [normal(rows, heads, n, length) / np.sqrt(dk) for n in (dk, dk, dv)]
+        gates = [-normal(rows, heads, length).abs(), torch.sigmoid(normal(rows, heads, length))]
+        logits = normal(rows * heads, vocab)
+
+        def run(ctx):
+            out, state = te.jeff_linear_attention_rows(*kv, *gates, None, *dims, ctx=ctx)
+            return (out, state, *te.token_log_probs(logits, None, rows * heads, vocab, top=4,
+                                                    ctx=ctx)[1:])
+        return run
+
+    runs = [problem(3, 2, 700, 8, 128, 128, 70001), problem(4, 24, 200, 8, 64, 96, 50000)]
+    streams = [torch.cuda.Stream() for _ in runs]
+    with te.Context(0, stream=streams[0].cuda_stream) as a, \
+            te.Context(0, stream=streams[1].cuda_stream) as b:
+        alone = []
+        for run, ctx, stream in zip(runs, (a, b), streams):
+            with torch.cuda.stream(stream):
+                alone.append([host(x) for x in run(ctx)])
+        torch.cuda.synchronize()
+        together = [[], []]
+        with te.asynchronous():
+            for _ in range(6):
+                for i, (run, ctx, stream) in enumerate(zip(runs, (a, b), streams)):
+                    with torch.cuda.stream(stream):
+                        together[i].append(run(ctx))
+        torch.cuda.synchronize()
+    for want, tries in zip(alone, together):
+        for got in tries:
+            assert all(np.array_equal(host(x), y) for x, y in zip(got, want))
