@@ -12,9 +12,10 @@
 // The `top` largest logits: every wave keeps its best 64 so far sorted across
 // its lanes, as unique 64-bit keys (value order, then the lower index first),
 // and compares the 16 bytes' maximum, which the softmax needs anyway, with
-// the top-th of them. What passes is collected in LDS and merged 64 at a time
-// by a bitonic network; for logits in random order that is a few merges in a
-// row of 10^5.
+// the top-th of them (of any of the position's waves: 1024 x 131072 bf16, top 5, 104
+// us with each wave's own, 82 with the highest). What passes is collected in LDS and
+// merged 64 at a time by a bitonic network; for logits in random order that is a few
+// merges in a row of 10^5.
 //
 // Bound by reading the logits. A position goes to one wave up to 2048 logits,
 // to one workgroup of four waves past that, and to several workgroups (joined
@@ -127,6 +128,10 @@ struct TopList {
   __device__ __forceinline__ void start(u64 most, int lane) {
     bar = key_at(sort64(most, lane), top - 1);
   }
+  __device__ __forceinline__ void raise(u64 other) {
+    other = key_at(other, 0);
+    bar = other > bar ? other : bar;
+  }
   // One key a lane (0: none). Keys are unique; the bar itself may still come.
   __device__ __forceinline__ void push(u64 key, int lane) {
     u64 pass = __ballot(key >= bar && key != 0);
@@ -204,6 +209,7 @@ __global__ __launch_bounds__(64 * NW) void log_probs_kernel(LogProbArgs a) {
   constexpr int U = 4;             // 16-byte pieces in flight per lane
   __shared__ u64 buf[NW][64];
   __shared__ float stats[NW][3];
+  __shared__ u64 bars;  // the highest of the waves' bars so far, a bar for all of them
   const int lane = threadIdx.x & 63, wave = NW == 1 ? 0 : threadIdx.x >> 6;
   const long pos = blockIdx.x / (unsigned)a.parts;
   const int part = (int)(blockIdx.x - (unsigned)pos * (unsigned)a.parts);
@@ -219,8 +225,11 @@ __global__ __launch_bounds__(64 * NW) void log_probs_kernel(LogProbArgs a) {
   TopList list;
   list.top = a.top;
   list.buf = buf[wave];
-  float bar_value = NAN;  // the bar's value, NaN while there is none
   bool begun = false;
+  if constexpr (TOP && NW > 1) {
+    if (threadIdx.x == 0) bars = 0;
+    __syncthreads();
+  }
 
   for (int p = p0 + wave * 64 + lane; p - lane < p1; p += 64 * NW * U) {
     float x[U][E];
@@ -281,18 +290,21 @@ __global__ __launch_bounds__(64 * NW) void log_probs_kernel(LogProbArgs a) {
             most = k > most ? k : most;
           }
         list.start(most, lane);
+        begun = true;
       }
+      if constexpr (NW > 1) {
+        if (lane == 0) atomicMax(&bars, list.bar);
+        list.raise(*const_cast<volatile u64 *>(&bars));
+      }
+      // Values are compared first: few keys are ever made.
+      const float bar_value = list.bar ? code_value((uint32_t)(list.bar >> 32)) : NAN;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        // Indices grow from piece to piece of a wave, so after its first pieces a
-        // value equal to the bar's comes too late; within the pieces the key decides.
-        const bool some = begun ? !(mx[u] <= bar_value) : true;
-        if (!__any(p + u * 64 * NW < p1 && some)) continue;
+        if (!__any(p + u * 64 * NW < p1 && !(mx[u] < bar_value))) continue;
 #pragma unroll
-        for (int e = 0; e < E; ++e) list.push(key(u, e), lane);
+        for (int e = 0; e < E; ++e)
+          if (__any(!(x[u][e] < bar_value))) list.push(key(u, e), lane);
       }
-      begun = true;
-      bar_value = list.bar ? code_value((uint32_t)(list.bar >> 32)) : NAN;
     }
   }
   s = wave_join(s);
@@ -389,7 +401,12 @@ void launch_parts(const LogProbArgs &a, int waves, hipStream_t stream, const Ker
 
 }  // namespace
 
-// Fewest 16-byte pieces of a part: one step of a workgroup's four waves. Fewer spread
+// Positions of up to so many 16-byte pieces stay whole: the join is a launch more and a
+// wave that reads what the others left (16 x 5000 f32, 1250 pieces: 4.1 us whole, 10.8
+// in two parts, with top 5 9.1 and 15.4; 256 x 32000 bf16, 4000 pieces: 8.7 and 11.9,
+// but with top 20 26.0 and 25.5, and 16 of them 25.5 and 19.1).
+constexpr size_t kLogProbWhole = 8192, kLogProbWholeTop = 2048;
+// Fewest pieces of a part: one step of a workgroup's four waves. Fewer spread
 // a position further, but every wave has to find its first `top` and the joining
 // wave reads them all (bf16, 100003 logits, top 20: 21.0 us with 256 pieces, 19.0 with
 // 512, 19.6 with 1024, 22.5 with 2048; 4 x 151936 f32, top 50: 61, 44, 30, 27).
@@ -400,7 +417,7 @@ void log_probs_plan(LogProbArgs &a, int cus) {
   const size_t pieces = (a.vocab + 2 * (per_piece - 1)) / per_piece;  // at any skew
   a.parts = 1;
   a.part_pieces = (int)pieces;
-  if (a.vocab <= kLogProbWaveVocab) return;
+  if (a.vocab <= kLogProbWaveVocab || pieces <= (a.top ? kLogProbWholeTop : kLogProbWhole)) return;
   // Parts of kLogProbPart pieces or more, until every CU has two workgroups.
   const size_t want = a.positions ? (2 * (size_t)cus + a.positions - 1) / a.positions : 1;
   const size_t most = (pieces + kLogProbPart - 1) / kLogProbPart;
