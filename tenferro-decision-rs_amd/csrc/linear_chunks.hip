@@ -678,12 +678,17 @@ struct Walk {
     }
     if constexpr (CT == 1) U[0] += A[0];
   }
-  __device__ __forceinline__ void store(Rsrc out, int at, float scale, const f32x4 (&O)[CT]) const {
-    const int t0 = at * kC, n = L - t0 - 16 * w - 4 * g;
+  // 0 for inactive tokens, whose queries are 0, but 0 times a state that is not finite is not.
+  __device__ __forceinline__ void store(Rsrc out, const Chunk &c, float scale,
+                                        const f32x4 (&O)[CT]) const {
+    const int t0 = c.at * kC, n = L - t0 - 16 * w - 4 * g;
+    const unsigned on = (unsigned)(c.act >> (16 * w + 4 * g));
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       const int off = (row_off + t0 + 16 * ct * L) * 4;
-      const f32x4 y = O[ct] * scale;
+      f32x4 y = O[ct] * scale;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = (on >> e) & 1u ? y[e] : 0.0f;
       if (t0 + kC <= L) {
         buffer_store4(y, out, off, 0);
       } else {
@@ -910,7 +915,7 @@ void linear_delta_kernel(LinearArgs a, LinearWork ws) {
     if (side) k.template add_tri<3>(tri, upl[0], sizeof(upl[0]), O[0]);
     if (!kRoles) state.put(k, spl);
     fetch_tri(far);
-    if (side) k.store(out, cur.at, a.scale, O[0]);
+    if (side) k.store(out, cur, a.scale, O[0]);
     if (!kRoles) lds_barrier();
     cur = next;
     next = chunks.next();
@@ -1003,7 +1008,7 @@ __global__ __launch_bounds__(512, 2) void linear_delta_path_kernel(LinearArgs a,
       k.template add_tri<3>(tri, upl[b][0], sizeof(upl[b][0]), O);
       k.fetch_tri(ahead, W::kScores, tri);
       between();
-      k.store(out, cur.at, a.scale, O);
+      k.store(out, cur, a.scale, O);
       between();
       advance();
     };
@@ -1106,7 +1111,7 @@ __global__ __launch_bounds__(512, 2) void linear_plain_kernel(LinearArgs a, Line
       start = k.factor(ahead, 0);
       k.template add_tri<NP>(scores, upl[b][0], sizeof(upl[b][0]), O);
       k.fetch_tri(ahead, W::kScores, scores);
-      k.store(out, cur.at, a.scale, O);
+      k.store(out, cur, a.scale, O);
       lds_barrier();
       advance();
     }

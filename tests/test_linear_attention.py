@@ -436,3 +436,39 @@ def test_the_longest_chunked_row_and_past_it(gpu_ctx, length):
     got = part(out.view(1, H, dv, length))
     assert (np.abs(got - want) <= tol * size)[..., 200:].all()
     assert (np.abs(state.view(1, H, dk, dv).cpu().numpy() - S) <= tol * A).all()
+
+
+# Shapes whose prompts take, of the delta rule: the token-by-token kernel, the path kernel on
+# one and two column tiles, four waves on two and four tiles, eight waves on one and two; the
+# same shapes without it: the plain kernel on one and two tiles.
+EVERY_KERNEL = [(2, 5, 4, 2, 40, 24), (2, 150, 4, 2, 40, 24), (5, 90, 8, 4, 50, 100),
+                (5, 90, 8, 4, 50, 213), (5, 90, 8, 4, 100, 213), (2, 150, 4, 2, 200, 24),
+                (5, 90, 8, 4, 200, 213)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("delta", [True, False], ids=["delta", "plain"])
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", EVERY_KERNEL, ids=str)
+def test_inactive_tokens_beside_inf_and_nan(gpu_ctx, shape, bf16, delta):
+    """A state and active tokens that hold inf and NaN: the outputs of inactive tokens are 0
+    all the same, and a value column without any of it has the bits it had before."""
+    R, L, H, HK, dk, dv = shape
+    p = Problem(*shape, bf16=bf16, delta=delta, mask="holes", state=True, decay=0.1)
+    p.mask[:, 1], p.mask[:, 2] = 1.0, 0.0
+    clean = [host(x) for x in p.run(gpu_ctx, cuda)]
+    p.state[:, :, dk // 2, 3], p.state[:, :, 0, 4] = np.inf, np.nan
+    p.v[:, :, 5, 1], p.v[:, :, 6, 1] = np.nan, -np.inf
+    out, state = [host(x) for x in p.run(gpu_ctx, cuda)]
+    off = p.mask == 0
+    tokens = lambda x: np.moveaxis(x.reshape(R, H, dv, L), 3, 1)  # (R, L, H, dv)
+    assert (tokens(out)[off] == 0).all()
+    whole = [j for j in range(dv) if j not in (3, 4, 5, 6)]
+    assert np.array_equal(tokens(out)[..., whole], tokens(clean[0])[..., whole])
+    cols = lambda x: x.reshape(R, H, dk, dv)[..., whole]
+    assert np.array_equal(cols(state), cols(clean[1]))
+    last = tokens(out)[np.arange(R), [np.flatnonzero(m)[-1] for m in p.mask]]
+    assert not np.isfinite(last[..., 3:7]).any()
+    p.k[:, :, 0, 1] = np.nan  # every column of the heads from here on
+    out = host(p.run(gpu_ctx, cuda)[0])
+    assert (tokens(out)[off] == 0).all()
