@@ -639,6 +639,16 @@ def jeff_full_attention_rows(q, k, v, gate, q_norm, k_norm, mask, rows: int, len
 
 # ------------------------------------------------------------------ linear attention
 
+def _check_result(x, name: str) -> None:
+    """Refuses a host buffer that results would not reach: anything but a contiguous
+    float32 array is converted, and what is written then is the copy."""
+    if not _is_torch(x) and not (
+            isinstance(x, np.ndarray) and x.dtype == np.float32
+            and x.flags.c_contiguous and x.flags.writeable):
+        raise InvalidArgument(
+            TFD_EINVAL, f"{name}: expected a contiguous float32 array to update")
+
+
 def jeff_linear_attention_rows(q, k, v, log_decay, beta, mask, rows: int, length: int, heads: int,
                                key_heads: int, key_dim: int, value_dim: int, *,
                                scale: Optional[float] = None, state=None, state_out=None,
@@ -655,7 +665,8 @@ def jeff_linear_attention_rows(q, k, v, log_decay, beta, mask, rows: int, length
     features contiguous. ``scale`` is 1/sqrt(key_dim) if None. ``state`` None starts
     from zeros; ``state_out`` may be ``state`` itself. bf16 takes q, k and v as
     bf16 bits. Returns (out, state after the last token), the state None unless
-    ``want_state`` or given a ``state_out``."""
+    ``want_state`` or given a ``state_out``. ``out`` and ``state_out`` are written where
+    they are: float32, contiguous."""
     ctx = ctx or default_context()
     dt = np.uint16 if bf16 else np.float32
     nk, nv = rows * length * key_heads * key_dim, rows * length * heads * value_dim
@@ -671,14 +682,17 @@ def jeff_linear_attention_rows(q, k, v, log_decay, beta, mask, rows: int, length
         out = _new_out(aq, nv)
         out_ptr = _ptr(out)
     else:
+        _check_result(out, "out")
         args.append(_Arg(out, np.float32, "out", nv))
         out, out_ptr = args[-1].obj, args[-1].ptr
     if state_out is None:
         state_out = _new_out(aq, ns) if want_state else None
         state_ptr = _ptr(state_out)
     elif state_out is state:
-        state_out, state_ptr = asi.obj, asi.ptr
+        _check_result(state, "state")
+        state_ptr = asi.ptr
     else:
+        _check_result(state_out, "state_out")
         args.append(_Arg(state_out, np.float32, "state_out", ns))
         state_out, state_ptr = args[-1].obj, args[-1].ptr
     flags = _flags(args, ctx)
@@ -698,10 +712,7 @@ def jeff_linear_attention_step(q, k, v, log_decay, beta, state, rows: int, heads
     """``jeff_linear_attention_rows`` for one token a row: ``state`` (f32, contiguous)
     is updated in place, also that of rows past a ``mask`` of zeros, which keep
     theirs. Returns out, rows x (heads*value_dim)."""
-    if not _is_torch(state) and not (
-            isinstance(state, np.ndarray) and state.dtype == np.float32
-            and state.flags.c_contiguous and state.flags.writeable):
-        raise InvalidArgument(TFD_EINVAL, "state: expected a contiguous float32 array to update")
+    _check_result(state, "state")
     return jeff_linear_attention_rows(q, k, v, log_decay, beta, mask, rows, 1, heads, key_heads,
                                       key_dim, value_dim, scale=scale, state=state,
                                       state_out=state, bf16=bf16, ctx=ctx, out=out)[0]

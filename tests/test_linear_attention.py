@@ -166,6 +166,35 @@ def test_refusals_before_any_device_call(ctx):
                                       dk, dv, ctx=ctx)
 
 
+def test_results_are_not_written_to_a_copy(ctx):
+    """A host array that would have to be converted is refused as a place for results, and
+    keeps what it holds; the caller would never see the copy that is written."""
+    R, L, H, dk, dv = 2, 3, 2, 4, 5
+    f = lambda n: np.zeros(n, np.float32)
+    nv, ns = R * L * H * dv, R * H * dk * dv
+    ops = (f(R * L * H * dk), f(R * L * H * dk), f(nv), f(R * L * H), None, None, R, L, H, H, dk, dv)
+
+    def wrong(n):
+        fixed = f(n)
+        fixed.flags.writeable = False
+        return [np.zeros(n), f(2 * n)[::2], fixed, [0.0] * n]
+
+    for x in wrong(nv):
+        with pytest.raises(te.InvalidArgument, match="out: expected a contiguous float32 array"):
+            te.jeff_linear_attention_rows(*ops, out=x, ctx=ctx)
+    for x in wrong(ns):
+        with pytest.raises(te.InvalidArgument, match="state_out: expected a contiguous float32"):
+            te.jeff_linear_attention_rows(*ops, state_out=x, ctx=ctx)
+        with pytest.raises(te.InvalidArgument, match="state: expected a contiguous float32"):
+            te.jeff_linear_attention_rows(*ops, state=x, state_out=x, ctx=ctx)
+        with pytest.raises(te.InvalidArgument, match="state: expected a contiguous float32"):
+            te.jeff_linear_attention_step(f(R * H * dk), f(R * H * dk), f(R * H * dv), f(R * H), None,
+                                          x, R, H, H, dk, dv, ctx=ctx)
+    with pytest.raises(te.InvalidArgument, match="state: expected a contiguous float32"):
+        te.jeff_linear_attention_step(f(R * H * dk), f(R * H * dk), f(R * H * dv), f(R * H), None,
+                                      None, R, H, H, dk, dv, ctx=ctx)
+
+
 def test_empty_problems_need_no_gpu(ctx):
     z = np.zeros(0, np.float32)
     out, state = te.jeff_linear_attention_rows(z, z, z, z, None, None, 0, 5, 2, 1, 4, 4, ctx=ctx)
