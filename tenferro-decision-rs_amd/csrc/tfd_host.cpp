@@ -1491,7 +1491,8 @@ int laya_forward(tfd_ctx *c, const tfd_laya_model *m, const int64_t *ids, const 
 constexpr size_t kLinearRecurrentF32 = 10, kLinearRecurrentBf16 = 6;
 // Workspace of the chunked form that is not passed while one row fits it.
 constexpr size_t kLinearWorkspace = (size_t)2 << 30;
-// Workgroups of a launch, likewise: 512 threads each, and a grid may have 2^32.
+// Workgroups of a launch: 512 threads each, and a grid may have 2^32. One head, of at most
+// 4096 column tiles, always fits.
 constexpr size_t kLinearBlocks = (size_t)1 << 22;
 
 int linear_run(tfd_ctx *c, bool bf16, size_t rows, size_t length, size_t heads, size_t key_heads,
@@ -1565,34 +1566,52 @@ int linear_run(tfd_ctx *c, bool bf16, size_t rows, size_t length, size_t heads, 
     if (!capturing && (rc = timing_events(c, &ev))) return rc;
     TFD_HIP(c, tfd::launch_linear_recurrent(a, c->stream, ev), "linear_recurrent launch");
   } else {
-    // As many rows at once as the workspace limit allows, at least one.
+    // As many rows at once as the limits allow, at least one. Where one row's blocks
+    // already pass theirs, its heads go in runs: whole groups of a key head, or, where a
+    // group is too long for that, parts of one.
+    const size_t tiles = (value_dim + 15) / 16, group = heads / key_heads;
+    size_t run = std::min(heads, kLinearBlocks / tiles);
+    if (run < heads && run > group) run -= run % group;
+    auto heads_of = [&](tfd::LinearArgs &b, size_t n) {
+      b.heads = (int)n;
+      b.key_heads = (int)std::max<size_t>(1, n / group);
+      b.group = (int)std::min(n, group);
+    };
     a.rows = 1;
+    heads_of(a, run);
     const size_t row = tfd::linear_space(a).total();
-    const size_t blocks = heads * ((value_dim + 15) / 16);
-    size_t at_once = std::min(kLinearWorkspace / row, kLinearBlocks / blocks);
+    size_t at_once = run < heads ? 1 : std::min(kLinearWorkspace / row, kLinearBlocks / (heads * tiles));
     at_once = std::min(rows, std::max<size_t>(1, at_once));
     if ((rc = reserve_capturable(c, op, c->linear, row * at_once, capturing))) return rc;
     if (!capturing && (rc = timing_events(c, &ev))) return rc;
     auto from = [](const void *p, size_t bytes) {
       return p ? static_cast<const char *>(p) + bytes : nullptr;
     };
-    for (size_t r0 = 0; r0 < rows; r0 += at_once) {
+    for (size_t r0 = 0, h0 = 0; r0 < rows;) {
       tfd::LinearArgs b = a;
       b.rows = (int)std::min(at_once, rows - r0);
-      b.q = from(q_d, es * (kn / rows) * r0);
-      b.k = from(k_d, es * (kn / rows) * r0);
-      b.v = from(v_d, es * (vn / rows) * r0);
-      const size_t f = sizeof(float);
-      b.log_decay = reinterpret_cast<const float *>(from(g_d, f * (gn / rows) * r0));
-      b.beta = reinterpret_cast<const float *>(from(b_d, f * (gn / rows) * r0));
+      const size_t n = std::min({run, heads - h0, run < group ? group - h0 % group : heads});
+      heads_of(b, n);
+      const size_t rh = r0 * heads + h0, kh = r0 * key_heads + h0 / group, f = sizeof(float);
+      b.q = from(q_d, es * (key_dim * length) * kh);
+      b.k = from(k_d, es * (key_dim * length) * kh);
+      b.v = from(v_d, es * (value_dim * length) * rh);
+      b.log_decay = reinterpret_cast<const float *>(from(g_d, f * length * rh));
+      b.beta = reinterpret_cast<const float *>(from(b_d, f * length * rh));
       b.mask = reinterpret_cast<const float *>(from(m_d, f * length * r0));
-      b.state_in = reinterpret_cast<const float *>(from(si_d, f * (sn / rows) * r0));
-      if (so_d) b.state_out = static_cast<float *>(so_d) + sn / rows * r0;
-      b.out = static_cast<float *>(out_d) + vn / rows * r0;
+      b.state_in = reinterpret_cast<const float *>(from(si_d, f * (key_dim * value_dim) * rh));
+      if (so_d) b.state_out = static_cast<float *>(so_d) + key_dim * value_dim * rh;
+      b.out = static_cast<float *>(out_d) + value_dim * length * rh;
+      const bool first = rh == 0;
+      h0 += n;
+      if (h0 == heads) {
+        h0 = 0;
+        r0 += (size_t)b.rows;
+      }
       TFD_HIP(c,
               tfd::launch_linear_chunks(b, c->linear.ptr, c->stream,
-                                        tfd::KernelEvents{r0 ? nullptr : ev.start,
-                                                          r0 + at_once < rows ? nullptr : ev.stop}),
+                                        tfd::KernelEvents{first ? ev.start : nullptr,
+                                                          r0 < rows ? nullptr : ev.stop}),
               "linear_chunks launch");
     }
   }

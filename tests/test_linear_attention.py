@@ -467,6 +467,57 @@ def test_the_longest_chunked_row_and_past_it(gpu_ctx, length):
     assert (np.abs(state.view(1, H, dk, dv).cpu().numpy() - S) <= tol * A).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("delta,key_heads", [(False, 820), (True, 2)])
+def test_a_row_of_more_columns_than_one_grid_has_threads_for(gpu_ctx, delta, key_heads):
+    """4100 heads of 65536 value features: 2^32 threads and more for one row, whose heads go in
+    runs, of whole groups of a key head (5 heads) and of parts of one (2050 heads)."""
+    import torch
+
+    L, H, dk, dv = 7, 4100, 8, 65536
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    new = lambda *s, **kw: torch.randn(*s, generator=gen, device="cuda", **kw)
+    q, k = (torch.nn.functional.normalize(new(key_heads, dk, L), dim=1).bfloat16() for _ in "qk")
+    v, g = new(H, dv, L, dtype=torch.bfloat16), -new(H, L).abs()
+    beta = torch.rand(H, L, generator=gen, device="cuda") if delta else None
+    mask = torch.tensor([1.0, 1, 0, 1, 1, 1, 1], device="cuda")
+    state = new(H, dk, dv)
+    heads = [0, 4, 5, 1019, 1020, 1023, 1024, 2047, 2048, 2049, 2050, 3073, 3074, 4097, 4098, H - 1]
+    cols = [*range(5), *range(32760, 32775), *range(dv - 20, dv)]
+    part = lambda x: x[heads][:, cols].float().cpu().numpy()[None]
+    of_key = [h // (H // key_heads) for h in heads]
+    p = Problem(1, L, len(heads), len(heads), dk, len(cols), delta=delta)
+    p.q, p.k = (x[of_key].float().cpu().numpy()[None] for x in (q, k))
+    p.v, p.state = part(v), part(state.transpose(1, 2)).transpose(0, 1, 3, 2)
+    p.g, p.mask = g[heads].cpu().numpy()[None], mask.cpu().numpy()[None]
+    p.beta = beta[heads].cpu().numpy()[None] if delta else None
+    flat = [x.reshape(-1) if x is not None else None for x in (q, k, v, g, beta)]
+    out, _ = te.jeff_linear_attention_rows(*flat, mask, 1, L, H, key_heads, dk, dv,
+                                           state=state.view(-1), state_out=state.view(-1),
+                                           bf16=True, ctx=gpu_ctx)
+    p.check(part(out.view(H, dv, L)), part(state.transpose(1, 2)).transpose(0, 1, 3, 2))
+
+
+@pytest.mark.gpu
+def test_single_tokens_of_more_rows_than_two_to_the_32_threads(gpu_ctx):
+    import torch
+
+    R, H, dk, dv = 65535, 260, 1, 32
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    new = lambda *s, **kw: torch.randn(*s, generator=gen, device="cuda", **kw)
+    q, k = (new(R, H, dk).sign().bfloat16() for _ in "qk")
+    v, g = new(R, H, dv, dtype=torch.bfloat16), -new(R, H).abs()
+    beta, state = torch.rand(R, H, generator=gen, device="cuda"), new(R, H, dk, dv)
+    rows = [0, 1, 32767, 32768, 64000, R - 1]
+    part = lambda x: x[rows].float().cpu().numpy()
+    p = Problem(len(rows), 1, H, H, dk, dv)
+    p.q, p.k, p.v, p.g, p.beta = (part(x)[..., None] for x in (q, k, v, g, beta))
+    p.state = part(state)
+    out = te.jeff_linear_attention_step(*(x.reshape(-1) for x in (q, k, v, g, beta)),
+                                        state.view(-1), R, H, H, dk, dv, bf16=True, ctx=gpu_ctx)
+    p.check(part(out.view(R, H, dv, 1)), part(state))
+
+
 # Shapes whose prompts take, of the delta rule: the token-by-token kernel, the path kernel on
 # one and two column tiles, four waves on two and four tiles, eight waves on one and two; the
 # same shapes without it: the plain kernel on one and two tiles.
