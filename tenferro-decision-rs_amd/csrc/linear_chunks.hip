@@ -332,7 +332,7 @@ __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearW
   const int chunk = blockIdx.x, h = blockIdx.y, r = blockIdx.z, nch = gridDim.x;
   const size_t rh = (size_t)r * a.heads + h, at = rh * nch + chunk;
   const int t0 = chunk * kC, n = min(kC, a.L - t0);
-  const int steps = linear_steps(a.dk), parts = DELTA ? 3 : 2;
+  const int steps = linear_steps(a.dk), parts = 1 + DELTA + FEATURES;
   const size_t kh = (size_t)r * a.key_heads + h / a.group;
   const uint32_t bytes = (uint32_t)a.dk * a.L * sizeof(T);
   const Rsrc q = buffer_rsrc(static_cast<const T *>(a.q) + kh * a.dk * a.L, bytes);
@@ -372,7 +372,7 @@ __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearW
   constexpr int SB = Pieces<T>::blocks * 1024;
   const size_t part = (size_t)4 * steps * SB;
   unsigned char *pq = ws.packed + (kh * nch + chunk) * parts * part;
-  unsigned char *pt = pq + part, *pk = pq + 2 * part;
+  unsigned char *pk = pq + part, *pt = pq + (1 + DELTA) * part;
   f32x4 score[4] = {}, keys[4] = {};
   auto slab = [&](int f0, Raw (&x)[2], Raw (&y)[2]) {
     if (f0) lds_barrier();
@@ -510,8 +510,8 @@ __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearW
 // Keys of more features take packed ones (4 x 1024 with 8 heads of 256 x 256 on 2 key
 // heads: 169, in place 179).
 template <typename T>
-constexpr bool keys_in_place(int NI) {
-  return sizeof(T) == 4 && NI <= 8;
+constexpr bool keys_packed(int NI) {
+  return linear_keys_packed(sizeof(T) == 2, NI / 2);
 }
 
 // A row's chunks with an active token, 64 at a time.
@@ -553,9 +553,9 @@ __device__ __forceinline__ void put_half(unsigned char *block, int lane, int hal
 template <typename T, bool DELTA, int NI, int CT>
 struct Walk {
   static constexpr int NP = Pieces<T>::n, NK = NI / 2, SB = Pieces<T>::blocks * 1024;
-  static constexpr int kPart = 4 * NK * SB, kParts = DELTA ? 3 : 2;
+  static constexpr int kPart = 4 * NK * SB, kParts = 1 + DELTA + keys_packed<T>(NI);
   static constexpr int kPlanes = DELTA ? 2 * kTri : kTri;
-  enum { kQueries, kByFeature, kKeys };  // parts of `packed`
+  enum { kQueries, kKeys, kByFeature = 1 + DELTA };  // parts of `packed`
   enum { kScores, kSolve };              // of `planes`
   typedef unsigned char State[NK * kPieces], Tokens[2 * kPieces];  // LDS, a column tile's
 
@@ -705,7 +705,7 @@ template <typename T, bool DELTA, int NI, int CT, int WAVES>
 struct StateTiles {
   typedef Walk<T, DELTA, NI, CT> W;
   static constexpr int TI = NI >= WAVES ? NI / WAVES : 1, NP = W::NP;
-  static constexpr bool kKeysPacked = !keys_in_place<T>(NI);
+  static constexpr bool kKeysPacked = keys_packed<T>(NI);
   f32x4 S[CT][TI];
   Stored<T> t[TI][2];
   float whole;
@@ -1142,7 +1142,7 @@ hipError_t launch(const LinearArgs &a, const LinearWork &ws, hipStream_t stream,
   auto grid = [&](int tiles) { return dim3((unsigned)(heads * ((jtiles + tiles - 1) / tiles))); };
   const bool few = heads * jtiles <= (size_t)a.cus, some = heads * jtiles <= 2 * (size_t)a.cus;
   const dim3 chunks((unsigned)((a.L + kC - 1) / kC), (unsigned)a.heads, (unsigned)a.rows);
-  hipExtLaunchKernelGGL((linear_pairs_kernel<T, DELTA, !keys_in_place<T>(NI)>), chunks, dim3(256),
+  hipExtLaunchKernelGGL((linear_pairs_kernel<T, DELTA, keys_packed<T>(NI)>), chunks, dim3(256),
                         0, stream, ev.start, nullptr, 0, a, ws);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;

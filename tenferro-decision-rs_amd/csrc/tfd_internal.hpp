@@ -359,9 +359,14 @@ constexpr int kLinearTriBytes = 6 * 3 * 1024;
 __host__ __device__ inline int linear_steps(int dk) {
   return dk <= 32 ? 1 : dk <= 64 ? 2 : dk <= 128 ? 4 : 8;
 }
-// Workspace of launch_linear_chunks: per (row, key head, chunk) the queries by tokens,
-// the keys by features (left out where they are read in place) and (delta rule) by tokens
-// as operands; per (row, head, chunk) the decayed scores (with the delta rule also the
+// Whether the walk takes the keys by features from the workspace; f32 keys of up to 128
+// features it reads where they are (linear_chunks.hip).
+__host__ __device__ constexpr bool linear_keys_packed(bool bf16, int steps) {
+  return bf16 || steps > 4;
+}
+// Workspace of launch_linear_chunks: per (row, key head, chunk) the queries by tokens, with
+// the delta rule the keys by tokens and, where linear_keys_packed, the keys by features as
+// operands; per (row, head, chunk) the decayed scores (with the delta rule also the
 // solve operand after them) and 64 factors each from the chunk's start, to its end and
 // beta; per (row, chunk) the active tokens.
 struct LinearWork {
@@ -375,8 +380,10 @@ struct LinearSpace {
 };
 inline LinearSpace linear_space(const LinearArgs &a) {
   const size_t nch = (size_t)((a.L + kLinearChunk - 1) / kLinearChunk) * a.rows;
-  const size_t parts = a.beta ? 3 : 2, block = a.bf16 ? 1024 : 2048;
-  return LinearSpace{nch * a.key_heads * parts * 4 * linear_steps(a.dk) * block,
+  const int steps = linear_steps(a.dk);
+  const size_t parts = 1 + (a.beta ? 1 : 0) + (linear_keys_packed(a.bf16, steps) ? 1 : 0);
+  const size_t block = a.bf16 ? 1024 : 2048;
+  return LinearSpace{nch * a.key_heads * parts * 4 * steps * block,
                      nch * a.heads * kLinearTriBytes * (a.beta ? 2 : 1),
                      nch * a.heads * 3 * kLinearChunk * 4, nch * 8};
 }

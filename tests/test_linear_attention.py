@@ -518,6 +518,28 @@ def test_single_tokens_of_more_rows_than_two_to_the_32_threads(gpu_ctx):
     p.check(part(out.view(R, H, dv, 1)), part(state))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("delta", [True, False], ids=["delta", "plain"])
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("dk", [30, 64, 128, 256])
+def test_the_workspace_holds_what_is_used(dk, bf16, delta):
+    """Per (row, key head, chunk): queries, with the delta rule keys by tokens, and keys by
+    features, except f32 keys of up to 128 features, which are read where they are. Per (row,
+    head, chunk): scores, with the delta rule the solve operand, and three factors a token."""
+    R, L, H, HK, dv = 2, 100, 4, 2, 20
+    p = Problem(R, L, H, HK, dk, dv, bf16=bf16, delta=delta, state=True)
+    with te.Context(0) as ctx:
+        ctx.stream()
+        before = ctx.retained_bytes()
+        out, state = p.run(ctx, cuda)
+        used = ctx.retained_bytes() - before
+    p.check(host(out), host(state))
+    chunks, wide = 2, max(32, 1 << (dk - 1).bit_length())
+    parts = 1 + delta + (bf16 or dk > 128)
+    assert used == R * chunks * (HK * parts * 64 * wide * (2 if bf16 else 4)
+                                 + H * (1 + delta) * 18 * 1024 + H * 3 * 64 * 4 + 8)
+
+
 # Shapes whose prompts take, of the delta rule: the token-by-token kernel, the path kernel on
 # one and two column tiles, four waves on two and four tiles, eight waves on one and two; the
 # same shapes without it: the plain kernel on one and two tiles.
