@@ -195,7 +195,7 @@ class Context:
         if rc != TFD_OK:
             raise DeviceError(rc, "tfd_ctx_create failed")
         self._h = handle
-        self._stream = None
+        self._stream = stream  # None until the context has made its own
         self.device = device
 
     @property
@@ -211,9 +211,11 @@ class Context:
         self.check(self._lib.tfd_ctx_synchronize(self._h))
 
     def stream(self) -> int:
-        if self._stream is None:  # the context keeps the stream of its first use
-            self._stream = self._lib.tfd_ctx_stream(self._h) or 0
-        return self._stream
+        if self._stream is None:
+            # Null means that the device could not be used, which a later call may be able
+            # to: it is not kept. Own streams are never null.
+            self._stream = self._lib.tfd_ctx_stream(self._h)
+        return self._stream or 0
 
     def retained_bytes(self) -> int:
         return self._lib.tfd_ctx_retained_bytes(self._h)
@@ -366,7 +368,11 @@ class _StreamOrder:
             return
         import torch
 
-        handle = ctx._stream if ctx._stream is not None else ctx.stream()
+        handle = ctx._stream
+        if handle is None:
+            handle = ctx.stream()
+            if not handle:  # the call might run all the same, on a stream not yet known
+                ctx.check(TFD_EHIP)
         if handle == torch._C._cuda_getCurrentRawStream(ctx.device):
             return
         cur = torch.cuda.current_stream(ctx.device)

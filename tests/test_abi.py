@@ -56,6 +56,35 @@ def test_context_does_not_touch_gpu_on_create(ctx):
     ctx.synchronize()  # nothing enqueued yet: a no-op
 
 
+class _StreamOnSecondAsk:
+    """The library, but the first use of a context's device fails."""
+
+    def __init__(self, lib, handle):
+        self._lib, self.handle, self.asked = lib, handle, 0
+
+    def __getattr__(self, name):
+        return getattr(self._lib, name)
+
+    def tfd_ctx_stream(self, ctx):
+        self.asked += 1
+        return None if self.asked == 1 else self.handle
+
+
+def test_a_failed_start_is_not_kept_as_the_stream(ctx):
+    """Null is a failure for a context with a stream of its own: the next use asks again, and
+    a call on device tensors does not run unordered meanwhile."""
+    ctx._lib = lib = _StreamOnSecondAsk(ctx._lib, 4096)
+    assert ctx.stream() == 0
+    assert ctx.stream() == 4096 and ctx.stream() == 4096 and lib.asked == 2
+    with te.Context(0) as other:
+        other._lib = _StreamOnSecondAsk(other._lib, 4096)
+        with pytest.raises(te.DeviceError):
+            te._StreamOrder(other, te.TFD_DEVICE_PTRS)
+    with te.Context(0, stream=0) as adopted:  # the device's default stream
+        adopted._lib = lib = _StreamOnSecondAsk(adopted._lib, 4096)
+        assert adopted.stream() == 0 and lib.asked == 0
+
+
 def _laya_call(ctx, shape, keep_len, hidden=8, heads=2, out_len=None, qkv_len=None):
     qkv = np.zeros(max(1, int(np.prod(shape))), np.float32)
     qkv_len = int(np.prod(shape)) if qkv_len is None else qkv_len
