@@ -415,7 +415,7 @@ def _ptr(x):
     """Address of an array or tensor that was just made."""
     if x is None:
         return None
-    return x.data_ptr() if _torch_types.get(type(x)) else x.ctypes.data
+    return x.data_ptr() if _is_torch(x) else x.ctypes.data
 
 
 # ------------------------------------------------------------------ op descriptors

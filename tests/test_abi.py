@@ -296,6 +296,17 @@ def test_wrapper_rejects_wrong_tensor_dtypes(ctx):
                                     H, KV, hd, hd, 1e7, 1e-6, bf16=True, ctx=ctx)
 
 
+def test_addresses_of_results_whatever_the_operands_types(monkeypatch):
+    """Operands of a tensor subclass (parameters) only: the results are plain tensors, of a
+    type that no call has met yet."""
+    import torch
+
+    monkeypatch.setattr(te, "_torch_types", {})
+    assert te._is_torch(torch.nn.Parameter(torch.zeros(3)))
+    x, y = torch.zeros(3), np.zeros(3, np.float32)
+    assert te._ptr(x) == x.data_ptr() and te._ptr(y) == y.ctypes.data and te._ptr(None) is None
+
+
 def test_wrapper_rejects_host_device_mix(ctx):
     """Host arrays and device tensors in one call are refused before any device
     call (a stand-in object reports itself as a CUDA tensor)."""

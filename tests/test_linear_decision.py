@@ -177,3 +177,28 @@ def test_two_contexts_at_once():
     for want, tries in zip(alone, together):
         for got in tries:
             assert all(np.array_equal(host(x), y) for x, y in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_operands_that_are_parameters(gpu_ctx, monkeypatch):
+    """A program whose first call passes a module's parameters and nothing else."""
+    import torch
+
+    rng = Lcg(17)
+    param = lambda *s: torch.nn.Parameter(cuda(rng.normal(int(np.prod(s))).astype(np.float32)),
+                                          requires_grad=False)
+    q, k, v, state = param(2, 8), param(2, 8), param(2, 4), param(2, 8, 4)
+    g, beta, logits = param(2), param(2), param(3, 50)
+    g.neg_().sub_(3), beta.sigmoid_()
+    ops = [x.data.view(-1) for x in (q, k, v, g, beta)]
+    want, after = te.jeff_linear_attention_rows(*ops, None, 1, 1, 2, 2, 8, 4,
+                                                state=state.data.view(-1), ctx=gpu_ctx)
+    marks = te.token_log_probs(logits.data.view(-1), None, 3, 50, top=3, ctx=gpu_ctx)
+    monkeypatch.setattr(te, "_torch_types", {})
+    out, new = te.jeff_linear_attention_rows(q, k, v, g, beta, None, 1, 1, 2, 2, 8, 4, state=state,
+                                             ctx=gpu_ctx)
+    assert torch.equal(out, want) and torch.equal(new, after)
+    monkeypatch.setattr(te, "_torch_types", {})
+    got = te.token_log_probs(logits, None, 3, 50, top=3, ctx=gpu_ctx)
+    assert got.log_probs is None
+    assert all(torch.equal(a, b) for a, b in zip(got[1:], marks[1:]))
