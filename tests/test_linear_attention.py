@@ -109,6 +109,64 @@ class Problem:
                 np.abs(state - S) / (A + 1e-30))
 
 
+def cut(x, bits):
+    """x to nearest with that many significant bits."""
+    m, e = np.frexp(x.astype(np.float64))
+    return np.ldexp(np.round(np.ldexp(m, bits)), e - bits)
+
+
+def column_norms(q, k, v, g, beta, mask, scale, state):
+    """The bounds of `reference` for each value column by itself: the largest norm a column of
+    the state has had, plus its largest write; the output's times the token's query."""
+    R, H, dv, L = v.shape
+    idx = np.arange(H) // (H // k.shape[1])
+    S = np.zeros((R, H, k.shape[2], dv)) if state is None else state.astype(np.float64)
+    norm, size = np.sqrt((S ** 2).sum(2)), np.zeros((R, H, dv, L))
+    write = np.zeros((R, H, dv))
+    for t in range(L):
+        on = np.ones(R, bool) if mask is None else mask[:, t] != 0
+        if not on.any():
+            continue
+        kt = k[on][..., t][:, idx].astype(np.float64)
+        S[on] *= np.exp(g[on, :, t].astype(np.float64))[..., None, None]
+        u = v[on, :, :, t].astype(np.float64)
+        if beta is not None:
+            u = beta[on, :, t].astype(np.float64)[..., None] * (
+                u - np.einsum("rhij,rhi->rhj", S[on], kt))
+        S[on] += kt[..., None] * u[:, :, None]
+        norm[on] = np.maximum(norm[on], np.sqrt((S[on] ** 2).sum(2)))
+        write[on] = np.maximum(write[on], np.abs(u))
+        size[on, :, :, t] = abs(scale) * (norm + write)[on] * np.sqrt(
+            (q[on][..., t].astype(np.float64) ** 2).sum(2))[:, idx][..., None]
+    return size, np.broadcast_to((norm + write)[:, :, None], S.shape)
+
+
+def check_columns(p, out, state):
+    """`Problem.check` with two bounds that lost bits of an operand do not stay within.
+
+    Each value column of the state evolves by itself, S_j <- e^g (I - beta k k^T) S_j + beta k
+    v_j, so that the count of the module's comment holds against the column's own norm.
+
+    Over all of a result the errors, independent and unbiased, add up in squares. From the
+    state and U to an output an element takes at most 48 + 12 + 3 roundings (8 steps of 32
+    features and 2 of 32 tokens, six products each, and the factors), to U as many, and 13 a
+    chunk to the state; more than a token by token sum in a tree. A rounding has a standard
+    deviation of at most 2^-24 / sqrt(3) of what is rounded, which is at most about twice the
+    result (two terms that partly cancel): 2 * 2^-24 sqrt((126 + 13 chunks) / 3) of the
+    result's 2-norm. An operand of 16 bits is off by 2^-16 / sqrt(3) or a little less."""
+    R, L, H, HK, dk, dv = p.dims
+    ops = (p.q, p.k, p.v, p.g, p.beta, p.mask, float(np.float32(dk ** -0.5)), p.state)
+    want, S, _, _ = reference(*ops)
+    size, A = column_norms(*ops)
+    tol = 2.0 ** -24 * (8 + 6 * np.sqrt(dk + 64 + L))
+    rms = 2 * 2.0 ** -24 * np.sqrt((126 + 13 * -(-L // 64)) / 3)
+    for got, exact, bound in ((out, want, size), (state, S, A)):
+        off = np.abs(np.asarray(got, np.float64).reshape(exact.shape) - exact)
+        assert (off <= tol * bound + 1e-37).all(), np.max(off / (bound + 1e-30))
+        whole = np.sqrt((exact ** 2).sum())
+        assert np.sqrt((off ** 2).sum()) <= rms * whole, np.sqrt((off ** 2).sum()) / whole
+
+
 def cuda(x):
     import torch
 
@@ -193,6 +251,32 @@ def test_results_are_not_written_to_a_copy(ctx):
     with pytest.raises(te.InvalidArgument, match="state: expected a contiguous float32"):
         te.jeff_linear_attention_step(f(R * H * dk), f(R * H * dk), f(R * H * dv), f(R * H), None,
                                       None, R, H, H, dk, dv, ctx=ctx)
+
+
+# rows, length, heads, key_heads, key_dim, value_dim
+COLUMNS = [(3, 17, 4, 2, 20, 33), (2, 65, 2, 1, 16, 130), (3, 127, 2, 2, 128, 128),
+           (1, 200, 2, 1, 256, 72), (1, 600, 2, 1, 64, 64), (5, 90, 8, 4, 50, 213),
+           (5, 90, 8, 4, 100, 213), (5, 90, 8, 4, 200, 100)]
+
+
+@pytest.mark.parametrize("bits", [17, 16])
+@pytest.mark.parametrize("delta", [True, False], ids=["delta", "plain"])
+@pytest.mark.parametrize("shape", COLUMNS[:5], ids=str)
+def test_the_check_finds_operands_of_fewer_bits(shape, delta, bits):
+    """What a kernel computes that drops the last piece of its operands: queries, keys, values
+    and every 64 tokens the state cut to 16 or 17 bits."""
+    for mask in (None, "left", "holes"):
+        p = Problem(*shape, delta=delta, mask=mask, state=True, decay=0.3)
+        outs, state, L = [], p.state, shape[1]
+        for a in range(0, L, 64):
+            at = lambda x: None if x is None else x[..., a:a + 64]
+            few = lambda x: cut(at(x), bits)
+            out, state, _, _ = reference(few(p.q), few(p.k), few(p.v), at(p.g), at(p.beta),
+                                         at(p.mask), float(np.float32(shape[4] ** -0.5)),
+                                         cut(state, bits))
+            outs.append(out)
+        with pytest.raises(AssertionError):
+            check_columns(p, np.concatenate(outs, -1), state)
 
 
 def test_empty_problems_need_no_gpu(ctx):
@@ -538,6 +622,80 @@ def test_the_workspace_holds_what_is_used(dk, bf16, delta):
     parts = 1 + delta + (bf16 or dk > 128)
     assert used == R * chunks * (HK * parts * 64 * wide * (2 if bf16 else 4)
                                  + H * (1 + delta) * 18 * 1024 + H * 3 * 64 * 4 + 8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("delta", [True, False], ids=["delta", "plain"])
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", COLUMNS, ids=str)
+def test_every_column_against_its_own_norm(gpu_ctx, shape, bf16, delta):
+    for mask in (None, "left", "holes"):
+        p = Problem(*shape, bf16=bf16, delta=delta, mask=mask, state=True, decay=0.3)
+        check_columns(p, *[host(x) for x in p.run(gpu_ctx, cuda)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("delta", [True, False], ids=["delta", "plain"])
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads,key_heads,dk,dv", [(4, 2, 40, 24), (8, 4, 50, 200),
+                                                   (8, 4, 100, 260), (4, 2, 200, 24)])
+def test_more_than_64_chunks_in_a_row_without_an_active_token(gpu_ctx, heads, key_heads, dk, dv,
+                                                              bf16, delta):
+    """Rows of 73 chunks with 150 active tokens: in the first and the last ones with 68 dead
+    chunks between, only in the last, only in the first, and none. The others hold NaN."""
+    R, n, L = 4, 150, 64 * 72 + 10
+    p = Problem(R, n, heads, key_heads, dk, dv, bf16=bf16, delta=delta, state=True, decay=0.3)
+    p.mask = np.ones((R, n), np.float32)
+    p.mask[3] = 0.0
+    at = np.array([[*range(75), *range(L - 75, L)], range(L - n, L), range(n), range(n)])
+    mask = np.zeros((R, L), np.float32)
+    for r in range(3):
+        mask[r, at[r]] = 1.0
+
+    def long(x, fill=np.nan):
+        if x is None:
+            return None
+        y = np.full((*x.shape[:-1], L), fill, np.float32)
+        for r in range(R):
+            y[r][..., at[r]] = x[r]
+        return y
+
+    w = Problem(1, 1, 1, 1, 1, 1, bf16=bf16)
+    w.dims = (R, L, heads, key_heads, dk, dv)
+    w.q, w.k, w.v, w.g, w.beta = (long(x) for x in (p.q, p.k, p.v, p.g, p.beta))
+    w.mask, w.state = mask, p.state
+    out, state = [host(x) for x in w.run(gpu_ctx, cuda)]
+    out = out.reshape(R, heads, dv, L)
+    assert (np.moveaxis(out, 3, 1)[mask == 0] == 0).all()
+    check_columns(p, np.stack([out[r][..., at[r]] for r in range(R)]), state)
+    assert np.array_equal(state.reshape(p.state.shape)[3], p.state[3])
+
+
+@pytest.mark.gpu
+def test_a_capture_that_would_grow_the_workspace_is_refused():
+    """And what the context had stays as it was: the call before it runs, captured and eager."""
+    import torch
+
+    stream = torch.cuda.Stream()
+    with te.Context(0, stream=stream.cuda_stream) as ctx, torch.cuda.stream(stream):
+        small, big = Problem(1, 100, 2, 2, 40, 24), Problem(3, 500, 2, 2, 40, 24)
+        want = [host(x) for x in small.run(ctx, cuda)]
+        held = ctx.retained_bytes()
+        ops, more = small.args(cuda), big.args(cuda)
+        stream.synchronize()
+        with te.asynchronous(), pytest.raises(te.Unsupported, match="workspace cannot grow"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+                te.jeff_linear_attention_rows(*more, *big.dims, ctx=ctx)
+                raise AssertionError("captured a call whose workspace is not there")
+        assert ctx.retained_bytes() == held
+        graph = torch.cuda.CUDAGraph()
+        with te.asynchronous(), torch.cuda.graph(graph, stream=stream):
+            got = te.jeff_linear_attention_rows(*ops, *small.dims, ctx=ctx)
+        for _ in range(3):
+            graph.replay()
+            stream.synchronize()
+            assert all(np.array_equal(host(a), b) for a, b in zip(got, want))
+            big.check(*[host(x) for x in big.run(ctx, cuda)])
 
 
 # Shapes whose prompts take, of the delta rule: the token-by-token kernel, the path kernel on

@@ -252,6 +252,34 @@ def test_repeats_streams_and_graphs():
 
 
 @pytest.mark.gpu
+def test_a_capture_that_would_grow_the_workspace_is_refused():
+    import torch
+
+    stream = torch.cuda.Stream()
+    with te.Context(0, stream=stream.cuda_stream) as ctx, torch.cuda.stream(stream):
+        x, t = logits(2, 50000, True), some_tokens(2, 50000, 4)
+        want = run(ctx, x, t, 9, True)
+        check(want, x, t, 9)
+        held = ctx.retained_bytes()
+        dx, dt = cuda(te.to_bf16_bits(x).reshape(-1)), cuda(t.reshape(-1))
+        big = cuda(logits(3, 160000, False).reshape(-1))
+        stream.synchronize()
+        with te.asynchronous(), pytest.raises(te.Unsupported, match="workspace cannot grow"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+                te.token_log_probs(big, None, 3, 160000, top=64, ctx=ctx)
+                raise AssertionError("captured a call whose workspace is not there")
+        assert ctx.retained_bytes() == held
+        graph = torch.cuda.CUDAGraph()
+        with te.asynchronous(), torch.cuda.graph(graph, stream=stream):
+            got = te.token_log_probs(dx, dt, 2, 50000, top=9, bf16=True, ctx=ctx)
+        for _ in range(3):
+            graph.replay()
+            stream.synchronize()
+            assert all(np.array_equal(a.cpu().numpy(), b) for a, b in zip(got, want))
+            te.token_log_probs(big, None, 3, 160000, top=64, ctx=ctx)
+
+
+@pytest.mark.gpu
 def test_logits_past_four_gigabytes(gpu_ctx):
     """More than 2^32 bytes of logits: the last positions are read where they are."""
     import torch
