@@ -292,7 +292,10 @@ int tfd_jeff_full_attention_layer_rows_f32(tfd_ctx *ctx, size_t rows, size_t len
  *   scale_bits: f32 bits of the factor on the output.
  * length 1 is the single-token form. key_dim is at most 256 (else
  * TFD_EUNSUPPORTED). A NaN or inf that an active token holds reaches this head's
- * later outputs, and may reach those up to 63 tokens before it.
+ * later outputs, and in prompts (over 10 tokens, over 6 in bf16) may reach those of active
+ * tokens up to 63 before it; so may f32 values past 3.39e38, which are inf in bf16. A
+ * log_decay above 0 is a growth: one past f32's range (e^88) within 64 tokens may give
+ * NaN even where the state it multiplies is 0.
  * Both this and tfd_token_log_probs may run under stream capture (with TFD_ASYNC)
  * once the context's workspace fits, that is, after one eager call of the same sizes,
  * else TFD_EUNSUPPORTED. Later, larger calls leave a captured workspace in

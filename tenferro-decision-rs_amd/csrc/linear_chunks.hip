@@ -313,10 +313,11 @@ __device__ __forceinline__ int tri_block(int tt, int ks) { return tt < 2 ? tt : 
 // by T_ij = -T_ii sum_(j <= k < i) M_ik T_kj on the f32 matrix cores, one distance
 // i - j after the other. The first head of a key head's group also leaves the
 // keys and queries behind in fragment order, the keys both ways: the walk's column
-// groups then each read whole lines with few loads (in the original order, where a
-// wave's token tile is 32 or 64 bytes of a feature row, this kernel and the walk took 14
-// + 222 us instead of 20 + 94 for 8 x 1024 tokens with 8 heads of 256 x 256 in bf16, 62 +
-// 586 instead of 109 + 424 for 2 x 8192 with 16 heads of 128 x 128).
+// groups then each read whole lines with few loads. This kernel and the walk take 15 + 95
+// us for 8 x 1024 tokens with 8 heads of 256 x 256 in bf16, 89 + 342 for 2 x 8192 with 16
+// heads of 128 x 128; the walks before them, on which the order was decided, 20 + 94 and 109
+// + 424 with it, 14 + 222 and 62 + 586 from the original order, where a wave's token tile is
+// 32 or 64 bytes of a feature row.
 // All loads are issued before anything waits for the first of them.
 template <typename T, bool DELTA, bool FEATURES>
 __global__ __launch_bounds__(256) void linear_pairs_kernel(LinearArgs a, LinearWork ws) {
@@ -822,8 +823,9 @@ struct StateTiles {
 // shared by four waves: wave w has token tile w of U and O, and the feature tiles TI w ..
 // of the state. Three times a chunk they hand their part to the others as operand
 // pieces in LDS: the state for K S0 and Q S0, V - d K S0 for U, U for O and the state.
-// Two or more workgroups a CU hide each other's exchanges; then the operands bound it
-// (8 TB/s out of L2 with bf16 keys).
+// Two or more workgroups a CU hide each other's exchanges; then the operands bound it (16
+// rows of 512 tokens with 16 heads of 128 x 128 in bf16: the workgroups load 744 MB, most of
+// it out of L2, in 114 us, 6.5 TB/s).
 // On eight waves the first four are on the path from one state to the next (K S0, V - d
 // K S0 and U), the others beside it (Q S0 and O, which nothing waits for), and the
 // state's tiles are dealt to all eight. `path` and `side` are both true on four.

@@ -157,7 +157,8 @@ __device__ __forceinline__ void move_reference(Stats &s, float m) {
   s.z = f * s.z;
   s.m = m;
 }
-// e^(x - m) and its product with x - m for one logit.
+// e^(x - m) and its product with x - m for one logit. The exponent's product is rounded, by
+// 2^-24 |d| log2 e: of the term, which is e^d, so of z by 2^-24 at most (|d| e^d <= 1 / e).
 __device__ __forceinline__ void add_logit(Stats &s, float x) {
   float d = x - s.m;
   d = d < kFar ? kFar : d;  // keeps a NaN
@@ -401,10 +402,23 @@ void launch_parts(const LogProbArgs &a, int waves, hipStream_t stream, const Ker
 
 }  // namespace
 
-// Positions of up to so many 16-byte pieces stay whole: the join is a launch more and a
-// wave that reads what the others left (16 x 5000 f32, 1250 pieces: 4.1 us whole, 10.8
-// in two parts, with top 5 9.1 and 15.4; 256 x 32000 bf16, 4000 pieces: 8.7 and 11.9,
-// but with top 20 26.0 and 25.5, and 16 of them 25.5 and 19.1).
+// Positions of up to so many 16-byte pieces stay whole: the join is a launch more, 2.6 us of
+// the host's time a call, and a wave that reads what the others left. Whole and in parts, us
+// per call (eager ones one after another, from Python; in brackets replays of a graph, where
+// the launch costs least):
+//   4096 pieces f32,  1 position 8.0, 10.6 (4.8, 4.9), 256: 8.0, 10.6 (5.6, 6.8)
+//   4096 pieces bf16, 1 position 8.0, 10.7 (7.3, 5.6), 256: 9.7, 10.3 (9.8, 8.3)
+//   8192 pieces f32,  1 position 8.0, 10.6 (7.3, 4.9), 256: 9.0, 10.2 (9.3, 9.2)
+//   8192 pieces bf16, 1 position 12.0, 10.5 (12.1, 5.5), 256: 15.4, 13.3 (15.6, 13.7)
+//   16384 pieces f32, 1 position 12.1, 10.4 (12.2, 4.9), 256: 16.8, 14.7 (17.3, 15.1)
+// With top 5:
+//   2048 pieces f32,  1 position 10.9, 13.5 (9.0, 11.4), 256: 11.0, 13.7 (10.1, 13.1)
+//   2048 pieces bf16, 1 position 11.9, 14.1 (11.5, 13.4), 256: 12.9, 15.7 (13.3, 15.7)
+//   4096 pieces f32,  1 position 11.1, 13.7 (12.2, 11.5), 256: 14.1, 15.4 (14.4, 15.1)
+//   4096 pieces bf16, 1 position 16.7, 14.1 (16.4, 13.4), 256: 20.3, 19.0 (20.1, 19.2)
+// With top 20 replays of 2048 pieces bf16 take 15.2 and 15.7 (1 position), 17.6 and 17.7
+// (256), of 4096 24.1 and 16.0, 27.5 and 22.6. The limits are where eager calls of both
+// types are about even.
 constexpr size_t kLogProbWhole = 8192, kLogProbWholeTop = 2048;
 // Fewest pieces of a part: one step of a workgroup's four waves. Fewer spread
 // a position further, but every wave has to find its first `top` and the joining
