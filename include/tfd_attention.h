@@ -13,7 +13,9 @@
  * plus entries that extend the same arithmetic without changing the drop-in
  * path (structured Laya masks, batched Jeff rows with native GQA, bf16 Jeff),
  * and what a hybrid Jeff model needs around them: linear attention over rows
- * (prompts and single tokens) and token log probabilities.
+ * (prompts and single tokens), token log probabilities, and for its full-attention
+ * layers while it generates: rotary positions, a paged cache of keys and values in
+ * 8 bits that new tokens are appended to, and the attention over it.
  *
  * Conventions
  *   - Every tensor is column-major exactly as the reference passes it:
@@ -57,6 +59,8 @@ extern "C" {
 #define TFD_ASYNC 2u       /* with TFD_DEVICE_PTRS: enqueue on the context stream and return */
 #define TFD_TRIM_LEADING 4u /* Jeff rows: drop each row's leading inactive keys and
                                restart RoPE positions at the first active one */
+#define TFD_INTERLEAVED 8u /* rotary pairs are features (2i, 2i+1), else (i, i + rotary_dim/2) */
+#define TFD_INVERSE 16u    /* rotary rows: turn back (the gradient of the turn) */
 /* Jeff drop-in on GQA-expanded K/V: the caller states kv_heads (bits 16..31),
  * heads / kv_heads consecutive heads of K and V being identical copies, as
  * jeff-infer's checkpoint expansion makes them (checkpoint.rs:307-319; the
@@ -349,6 +353,131 @@ int tfd_token_log_probs_bf16(tfd_ctx *ctx, const uint16_t *logits, size_t vocab,
                              size_t positions, const int64_t *tokens, size_t per_position,
                              size_t top, float *log_probs, float *entropy, int64_t *top_tokens,
                              float *top_log_probs, unsigned flags);
+
+/*
+ * Rotary positions of rows of heads (no counterpart among the reference's ops, which
+ * turn queries and keys inside the Jeff op, cpu-kernels lib.rs:692-709). Per token at
+ * position p and each of the first rotary_dim / 2 pairs (a, b) of a head's features, with
+ * u = p frequencies[i] turns, whole ones dropped in 64 bits:
+ *   a' = magnitude (a cos 2 pi u - b sin 2 pi u)
+ *   b' = magnitude (a sin 2 pi u + b cos 2 pi u)
+ * The features behind rotary_dim are copied.
+ *   x, out:      rows x (length, heads*head_dim); out may be x (in place), no other
+ *                overlap is allowed.
+ *   positions:   rows x (length), any 32-bit value, or NULL: 0, 1, ...
+ *   frequencies: rotary_dim / 2 doubles in HOST memory whatever the flags (turns per token:
+ *                theta^(-2i/rotary_dim) / 2 pi, stretched for long contexts as the caller
+ *                likes); read before the call returns. rotary_dim is even and at most 256
+ *                (else TFD_EUNSUPPORTED).
+ *   magnitude_bits: f32 bits of the factor on the turned features.
+ * flags may carry TFD_INTERLEAVED and TFD_INVERSE (turns by -u; with the same magnitude
+ * the gradient of the forward call).
+ * This and the two cache entries may run under stream capture (with TFD_ASYNC); the
+ * attention needs one eager call of the same sizes before, whose workspace the graphs of
+ * a context share, with each other and with its eager calls: replay them in the order
+ * of one stream.
+ */
+int tfd_rotary_rows_f32(tfd_ctx *ctx, size_t rows, size_t length, size_t heads, size_t head_dim,
+                        size_t rotary_dim, const float *x, const int32_t *positions,
+                        const double *frequencies, uint32_t magnitude_bits, float *out,
+                        unsigned flags);
+
+/* As tfd_rotary_rows_f32 on bf16 bits; the turn is f32, rounded once. */
+int tfd_rotary_rows_bf16(tfd_ctx *ctx, size_t rows, size_t length, size_t heads, size_t head_dim,
+                         size_t rotary_dim, const uint16_t *x, const int32_t *positions,
+                         const double *frequencies, uint32_t magnitude_bits, uint16_t *out,
+                         unsigned flags);
+
+/*
+ * A paged cache of keys and values in e4m3 (the OCP 8-bit float of range 448), with a
+ * scale for each block of 64 tokens and kv head. `wide` is head_dim rounded up to a
+ * multiple of 64.
+ *   keys:   pages x kv_heads x (page_tokens, wide), a token's features contiguous; features
+ *           behind head_dim hold 0.
+ *   values: pages x kv_heads x page_tokens/64 x (wide, 64), a block's tokens contiguous;
+ *           features behind head_dim are not read.
+ *   key_scales, value_scales: pages x kv_heads x page_tokens/64, powers of two; a code
+ *           stands for its e4m3 value times its block's scale.
+ * page_tokens is a power of two of at least 64; keys and values are 16-byte aligned.
+ * No page has to be cleared before its first use.
+ */
+typedef struct tfd_paged_cache {
+  uint8_t *keys, *values;
+  float *key_scales, *value_scales;
+  size_t pages, page_tokens;
+} tfd_paged_cache;
+
+/*
+ * Appends the keys and values of new tokens to the rows' pages.
+ *   k, v:     rows x (length, kv_heads*head_dim), as for the Jeff rows op. A row's new tokens
+ *             are its last counts[r] ones (left padding); what the others hold is not used.
+ *   k_norm:   (head_dim): keys become x / sqrt(mean(x^2) + eps) (1 + k_norm), as in the Jeff
+ *             op; NULL leaves them as they are. They are then turned (rotary_dim,
+ *             frequencies, magnitude as for tfd_rotary_rows_f32; rotary_dim 0: not) to
+ *             their place in the row, lengths[r] + i for its i-th new token.
+ *   pages:    rows x (pages_per_row): token j of row r is in page
+ *             pages[r * pages_per_row + j / page_tokens]. Rows may share pages that no call
+ *             appends to; rows of one call that append to the same page leave undefined
+ *             codes in it.
+ *   lengths:  (rows) tokens that the rows hold before the call, NULL: none. Not updated.
+ *   counts:   (rows), NULL: length for every row. 0 leaves a row as it is.
+ * A block's scale is the smallest power of two (of at least 2^-100) with which every
+ * finite value appended to the block is within 448; while the block fills it only grows,
+ * and the codes of its earlier tokens are rounded again under the new scale. Codes are
+ * rounded to nearest even from 64-bit keys; NaN and inf become the code of NaN.
+ * head_dim is at most 256 (else TFD_EUNSUPPORTED). A row whose length or count is negative, whose
+ * count exceeds length, or that its pages cannot hold, and pages outside the
+ * cache: with host operands TFD_EINVAL; with device operands, which the host does not
+ * read, nothing is written for that row or page.
+ */
+int tfd_jeff_cache_append_f32(tfd_ctx *ctx, size_t rows, size_t length, size_t kv_heads,
+                              size_t head_dim, size_t rotary_dim, const float *k, const float *v,
+                              const float *k_norm, const double *frequencies,
+                              uint32_t magnitude_bits, uint32_t eps_bits,
+                              const tfd_paged_cache *cache, const int32_t *pages,
+                              size_t pages_per_row, const int32_t *lengths,
+                              const int32_t *counts, unsigned flags);
+
+/* As tfd_jeff_cache_append_f32 with k and v given as bf16 bits. */
+int tfd_jeff_cache_append_bf16(tfd_ctx *ctx, size_t rows, size_t length, size_t kv_heads,
+                               size_t head_dim, size_t rotary_dim, const uint16_t *k,
+                               const uint16_t *v, const float *k_norm, const double *frequencies,
+                               uint32_t magnitude_bits, uint32_t eps_bits,
+                               const tfd_paged_cache *cache, const int32_t *pages,
+                               size_t pages_per_row, const int32_t *lengths,
+                               const int32_t *counts, unsigned flags);
+
+/*
+ * The Jeff full-attention op of new tokens over a paged cache that holds them already
+ * (tfd_jeff_cache_append_* with the same pages, lengths and counts) and the rows'
+ * earlier ones: q normalized (q_norm NULL: not) and turned to its place, a softmax over the
+ * keys up to its own, times sigmoid(gate) (gate NULL: 1). Query head h reads kv head
+ * h / (heads / kv_heads).
+ *   q, gate, out: rows x (length, heads*head_dim). out of the tokens before a row's last
+ *                 counts[r] ones is 0. A row that lengths, counts and pages do not describe
+ *                 (see the append) has NaN for every out; a page outside the cache gives
+ *                 NaN to the tokens that see it. With host operands both are TFD_EINVAL.
+ * Every sum is f32 or more, no operand is rounded below f32. A NaN that a key or value
+ * holds reaches the outputs that see its token, and no other.
+ */
+int tfd_jeff_cached_attention_f32(tfd_ctx *ctx, size_t rows, size_t length, size_t heads,
+                                  size_t kv_heads, size_t head_dim, size_t rotary_dim,
+                                  const float *q, const float *gate, const float *q_norm,
+                                  const double *frequencies, uint32_t magnitude_bits,
+                                  uint32_t eps_bits, const tfd_paged_cache *cache,
+                                  const int32_t *pages, size_t pages_per_row,
+                                  const int32_t *lengths, const int32_t *counts, float *out,
+                                  unsigned flags);
+
+/* As tfd_jeff_cached_attention_f32 with q and gate given as bf16 bits. */
+int tfd_jeff_cached_attention_bf16(tfd_ctx *ctx, size_t rows, size_t length, size_t heads,
+                                   size_t kv_heads, size_t head_dim, size_t rotary_dim,
+                                   const uint16_t *q, const uint16_t *gate, const float *q_norm,
+                                   const double *frequencies, uint32_t magnitude_bits,
+                                   uint32_t eps_bits, const tfd_paged_cache *cache,
+                                   const int32_t *pages, size_t pages_per_row,
+                                   const int32_t *lengths, const int32_t *counts, float *out,
+                                   unsigned flags);
 
 #ifdef __cplusplus
 }

@@ -66,6 +66,7 @@ struct tfd_ctx {
   DevBuf planes;      // bf16 planes of the linears' operands
   DevBuf linear;      // chunk operands of the linear attention
   DevBuf readout;     // partial statistics of the token log probabilities
+  DevBuf cached;      // partial outputs of the attention over a cache
   // Workspaces that a captured graph may still use, outgrown since.
   std::vector<void *> retired;
   size_t retired_bytes = 0;
@@ -1700,6 +1701,302 @@ int log_probs_run(tfd_ctx *c, bool bf16, const void *logits, size_t vocab, size_
   return finish(c, flags, log_probs, lp_d, sizeof(float) * pn);
 }
 
+// ------------------------------------------------ rotary positions
+
+// The plan of a call's rotary arguments, checked.
+int rotary_plan(tfd_ctx *c, const char *op, size_t head_dim, size_t rotary_dim,
+                const double *frequencies, uint32_t magnitude_bits, unsigned flags,
+                tfd::RotaryPlan *plan) {
+  if (rotary_dim > head_dim)
+    return invalid(c, op, "rotary_dim", "rotary_dim must not exceed head_dim");
+  if (rotary_dim % 2) return invalid(c, op, "rotary_dim", "rotary_dim must be even");
+  const size_t pairs = rotary_dim / 2;
+  if (pairs > (size_t)tfd::kRotaryMaxPairs)
+    return fail(c, TFD_EUNSUPPORTED, "%s: rotary_dim %zu exceeds %d", op, rotary_dim,
+                2 * tfd::kRotaryMaxPairs);
+  if (pairs && !frequencies) return invalid(c, op, "frequencies", "null buffer");
+  *plan = tfd::RotaryPlan{};
+  plan->pairs = (int)pairs;
+  plan->interleaved = (flags & TFD_INTERLEAVED) ? 1 : 0;
+  plan->magnitude = bits_to_f32(magnitude_bits);
+  for (size_t i = 0; i < pairs; ++i) {
+    if (!std::isfinite(frequencies[i]))
+      return invalid(c, op, "frequencies", "frequencies must be finite");
+    plan->turns[i] = frequencies[i];
+  }
+  return TFD_OK;
+}
+
+// Workgroups of a launch of 512 threads each at most; a grid may have 2^32 threads.
+constexpr size_t kGridBlocks = (size_t)1 << 22;
+
+int rotary_run(tfd_ctx *c, bool bf16, size_t rows, size_t length, size_t heads, size_t head_dim,
+               size_t rotary_dim, const void *x, const int32_t *positions,
+               const double *frequencies, uint32_t magnitude_bits, void *out, unsigned flags) {
+  const char *op = bf16 ? "tfd_rotary_rows_bf16" : "tfd_rotary_rows_f32";
+  if (!c) return TFD_EINVAL;
+  c->err.clear();
+  int rc = check_flags(c, op, flags, TFD_DEVICE_PTRS | TFD_ASYNC | TFD_INTERLEAVED | TFD_INVERSE);
+  if (rc) return rc;
+  size_t mn = 0, n = 0;
+  if (!mul_ok(rows, length, &mn) || !mul_ok(mn, heads, &n) || !mul_ok(n, head_dim, &n) ||
+      n > SIZE_MAX / 64)
+    return invalid(c, op, "shape", "attention dimensions overflow");
+  tfd::RotaryArgs a{};
+  if ((rc = rotary_plan(c, op, head_dim, rotary_dim, frequencies, magnitude_bits, flags, &a.plan)))
+    return rc;
+  if (n == 0) return TFD_OK;
+  if (length > (size_t)1 << 28 || head_dim > (size_t)1 << 20 || heads > 65535 || rows > 65535 ||
+      ((length + 3) / 4 * ((head_dim + 1) / 2) / 256 + 1) * rows > kGridBlocks)
+    return fail(c, TFD_EUNSUPPORTED, "%s: length/head_dim/heads/rows exceed the launch grid", op);
+  if (!x || !out) return invalid(c, op, "inputs", "null buffer");
+  if ((rc = ensure_ready(c))) return rc;
+  bool capturing = false;
+  if ((rc = capture_state(c, op, flags, &capturing))) return rc;
+  const size_t es = bf16 ? 2 : 4;
+  const void *x_d = nullptr, *p_d = nullptr;
+  void *out_d = nullptr;
+  if ((rc = operand(c, flags, 1, x, es * n, &x_d))) return rc;
+  if (positions && (rc = operand(c, flags, 2, positions, sizeof(int32_t) * mn, &p_d))) return rc;
+  if ((rc = output(c, flags, 0, out, es * n, &out_d))) return rc;
+  a.x = x_d;
+  a.positions = static_cast<const int32_t *>(p_d);
+  a.out = out_d;
+  a.L = (int)length;
+  a.heads = (int)heads;
+  a.hd = (int)head_dim;
+  a.inverse = (flags & TFD_INVERSE) ? 1 : 0;
+  a.bf16 = bf16;
+  a.cus = c->cus;
+  tfd::KernelEvents ev;
+  if (!capturing && (rc = timing_events(c, &ev))) return rc;
+  TFD_HIP(c, tfd::launch_rotary(a, (int)rows, c->stream, ev), "rotary launch");
+  return finish(c, flags, out, out_d, es * n);
+}
+
+// ------------------------------------------------ paged 8-bit cache
+
+// What the append and the attention have in common: the cache's and the rows' arguments.
+struct CacheCall {
+  const tfd_paged_cache *cache;
+  const int32_t *pages;
+  size_t per_row;
+  const int32_t *lengths, *counts;
+  size_t rows, length, kv_heads, head_dim;
+  size_t wide, code_bytes, scale_bytes;
+};
+
+int check_cache(tfd_ctx *c, const char *op, CacheCall &m, unsigned flags) {
+  if (!m.cache) return invalid(c, op, "cache", "null cache");
+  const tfd_paged_cache &k = *m.cache;
+  if (k.page_tokens < 64 || (k.page_tokens & (k.page_tokens - 1)))
+    return invalid(c, op, "page_tokens", "page_tokens must be a power of two of at least 64");
+  if (m.head_dim > (size_t)tfd::kCacheMaxHd)
+    return fail(c, TFD_EUNSUPPORTED, "%s: head_dim %zu exceeds %d", op, m.head_dim,
+                tfd::kCacheMaxHd);
+  size_t room = 0, n = 0;
+  m.wide = tfd::cache_wide((int)m.head_dim);
+  if (!mul_ok(m.per_row, k.page_tokens, &room) || !mul_ok(k.pages, m.kv_heads, &n) ||
+      !mul_ok(n, k.page_tokens, &n) || !mul_ok(n, m.wide, &m.code_bytes) ||
+      m.code_bytes > SIZE_MAX / 64)
+    return invalid(c, op, "shape", "cache dimensions overflow");
+  m.scale_bytes = n / 64 * sizeof(float);
+  if (room > (size_t)INT32_MAX || k.pages > (size_t)INT32_MAX)
+    return fail(c, TFD_EUNSUPPORTED, "%s: a row's tokens or the pages exceed 31 bits", op);
+  if (m.rows == 0 || m.length == 0 || m.kv_heads == 0 || m.head_dim == 0) return TFD_OK;
+  if (m.length > (size_t)1 << 24 || m.kv_heads > 32767 || m.rows > 65535)
+    return fail(c, TFD_EUNSUPPORTED, "%s: length/kv_heads/rows exceed the launch grid", op);
+  if (k.pages == 0 || m.per_row == 0)
+    return invalid(c, op, "pages", "the cache and the rows need a page");
+  if (!k.keys || !k.values || !k.key_scales || !k.value_scales || !m.pages)
+    return invalid(c, op, "inputs", "null buffer");
+  if (flags & TFD_DEVICE_PTRS) {
+    if (!aligned16(k.keys) || !aligned16(k.values))
+      return invalid(c, op, "cache", "keys and values must be 16-byte aligned");
+    return TFD_OK;
+  }
+  for (size_t r = 0; r < m.rows; ++r) {
+    const int64_t first = m.lengths ? m.lengths[r] : 0;
+    const int64_t count = m.counts ? m.counts[r] : (int64_t)m.length;
+    if (first < 0) return invalid(c, op, "lengths", "a row's length is negative");
+    if (count < 0 || count > (int64_t)m.length)
+      return invalid(c, op, "counts", "a row's count is negative or more than its tokens");
+    if (first + count > (int64_t)room)
+      return invalid(c, op, "lengths", "a row's pages do not hold its tokens");
+    if (count == 0) continue;
+    const size_t used = ((size_t)(first + count) + k.page_tokens - 1) / k.page_tokens;
+    for (size_t j = 0; j < used; ++j) {
+      const int32_t p = m.pages[r * m.per_row + j];
+      if (p < 0 || (size_t)p >= k.pages)
+        return invalid(c, op, "pages", "a page is outside the cache");
+    }
+  }
+  return TFD_OK;
+}
+
+// Staging slots of the cache's and the rows' operands.
+enum : int { kSlotKeys = 4, kSlotValues, kSlotKeyScales, kSlotValueScales, kSlotPages, kSlotLengths,
+             kSlotCounts };
+
+int cache_view(tfd_ctx *c, const CacheCall &m, unsigned flags, tfd::CacheView *v) {
+  int rc;
+  const void *p = nullptr;
+  const tfd_paged_cache &k = *m.cache;
+  if ((rc = operand(c, flags, kSlotKeys, k.keys, m.code_bytes, &p))) return rc;
+  v->keys = static_cast<uint8_t *>(const_cast<void *>(p));
+  if ((rc = operand(c, flags, kSlotValues, k.values, m.code_bytes, &p))) return rc;
+  v->values = static_cast<uint8_t *>(const_cast<void *>(p));
+  if ((rc = operand(c, flags, kSlotKeyScales, k.key_scales, m.scale_bytes, &p))) return rc;
+  v->key_scales = static_cast<float *>(const_cast<void *>(p));
+  if ((rc = operand(c, flags, kSlotValueScales, k.value_scales, m.scale_bytes, &p))) return rc;
+  v->value_scales = static_cast<float *>(const_cast<void *>(p));
+  if ((rc = operand(c, flags, kSlotPages, m.pages, sizeof(int32_t) * m.rows * m.per_row, &p)))
+    return rc;
+  v->table = static_cast<const int32_t *>(p);
+  if (m.lengths) {
+    if ((rc = operand(c, flags, kSlotLengths, m.lengths, sizeof(int32_t) * m.rows, &p))) return rc;
+    v->lengths = static_cast<const int32_t *>(p);
+  }
+  if (m.counts) {
+    if ((rc = operand(c, flags, kSlotCounts, m.counts, sizeof(int32_t) * m.rows, &p))) return rc;
+    v->counts = static_cast<const int32_t *>(p);
+  }
+  v->pages = (int)k.pages;
+  v->per_row = (int)m.per_row;
+  v->blocks_log2 = 0;
+  while (((size_t)64 << v->blocks_log2) < k.page_tokens) ++v->blocks_log2;
+  v->kv_heads = (int)m.kv_heads;
+  v->hd = (int)m.head_dim;
+  v->wide = (int)m.wide;
+  v->L = (int)m.length;
+  return TFD_OK;
+}
+
+int append_run(tfd_ctx *c, bool bf16, CacheCall m, size_t rotary_dim, const void *k,
+               const void *v, const float *k_norm, const double *frequencies,
+               uint32_t magnitude_bits, uint32_t eps_bits, unsigned flags) {
+  const char *op = bf16 ? "tfd_jeff_cache_append_bf16" : "tfd_jeff_cache_append_f32";
+  if (!c) return TFD_EINVAL;
+  c->err.clear();
+  int rc = check_flags(c, op, flags, TFD_DEVICE_PTRS | TFD_ASYNC | TFD_INTERLEAVED);
+  if (rc) return rc;
+  size_t n = 0;
+  if (!mul_ok(m.rows, m.length, &n) || !mul_ok(n, m.kv_heads, &n) || !mul_ok(n, m.head_dim, &n) ||
+      n > SIZE_MAX / 64)
+    return invalid(c, op, "shape", "attention dimensions overflow");
+  tfd::AppendArgs a{};
+  if ((rc = rotary_plan(c, op, m.head_dim, rotary_dim, frequencies, magnitude_bits, flags,
+                        &a.plan)))
+    return rc;
+  if ((rc = check_cache(c, op, m, flags))) return rc;
+  if (n == 0) return TFD_OK;
+  if ((m.length / 64 + 2) * m.kv_heads * 2 * m.rows > kGridBlocks)
+    return fail(c, TFD_EUNSUPPORTED, "%s: length/kv_heads/rows exceed the launch grid", op);
+  if (!k || !v) return invalid(c, op, "inputs", "null buffer");
+  if (!(flags & TFD_DEVICE_PTRS)) {
+    // Two rows that append to one page would each scale it by itself.
+    std::vector<int32_t> written;
+    try {
+      for (size_t r = 0; r < m.rows; ++r) {
+        const size_t first = m.lengths ? (size_t)m.lengths[r] : 0;
+        const size_t count = m.counts ? (size_t)m.counts[r] : m.length;
+        for (size_t j = first / m.cache->page_tokens;
+             count && j <= (first + count - 1) / m.cache->page_tokens; ++j)
+          written.push_back(m.pages[r * m.per_row + j]);
+      }
+    } catch (const std::bad_alloc &) {
+      return fail(c, TFD_EHIP, "%s: out of host memory", op);
+    }
+    std::sort(written.begin(), written.end());
+    if (std::adjacent_find(written.begin(), written.end()) != written.end())
+      return invalid(c, op, "pages", "two rows append to one page");
+  }
+  if ((rc = ensure_ready(c))) return rc;
+  bool capturing = false;
+  if ((rc = capture_state(c, op, flags, &capturing))) return rc;
+  const size_t es = bf16 ? 2 : 4;
+  const void *k_d = nullptr, *v_d = nullptr, *n_d = nullptr;
+  if ((rc = operand(c, flags, 1, k, es * n, &k_d))) return rc;
+  if ((rc = operand(c, flags, 2, v, es * n, &v_d))) return rc;
+  if (k_norm && (rc = operand(c, flags, 3, k_norm, sizeof(float) * m.head_dim, &n_d))) return rc;
+  if ((rc = cache_view(c, m, flags, &a.cache))) return rc;
+  a.k = k_d;
+  a.v = v_d;
+  a.k_norm = static_cast<const float *>(n_d);
+  a.eps = bits_to_f32(eps_bits);
+  a.bf16 = bf16;
+  tfd::KernelEvents ev;
+  if (!capturing && (rc = timing_events(c, &ev))) return rc;
+  TFD_HIP(c, tfd::launch_cache_append(a, (int)m.rows, c->stream, ev), "cache_append launch");
+  if (!(flags & TFD_DEVICE_PTRS)) {
+    const struct { void *host, *dev; size_t bytes; } back[3] = {
+        {m.cache->values, a.cache.values, m.code_bytes},
+        {m.cache->key_scales, a.cache.key_scales, m.scale_bytes},
+        {m.cache->value_scales, a.cache.value_scales, m.scale_bytes}};
+    for (const auto &b : back)
+      TFD_HIP(c, hipMemcpyAsync(b.host, b.dev, b.bytes, hipMemcpyDeviceToHost, c->stream),
+              "hipMemcpyAsync D2H");
+  }
+  return finish(c, flags, m.cache->keys, a.cache.keys, m.code_bytes);
+}
+
+int cached_run(tfd_ctx *c, bool bf16, CacheCall m, size_t heads, size_t rotary_dim, const void *q,
+               const void *gate, const float *q_norm, const double *frequencies,
+               uint32_t magnitude_bits, uint32_t eps_bits, float *out, unsigned flags) {
+  const char *op = bf16 ? "tfd_jeff_cached_attention_bf16" : "tfd_jeff_cached_attention_f32";
+  if (!c) return TFD_EINVAL;
+  c->err.clear();
+  int rc = check_flags(c, op, flags, TFD_DEVICE_PTRS | TFD_ASYNC | TFD_INTERLEAVED);
+  if (rc) return rc;
+  if (m.kv_heads == 0 || heads % m.kv_heads != 0)
+    return invalid(c, op, "kv_heads", "heads must be a multiple of kv_heads");
+  size_t n = 0;
+  if (!mul_ok(m.rows, m.length, &n) || !mul_ok(n, heads, &n) || !mul_ok(n, m.head_dim, &n) ||
+      n > SIZE_MAX / 64)
+    return invalid(c, op, "shape", "attention dimensions overflow");
+  tfd::CachedArgs a{};
+  if ((rc = rotary_plan(c, op, m.head_dim, rotary_dim, frequencies, magnitude_bits, flags,
+                        &a.plan)))
+    return rc;
+  if ((rc = check_cache(c, op, m, flags))) return rc;
+  if (n == 0) return TFD_OK;
+  if (heads > 65535 || (m.length * (heads / m.kv_heads) / 16 + 1) * m.kv_heads * m.rows > kGridBlocks)
+    return fail(c, TFD_EUNSUPPORTED, "%s: length/heads/rows exceed the launch grid", op);
+  if (!q || !out) return invalid(c, op, "inputs", "null buffer");
+  if ((rc = ensure_ready(c))) return rc;
+  bool capturing = false;
+  if ((rc = capture_state(c, op, flags, &capturing))) return rc;
+  const size_t es = bf16 ? 2 : 4;
+  const void *q_d = nullptr, *g_d = nullptr, *n_d = nullptr;
+  void *out_d = nullptr;
+  if ((rc = operand(c, flags, 1, q, es * n, &q_d))) return rc;
+  if (gate && (rc = operand(c, flags, 2, gate, es * n, &g_d))) return rc;
+  if (q_norm && (rc = operand(c, flags, 3, q_norm, sizeof(float) * m.head_dim, &n_d))) return rc;
+  if ((rc = cache_view(c, m, flags, &a.cache))) return rc;
+  if ((rc = output(c, flags, 0, out, sizeof(float) * n, &out_d))) return rc;
+  a.q = q_d;
+  a.gate = g_d;
+  a.q_norm = static_cast<const float *>(n_d);
+  a.out = static_cast<float *>(out_d);
+  a.eps = bits_to_f32(eps_bits);
+  a.c1 = (1.0f / sqrtf((float)m.head_dim)) * kLog2e;
+  a.heads = (int)heads;
+  a.group = (int)(heads / m.kv_heads);
+  a.bf16 = bf16;
+  a.cus = c->cus;
+  tfd::cached_plan(a, (int)m.rows);
+  if (const size_t bytes = tfd::cached_work_bytes(a, (int)m.rows)) {
+    if ((rc = reserve_capturable(c, op, c->cached, bytes, capturing))) return rc;
+    a.part_out = static_cast<float *>(c->cached.ptr);
+    a.part_stats = a.part_out + bytes / sizeof(float) / (m.wide + 2) * m.wide;
+  }
+  tfd::KernelEvents ev;
+  if (!capturing && (rc = timing_events(c, &ev))) return rc;
+  TFD_HIP(c, tfd::launch_cached_attention(a, (int)m.rows, c->stream, ev),
+          "cached_attention launch");
+  return finish(c, flags, out, out_d, sizeof(float) * n);
+}
+
 }  // namespace
 
 // ---------------------------------------------------------------- C ABI
@@ -1741,6 +2038,7 @@ void tfd_ctx_destroy(tfd_ctx *c) {
     if (c->model.ptr) (void)hipFree(c->model.ptr);
     if (c->linear.ptr) (void)hipFree(c->linear.ptr);
     if (c->readout.ptr) (void)hipFree(c->readout.ptr);
+    if (c->cached.ptr) (void)hipFree(c->cached.ptr);
     for (void *p : c->retired) (void)hipFree(p);
     if (c->blas) (void)rocblas_destroy_handle(c->blas);
     for (auto &e : c->rope) {
@@ -1773,6 +2071,7 @@ size_t tfd_ctx_retained_bytes(const tfd_ctx *c) {
   if (!c) return 0;
   size_t total = sizeof(tfd_ctx) + c->bits.cap + c->kp.cap + c->layer.cap + c->model.cap + c->planes.cap +
                  c->model_host.capacity() + c->linear.cap + c->readout.cap +
+                 c->cached.cap +
                  c->retired_bytes;
   for (const auto &b : c->staging) total += b.cap;
   for (const auto &e : c->rope) total += e.bytes;
@@ -2010,6 +2309,78 @@ int tfd_token_log_probs_bf16(tfd_ctx *c, const uint16_t *logits, size_t vocab, s
                              float *top_log_probs, unsigned flags) {
   return log_probs_run(c, true, logits, vocab, ld, positions, tokens, per_position, top, log_probs,
                        entropy, top_tokens, top_log_probs, flags);
+}
+
+int tfd_rotary_rows_f32(tfd_ctx *c, size_t rows, size_t length, size_t heads, size_t head_dim,
+                        size_t rotary_dim, const float *x, const int32_t *positions,
+                        const double *frequencies, uint32_t magnitude_bits, float *out,
+                        unsigned flags) {
+  return rotary_run(c, false, rows, length, heads, head_dim, rotary_dim, x, positions, frequencies,
+                    magnitude_bits, out, flags);
+}
+
+int tfd_jeff_cache_append_f32(tfd_ctx *c, size_t rows, size_t length, size_t kv_heads,
+                              size_t head_dim, size_t rotary_dim, const float *k,
+                              const float *v, const float *k_norm, const double *frequencies,
+                              uint32_t magnitude_bits, uint32_t eps_bits,
+                              const tfd_paged_cache *cache, const int32_t *pages,
+                              size_t pages_per_row, const int32_t *lengths,
+                              const int32_t *counts, unsigned flags) {
+  return append_run(c, false,
+                    CacheCall{cache, pages, pages_per_row, lengths, counts, rows, length, kv_heads,
+                              head_dim, 0, 0, 0},
+                    rotary_dim, k, v, k_norm, frequencies, magnitude_bits, eps_bits, flags);
+}
+
+int tfd_jeff_cached_attention_f32(tfd_ctx *c, size_t rows, size_t length, size_t heads,
+                                  size_t kv_heads, size_t head_dim, size_t rotary_dim,
+                                  const float *q, const float *gate, const float *q_norm,
+                                  const double *frequencies, uint32_t magnitude_bits,
+                                  uint32_t eps_bits, const tfd_paged_cache *cache,
+                                  const int32_t *pages, size_t pages_per_row,
+                                  const int32_t *lengths, const int32_t *counts, float *out,
+                                  unsigned flags) {
+  return cached_run(c, false,
+                    CacheCall{cache, pages, pages_per_row, lengths, counts, rows, length, kv_heads,
+                              head_dim, 0, 0, 0},
+                    heads, rotary_dim, q, gate, q_norm, frequencies, magnitude_bits, eps_bits, out,
+                    flags);
+}
+
+int tfd_rotary_rows_bf16(tfd_ctx *c, size_t rows, size_t length, size_t heads, size_t head_dim,
+                        size_t rotary_dim, const uint16_t *x, const int32_t *positions,
+                        const double *frequencies, uint32_t magnitude_bits, uint16_t *out,
+                        unsigned flags) {
+  return rotary_run(c, true, rows, length, heads, head_dim, rotary_dim, x, positions, frequencies,
+                    magnitude_bits, out, flags);
+}
+
+int tfd_jeff_cache_append_bf16(tfd_ctx *c, size_t rows, size_t length, size_t kv_heads,
+                              size_t head_dim, size_t rotary_dim, const uint16_t *k,
+                              const uint16_t *v, const float *k_norm, const double *frequencies,
+                              uint32_t magnitude_bits, uint32_t eps_bits,
+                              const tfd_paged_cache *cache, const int32_t *pages,
+                              size_t pages_per_row, const int32_t *lengths,
+                              const int32_t *counts, unsigned flags) {
+  return append_run(c, true,
+                    CacheCall{cache, pages, pages_per_row, lengths, counts, rows, length, kv_heads,
+                              head_dim, 0, 0, 0},
+                    rotary_dim, k, v, k_norm, frequencies, magnitude_bits, eps_bits, flags);
+}
+
+int tfd_jeff_cached_attention_bf16(tfd_ctx *c, size_t rows, size_t length, size_t heads,
+                                  size_t kv_heads, size_t head_dim, size_t rotary_dim,
+                                  const uint16_t *q, const uint16_t *gate, const float *q_norm,
+                                  const double *frequencies, uint32_t magnitude_bits,
+                                  uint32_t eps_bits, const tfd_paged_cache *cache,
+                                  const int32_t *pages, size_t pages_per_row,
+                                  const int32_t *lengths, const int32_t *counts, float *out,
+                                  unsigned flags) {
+  return cached_run(c, true,
+                    CacheCall{cache, pages, pages_per_row, lengths, counts, rows, length, kv_heads,
+                              head_dim, 0, 0, 0},
+                    heads, rotary_dim, q, gate, q_norm, frequencies, magnitude_bits, eps_bits, out,
+                    flags);
 }
 
 int tfd_laya_forward_f32(tfd_ctx *c, const tfd_laya_model *model, const int64_t *ids,

@@ -415,4 +415,95 @@ struct LogProbArgs {
 void log_probs_plan(LogProbArgs &a, int cus);
 hipError_t launch_log_probs(const LogProbArgs &a, hipStream_t stream, const KernelEvents &ev);
 
+// ------------------------------------------------ rotary positions
+
+// Pairs of features that may be turned.
+constexpr int kRotaryMaxPairs = 128;
+struct RotaryPlan {
+  int pairs;
+  int interleaved;   // pairs (2i, 2i + 1), else (i, i + pairs)
+  float magnitude;   // of the turned features
+  double turns[kRotaryMaxPairs];  // per token
+};
+struct RotaryArgs {
+  const void *x;             // rows x (L, heads * hd), f32 or bf16
+  const int32_t *positions;  // rows x (L), or null: 0, 1, ..
+  void *out;                 // as x, may be x
+  int L, heads, hd, inverse;
+  bool bf16;
+  int cus;
+  // Set by the launcher: tokens and features a thread takes.
+  int steps, groups;
+  RotaryPlan plan;
+};
+hipError_t launch_rotary(RotaryArgs a, int rows, hipStream_t stream, const KernelEvents &ev);
+
+// ------------------------------------------------ paged 8-bit cache
+
+// Tokens that share a scale (per kv head, keys and values apart).
+constexpr int kCacheBlock = 64;
+// Features of a head that the cache may hold; a head takes whole 64s of them.
+constexpr int kCacheMaxHd = 256;
+__host__ __device__ constexpr int cache_wide(int hd) { return (hd + 63) & ~63; }
+// Exponent of the smallest scale: a block whose values are smaller loses them.
+constexpr int kCacheLowest = -100;
+// Per page and kv head `blocks` blocks of 64 tokens: keys (64, wide) each, features
+// contiguous; values (wide, 64), tokens contiguous; a scale each.
+struct CacheView {
+  uint8_t *keys, *values;  // e4m3
+  float *key_scales, *value_scales;
+  const int32_t *table;    // rows x (per_row) pages
+  const int32_t *lengths;  // rows: tokens cached before the call, or null: none
+  const int32_t *counts;   // rows: active tokens, the last ones, or null: all
+  int pages, per_row;
+  int blocks_log2;         // blocks of a page
+  int kv_heads, hd, wide, L;
+};
+// A row's tokens before the call (first) and of it (count); false where they do not
+// fit the row's pages.
+__device__ __forceinline__ bool cache_row(const CacheView &c, int r, int &first, int &count) {
+  first = c.lengths ? c.lengths[r] : 0;
+  count = c.counts ? c.counts[r] : c.L;
+  const long long room = (long long)c.per_row << (c.blocks_log2 + 6);
+  return first >= 0 && count >= 0 && count <= c.L && (long long)first + count <= room;
+}
+// Place of block b of row r and head h in the pool of blocks, or -1.
+__device__ __forceinline__ long long cache_block(const CacheView &c, int r, int h, int b) {
+  const int page = c.table[(size_t)r * c.per_row + (b >> c.blocks_log2)];
+  if ((uint32_t)page >= (uint32_t)c.pages) return -1;
+  return (((long long)page * c.kv_heads + h) << c.blocks_log2) + (b & ((1 << c.blocks_log2) - 1));
+}
+
+struct AppendArgs {
+  CacheView cache;
+  const void *k, *v;    // rows x (L, kv_heads * hd)
+  const float *k_norm;  // (hd), or null: keys as they are
+  float eps;
+  bool bf16;
+  RotaryPlan plan;
+};
+hipError_t launch_cache_append(const AppendArgs &a, int rows, hipStream_t stream,
+                               const KernelEvents &ev);
+
+struct CachedArgs {
+  CacheView cache;
+  const void *q, *gate;  // rows x (L, heads * hd); gate may be null
+  const float *q_norm;   // (hd), or null
+  float *out;
+  float eps, c1;         // c1: log2(e) / sqrt(hd)
+  int heads, group;
+  bool bf16;
+  int cus;
+  // Set by cached_plan: query tiles per (row, kv head), parts of a tile's blocks.
+  int tiles, parts;
+  float *part_out, *part_stats;
+  RotaryPlan plan;
+};
+// Columns (token, query head) of a query tile.
+constexpr int kCachedColumns = 16;
+void cached_plan(CachedArgs &a, int rows);
+size_t cached_work_bytes(const CachedArgs &a, int rows);
+hipError_t launch_cached_attention(const CachedArgs &a, int rows, hipStream_t stream,
+                                   const KernelEvents &ev);
+
 }  // namespace tfd

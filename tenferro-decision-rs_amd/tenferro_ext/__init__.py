@@ -11,7 +11,9 @@ The reference exposes the two ops as eager-session extension methods:
 and as ``ExtensionOp`` descriptors (``LayaAttentionBlockOp``,
 ``JeffFullAttentionOp``) whose payload stores the f64 parameters as f32 bits.
 Beside them stand the operators a hybrid Jeff model needs around its full-attention
-layers: ``jeff_linear_attention_rows`` / ``_step`` and ``token_log_probs``.
+layers: ``jeff_linear_attention_rows`` / ``_step`` and ``token_log_probs``, and for those
+layers while it generates: ``rotary_rows``, ``jeff_cache_append`` and
+``jeff_cached_attention`` over a ``PagedCache`` in 8 bits.
 This module keeps those names, argument meanings and error behaviour, and runs
 every call on the GPU through ``libtfd_attention.so``. There is no CPU
 fallback: if the library or a GPU is missing, calls raise.
@@ -46,6 +48,8 @@ TFD_HOST_PTRS = 0
 TFD_DEVICE_PTRS = 1
 TFD_ASYNC = 2
 TFD_TRIM_LEADING = 4
+TFD_INTERLEAVED = 8
+TFD_INVERSE = 16
 TFD_KV_HEADS_MASK = 0xFFFF0000
 
 
@@ -79,6 +83,12 @@ EXPORTED_SYMBOLS = (
     "tfd_jeff_linear_attention_rows_bf16",
     "tfd_token_log_probs_f32",
     "tfd_token_log_probs_bf16",
+    "tfd_rotary_rows_f32",
+    "tfd_rotary_rows_bf16",
+    "tfd_jeff_cache_append_f32",
+    "tfd_jeff_cache_append_bf16",
+    "tfd_jeff_cached_attention_f32",
+    "tfd_jeff_cached_attention_bf16",
     "tfd_laya_forward_f32",
 )
 
@@ -164,6 +174,11 @@ def load_library(path: Optional[str] = None) -> ctypes.CDLL:
         sig[f"tfd_jeff_linear_attention_rows_{kind}"] = (
             I, [P, S, S, S, S, S, S, P, P, P, P, P, P, U32, P, P, P, F])
         sig[f"tfd_token_log_probs_{kind}"] = (I, [P, P, S, S, S, P, S, S, P, P, P, P, F])
+        sig[f"tfd_rotary_rows_{kind}"] = (I, [P, S, S, S, S, S, P, P, P, U32, P, F])
+        sig[f"tfd_jeff_cache_append_{kind}"] = (
+            I, [P, S, S, S, S, S, P, P, P, P, U32, U32, P, P, S, P, P, F])
+        sig[f"tfd_jeff_cached_attention_{kind}"] = (
+            I, [P, S, S, S, S, S, S, P, P, P, P, U32, U32, P, P, S, P, P, P, F])
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
         fn.restype = res
@@ -276,6 +291,8 @@ _TORCH_DTYPES = {
     np.dtype(np.uint8): ("uint8", "bool"),
     np.dtype(np.uint16): ("uint16", "int16", "bfloat16"),
     np.dtype(np.int64): ("int64",),
+    np.dtype(np.int32): ("int32",),
+    "e4m3": ("float8_e4m3fn", "uint8"),  # codes, bytes on the host
 }
 _accepted: set = set()  # (torch dtype, host dtype) pairs that passed the check by name
 
@@ -299,7 +316,7 @@ class _Arg:
             return
         if _torch_types.get(type(x)) or _is_torch(x):
             if (x.dtype, dtype) not in _accepted:
-                allowed = _TORCH_DTYPES[np.dtype(dtype)]
+                allowed = _TORCH_DTYPES[dtype if dtype == "e4m3" else np.dtype(dtype)]
                 got = str(x.dtype).replace("torch.", "")
                 if got not in allowed:
                     raise InvalidArgument(
@@ -311,7 +328,7 @@ class _Arg:
             self.n = x.numel()
             self.device = x.is_cuda
         else:
-            arr = np.ascontiguousarray(x, dtype=dtype)
+            arr = np.ascontiguousarray(x, dtype=np.uint8 if dtype == "e4m3" else dtype)
             self.obj = arr
             self.ptr = arr.ctypes.data
             self.n = arr.size
@@ -645,14 +662,14 @@ def jeff_full_attention_rows(q, k, v, gate, q_norm, k_norm, mask, rows: int, len
 
 # ------------------------------------------------------------------ linear attention
 
-def _check_result(x, name: str) -> None:
+def _check_result(x, name: str, dtype=np.float32) -> None:
     """Refuses a host buffer that results would not reach: anything but a contiguous
-    float32 array is converted, and what is written then is the copy."""
+    array of the type is converted, and what is written then is the copy."""
     if not _is_torch(x) and not (
-            isinstance(x, np.ndarray) and x.dtype == np.float32
+            isinstance(x, np.ndarray) and x.dtype == dtype
             and x.flags.c_contiguous and x.flags.writeable):
         raise InvalidArgument(
-            TFD_EINVAL, f"{name}: expected a contiguous float32 array to update")
+            TFD_EINVAL, f"{name}: expected a contiguous {np.dtype(dtype).name} array to update")
 
 
 def jeff_linear_attention_rows(q, k, v, log_decay, beta, mask, rows: int, length: int, heads: int,
@@ -722,6 +739,228 @@ def jeff_linear_attention_step(q, k, v, log_decay, beta, state, rows: int, heads
     return jeff_linear_attention_rows(q, k, v, log_decay, beta, mask, rows, 1, heads, key_heads,
                                       key_dim, value_dim, scale=scale, state=state,
                                       state_out=state, bf16=bf16, ctx=ctx, out=out)[0]
+
+
+# ------------------------------------------------------------------ rotary positions
+
+class Rotary(NamedTuple):
+    """How pairs of features turn with their token's position p: pair i by p frequencies[i]
+    turns, then times ``magnitude``. frequencies: float64, in host memory, one a pair; the
+    pairs are (2i, 2i+1) where ``interleaved``, else (i, i + pairs), and stand first in a head."""
+
+    frequencies: Any
+    interleaved: bool = False
+    magnitude: float = 1.0
+
+
+def rotary_frequencies(rotary_dim: int, theta: float, *, scaling: str = "none", factor: float = 1.0,
+                       trained_length: int = 0, low_turns: float = 1.0,
+                       high_turns: float = 32.0) -> np.ndarray:
+    """Turns per token of the rotary_dim / 2 pairs, theta^(-2i/rotary_dim) / 2 pi, stretched for
+    contexts ``factor`` times as long by ``scaling``:
+
+    * ``"none"``
+    * ``"linear"``: every frequency divided by ``factor``
+    * ``"base"``: theta times factor^(rotary_dim/(rotary_dim-2)), which divides the lowest
+      frequency by ``factor`` and keeps the highest
+    * ``"bands"``: a pair that turns at least ``high_turns`` times in ``trained_length`` tokens keeps
+      its frequency, one that turns at most ``low_turns`` times has it divided by ``factor``, between
+      them the two are blended by the number of turns
+    """
+    if rotary_dim < 0 or rotary_dim % 2:
+        raise InvalidArgument(TFD_EINVAL, "rotary_dim: rotary_dim must be even")
+    if not theta > 0 or not factor > 0:
+        raise InvalidArgument(TFD_EINVAL, "rotary_frequencies: theta and factor must be positive")
+    if scaling == "base":
+        if rotary_dim <= 2:
+            raise InvalidArgument(TFD_EINVAL, "scaling: \"base\" needs a rotary_dim over 2")
+        theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
+    i = np.arange(rotary_dim // 2, dtype=np.float64)
+    f = np.float64(theta) ** (-2.0 * i / max(rotary_dim, 1)) / (2.0 * np.pi)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "bands":
+        if not trained_length > 0 or not high_turns > low_turns:
+            raise InvalidArgument(TFD_EINVAL, "scaling: \"bands\" needs a trained_length and "
+                                  "high_turns over low_turns")
+        keep = np.clip((f * trained_length - low_turns) / (high_turns - low_turns), 0.0, 1.0)
+        f = f * (keep + (1.0 - keep) / factor)
+    elif scaling not in ("none", "base"):
+        raise InvalidArgument(TFD_EINVAL, f"scaling: unknown scaling {scaling!r}")
+    return f
+
+
+_NO_ROTARY = Rotary(None)
+
+
+def _rotary_args(rotary):
+    """(the array that has to live until the call returns, rotary_dim, address, magnitude bits,
+    flags)."""
+    frequencies, interleaved, magnitude = _NO_ROTARY if rotary is None else rotary
+    if frequencies is None:
+        return None, 0, None, f32_bits(magnitude), 0
+    f = np.ascontiguousarray(frequencies, dtype=np.float64)
+    return (f, 2 * f.size, f.ctypes.data, f32_bits(magnitude), TFD_INTERLEAVED if interleaved else 0)
+
+
+def rotary_rows(x, positions, rows: int, length: int, heads: int, head_dim: int, rotary, *,
+                inverse: bool = False, bf16: bool = False, ctx: Optional[Context] = None, out=None):
+    """Rotary positions of rows of heads (include/tfd_attention.h). x: rows x (length,
+    heads*head_dim). positions: int32 rows x (length), or None for 0, 1, ... ``rotary``: a
+    ``Rotary``. ``inverse`` turns back, which is the gradient: of out to that of x. bf16 takes
+    and returns bf16 bits. ``out`` may be ``x``. Returns out, of x's type."""
+    ctx = ctx or default_context()
+    dt = np.uint16 if bf16 else np.float32
+    n = rows * length * heads * head_dim
+    ax = _Arg(x, dt, "x", n)
+    ap = _Arg(positions, np.int32, "positions", None if positions is None else rows * length)
+    args = [ax, ap]
+    if out is None:
+        if ax.device:
+            out = ax.obj.new_empty(n)
+            out_ptr = out.data_ptr()
+        else:
+            out = np.empty(n, dtype=dt)
+            out_ptr = out.ctypes.data
+    else:
+        _check_result(out, "out", dt)
+        args.append(_Arg(out, dt, "out", n))
+        out, out_ptr = args[-1].obj, args[-1].ptr
+    kept, dim, freq, magnitude, rotary_flags = _rotary_args(rotary)
+    flags = _flags(args, ctx)
+    fn = ctx._lib.tfd_rotary_rows_bf16 if bf16 else ctx._lib.tfd_rotary_rows_f32
+    flags |= rotary_flags | (TFD_INVERSE if inverse else 0)
+    _call(ctx, flags, fn, ctx.handle, rows, length, heads, head_dim, dim, ax.ptr, ap.ptr, freq,
+          magnitude, out_ptr, flags)
+    return out
+
+
+# ------------------------------------------------------------------ paged 8-bit cache
+
+class PagedCache(NamedTuple):
+    """A paged cache of keys and values in e4m3 with a scale for each block of 64 tokens
+    and kv head (include/tfd_attention.h). Flat: keys pages x kv_heads x (page_tokens, wide),
+    features contiguous; values pages x kv_heads x page_tokens/64 x (wide, 64), tokens contiguous
+    (float8_e4m3fn or uint8 tensors, uint8 arrays); the scales float32, pages x kv_heads x
+    page_tokens/64. ``wide`` is head_dim rounded up to a multiple of 64."""
+
+    keys: Any
+    values: Any
+    key_scales: Any
+    value_scales: Any
+    page_tokens: int
+
+
+def paged_cache(pages: int, kv_heads: int, head_dim: int, page_tokens: int = 64, *,
+                device=None) -> PagedCache:
+    """An empty ``PagedCache``, of torch tensors on ``device`` or, if None, of numpy arrays."""
+    if page_tokens < 64 or page_tokens & (page_tokens - 1):
+        raise InvalidArgument(
+            TFD_EINVAL, "page_tokens: page_tokens must be a power of two of at least 64")
+    n = pages * kv_heads * page_tokens
+    size, blocks = n * (-(-head_dim // 64) * 64), n // 64
+    if device is None:
+        return PagedCache(np.zeros(size, np.uint8), np.zeros(size, np.uint8),
+                          np.ones(blocks, np.float32), np.ones(blocks, np.float32), page_tokens)
+    import torch
+
+    codes = [torch.zeros(size, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+             for _ in range(2)]
+    scales = [torch.ones(blocks, dtype=torch.float32, device=device) for _ in range(2)]
+    return PagedCache(*codes, *scales, page_tokens)
+
+
+class _PagedCacheStruct(ctypes.Structure):
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p),
+                ("key_scales", ctypes.c_void_p), ("value_scales", ctypes.c_void_p),
+                ("pages", ctypes.c_size_t), ("page_tokens", ctypes.c_size_t)]
+
+
+def _cache_args(cache, pages, lengths, counts, rows: int, kv_heads: int, head_dim: int):
+    """(the arguments to check, the C struct, pages a row)."""
+    keys, values, key_scales, value_scales, page_tokens = cache
+    if page_tokens < 64 or page_tokens & (page_tokens - 1):
+        raise InvalidArgument(
+            TFD_EINVAL, "page_tokens: page_tokens must be a power of two of at least 64")
+    ak = _Arg(keys, "e4m3", "keys")
+    per_page = kv_heads * page_tokens * (-(-head_dim // 64) * 64)
+    held = ak.n // per_page if per_page else 0
+    av = _Arg(values, "e4m3", "values", ak.n)
+    blocks = held * kv_heads * (page_tokens // 64)
+    aks = _Arg(key_scales, np.float32, "key_scales", blocks)
+    avs = _Arg(value_scales, np.float32, "value_scales", blocks)
+    if ak.n != held * per_page:
+        raise InvalidArgument(TFD_EINVAL, f"keys: {ak.n} elements, not whole pages of {per_page}")
+    ap = _Arg(pages, np.int32, "pages")
+    per_row = ap.n // rows if rows else 0
+    if ap.n != per_row * rows:
+        raise InvalidArgument(
+            TFD_EINVAL, f"pages: {ap.n} elements, not a whole number for each of {rows} rows")
+    al = _Arg(lengths, np.int32, "lengths", None if lengths is None else rows)
+    ac = _Arg(counts, np.int32, "counts", None if counts is None else rows)
+    struct_ = _PagedCacheStruct(ak.ptr, av.ptr, aks.ptr, avs.ptr, held, page_tokens)
+    return [ak, av, aks, avs, ap, al, ac], struct_, per_row
+
+
+def jeff_cache_append(k, v, k_norm, cache, pages, lengths, counts, rows: int, length: int,
+                      kv_heads: int, head_dim: int, rotary, eps: float, *, bf16: bool = False,
+                      ctx: Optional[Context] = None):
+    """Appends keys (normalized and turned) and values of new tokens to the rows' pages of a
+    ``PagedCache``, in place (include/tfd_attention.h).
+
+    k, v: rows x (length, kv_heads*head_dim); the last counts[r] tokens of row r are new
+    (counts None: all). k_norm (head_dim) or None: keys as they are. ``rotary``: a ``Rotary``
+    or None. pages: int32 (rows, pages a row); lengths: int32 (rows), the tokens that the
+    rows hold before the call (None: none), not updated. bf16 takes k and v as bf16 bits."""
+    ctx = ctx or default_context()
+    dt = np.uint16 if bf16 else np.float32
+    n = rows * length * kv_heads * head_dim
+    ak, av = _Arg(k, dt, "k", n), _Arg(v, dt, "v", n)
+    an = _Arg(k_norm, np.float32, "k_norm", None if k_norm is None else head_dim)
+    for x, name, kind in zip(cache, PagedCache._fields, (np.uint8, np.uint8, np.float32, np.float32)):
+        _check_result(x, name, kind)
+    args, held, per_row = _cache_args(cache, pages, lengths, counts, rows, kv_heads, head_dim)
+    kept, dim, freq, magnitude, rotary_flags = _rotary_args(rotary)
+    flags = _flags([ak, av, an] + args, ctx) | rotary_flags
+    fn = ctx._lib.tfd_jeff_cache_append_bf16 if bf16 else ctx._lib.tfd_jeff_cache_append_f32
+    _call(ctx, flags, fn, ctx.handle, rows, length, kv_heads, head_dim, dim, ak.ptr, av.ptr, an.ptr,
+          freq, magnitude, f32_bits(eps), ctypes.byref(held), args[4].ptr, per_row, args[5].ptr,
+          args[6].ptr, flags)
+
+
+def jeff_cached_attention(q, gate, q_norm, cache, pages, lengths, counts, rows: int, length: int,
+                          heads: int, kv_heads: int, head_dim: int, rotary, eps: float, *,
+                          bf16: bool = False, ctx: Optional[Context] = None, out=None):
+    """Causal attention of new tokens over the ``PagedCache`` that holds them already
+    (``jeff_cache_append`` with the same pages, lengths and counts) and their row's earlier
+    ones: q normalized and turned, outputs times sigmoid(gate) (include/tfd_attention.h).
+
+    q, gate: rows x (length, heads*head_dim), gate may be None; q_norm (head_dim) or None. bf16
+    takes q and gate as bf16 bits. Returns out (f32), rows x (length, heads*head_dim), 0 at the
+    tokens before a row's last counts[r]."""
+    ctx = ctx or default_context()
+    dt = np.uint16 if bf16 else np.float32
+    n = rows * length * heads * head_dim
+    aq = _Arg(q, dt, "q", n)
+    ag = _Arg(gate, dt, "gate", None if gate is None else n)
+    an = _Arg(q_norm, np.float32, "q_norm", None if q_norm is None else head_dim)
+    args, held, per_row = _cache_args(cache, pages, lengths, counts, rows, kv_heads, head_dim)
+    checked = [aq, ag, an] + args
+    if out is None:
+        out = _new_out(aq, n)
+        out_ptr = _ptr(out)
+    else:
+        _check_result(out, "out")
+        checked.append(_Arg(out, np.float32, "out", n))
+        out, out_ptr = checked[-1].obj, checked[-1].ptr
+    kept, dim, freq, magnitude, rotary_flags = _rotary_args(rotary)
+    flags = _flags(checked, ctx) | rotary_flags
+    fn = (ctx._lib.tfd_jeff_cached_attention_bf16 if bf16
+          else ctx._lib.tfd_jeff_cached_attention_f32)
+    _call(ctx, flags, fn, ctx.handle, rows, length, heads, kv_heads, head_dim, dim, aq.ptr, ag.ptr,
+          an.ptr, freq, magnitude, f32_bits(eps), ctypes.byref(held), args[4].ptr, per_row,
+          args[5].ptr, args[6].ptr, out_ptr, flags)
+    return out
 
 
 # ------------------------------------------------------------------ readout
