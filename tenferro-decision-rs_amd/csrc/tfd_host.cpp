@@ -1984,16 +1984,22 @@ int cached_run(tfd_ctx *c, bool bf16, CacheCall m, size_t heads, size_t rotary_d
   a.group = (int)(heads / m.kv_heads);
   a.bf16 = bf16;
   a.cus = c->cus;
-  tfd::cached_plan(a, (int)m.rows);
-  if (const size_t bytes = tfd::cached_work_bytes(a, (int)m.rows)) {
-    if ((rc = reserve_capturable(c, op, c->cached, bytes, capturing))) return rc;
-    a.part_out = static_cast<float *>(c->cached.ptr);
-    a.part_stats = a.part_out + bytes / sizeof(float) / (m.wide + 2) * m.wide;
-  }
+  a.rows = (int)m.rows;
+  tfd::cached_plan(a);
+  // The counters at the workspace's start are zero between calls, whatever sizes a call has.
+  const tfd::CachedSpace space = tfd::cached_space(a);
+  const size_t bytes = space.done + space.stats + space.out;
+  const bool grows = bytes > c->cached.cap;
+  if ((rc = reserve_capturable(c, op, c->cached, bytes, capturing))) return rc;
+  if (grows)
+    TFD_HIP(c, tfd::launch_fill_zero(static_cast<float *>(c->cached.ptr),
+                                     space.done / sizeof(float), c->stream), "fill_zero launch");
+  a.part_done = static_cast<unsigned *>(c->cached.ptr);
+  a.part_stats = reinterpret_cast<float *>(a.part_done + space.done / sizeof(unsigned));
+  a.part_out = a.part_stats + space.stats / sizeof(float);
   tfd::KernelEvents ev;
   if (!capturing && (rc = timing_events(c, &ev))) return rc;
-  TFD_HIP(c, tfd::launch_cached_attention(a, (int)m.rows, c->stream, ev),
-          "cached_attention launch");
+  TFD_HIP(c, tfd::launch_cached_attention(a, c->stream, ev), "cached_attention launch");
   return finish(c, flags, out, out_d, sizeof(float) * n);
 }
 

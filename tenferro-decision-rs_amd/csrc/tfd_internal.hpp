@@ -494,16 +494,23 @@ struct CachedArgs {
   int heads, group;
   bool bf16;
   int cus;
-  // Set by cached_plan: query tiles per (row, kv head), parts of a tile's blocks.
-  int tiles, parts;
-  float *part_out, *part_stats;
+  int rows;
+  // Set by cached_plan: tiles of columns per (row, kv head), workgroups beside the tiles' that
+  // long rows are spread over (0: the grid's, whatever the tiles), the least blocks that make
+  // a part, places for partial results; grid: workgroups of the launch.
+  int tiles, spread, grid, least, slots;
+  unsigned *part_done;  // zeroed once, and left at zero by every launch
+  float *part_stats, *part_out;
   RotaryPlan plan;
 };
 // Columns (token, query head) of a query tile.
 constexpr int kCachedColumns = 16;
-void cached_plan(CachedArgs &a, int rows);
-size_t cached_work_bytes(const CachedArgs &a, int rows);
-hipError_t launch_cached_attention(const CachedArgs &a, int rows, hipStream_t stream,
+struct CachedSpace {
+  size_t done, stats, out;  // bytes of the workspace's parts
+};
+void cached_plan(CachedArgs &a);
+CachedSpace cached_space(const CachedArgs &a);
+hipError_t launch_cached_attention(const CachedArgs &a, hipStream_t stream,
                                    const KernelEvents &ev);
 
 }  // namespace tfd

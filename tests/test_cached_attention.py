@@ -1,14 +1,19 @@
 """Attention over the paged 8-bit cache against the formula in 64 bits, on the codes and scales
 that the cache holds.
 
-Tolerance, in units of u = 2^-24. A normalized, turned query feature carries at most 24 roundings
+Tolerance, in units of u = 2^-24. A normalized, turned query feature carries at most 28 roundings
 (norm: 9 of a sum of 256 squares, its root, reciprocal, two products; turn: 9 of
-test_rotary), each at most u of the features that enter it; a score's sum of 3 hd products
+test_rotary; two fp16 pieces of 11 bits: 2^-22, which is 4), each at most u of the features that
+enter it; a score's sum of 3 hd products
 six standard deviations of independent roundings, 6 sqrt(3 hd). All are taken on the sum of the
 products' absolute values (`size`; a turned pair mixes two features, which 2 covers), and
 e^score is off by twice that (numerator and denominator) plus 4 u |score| of the score's scaling and
-its difference from the reference. exp2, the pieces, scales and sums over T keys add 16 + 6 sqrt(3 T)
-u, the gate 8 + 2 |gate|. All on the sum of p |v| times the gate.
+its difference from the reference. exp2, two fp16 pieces, scales and sums over T keys add 20 + 6 sqrt(3 T)
+u, the gate 8 + 2 |gate|. All on the sum of p |v| times the gate. Beside it a probability, which
+is at most 1 against the row's largest, is held times 2^15 in fp16 pieces whose last step is 2^-24:
+it is off by up to 2^-25 / 2^15 = 2^-40 however small it is, on the sum of |v| (the sum of the
+probabilities, which divides it, is at least 1). That shows where the largest probabilities meet
+values of 0.
 """
 import numpy as np
 import pytest
@@ -56,13 +61,14 @@ def reference(ref, q, gate, norm, rotary, before, counts):
                     p /= p.sum(1, keepdims=True)
                     pv = np.where(seen[:, :, None], p[:, :, None] * v, 0).sum(1) if np.isnan(
                         v).any() else p @ v
-                    e = 2 * ((24 + 6 * np.sqrt(3 * hd)) * 2 * np.where(seen, size, 0).max(1)
-                             + 4 * np.where(seen, np.abs(s), 0).max(1)) + 16 + 6 * np.sqrt(3 * (n + c))
+                    e = 2 * ((28 + 6 * np.sqrt(3 * hd)) * 2 * np.where(seen, size, 0).max(1)
+                             + 4 * np.where(seen, np.abs(s), 0).max(1)) + 20 + 6 * np.sqrt(3 * (n + c))
                     g = 1.0 if gate is None else 1 / (1 + np.exp(-gate[r, j].T[L - c:].astype(float)))
                     extra = 8 if gate is None else 8 + 2 * np.abs(gate[r, j].T[L - c:])
                     out[r, j, :, L - c:] = (pv * g).T
                     tol[r, j, :, L - c:] = ((e[:, None] + extra) * U * (p @ np.abs(np.nan_to_num(v)))
                                             * g).T
+                    tol[r, j, :, L - c:] += 2.0**-40 * (seen @ np.abs(np.nan_to_num(v)) * g).T
     return out, tol
 
 
