@@ -459,13 +459,17 @@ struct CacheView {
   int blocks_log2;         // blocks of a page
   int kv_heads, hd, wide, L;
 };
+// Whether a row's pages hold `count` tokens of the call's behind `first`.
+__device__ __forceinline__ bool cache_holds(const CacheView &c, int first, int count) {
+  const long long room = (long long)c.per_row << (c.blocks_log2 + 6);
+  return first >= 0 && count >= 0 && count <= c.L && (long long)first + count <= room;
+}
 // A row's tokens before the call (first) and of it (count); false where they do not
 // fit the row's pages.
 __device__ __forceinline__ bool cache_row(const CacheView &c, int r, int &first, int &count) {
   first = c.lengths ? c.lengths[r] : 0;
   count = c.counts ? c.counts[r] : c.L;
-  const long long room = (long long)c.per_row << (c.blocks_log2 + 6);
-  return first >= 0 && count >= 0 && count <= c.L && (long long)first + count <= room;
+  return cache_holds(c, first, count);
 }
 // Place of block b of row r and head h in the pool of blocks, or -1.
 __device__ __forceinline__ long long cache_block(const CacheView &c, int r, int h, int b) {
@@ -495,10 +499,9 @@ struct CachedArgs {
   bool bf16;
   int cus;
   int rows;
-  // Set by cached_plan: tiles of columns per (row, kv head), workgroups beside the tiles' that
-  // long rows are spread over (0: the grid's, whatever the tiles), the least blocks that make
-  // a part, places for partial results; grid: workgroups of the launch.
-  int tiles, spread, grid, least, slots;
+  // Set by cached_plan: tiles of columns per (row, kv head), workgroups, the least blocks
+  // that make a part, places for partial results.
+  int tiles, grid, least, slots;
   unsigned *part_done;  // zeroed once, and left at zero by every launch
   float *part_stats, *part_out;
   RotaryPlan plan;
