@@ -499,15 +499,17 @@ struct CachedArgs {
   bool bf16;
   int cus;
   int rows;
-  // Set by cached_plan: tiles of columns per (row, kv head), workgroups, the least blocks
-  // that make a part, places for partial results.
-  int tiles, grid, least, slots;
+  // Set by cached_plan: the kernel, columns of a tile, tiles per (row, kv head), workgroups,
+  // the least blocks that make a part, pieces of an even share, most parts of a tile, places
+  // for partial results.
+  bool prompt;
+  int columns, tiles, grid, least, finer, cap, slots;
   unsigned *part_done;  // zeroed once, and left at zero by every launch
   float *part_stats, *part_out;
   RotaryPlan plan;
 };
-// Columns (token, query head) of a query tile.
-constexpr int kCachedColumns = 16;
+// Up to this many (token, query head of a group) columns of a row take the rows kernel.
+constexpr int kCachedPromptColumns = 32;
 struct CachedSpace {
   size_t done, stats, out;  // bytes of the workspace's parts
 };
@@ -515,5 +517,6 @@ void cached_plan(CachedArgs &a);
 CachedSpace cached_space(const CachedArgs &a);
 hipError_t launch_cached_attention(const CachedArgs &a, hipStream_t stream,
                                    const KernelEvents &ev);
+hipError_t launch_cached_prompt(const CachedArgs &a, hipStream_t stream, const KernelEvents &ev);
 
 }  // namespace tfd
