@@ -9,8 +9,9 @@
 // products, one for each piece of the f32 one: hi the nearest fp16, lo that of the rest, 22
 // significant bits. A column's queries are taken times a power of two that brings the largest
 // to [2^13, 2^14), so that what fp16's range cuts off is below 2^-37 of the column's
-// largest; probabilities (at most 1) times 2^15, which leaves 2^-40. The blocks' key scales
-// are applied to the scores; the outputs are kept in units of the last block's value scale.
+// largest; probabilities (at most 1) times 2^11 to 2^15, which leaves 2^-36. The blocks' key
+// scales are applied to the scores, their value scales to the probabilities, against a unit
+// that the outputs are kept in.
 //
 // Tiles. The columns of a product are (token, query head of the group) pairs of one
 // (row, kv head), 16 of them; its rows are keys, then features. S^T = K Q^T leaves lane
@@ -342,11 +343,12 @@ __device__ __forceinline__ bool open_tile(const CachedArgs &a, const Share &shar
   return true;
 }
 
-// Walks the (query head, feature) rows of a tile, lanes along its tokens: fn(column of the
-// tile, feature, place in rows x (L, heads * hd)).
-template <int THREADS, typename F>
+// Walks the (query head, feature) rows of a tile, lanes along its tokens: use(column of the
+// tile, feature, place in rows x (L, heads * hd), load(that place)), with eight loads on
+// their way at once.
+template <int THREADS, typename F, typename G>
 __device__ __forceinline__ void along_tokens(const CachedArgs &a, const Share &share, const Tile &t,
-                                             F fn) {
+                                             F load, G use) {
   const int L = a.cache.L, hd = a.cache.hd, group = a.group;
   const int tokens = t.u1 - t.u0 + 1;
   const int bits = tokens > 1 ? 32 - __builtin_clz(tokens - 1) : 0;  // at most COLS tokens
@@ -362,15 +364,27 @@ __device__ __forceinline__ void along_tokens(const CachedArgs &a, const Share &s
   const int token = L - t.count + t.u0 + u;
   const int jump = step / hd, rest = step - jump * hd;
   while (g < high) {
-    const int c = (t.u0 + u) * group + g - t.c0;
-    if (u < tokens && c >= 0 && c < t.used)
-      fn(c, row, (base + (size_t)g * hd + row) * L + token);
-    g += jump;
-    row += rest;
-    if (row >= hd) {
-      row -= hd;
-      ++g;
+    constexpr int kBatch = 8;
+    int c[kBatch], f[kBatch];
+    size_t at[kBatch];
+    float v[kBatch];
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e) {
+      c[e] = (t.u0 + u) * group + g - t.c0;
+      f[e] = row;
+      if (g >= high || u >= tokens || c[e] >= t.used) c[e] = -1;
+      at[e] = (base + (size_t)g * hd + row) * L + token;
+      v[e] = c[e] >= 0 ? load(at[e]) : 0.0f;
+      g += jump;
+      row += rest;
+      if (row >= hd) {
+        row -= hd;
+        ++g;
+      }
     }
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e)
+      if (c[e] >= 0) use(c[e], f[e], at[e], v[e]);
   }
 }
 
@@ -380,7 +394,7 @@ __device__ __forceinline__ void along_tokens(const CachedArgs &a, const Share &s
 template <int N>
 struct Softmax {
   float m = -INFINITY, l = 0.0f;   // reference in log2 units and sum
-  float unit = 1.0f, top = 0.0f;   // the outputs' unit, the largest value scale so far
+  float unit = 1.0f, top = 0.0f;   // the outputs' unit, the largest so far
   f32x4 o[N];
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -407,17 +421,17 @@ struct Softmax {
     const float ref = mn == -INFINITY ? 0.0f : mn;
     const float alpha = m == -INFINITY ? 0.0f : fast_exp2(m - ref);
     m = mn;
-    // The block's value scale becomes the unit, unless it is so far below the largest one
-    // that the outputs could leave f32's range in it: then the probabilities carry the
-    // difference.
-    float turn = alpha, p15 = 0x1p15f;
-    if (vs != unit) {
+    // The outputs' unit is a value scale that blocks have had: a block's own up to 16 times
+    // smaller is made up for in the probabilities; another one becomes the unit, unless it is
+    // so far below the largest that the outputs could leave f32's range in it.
+    float turn = alpha;
+    if (vs > unit || vs < unit * 0x1p-4f) {
       top = fmaxf(top, vs);
       const float to = fmaxf(vs, top * 0x1p-90f);
       turn = alpha * (unit / to);
-      p15 = 0x1p15f * (vs / to);
       unit = to;
     }
+    const float p15 = vs == unit ? 0x1p15f : 0x1p15f * (vs / unit);
     float rs = 0.0f;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
@@ -439,68 +453,75 @@ struct Softmax {
       p[1][k] = join_f16(lo.lo, hi.lo);
     }
   }
-  // Adds the block's values; raw(f): the lane's 16 bytes of features 16 f + lane % 16.
-  template <typename F>
-  __device__ __forceinline__ void add(F raw, bool masked, int limit, const f16x8 (&p)[2][2]) {
-    if (!masked) {
-      // Four operands ahead of the products.
-      u32x4 c[4], next[4];
+};
+
+// Adds a block's values to CT tiles' outputs; raw(f): the lane's 16 bytes of features
+// 16 f + lane % 16.
+template <int N, int CT, typename F>
+__device__ __forceinline__ void add_values(Softmax<N> (&soft)[CT], F raw, bool masked,
+                                           const int (&limit)[CT], const f16x8 (&p)[CT][2][2]) {
+  auto multiply = [&](int f, u32x4 c) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) c[e] = raw(e);
+    for (int k = 0; k < 2; ++k) {
+      const f16x8 v = codes_f16(c[2 * k], c[2 * k + 1]);
 #pragma unroll
-      for (int f = 0; f < N; f += 4) {
+      for (int i = 1; i >= 0; --i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (f + 4 < N) next[e] = raw(f + 4 + e);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const f16x8 v = codes_f16(c[e][2 * k], c[e][2 * k + 1]);
-            o[f + e] = mfma_16x16x32_f16(v, p[1][k], o[f + e]);
-            o[f + e] = mfma_16x16x32_f16(v, p[0][k], o[f + e]);
-          }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c[e] = next[e];
-      }
-      return;
+        for (int ct = 0; ct < CT; ++ct)
+          soft[ct].o[f] = mfma_16x16x32_f16(v, p[ct][i][k], soft[ct].o[f]);
     }
-    // What a column does not see must not reach it: the product of a probability of 0 and a
-    // NaN (a later token's, or what was in memory) is NaN. The block's NaN codes become 0,
-    // and the columns that do see one get it back.
-    f16x8 sees[2];
+  };
+  if (!masked) {
+    // Operands ahead of the products, which take long enough for them to arrive.
+    constexpr int kAhead = 4 / CT;
+    u32x4 c[kAhead], next[kAhead];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int e = 0; e < kAhead; ++e) c[e] = raw(e);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sees[k][e] = (_Float16)(8 * k + e <= limit ? 1.0f : 0.0f);
+    for (int f = 0; f < N; f += kAhead) {
 #pragma unroll
-    for (int f = 0; f < N; ++f) {
-      u32x4 c = raw(f);
-      u32x4 bad;
+      for (int e = 0; e < kAhead; ++e)
+        if (f + kAhead < N) next[e] = raw(f + kAhead + e);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        bad[e] = nan_codes(c[e]) >> 7;
-        c[e] &= ~(bad[e] * 0xffu);
-      }
+      for (int e = 0; e < kAhead; ++e) multiply(f + e, c[e]);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const f16x8 v = codes_f16(c[2 * k], c[2 * k + 1]);
-        o[f] = mfma_16x16x32_f16(v, p[1][k], o[f]);
-        o[f] = mfma_16x16x32_f16(v, p[0][k], o[f]);
-      }
-      if (__any((bad[0] | bad[1] | bad[2] | bad[3]) != 0)) {
+      for (int e = 0; e < kAhead; ++e) c[e] = next[e];
+    }
+    return;
+  }
+  // What a column does not see must not reach it: the product of a probability of 0 and a
+  // NaN (a later token's, or what was in memory) is NaN. The block's NaN codes become 0,
+  // and the columns that do see one get it back.
+#pragma unroll
+  for (int f = 0; f < N; ++f) {
+    u32x4 c = raw(f), bad;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      bad[e] = nan_codes(c[e]) >> 7;
+      c[e] &= ~(bad[e] * 0xffu);
+    }
+    multiply(f, c);
+    if (__any((bad[0] | bad[1] | bad[2] | bad[3]) != 0)) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
         f32x4 n = {0, 0, 0, 0};
 #pragma unroll
-        for (int k = 0; k < 2; ++k)  // 0x38: e4m3's 1
-          n = mfma_16x16x32_f16(codes_f16(bad[2 * k] * 0x38u, bad[2 * k + 1] * 0x38u), sees[k], n);
+        for (int k = 0; k < 2; ++k) {
+          f16x8 sees;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[f][i] = n[i] > 0.0f ? __builtin_nanf("") : o[f][i];
+          for (int e = 0; e < 8; ++e) sees[e] = (_Float16)(8 * k + e <= limit[ct] ? 1.0f : 0.0f);
+          // 0x38: e4m3's 1.
+          n = mfma_16x16x32_f16(codes_f16(bad[2 * k] * 0x38u, bad[2 * k + 1] * 0x38u), sees, n);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          soft[ct].o[f][i] = n[i] > 0.0f ? __builtin_nanf("") : soft[ct].o[f][i];
       }
     }
   }
-};
+}
 
 // What the waves of a share left in LDS (o, m, l and unit of PER waves a column) to its outputs
 // or, where the tile has several parts, to its place, and the join by the last workgroup.
@@ -509,14 +530,13 @@ __device__ __forceinline__ void finish_share(const Share &share, const Tile &t, 
   constexpr int WIDE = 64 * W;
   const CachedArgs &a = args_again();
   const Parts parts = Parts::of<COLS, WIDE>(a);
-  // sh.o[0] to the outputs.
-  auto leave = [&]() {
-    __syncthreads();
-    along_tokens<THREADS>(a, share, t, [&](int c, int f, size_t at) {
-      float y = sh.o[0][c][f];
-      if (a.gate) y *= fast_sigmoid(load_as_f32<T>(a.gate, at));
-      a.out[at] = y;
-    });
+  // Joined outputs, times the gate, from LDS to where they belong.
+  auto give = [&](const float(&from)[COLS][WIDE + 4]) {
+    along_tokens<THREADS>(
+        a, share, t, [&](size_t at) { return a.gate ? load_as_f32<T>(a.gate, at) : 0.0f; },
+        [&](int c, int f, size_t at, float gate) {
+          a.out[at] = a.gate ? from[c][f] * fast_sigmoid(gate) : from[c][f];
+        });
   };
   for (int at = threadIdx.x; at < t.used * (WIDE / 4); at += THREADS) {
     const int f = 4 * (at % (WIDE / 4)), c = at / (WIDE / 4);
@@ -541,7 +561,8 @@ __device__ __forceinline__ void finish_share(const Share &share, const Tile &t, 
     }
   }
   if (share.parts == 1) {
-    leave();
+    __syncthreads();
+    give(sh.o[0]);
     return;
   }
   // The last workgroup of 16 parts to get here joins them, in the first one's place; the last
@@ -595,11 +616,7 @@ __device__ __forceinline__ void finish_share(const Share &share, const Tile &t, 
     }
     if (!finish) return;
     __syncthreads();
-    along_tokens<THREADS>(a, share, t, [&](int c, int f, size_t at) {
-      float y = sh.joined[c][f];
-      if (a.gate) y *= fast_sigmoid(load_as_f32<T>(a.gate, at));
-      a.out[at] = y;
-    });
+    give(sh.joined);
   };
   const int lead = share.part & ~(kJoin - 1), members = min(kJoin, share.parts - lead);
   if (!arrived_last(a.part_done + share.slot + lead, members)) return;

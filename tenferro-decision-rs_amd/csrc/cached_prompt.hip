@@ -9,29 +9,36 @@
 namespace tfd {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
-constexpr int kCols = 64;
 constexpr int kPromptCap = 256;
 
-// Values as keys (KeyStage): feature f's 64 tokens are four pieces, turned by f / 4.
+// Values as keys (KeyStage): feature f's 64 tokens are four pieces, at places that f / 4 turns.
+// Which quarter is first turned is chosen for the lanes that LDS serves at once, 0 to 3, 12 to
+// 15 and 20 to 27 of 32.
 template <int W>
 struct ValueStage {
   u32x4 piece[64 * 4 * W];
+  static __device__ __forceinline__ int turn(int quarter) {  // 0, 3, 1, 2
+    return (0x9c >> (2 * quarter)) & 3;
+  }
+  static __device__ __forceinline__ int unturn(int place) {  // and back
+    return (0x78 >> (2 * place)) & 3;
+  }
   static __device__ __forceinline__ int source(int lane) {
-    return 16 * ((lane & ~3) | ((lane & 3) ^ ((lane >> 4) & 3)));
+    return 16 * ((lane & ~3) | unturn((lane & 3) ^ ((lane >> 4) & 3)));
   }
   __device__ __forceinline__ u32x4 get(int f, int col, int grp) const {
-    return piece[64 * f + 4 * col + (grp ^ ((col >> 2) & 3))];
+    return piece[64 * f + 4 * col + (turn(grp) ^ ((col >> 2) & 3))];
   }
 };
 
-template <int W>
+template <int W, int CT, int NW>
 struct PromptLds {
+  static constexpr int kCols = 16 * CT * NW;
   union {
     struct {
       KeyStage<W> keys[2];
       ValueStage<W> values[2];
+      _Float16 low[CT > 1 ? kCols : 1][64 * W + 8];  // the queries' lower pieces
     };
     float x[kCols][64 * W + 4];     // queries before they are split
     float o[1][kCols][64 * W + 4];  // outputs
@@ -45,9 +52,11 @@ struct PromptLds {
   Deal::Lanes lanes;
 };
 
-template <typename T, int W>
-__device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W> &sh) {
-  constexpr int WIDE = 64 * W;
+// NW waves of CT tiles of 16 columns.
+template <typename T, int W, int CT, int NW>
+__device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W, CT, NW> &sh) {
+  constexpr int WIDE = 64 * W, kCols = 16 * CT * NW, kThreads = 64 * NW;
+  constexpr bool kLowInLds = CT > 1;
   const CachedArgs &a = args_again();
   const CacheView &cv = a.cache;
   int lane = threadIdx.x;
@@ -66,19 +75,27 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W> &s
       *reinterpret_cast<f32x4 *>(&sh.x[at / (WIDE / 4)][4 * (at % (WIDE / 4))]) = f32x4{0, 0, 0, 0};
     __syncthreads();
   }
-  along_tokens<kThreads>(a, share, tile,
-                         [&](int c, int f, size_t at) { sh.x[c][f] = load_as_f32<T>(a.q, at); });
+  along_tokens<kThreads>(a, share, tile, [&](size_t at) { return load_as_f32<T>(a.q, at); },
+                         [&](int c, int f, size_t, float v) { sh.x[c][f] = v; });
   __syncthreads();
-  float *x = sh.x[16 * wave + col];
-  const int c = 16 * wave + col, used = tile.used;
-  const int own = min(c, used - 1);  // columns past the last see what it sees
-  const int mine = first + (tile.c0 + own) / group;
-  {
-    // Each of the column's four lanes has a quarter of the features.
-    f32x4 y[4 * W];
+  const int used = tile.used, w0 = 16 * CT * wave;  // the wave's first column
+  // Operand of step (j, k): features 64 j + 16 grp + 8 k .. + 7 of the lane's columns (the lower
+  // pieces go to LDS: with them in registers, those of two tiles do not fit), and the last
+  // key that they see (columns past the last: what it sees).
+  f16x8 q[CT][2 * W], low[CT][2 * W];
+  float c1[CT];
+  int mine[CT];
 #pragma unroll
-    for (int n = 0; n < 4 * W; ++n) y[n] = *reinterpret_cast<const f32x4 *>(x + 16 * W * grp + 4 * n);
+  for (int ct = 0; ct < CT; ++ct) {
+    const int c = w0 + 16 * ct + col;
+    float *x = sh.x[c];
+    mine[ct] = first + (tile.c0 + min(c, used - 1)) / group;
+    f32x4 y[4 * W];
     if (a.q_norm) {
+      // Each of the column's four lanes has a quarter of the features.
+#pragma unroll
+      for (int n = 0; n < 4 * W; ++n)
+        y[n] = *reinterpret_cast<const f32x4 *>(x + 16 * W * grp + 4 * n);
       float sq = 0.0f;
 #pragma unroll
       for (int n = 0; n < 4 * W; ++n)
@@ -87,33 +104,27 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W> &s
       sq = pair_sum(pair16_sum(sq));
       const float inv = 1.0f / sqrtf(sq / (float)hd + a.eps);
 #pragma unroll
-      for (int n = 0; n < 4 * W; ++n)
+      for (int n = 0; n < 4 * W; ++n) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int f = 16 * W * grp + 4 * n + e;
           y[n][e] *= inv * (1.0f + a.q_norm[f < hd ? f : 0]);
         }
-#pragma unroll
-      for (int n = 0; n < 4 * W; ++n) *reinterpret_cast<f32x4 *>(x + 16 * W * grp + 4 * n) = y[n];
+        *reinterpret_cast<f32x4 *>(x + 16 * W * grp + 4 * n) = y[n];
+      }
+      __builtin_amdgcn_wave_barrier();
     }
-  }
-  __builtin_amdgcn_wave_barrier();
-  for (int i = grp; i < a.plan.pairs; i += 4) {
-    const int fa = pair_first(a.plan, i), fb = pair_second(a.plan, i);
-    float s, k;
-    sincospif(2.0f * (float)turn_of((double)mine, a.plan.turns[i]), &s, &k);
-    s *= a.plan.magnitude;
-    k *= a.plan.magnitude;
-    const float p = x[fa], q = x[fb];
-    x[fa] = fmaf(p, k, -(q * s));
-    x[fb] = fmaf(p, s, q * k);
-  }
-  __builtin_amdgcn_wave_barrier();
-  // Operand of step (j, k): features 64 j + 16 grp + 8 k .. + 7 of the lane's column.
-  f16x8 q[2][2 * W];
-  float c1;
-  {
-    f32x4 y[4 * W];
+    for (int i = grp; i < a.plan.pairs; i += 4) {
+      const int fa = pair_first(a.plan, i), fb = pair_second(a.plan, i);
+      float s, k;
+      sincospif(2.0f * (float)turn_of((double)mine[ct], a.plan.turns[i]), &s, &k);
+      s *= a.plan.magnitude;
+      k *= a.plan.magnitude;
+      const float p = x[fa], r = x[fb];
+      x[fa] = fmaf(p, k, -(r * s));
+      x[fb] = fmaf(p, s, r * k);
+    }
+    __builtin_amdgcn_wave_barrier();
     float most = 0.0f;
 #pragma unroll
     for (int j = 0; j < W; ++j)
@@ -127,7 +138,7 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W> &s
     int e = 0;
     if (most > 0.0f && most <= 3.402823466e38f) (void)frexpf(most, &e);
     e = 14 - max(-100, e);
-    c1 = ldexpf(a.c1, -e);
+    c1[ct] = ldexpf(a.c1, -e);
 #pragma unroll
     for (int n = 0; n < 2 * W; ++n) {
       F16x2 s[2];
@@ -138,106 +149,175 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W> &s
         for (int i = 0; i < 4; ++i) v[i] = ldexpf(v[i], e);
         s[k] = split_f16x2(v);
       }
-      q[0][n] = join_f16(s[0].hi, s[1].hi);
-      q[1][n] = join_f16(s[0].lo, s[1].lo);
+      q[ct][n] = join_f16(s[0].hi, s[1].hi);
+      low[ct][n] = join_f16(s[0].lo, s[1].lo);
     }
   }
   // The wave's columns see keys up to here, all of them up to the first's.
-  const int wave_sees = first + (tile.c0 + min(16 * wave + 15, used - 1)) / group;
-  const int seen_by_all = first + (tile.c0 + min(16 * wave, used - 1)) / group;
+  const int wave_sees = first + (tile.c0 + min(w0 + 16 * CT - 1, used - 1)) / group;
+  const int seen_by_all = first + (tile.c0 + min(w0, used - 1)) / group;
 
   // A wave brings a quarter of a block. The loads are waited for by hand: by all before
   // the barrier behind which they are read.
-  float ks[2], vs[2];
-  auto load = [&](int b, int to) {
-    const long long place = shared_block(cv, r, h, b);
+  float ks = 0.0f, vs = 1.0f;  // of the block that is on its way, then of the one that is read
+  long long place = 0;         // of the next block to load
+  auto look_up = [&](int b) { place = shared_block(cv, r, h, min(b, b1 - 1)); };
+  auto load = [&](int to) {
     const size_t at = (size_t)(place < 0 ? 0 : place) * 64 * WIDE;
     const u32x4r keys = rsrc_words(cv.keys + at, 64 * WIDE);
     const u32x4r values = rsrc_words(cv.values + at, 64 * WIDE);
 #pragma unroll
-    for (int n = 0; n < W; ++n) {
-      const int i = wave * W + n;
+    for (int n = 0; n < (4 * W + NW - 1) / NW; ++n) {
+      const int i = wave + NW * n;
+      if (4 * W % NW && i >= 4 * W) break;
       load_lds16(keys, KeyStage<W>::source(i, lane), 1024 * i,
                  reinterpret_cast<unsigned char *>(&sh.keys[to].piece[64 * i]));
       load_lds16(values, ValueStage<W>::source(lane), 1024 * i,
                  reinterpret_cast<unsigned char *>(&sh.values[to].piece[64 * i]));
     }
-    ks[to] = place < 0 ? __builtin_nanf("") : scalar_read(cv.key_scales, place);
-    vs[to] = place < 0 ? 1.0f : scalar_read(cv.value_scales, place);
   };
-  Softmax<4 * W> soft;
-  soft.clear();
+  auto scales = [&](float &k, float &v) {
+    k = place < 0 ? __builtin_nanf("") : scalar_read(cv.key_scales, place);
+    v = place < 0 ? 1.0f : scalar_read(cv.value_scales, place);
+  };
+  Softmax<4 * W> soft[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) soft[ct].clear();
   __syncthreads();  // the queries' place is the blocks'
-  if (b0 < b1) load(b0, 0);
-  auto step = [&](int b, int at) {
+  if constexpr (kLowInLds) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int n = 0; n < 2 * W; ++n)
+        *reinterpret_cast<f16x8 *>(
+            &sh.low[w0 + 16 * ct + col][64 * (n >> 1) + 16 * grp + 8 * (n & 1)]) = low[ct][n];
+  }
+  float next_ks = 0.0f, next_vs = 1.0f;
+  if (b0 < b1) {
+    look_up(b0);
+    load(0);
+    scales(ks, vs);
+    look_up(b0 + 1);
+  }
+  int at = 0;
+  for (int b = b0; b < b1; ++b, at ^= 1) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (b + 1 < b1) load(b + 1, at ^ 1);
-    if (16 * wave >= used || b * 64 > wave_sees) return;
-    f32x4 s[4];
+    if (b > b0) {
+      ks = next_ks;
+      vs = next_vs;
+    }
+    if (b + 1 < b1) load(at ^ 1);
+    // What the next round needs of the scales and the table is asked for where no LDS read
+    // follows at once: it would wait for it.
+    const bool sees = w0 < used && b * 64 <= wave_sees;
+    if (!sees) {
+      scales(next_ks, next_vs);
+      look_up(b + 2);
+      continue;
+    }
+    // Taken anew for every block: the places made of it would be kept, and spilt.
+    int here = threadIdx.x;
+    asm volatile("" : "+v"(here));
+    const int row = here & 15, quarter = (here >> 4) & 3;
+    const KeyStage<W> &keys = sh.keys[at];
+    const ValueStage<W> &values = sh.values[at];
+    f32x4 s[CT][4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) s[t] = f32x4{0, 0, 0, 0};
-    u32x4 c[4], next[4];
+    for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) c[t] = sh.keys[at].get(t, 0, col, grp);
+      for (int t = 0; t < 4; ++t) s[ct][t] = f32x4{0, 0, 0, 0};
+    constexpr int kAhead = 4 / CT;
+    u32x4 c[kAhead], next[kAhead];
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) c[e] = keys.get(e, 0, row, quarter);
 #pragma unroll
     for (int j = 0; j < W; ++j) {
+      f16x8 lo[CT][2];
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-        if (j + 1 < W) next[t] = sh.keys[at].get(t, j + 1, col, grp);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+        for (int k = 0; k < 2; ++k)
+          lo[ct][k] = kLowInLds ? *reinterpret_cast<const f16x8 *>(
+                                      &sh.low[w0 + 16 * ct + row][64 * j + 16 * quarter + 8 * k])
+                                : low[ct][2 * j + k];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const f16x8 key = codes_f16(c[t][2 * k], c[t][2 * k + 1]);
-          s[t] = mfma_16x16x32_f16(key, q[1][2 * j + k], s[t]);
-          s[t] = mfma_16x16x32_f16(key, q[0][2 * j + k], s[t]);
+      for (int t = 0; t < 4; t += kAhead) {
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+          const int n = 4 * j + t + kAhead + e;
+          if (n < 4 * W) next[e] = keys.get(n & 3, n >> 2, row, quarter);
         }
-      __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) c[t] = next[t];
+        for (int e = 0; e < kAhead; ++e)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const f16x8 key = codes_f16(c[e][2 * k], c[e][2 * k + 1]);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+              s[ct][t + e] = mfma_16x16x32_f16(key, lo[ct][k], s[ct][t + e]);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+              s[ct][t + e] = mfma_16x16x32_f16(key, q[ct][2 * j + k], s[ct][t + e]);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) c[e] = next[e];
+      }
     }
+    scales(next_ks, next_vs);
+    look_up(b + 2);
     const bool masked = b * 64 + 63 > seen_by_all;
-    const int limit = mine - b * 64 - 16 * grp;
-    f16x8 p[2][2];
-    soft.step(s, ks[at] * c1, masked, limit, vs[at], p);
-    soft.add([&](int f) { return sh.values[at].get(f, col, grp); }, masked, limit, p);
-  };
-  for (int b = b0; b < b1; b += 2) {
-    step(b, 0);
-    if (b + 1 < b1) step(b + 1, 1);
-  }
-  const float l = pair_sum(pair16_sum(soft.l));
-  __syncthreads();  // the blocks' place is the outputs'
-  if (grp == 0) {
-    sh.m[0][c] = soft.m;
-    sh.l[0][c] = l;
-    sh.unit[0][c] = soft.unit * 0x1p-15f;
-  }
+    int limit[CT];
+    f16x8 p[CT][2][2];
 #pragma unroll
-  for (int f = 0; f < 4 * W; ++f) *reinterpret_cast<f32x4 *>(&sh.o[0][c][16 * f + 4 * grp]) = soft.o[f];
+    for (int ct = 0; ct < CT; ++ct) {
+      limit[ct] = mine[ct] - b * 64 - 16 * quarter;
+      soft[ct].step(s[ct], ks * c1[ct], masked, limit[ct], vs, p[ct]);
+    }
+    add_values<4 * W, CT>(soft, [&](int f) { return values.get(f, row, quarter); }, masked, limit,
+                          p);
+  }
+  __syncthreads();  // the blocks' place is the outputs'
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int c = w0 + 16 * ct + col;
+    const float l = pair_sum(pair16_sum(soft[ct].l));
+    if (grp == 0) {
+      sh.m[0][c] = soft[ct].m;
+      sh.l[0][c] = l;
+      sh.unit[0][c] = soft[ct].unit * 0x1p-15f;
+    }
+#pragma unroll
+    for (int f = 0; f < 4 * W; ++f)
+      *reinterpret_cast<f32x4 *>(&sh.o[0][c][16 * f + 4 * grp]) = soft[ct].o[f];
+  }
   __syncthreads();
   finish_share<T, W, kCols, 1, kThreads>(share, tile, sh);
 }
 
-template <typename T, int W>
-__global__ __launch_bounds__(256, 2) void cached_prompt_kernel(CachedArgs a) {
-  __shared__ PromptLds<W> sh;
+template <typename T, int W, int CT, int NW>
+__global__ __launch_bounds__(64 * NW, 3 - CT) void cached_prompt_kernel(CachedArgs a) {
+  __shared__ PromptLds<W, CT, NW> sh;
   Deal deal;
   deal.make(a, sh.lanes);
   Share share;
   for (uint32_t w = blockIdx.x; deal.find(args_again(), sh.lanes, w, share); w += gridDim.x) {
-    prompt_share<T, W>(share, sh);
+    prompt_share<T, W, CT, NW>(share, sh);
     __syncthreads();
   }
 }
 
 template <typename T, int W>
 hipError_t launch_wide(const CachedArgs &a, hipStream_t stream, const KernelEvents &ev) {
-  hipExtLaunchKernelGGL((cached_prompt_kernel<T, W>), dim3((unsigned)a.grid), dim3(kThreads), 0,
-                        stream, ev.start, ev.stop, 0, a);
+  if (a.columns == 128)
+    hipExtLaunchKernelGGL((cached_prompt_kernel<T, W, 1, 8>), dim3((unsigned)a.grid), dim3(512),
+                          0, stream, ev.start, ev.stop, 0, a);
+  else
+    hipExtLaunchKernelGGL((cached_prompt_kernel<T, W, 1, 4>), dim3((unsigned)a.grid), dim3(256),
+                          0, stream, ev.start, ev.stop, 0, a);
   return hipGetLastError();
 }
 

@@ -169,15 +169,15 @@ __device__ __forceinline__ void rows_share(const Share &share, RowsLds<W> &sh) {
   const int mine = first + min(c0 + col, last) / group;
   const int seen_by_all = first + tile.u0;
 
-  Softmax<4 * W> soft;
-  soft.clear();
+  Softmax<4 * W> soft[1];
+  soft[0].clear();
   // A wave's last block apart: the loads of another one without a branch, so that the waits
   // for the values count the next keys behind them (with it 64 ragged rows 43 us and 128 x 8192
   // 190, without 38 and 172). No other block holds a key that some column does not see:
   // a tile's columns are 16 tokens at most, its blocks dealt to eight waves in turn.
+  long long next = 0;  // place of the wave's next block
   auto block = [&](int b, auto is_last) {
     constexpr bool kLast = decltype(is_last)::value;
-    const long long next = kLast ? 0 : shared_block(cv, r, h, b + kWaves);
     // The queries' operands are read again for every block: kept, they would take the
     // registers of the SIMD's other wave.
     asm volatile("" ::: "memory");
@@ -210,28 +210,32 @@ __device__ __forceinline__ void rows_share(const Share &share, RowsLds<W> &sh) {
     if constexpr (!kLast) load_keys(next);
     __builtin_amdgcn_sched_barrier(0);
     const bool masked = kLast && b * 64 + 63 > seen_by_all;
-    const int limit = mine - b * 64 - 16 * grp;  // of the lane's 16 keys: those <= limit
-    f16x8 p[2][2];
-    soft.step(s, factor, masked, limit, vs, p);
-    soft.add([&](int f) { return vr[f]; }, masked, limit, p);
+    const int limit[1] = {mine - b * 64 - 16 * grp};  // of the lane's 16 keys: those <= limit
+    f16x8 p[1][2][2];
+    soft[0].step(s, factor, masked, limit[0], vs, p[0]);
+    add_values<4 * W, 1>(soft, [&](int f) { return vr[f]; }, masked, limit, p);
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (!kLast) load_values(next);
+    if constexpr (!kLast) {
+      load_values(next);
+      next = shared_block(cv, r, h, min(b + 2 * kWaves, b1 - 1));
+    }
   };
   int b = b0 + wave;
+  if (b + kWaves < b1) next = shared_block(cv, r, h, b + kWaves);
   for (; b + kWaves < b1; b += kWaves) block(b, std::false_type{});
   if (b < b1) block(b, std::true_type{});
-  const float l = pair_sum(pair16_sum(soft.l));
+  const float l = pair_sum(pair16_sum(soft[0].l));
   __syncthreads();  // the keys' place is the outputs'
   // The waves' sums, joined by all of them, in units of 1 and 2^-15 probabilities.
   if (grp == 0) {
-    sh.m[wave][col] = soft.m;
+    sh.m[wave][col] = soft[0].m;
     sh.l[wave][col] = l;
-    sh.unit[wave][col] = soft.unit * 0x1p-15f;
+    sh.unit[wave][col] = soft[0].unit * 0x1p-15f;
   }
 #pragma unroll
   for (int f = 0; f < 4 * W; ++f)
     if (col < tile.used)
-      *reinterpret_cast<f32x4 *>(&sh.o[wave][col][16 * f + 4 * grp]) = soft.o[f];
+      *reinterpret_cast<f32x4 *>(&sh.o[wave][col][16 * f + 4 * grp]) = soft[0].o[f];
   __syncthreads();
   finish_share<T, W, kCols, kWaves, kThreads>(share, tile, sh);
 }
@@ -270,11 +274,12 @@ hipError_t launch_typed(const CachedArgs &a, hipStream_t stream, const KernelEve
 void cached_plan(CachedArgs &a) {
   const long long columns = (long long)a.group * a.cache.L;
   a.prompt = columns > kCachedPromptColumns;
-  a.columns = a.prompt ? 64 : 16;
+  a.columns = !a.prompt ? 16 : columns > 64 ? 128 : 64;
   a.tiles = (int)((columns + a.columns - 1) / a.columns);
-  // What the CUs hold at once: one workgroup of eight waves, two of four.
+  // What the CUs hold at once: one workgroup of eight waves or of four with 128 columns, two of
+  // four with 64.
   const int cus = a.cus < 256 ? a.cus : 256;
-  a.grid = a.prompt ? 2 * cus : cus;
+  a.grid = a.columns == 64 ? 2 * cus : cus;
   a.least = a.prompt ? 4 : kWaves;
   a.finer = a.prompt ? 2 : 4;
   a.cap = a.prompt ? 256 : kRowsCap;
@@ -284,8 +289,9 @@ void cached_plan(CachedArgs &a) {
 }
 
 CachedSpace cached_space(const CachedArgs &a) {
+  // As many counters for every call: what is behind them is not zero between calls.
   const size_t slots = (size_t)a.slots;
-  return CachedSpace{2 * slots * sizeof(unsigned), slots * a.columns * 2 * sizeof(float),
+  return CachedSpace{2 * kCachedSlots * sizeof(unsigned), slots * a.columns * 2 * sizeof(float),
                      slots * a.columns * a.cache.wide * sizeof(float)};
 }
 

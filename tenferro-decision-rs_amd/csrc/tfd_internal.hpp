@@ -510,6 +510,8 @@ struct CachedArgs {
 };
 // Up to this many (token, query head of a group) columns of a row take the rows kernel.
 constexpr int kCachedPromptColumns = 32;
+// Most places for partial results; two counters each.
+constexpr size_t kCachedSlots = 2048;
 struct CachedSpace {
   size_t done, stats, out;  // bytes of the workspace's parts
 };

@@ -10,8 +10,8 @@ products' absolute values (`size`; a turned pair mixes two features, which 2 cov
 e^score is off by twice that (numerator and denominator) plus 4 u |score| of the score's scaling and
 its difference from the reference. exp2, two fp16 pieces, scales and sums over T keys add 20 + 6 sqrt(3 T)
 u, the gate 8 + 2 |gate|. All on the sum of p |v| times the gate. Beside it a probability, which
-is at most 1 against the row's largest, is held times 2^15 in fp16 pieces whose last step is 2^-24:
-it is off by up to 2^-25 / 2^15 = 2^-40 however small it is, on the sum of |v| (the sum of the
+is at most 1 against the row's largest, is held times 2^11 to 2^15 in fp16 pieces whose last step is 2^-24:
+it is off by up to 2^-25 / 2^11 = 2^-36 however small it is, on the sum of |v| (the sum of the
 probabilities, which divides it, is at least 1). That shows where the largest probabilities meet
 values of 0.
 """
@@ -68,7 +68,7 @@ def reference(ref, q, gate, norm, rotary, before, counts):
                     out[r, j, :, L - c:] = (pv * g).T
                     tol[r, j, :, L - c:] = ((e[:, None] + extra) * U * (p @ np.abs(np.nan_to_num(v)))
                                             * g).T
-                    tol[r, j, :, L - c:] += 2.0**-40 * (seen @ np.abs(np.nan_to_num(v)) * g).T
+                    tol[r, j, :, L - c:] += 2.0**-36 * (seen @ np.abs(np.nan_to_num(v)) * g).T
     return out, tol
 
 
