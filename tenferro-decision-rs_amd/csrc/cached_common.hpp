@@ -24,6 +24,8 @@
 // cached_prompt.hip for many, whose time is the products.
 #pragma once
 
+#include <type_traits>
+
 #include "rotary.hpp"
 #include "tfd_device.hpp"
 #include "tfd_internal.hpp"
@@ -343,16 +345,17 @@ __device__ __forceinline__ bool open_tile(const CachedArgs &a, const Share &shar
   return true;
 }
 
-// Walks the (query head, feature) rows of a tile, lanes along its tokens: use(column of the
-// tile, feature, place in rows x (L, heads * hd), load(that place)), with eight loads on
-// their way at once.
-template <int THREADS, typename F, typename G>
+// Walks the (query head, feature) rows of a tile, V tokens a lane: use(first column of the
+// tile, feature, place in rows x (L, heads * hd), tokens (1 to V; columns a group apart),
+// load(that place, tokens)), with several loads on their way at once. A first or last token
+// may have columns outside of the tile.
+template <int THREADS, int V, typename F, typename G>
 __device__ __forceinline__ void along_tokens(const CachedArgs &a, const Share &share, const Tile &t,
                                              F load, G use) {
   const int L = a.cache.L, hd = a.cache.hd, group = a.group;
-  const int tokens = t.u1 - t.u0 + 1;
-  const int bits = tokens > 1 ? 32 - __builtin_clz(tokens - 1) : 0;  // at most COLS tokens
-  const int u = threadIdx.x & ((1 << bits) - 1), step = THREADS >> bits;
+  const int tokens = t.u1 - t.u0 + 1, runs = (tokens + V - 1) / V;
+  const int bits = runs > 1 ? 32 - __builtin_clz(runs - 1) : 0;  // at most COLS of them
+  const int u = V * (threadIdx.x & ((1 << bits) - 1)), step = THREADS >> bits;
   // Heads of a tile within one token.
   const int low = tokens == 1 ? t.c0 - t.u0 * group : 0;
   const int high = tokens == 1 ? low + t.used : group;
@@ -361,20 +364,20 @@ __device__ __forceinline__ void along_tokens(const CachedArgs &a, const Share &s
   g += skip;
   row -= skip * hd;
   const size_t base = ((size_t)share.r * a.heads + share.h * group) * hd;
-  const int token = L - t.count + t.u0 + u;
+  const int token = L - t.count + t.u0 + u, n = min(V, tokens - u);
   const int jump = step / hd, rest = step - jump * hd;
   while (g < high) {
-    constexpr int kBatch = 8;
+    constexpr int kBatch = V > 1 ? 4 : 8;
     int c[kBatch], f[kBatch];
     size_t at[kBatch];
-    float v[kBatch];
+    decltype(load(size_t(0), 0)) v[kBatch];
 #pragma unroll
     for (int e = 0; e < kBatch; ++e) {
       c[e] = (t.u0 + u) * group + g - t.c0;
       f[e] = row;
-      if (g >= high || u >= tokens || c[e] >= t.used) c[e] = -1;
       at[e] = (base + (size_t)g * hd + row) * L + token;
-      v[e] = c[e] >= 0 ? load(at[e]) : 0.0f;
+      if (g >= high || n <= 0) c[e] = INT32_MAX;
+      if (c[e] != INT32_MAX) v[e] = load(at[e], n);
       g += jump;
       row += rest;
       if (row >= hd) {
@@ -384,9 +387,28 @@ __device__ __forceinline__ void along_tokens(const CachedArgs &a, const Share &s
     }
 #pragma unroll
     for (int e = 0; e < kBatch; ++e)
-      if (c[e] >= 0) use(c[e], f[e], at[e], v[e]);
+      if (c[e] != INT32_MAX) use(c[e], f[e], at[e], n, v[e]);
   }
 }
+// V values side by side, at any alignment.
+template <typename T, int V>
+struct Run {
+  T e[V];
+  static __device__ __forceinline__ Run load(const void *p, size_t at, int n) {
+    Run r;
+    const T *from = static_cast<const T *>(p) + at;
+    if (n == V) {
+      __builtin_memcpy(&r, from, sizeof r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i < n) r.e[i] = from[i];
+    }
+    return r;
+  }
+};
+__device__ __forceinline__ float as_f32(unsigned short x) { return bf16_to_f32(x); }
+__device__ __forceinline__ float as_f32(float x) { return x; }
 
 // One block's step of the online softmax of a lane's 16 scores (keys 16 grp + 4 t + i of its
 // column; those > limit are not seen): the state moves on, and p becomes the pieces of the
@@ -532,11 +554,39 @@ __device__ __forceinline__ void finish_share(const Share &share, const Tile &t, 
   const Parts parts = Parts::of<COLS, WIDE>(a);
   // Joined outputs, times the gate, from LDS to where they belong.
   auto give = [&](const float(&from)[COLS][WIDE + 4]) {
-    along_tokens<THREADS>(
-        a, share, t, [&](size_t at) { return a.gate ? load_as_f32<T>(a.gate, at) : 0.0f; },
-        [&](int c, int f, size_t at, float gate) {
-          a.out[at] = a.gate ? from[c][f] * fast_sigmoid(gate) : from[c][f];
-        });
+    auto run = [&](auto width) {
+      constexpr int V = decltype(width)::value;
+      along_tokens<THREADS, V>(
+          a, share, t,
+          [&](size_t at, int n) {
+            return a.gate ? Run<T, V>::load(a.gate, at, n) : Run<T, V>{};
+          },
+          [&](int c, int f, size_t at, int n, const Run<T, V> &gate) {
+            Run<float, V> y;
+            bool whole = n == V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const int ci = c + i * a.group;
+              const bool in = i < n && ci >= 0 && ci < t.used;
+              whole = whole && in;
+              y.e[i] = in ? from[ci][f] : 0.0f;
+              if (a.gate) y.e[i] *= fast_sigmoid(as_f32(gate.e[i]));
+            }
+            if (whole) {
+              __builtin_memcpy(a.out + at, &y, sizeof y);
+            } else {
+#pragma unroll
+              for (int i = 0; i < V; ++i) {
+                const int ci = c + i * a.group;
+                if (i < n && ci >= 0 && ci < t.used) a.out[at + i] = y.e[i];
+              }
+            }
+          });
+    };
+    if (t.u1 - t.u0 >= 4)
+      run(std::integral_constant<int, 4>{});
+    else
+      run(std::integral_constant<int, 1>{});
   };
   for (int at = threadIdx.x; at < t.used * (WIDE / 4); at += THREADS) {
     const int f = 4 * (at % (WIDE / 4)), c = at / (WIDE / 4);
@@ -601,17 +651,32 @@ __device__ __forceinline__ void finish_share(const Share &share, const Tile &t, 
       sh.l[0][c] = total;
     }
     __syncthreads();
-    for (int at = threadIdx.x; at < t.used * (WIDE / 4); at += THREADS) {
-      const int f = 4 * (at % (WIDE / 4)), c = at / (WIDE / 4);
-      f32x4 sum = {0, 0, 0, 0};
-#pragma unroll 8
+    // Several places a thread at once, and of few of them several parts.
+    constexpr int kPlaces = COLS > 16 ? 8 : 1;
+    const int places = t.used * (WIDE / 4);
+    for (int at0 = threadIdx.x; at0 < places; at0 += kPlaces * THREADS) {
+      f32x4 sum[kPlaces];
+#pragma unroll
+      for (int i = 0; i < kPlaces; ++i) sum[i] = f32x4{0, 0, 0, 0};
+#pragma unroll 8 / kPlaces
       for (int p = 0; p < n; ++p)
-        sum += get4(parts.out, (((from + p * step) * COLS + c) * WIDE + f) * 4) * sh.weight[p][c];
-      if (finish) {
-        *reinterpret_cast<f32x4 *>(&sh.joined[c][f]) = sum * (1.0f / sh.l[0][c]);
-      } else {
-        put4(parts.out, sum, ((from * COLS + c) * WIDE + f) * 4);
-        if (f == 0) put2(parts.stats, sh.m[0][c], sh.l[0][c], (from * COLS + c) * 8);
+#pragma unroll
+        for (int i = 0; i < kPlaces; ++i) {
+          const int at = min(at0 + i * THREADS, places - 1);
+          const int f = 4 * (at % (WIDE / 4)), c = at / (WIDE / 4);
+          sum[i] += get4(parts.out, (((from + p * step) * COLS + c) * WIDE + f) * 4) * sh.weight[p][c];
+        }
+#pragma unroll
+      for (int i = 0; i < kPlaces; ++i) {
+        const int at = at0 + i * THREADS;
+        if (at >= places) break;
+        const int f = 4 * (at % (WIDE / 4)), c = at / (WIDE / 4);
+        if (finish) {
+          *reinterpret_cast<f32x4 *>(&sh.joined[c][f]) = sum[i] * (1.0f / sh.l[0][c]);
+        } else {
+          put4(parts.out, sum[i], ((from * COLS + c) * WIDE + f) * 4);
+          if (f == 0) put2(parts.stats, sh.m[0][c], sh.l[0][c], (from * COLS + c) * 8);
+        }
       }
     }
     if (!finish) return;

@@ -75,8 +75,16 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W, CT
       *reinterpret_cast<f32x4 *>(&sh.x[at / (WIDE / 4)][4 * (at % (WIDE / 4))]) = f32x4{0, 0, 0, 0};
     __syncthreads();
   }
-  along_tokens<kThreads>(a, share, tile, [&](size_t at) { return load_as_f32<T>(a.q, at); },
-                         [&](int c, int f, size_t, float v) { sh.x[c][f] = v; });
+  constexpr int kRun = sizeof(T) == 2 ? 8 : 4;
+  along_tokens<kThreads, kRun>(
+      a, share, tile, [&](size_t at, int n) { return Run<T, kRun>::load(a.q, at, n); },
+      [&](int c, int f, size_t, int n, const Run<T, kRun> &v) {
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) {
+          const int ci = c + i * group;
+          if (i < n && ci >= 0 && ci < tile.used) sh.x[ci][f] = as_f32(v.e[i]);
+        }
+      });
   __syncthreads();
   const int used = tile.used, w0 = 16 * CT * wave;  // the wave's first column
   // Operand of step (j, k): features 64 j + 16 grp + 8 k .. + 7 of the lane's columns (the lower
@@ -208,13 +216,17 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W, CT
       ks = next_ks;
       vs = next_vs;
     }
-    if (b + 1 < b1) load(at ^ 1);
-    // What the next round needs of the scales and the table is asked for where no LDS read
-    // follows at once: it would wait for it.
-    const bool sees = w0 < used && b * 64 <= wave_sees;
-    if (!sees) {
+    // The next block, and what the one after it needs of the scales and the table, are asked for
+    // behind the scores, where no LDS read (which would wait for the scalar ones) follows at
+    // once.
+    auto ahead = [&]() {
+      if (b + 1 < b1) load(at ^ 1);
       scales(next_ks, next_vs);
       look_up(b + 2);
+    };
+    const bool sees = w0 < used && b * 64 <= wave_sees;
+    if (!sees) {
+      ahead();
       continue;
     }
     // Taken anew for every block: the places made of it would be kept, and spilt.
@@ -267,8 +279,7 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W, CT
         for (int e = 0; e < kAhead; ++e) c[e] = next[e];
       }
     }
-    scales(next_ks, next_vs);
-    look_up(b + 2);
+    ahead();
     const bool masked = b * 64 + 63 > seen_by_all;
     int limit[CT];
     f16x8 p[CT][2][2];
