@@ -39,15 +39,47 @@ __device__ __forceinline__ float odd_f32(double x) {
   return __uint_as_float(u);
 }
 
+// 1 / scale, a power of two from 2^-100 to 2^120.
+__device__ __forceinline__ float inverse_of(float scale) {
+  return __uint_as_float((254u << 23) - __float_as_uint(scale));
+}
+
 constexpr uint32_t kNanCode = 0x7f;
 
-// Code of the nearest e4m3 value of |x| <= 448, else (and for NaN) the code of NaN.
-__device__ __forceinline__ uint32_t to_code(float x) {
-  const uint32_t c = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 0xffu;
-  return fabsf(x) <= 448.0f ? c : kNanCode;
-}
 __device__ __forceinline__ float from_code(uint32_t c) {
   return __builtin_amdgcn_cvt_f32_fp8((int)c, 0);
+}
+__device__ __forceinline__ uint32_t four_codes(const float (&x)[4]) {
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
+}
+// Codes of the nearest e4m3 values of |x| <= 448, of others (and of NaN) the code of NaN.
+__device__ __forceinline__ uint32_t to_codes(const float (&x)[4]) {
+  uint32_t c = four_codes(x);
+  const float most = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+  if (most > 448.0f || (((c & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (!(fabsf(x[e]) <= 448.0f)) c = (c & ~(0xffu << (8 * e))) | kNanCode << (8 * e);
+  }
+  return c;
+}
+// The same from 64 bits, rounded once: f32 is rounded to on the way, which can only change a
+// code where it ends on the middle between two e4m3 values, whose significands have at most
+// five bits.
+__device__ __forceinline__ uint32_t to_codes(const double (&x)[4]) {
+  float f[4];
+  uint32_t least = ~0u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    f[e] = (float)x[e];
+    least = min(least, __float_as_uint(f[e]) & 0x7ffffu);
+  }
+  if (least == 0) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = odd_f32(x[e]);
+  }
+  return to_codes(f);
 }
 
 // Smallest e with most <= 448 * 2^e, at least kCacheLowest.
@@ -72,8 +104,9 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
   constexpr int LANES = THREADS / QUADS;  // feature pairs side by side
   constexpr int WAVES = THREADS / 64;
   __shared__ int need_s[WAVES];
-  __shared__ double sums[WAVES][64];
-  __shared__ uint32_t rows_s[QUADS == 16 ? 64 * 64 : 64];  // codes by token, 256 features
+  __shared__ double sums[WAVES][64], inv_s[64];
+  // Codes by token, 256 features; rows four bytes apart, so that 16 quads are in 16 banks.
+  __shared__ uint32_t rows_s[QUADS == 16 ? 64 * 65 : 1];
   const CacheView &cv = a.cache;
   const int r = blockIdx.z, h = blockIdx.y >> 1, L = cv.L, hd = cv.hd;
   const bool keys = (blockIdx.y & 1) == 0;
@@ -81,8 +114,6 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
   if (!cache_row(cv, r, first, count) || count == 0) return;
   const int b = (first >> 6) + blockIdx.x;
   if (b * 64LL >= (long long)first + count) return;
-  const long long place = cache_block(cv, r, h, b);
-  if (place < 0) return;
   // Slots [lo, hi) of the block are new; slot s is token t = s + shift.
   const int lo = max(first - b * 64, 0);
   const int hi = (int)min(64LL, (long long)first + count - b * 64LL);
@@ -123,6 +154,8 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
       vb[n][e] = widen(q.e[e]);
     }
   }
+  const long long place = cache_block(cv, r, h, b);
+  if (place < 0) return;
   float *scale_at = (keys ? cv.key_scales : cv.value_scales) + place;
   const float before = lo > 0 ? *scale_at : 0.0f;
   const size_t block0 = (size_t)place * 64 * cv.wide;
@@ -163,13 +196,15 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) sums[wave][4 * quad + e] = sq[e];
       __syncthreads();
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      if (threadIdx.x < 4 * QUADS) {  // each token's once: the root and its inverse cost 60 operations
         double t = 0.0;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) t += sums[w][4 * quad + e];
-        inv[e] = 1.0 / sqrt(t / hd + (double)a.eps);
+        for (int w = 0; w < WAVES; ++w) t += sums[w][threadIdx.x];
+        inv_s[threadIdx.x] = 1.0 / sqrt(t / hd + (double)a.eps);
       }
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 4; ++e) inv[e] = inv_s[4 * quad + e];
     }
     double most = 0.0;
 #pragma unroll
@@ -195,20 +230,30 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
           ya[n][e] = fa[n] < hd ? p : 0.0;  // also beside a NaN in the token
           yb[n][e] = fb[n] < hd ? q : 0.0;
         }
-        if (fabs(ya[n][e]) <= 1e300) most = fmax(most, fabs(ya[n][e]));
-        if (fabs(yb[n][e]) <= 1e300) most = fmax(most, fabs(yb[n][e]));
+        most = fmax(most, fmax(fabs(ya[n][e]), fabs(yb[n][e])));
       }
     }
+    if (most > 1e300) {  // inf, which counts as little as NaN
+      most = 0.0;
+#pragma unroll
+      for (int n = 0; n < NP; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (fabs(ya[n][e]) <= 1e300) most = fmax(most, fabs(ya[n][e]));
+          if (fabs(yb[n][e]) <= 1e300) most = fmax(most, fabs(yb[n][e]));
+        }
+    }
     agree(need_exponent(most));
-    const double to = 1.0 / (double)scale;
+    const double to = (double)inverse_of(scale);
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
-      ca[n] = cb[n] = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        ca[n] |= to_code(odd_f32(ya[n][e] * to)) << (8 * e);
-        cb[n] |= to_code(odd_f32(yb[n][e] * to)) << (8 * e);
+        ya[n][e] *= to;
+        yb[n][e] *= to;
       }
+      ca[n] = to_codes(ya[n]);
+      cb[n] = to_codes(yb[n]);
     }
   } else {
     float most = 0.0f;
@@ -216,19 +261,29 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
     for (int n = 0; n < NP; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (fabsf(va[n][e]) <= 3.402823466e38f) most = fmaxf(most, fabsf(va[n][e]));
-        if (fabsf(vb[n][e]) <= 3.402823466e38f) most = fmaxf(most, fabsf(vb[n][e]));
+        most = fmaxf(most, fmaxf(fabsf(va[n][e]), fabsf(vb[n][e])));
       }
+    if (most > 3.402823466e38f) {
+      most = 0.0f;
+#pragma unroll
+      for (int n = 0; n < NP; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (fabsf(va[n][e]) <= 3.402823466e38f) most = fmaxf(most, fabsf(va[n][e]));
+          if (fabsf(vb[n][e]) <= 3.402823466e38f) most = fmaxf(most, fabsf(vb[n][e]));
+        }
+    }
     agree(need_exponent(most));
-    const float to = 1.0f / scale;
+    const float to = inverse_of(scale);
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
-      ca[n] = cb[n] = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        ca[n] |= to_code(va[n][e] * to) << (8 * e);
-        cb[n] |= to_code(vb[n][e] * to) << (8 * e);
+        va[n][e] *= to;
+        vb[n][e] *= to;
       }
+      ca[n] = to_codes(va[n]);
+      cb[n] = to_codes(vb[n]);
     }
   }
   // Earlier tokens under a scale that grew.
@@ -238,7 +293,9 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
       const int s = keys ? j / cv.wide : j % lo, f = keys ? j % cv.wide : j / lo;
       uint8_t *p = codes + (keys ? s * cv.wide + f : f * 64 + s);
       const uint32_t c = *p;
-      *p = (c & 0x7f) == kNanCode ? (uint8_t)c : (uint8_t)to_code(from_code(c) * again);
+      const float x = from_code(c) * again;
+      if ((c & 0x7f) != kNanCode)
+        *p = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false);
     }
   }
   if (threadIdx.x == 0) *scale_at = scale;
@@ -278,13 +335,13 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
       if (lane0 + LANES * n < half)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          bytes[(s0 + e) * cv.wide + fa[n]] = (uint8_t)(ca[n] >> (8 * e));
-          bytes[(s0 + e) * cv.wide + fb[n]] = (uint8_t)(cb[n] >> (8 * e));
+          bytes[(s0 + e) * (cv.wide + 4) + fa[n]] = (uint8_t)(ca[n] >> (8 * e));
+          bytes[(s0 + e) * (cv.wide + 4) + fb[n]] = (uint8_t)(cb[n] >> (8 * e));
         }
     __syncthreads();
     uint32_t *to = reinterpret_cast<uint32_t *>(codes);
     const int row = cv.wide / 4;
-    for (int j = threadIdx.x + lo * row; j < hi * row; j += THREADS) to[j] = rows_s[j];
+    for (int j = threadIdx.x + lo * row; j < hi * row; j += THREADS) to[j] = rows_s[j + j / row];
   }
 }
 
