@@ -11,6 +11,17 @@
 // Keys are computed in 64 bits, whose vector rate is that of 32 bits here: a code then does
 // not depend on the order of a sum or on the shape of the launch, so tokens appended
 // one by one leave the codes that a prompt of them leaves, as long as no scale grew between.
+//
+// A workgroup has one block of one head, as all of it decides the scale: loads are runs of
+// tokens of a feature, a key's codes change to a token's features side by side in LDS.
+// Measured: 4 rows of 8192 bf16 tokens, 4 heads of 128 features (66 MB read, 33 MB written):
+// 70 us, 1.4 TB/s. Of it the values are 21 us and the keys 50, whose loads alone
+// take 26 (runs of 128 bytes, 16 KB apart), sines 15, norms, codes and stores the rest. 512
+// threads with 8 pairs of features each (88 registers): 70 us; 1024 with 4: 93; 256 with
+// 16: 73; held to 64 registers, which spills: 88; a workgroup for all heads of a block,
+// which takes sines once but holds them (over 126 registers): 91 to 117. For over 128
+// features 1024 threads and 512 measured the same (16 rows of up to 256 tokens: 14 us, a chain of
+// waits). A single token of 64 rows: 5 us, of which 3.5 are an empty launch's.
 #include <hip/hip_ext.h>
 #include <string.h>
 
@@ -39,7 +50,11 @@ __device__ __forceinline__ float odd_f32(double x) {
   return __uint_as_float(u);
 }
 
-// 1 / scale, a power of two from 2^-100 to 2^120.
+// 2^e, e from -100 to 127.
+__device__ __forceinline__ float power_of_two(int e) {
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+// 1 / scale, a power of two from 2^-100 to 2^126.
 __device__ __forceinline__ float inverse_of(float scale) {
   return __uint_as_float((254u << 23) - __float_as_uint(scale));
 }
@@ -64,10 +79,10 @@ __device__ __forceinline__ uint32_t to_codes(const float (&x)[4]) {
   }
   return c;
 }
-// The same from 64 bits, rounded once: f32 is rounded to on the way, which can only change a
-// code where it ends on the middle between two e4m3 values, whose significands have at most
-// five bits.
-__device__ __forceinline__ uint32_t to_codes(const double (&x)[4]) {
+// The same of x * to from 64 bits, rounded once: f32 is rounded to on the way, which can only
+// change a code where it ends on the middle between two e4m3 values, whose significands have
+// at most five bits. (What f32 does not hold is far below the least code, or above the last.)
+__device__ __forceinline__ uint32_t to_codes(const double (&x)[4], float to) {
   float f[4];
   uint32_t least = ~0u;
 #pragma unroll
@@ -79,37 +94,43 @@ __device__ __forceinline__ uint32_t to_codes(const double (&x)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) f[e] = odd_f32(x[e]);
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] *= to;
   return to_codes(f);
 }
 
-// Smallest e with most <= 448 * 2^e, at least kCacheLowest.
-__device__ __forceinline__ int need_exponent(float most) {
-  if (!(most > 0.0f)) return kCacheLowest;
-  int e;
-  const float m = frexpf(most, &e);
-  return min(127, max(kCacheLowest, e - 9 + (m > 0.875f ? 1 : 0)));
+// Numbers ordered as |x|, with what the scale depends on: the exponent, and whether the
+// significand is above 1.75.
+__device__ __forceinline__ uint32_t size_of(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x);
+  return ((uint32_t)(u >> 32) << 1) + ((uint32_t)u != 0);
 }
-__device__ __forceinline__ int need_exponent(double most) {
-  if (!(most > 0.0)) return kCacheLowest;
-  int e;
-  const double m = frexp(most, &e);
-  return min(127, max(kCacheLowest, e - 9 + (m > 0.875 ? 1 : 0)));
+__device__ __forceinline__ uint32_t size_of(float x) { return __float_as_uint(x) << 1; }
+// Those of inf and NaN, which the scale does not count.
+constexpr uint32_t kInfinite64 = 0x7ffu << 21, kInfinite32 = 0xffu << 24;
+// Smallest e with |x| <= 448 * 2^e, in range.
+__device__ __forceinline__ int need_exponent64(uint32_t size) {
+  return min(127, max(kCacheLowest, (int)(size >> 21) - 1031 + ((size & 0x1fffff) > 0x180000)));
+}
+__device__ __forceinline__ int need_exponent32(uint32_t size) {
+  return min(127, max(kCacheLowest, (int)(size >> 24) - 135 + ((size & 0xffffff) > 0xc00000)));
 }
 
-// One block of one (row, kv head), its keys or its values. Thread tid holds the four
-// slots 4 (tid % QUADS) .. + 3 of the feature pairs tid / QUADS + n * THREADS / QUADS,
-// n < NP. QUADS 16: whole blocks; 1: one token a row.
+// One block of one (row, kv head): its keys, or (blockIdx.z behind the rows) its values. Thread tid holds the E slots E (tid % QUADS) .. + E - 1 of the feature pairs
+// tid / QUADS + n * THREADS / QUADS, n < NP. QUADS 16, E 4: whole blocks; 1, 1: one token a row.
 template <typename T, int QUADS, int THREADS, int NP>
 __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
   constexpr int LANES = THREADS / QUADS;  // feature pairs side by side
   constexpr int WAVES = THREADS / 64;
+  constexpr int E = QUADS == 1 ? 1 : 4;
   __shared__ int need_s[WAVES];
-  __shared__ double sums[WAVES][64], inv_s[64];
+  __shared__ double sums[WAVES][E * QUADS], inv_s[E * QUADS];
   // Codes by token, 256 features; rows four bytes apart, so that 16 quads are in 16 banks.
   __shared__ uint32_t rows_s[QUADS == 16 ? 64 * 65 : 1];
   const CacheView &cv = a.cache;
-  const int r = blockIdx.z, h = blockIdx.y >> 1, L = cv.L, hd = cv.hd;
-  const bool keys = (blockIdx.y & 1) == 0;
+  const bool keys = blockIdx.z < gridDim.z / 2;
+  const int r = keys ? blockIdx.z : blockIdx.z - gridDim.z / 2, h = blockIdx.y;
+  const int L = cv.L, hd = cv.hd;
   int first, count;
   if (!cache_row(cv, r, first, count) || count == 0) return;
   const int b = (first >> 6) + blockIdx.x;
@@ -119,37 +140,40 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
   const int hi = (int)min(64LL, (long long)first + count - b * 64LL);
   const long long shift = (long long)b * 64 - first + (L - count);
   const int quad = threadIdx.x % QUADS, lane0 = threadIdx.x / QUADS;
-  const int s0 = QUADS == 16 ? 4 * quad : lo & ~3;
+  const int s0 = QUADS == 16 ? 4 * quad : lo;
   const int wave = threadIdx.x >> 6;
   const int pairs = keys ? a.plan.pairs : 0;
   const int half = cv.wide / 2;
-  const T *x = static_cast<const T *>(keys ? a.k : a.v) +
-               ((size_t)r * cv.kv_heads + h) * hd * L;
+  const T *x = static_cast<const T *>(keys ? a.k : a.v) + ((size_t)r * cv.kv_heads + h) * hd * L;
   int fa[NP], fb[NP];
-  float va[NP][4], vb[NP][4];
-  const bool whole = s0 >= lo && s0 + 4 <= hi;
 #pragma unroll
   for (int n = 0; n < NP; ++n) {
     const int i = lane0 + LANES * n;
     fa[n] = i < pairs ? pair_first(a.plan, i) : 2 * i;
     fb[n] = i < pairs ? pair_second(a.plan, i) : 2 * i + 1;
+  }
+  float va[NP][4] = {}, vb[NP][4] = {};
+  const bool whole = s0 >= lo && s0 + E <= hi;
+#pragma unroll
+  for (int n = 0; n < NP; ++n) {
     struct {
-      T e[4];
+      T e[E];
     } p = {}, q = {};
-    const T *pa = x + (long long)fa[n] * L + (s0 + shift), *pb = x + (long long)fb[n] * L + (s0 + shift);
+    const T *pa = x + (long long)fa[n] * L + (s0 + shift);
+    const T *pb = x + (long long)fb[n] * L + (s0 + shift);
     if (whole) {
       if (fa[n] < hd) memcpy(&p, pa, sizeof p);
       if (fb[n] < hd) memcpy(&q, pb, sizeof q);
-    } else {
+    } else if constexpr (E > 1) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < E; ++e)
         if (s0 + e >= lo && s0 + e < hi) {
           if (fa[n] < hd) p.e[e] = pa[e];
           if (fb[n] < hd) q.e[e] = pb[e];
         }
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < E; ++e) {
       va[n][e] = widen(p.e[e]);
       vb[n][e] = widen(q.e[e]);
     }
@@ -158,45 +182,43 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
   if (place < 0) return;
   float *scale_at = (keys ? cv.key_scales : cv.value_scales) + place;
   const float before = lo > 0 ? *scale_at : 0.0f;
-  const size_t block0 = (size_t)place * 64 * cv.wide;
-  uint8_t *codes = (keys ? cv.keys : cv.values) + block0;
-
-  uint32_t ca[NP], cb[NP];  // four codes each
-  int need;
+  uint8_t *codes = (keys ? cv.keys : cv.values) + (size_t)place * 64 * cv.wide;
+  uint32_t ca[NP], cb[NP];  // E codes each
   float scale;
   auto agree = [&](int mine) {  // the block's scale
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) mine = max(mine, __shfl_xor(mine, o));
     if ((threadIdx.x & 63) == 0) need_s[wave] = mine;
     __syncthreads();
-    need = need_s[0];
+    int need = need_s[0];
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) need = max(need, need_s[w]);
-    const float s = ldexpf(1.0f, need);
-    scale = fmaxf(s, before);
+    scale = fmaxf(power_of_two(need), before);
   };
   if (keys) {
-    double ya[NP][4], yb[NP][4];
-    double inv[4] = {1.0, 1.0, 1.0, 1.0};
+    double ya[NP][4] = {}, yb[NP][4] = {};
+    double inv[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) inv[e] = 1.0;
     if (a.k_norm) {
-      double sq[4] = {};
+      double sq[E] = {};
 #pragma unroll
       for (int n = 0; n < NP; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < E; ++e) {
           const double p = va[n][e], q = vb[n][e];
           sq[e] = fma(p, p, fma(q, q, sq[e]));
         }
-      // Lanes with the same quad: tid % QUADS.
+      // Lanes with the same slots: tid % QUADS.
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < E; ++e)
 #pragma unroll
         for (int o = QUADS; o < 64; o <<= 1) sq[e] += __shfl_xor(sq[e], o);
       if ((threadIdx.x & 63) < QUADS)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sums[wave][4 * quad + e] = sq[e];
+        for (int e = 0; e < E; ++e) sums[wave][E * quad + e] = sq[e];
       __syncthreads();
-      if (threadIdx.x < 4 * QUADS) {  // each token's once: the root and its inverse cost 60 operations
+      if (threadIdx.x < E * QUADS) {  // a token's once: root and inverse cost 60 operations
         double t = 0.0;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) t += sums[w][threadIdx.x];
@@ -204,9 +226,9 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
       }
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < 4; ++e) inv[e] = inv_s[4 * quad + e];
+      for (int e = 0; e < E; ++e) inv[e] = inv_s[E * quad + e];
     }
-    double most = 0.0;
+    uint32_t most = 0;
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
       const int i = lane0 + LANES * n;
@@ -217,68 +239,68 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
       }
       const double f = i < pairs ? a.plan.turns[i] : 0.0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < E; ++e) {
         const double p = (double)va[n][e] * inv[e] * wa, q = (double)vb[n][e] * inv[e] * wb;
-        if (i < pairs) {
-          double c, s;
-          sincospi(2.0 * turn_of((double)(b * 64LL + s0 + e), f), &s, &c);
-          c *= (double)a.plan.magnitude;
-          s *= (double)a.plan.magnitude;
-          ya[n][e] = fma(p, c, -(q * s));
-          yb[n][e] = fma(p, s, q * c);
-        } else {
-          ya[n][e] = fa[n] < hd ? p : 0.0;  // also beside a NaN in the token
-          yb[n][e] = fb[n] < hd ? q : 0.0;
-        }
-        most = fmax(most, fmax(fabs(ya[n][e]), fabs(yb[n][e])));
+        double c, s;
+        sincos_turns(turn_of((double)(b * 64LL + s0 + e), f), s, c);
+        c *= (double)a.plan.magnitude;
+        s *= (double)a.plan.magnitude;
+        const double ta = fma(p, c, -(q * s)), tb = fma(p, s, q * c);
+        // Features that are not turned: also beside a NaN in the token, and past the last.
+        ya[n][e] = i < pairs ? ta : fa[n] < hd ? p : 0.0;
+        yb[n][e] = i < pairs ? tb : fb[n] < hd ? q : 0.0;
+        most = max(most, max(size_of(ya[n][e]), size_of(yb[n][e])));
       }
     }
-    if (most > 1e300) {  // inf, which counts as little as NaN
-      most = 0.0;
+    if (most >= kInfinite64) {
+      most = 0;
 #pragma unroll
       for (int n = 0; n < NP; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (fabs(ya[n][e]) <= 1e300) most = fmax(most, fabs(ya[n][e]));
-          if (fabs(yb[n][e]) <= 1e300) most = fmax(most, fabs(yb[n][e]));
+        for (int e = 0; e < E; ++e) {
+          const uint32_t sa = size_of(ya[n][e]), sb = size_of(yb[n][e]);
+          most = max(most, max(sa < kInfinite64 ? sa : 0u, sb < kInfinite64 ? sb : 0u));
         }
     }
-    agree(need_exponent(most));
-    const double to = (double)inverse_of(scale);
+    agree(need_exponent64(most));
+    float to = inverse_of(scale);
+    if (scale >= 0x1p119f) {  // past what 32 bits hold
+      to = 1.0f;
+#pragma unroll
+      for (int n = 0; n < NP; ++n)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          ya[n][e] *= 1.0 / (double)scale;
+          yb[n][e] *= 1.0 / (double)scale;
+        }
+    }
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        ya[n][e] *= to;
-        yb[n][e] *= to;
-      }
-      ca[n] = to_codes(ya[n]);
-      cb[n] = to_codes(yb[n]);
+      ca[n] = to_codes(ya[n], to);
+      cb[n] = to_codes(yb[n], to);
     }
   } else {
-    float most = 0.0f;
+    uint32_t most = 0;
 #pragma unroll
     for (int n = 0; n < NP; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        most = fmaxf(most, fmaxf(fabsf(va[n][e]), fabsf(vb[n][e])));
-      }
-    if (most > 3.402823466e38f) {
-      most = 0.0f;
+      for (int e = 0; e < E; ++e) most = max(most, max(size_of(va[n][e]), size_of(vb[n][e])));
+    if (most >= kInfinite32) {
+      most = 0;
 #pragma unroll
       for (int n = 0; n < NP; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (fabsf(va[n][e]) <= 3.402823466e38f) most = fmaxf(most, fabsf(va[n][e]));
-          if (fabsf(vb[n][e]) <= 3.402823466e38f) most = fmaxf(most, fabsf(vb[n][e]));
+        for (int e = 0; e < E; ++e) {
+          const uint32_t sa = size_of(va[n][e]), sb = size_of(vb[n][e]);
+          most = max(most, max(sa < kInfinite32 ? sa : 0u, sb < kInfinite32 ? sb : 0u));
         }
     }
-    agree(need_exponent(most));
+    agree(need_exponent32(most));
     const float to = inverse_of(scale);
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < E; ++e) {
         va[n][e] *= to;
         vb[n][e] *= to;
       }
@@ -293,9 +315,9 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
       const int s = keys ? j / cv.wide : j % lo, f = keys ? j % cv.wide : j / lo;
       uint8_t *p = codes + (keys ? s * cv.wide + f : f * 64 + s);
       const uint32_t c = *p;
-      const float x = from_code(c) * again;
+      const float y = from_code(c) * again;
       if ((c & 0x7f) != kNanCode)
-        *p = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false);
+        *p = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
     }
   }
   if (threadIdx.x == 0) *scale_at = scale;
@@ -308,25 +330,23 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
         const uint32_t c = k ? cb[n] : ca[n];
         if (f >= hd) continue;
         uint8_t *p = codes + f * 64 + s0;
-        if (whole) {
+        if constexpr (E == 1) {
+          *p = (uint8_t)c;
+        } else if (whole) {
           *reinterpret_cast<uint32_t *>(p) = c;
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < E; ++e)
             if (s0 + e >= lo && s0 + e < hi) p[e] = (uint8_t)(c >> (8 * e));
         }
       }
-    return;
-  }
-  if constexpr (QUADS == 1) {
+  } else if constexpr (E == 1) {
 #pragma unroll
     for (int n = 0; n < NP; ++n)
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-        if (s0 + s >= lo && s0 + s < hi && lane0 + LANES * n < half) {
-          codes[(s0 + s) * cv.wide + fa[n]] = (uint8_t)(ca[n] >> (8 * s));
-          codes[(s0 + s) * cv.wide + fb[n]] = (uint8_t)(cb[n] >> (8 * s));
-        }
+      if (lane0 + LANES * n < half) {
+        codes[s0 * cv.wide + fa[n]] = (uint8_t)ca[n];
+        codes[s0 * cv.wide + fb[n]] = (uint8_t)cb[n];
+      }
   } else {
     // Through LDS, so that a token's features leave side by side.
     uint8_t *bytes = reinterpret_cast<uint8_t *>(rows_s);
@@ -334,7 +354,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
     for (int n = 0; n < NP; ++n)
       if (lane0 + LANES * n < half)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < E; ++e) {
           bytes[(s0 + e) * (cv.wide + 4) + fa[n]] = (uint8_t)(ca[n] >> (8 * e));
           bytes[(s0 + e) * (cv.wide + 4) + fb[n]] = (uint8_t)(cb[n] >> (8 * e));
         }
@@ -346,14 +366,15 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
 }
 
 template <typename T>
-hipError_t launch_append(const AppendArgs &a, int rows, hipStream_t stream,
-                         const KernelEvents &ev) {
+hipError_t launch_append(const AppendArgs &a, int rows, hipStream_t stream, const KernelEvents &ev) {
   const int L = a.cache.L, half = a.cache.wide / 2;
   // Blocks that L tokens from any slot on may touch.
   const unsigned blocks = (unsigned)((L + 62) / 64 + 1);
-  const dim3 grid(blocks, (unsigned)a.cache.kv_heads * 2, (unsigned)rows);
+  const dim3 grid(blocks, (unsigned)a.cache.kv_heads, (unsigned)rows * 2);
 #define TFD_APPEND(Q, N, P)                                                                     \
   hipExtLaunchKernelGGL((append_kernel<T, Q, N, P>), grid, dim3(N), 0, stream, ev.start, ev.stop, 0, a)
+  // For single tokens a thread for each pair of features; for runs 8 pairs and slots a
+  // thread, or 4 where the features are few.
   if (L == 1)
     TFD_APPEND(1, 128, 1);
   else if (half <= 32)
@@ -361,7 +382,7 @@ hipError_t launch_append(const AppendArgs &a, int rows, hipStream_t stream,
   else if (half <= 64)
     TFD_APPEND(16, 512, 2);
   else
-    TFD_APPEND(16, 512, 4);
+    TFD_APPEND(16, 1024, 2);
 #undef TFD_APPEND
   return hipGetLastError();
 }
