@@ -477,25 +477,22 @@ struct Softmax {
   }
 };
 
-// Adds a block's values to CT tiles' outputs; raw(f): the lane's 16 bytes of features
+// Adds a block's values to a tile's outputs; raw(f): the lane's 16 bytes of features
 // 16 f + lane % 16.
-template <int N, int CT, typename F>
-__device__ __forceinline__ void add_values(Softmax<N> (&soft)[CT], F raw, bool masked,
-                                           const int (&limit)[CT], const f16x8 (&p)[CT][2][2]) {
+template <int N, typename F>
+__device__ __forceinline__ void add_values(Softmax<N> &soft, F raw, bool masked, int limit,
+                                           const f16x8 (&p)[2][2]) {
   auto multiply = [&](int f, u32x4 c) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const f16x8 v = codes_f16(c[2 * k], c[2 * k + 1]);
 #pragma unroll
-      for (int i = 1; i >= 0; --i)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-          soft[ct].o[f] = mfma_16x16x32_f16(v, p[ct][i][k], soft[ct].o[f]);
+      for (int i = 1; i >= 0; --i) soft.o[f] = mfma_16x16x32_f16(v, p[i][k], soft.o[f]);
     }
   };
   if (!masked) {
     // Operands ahead of the products, which take long enough for them to arrive.
-    constexpr int kAhead = 4 / CT;
+    constexpr int kAhead = 4;
     u32x4 c[kAhead], next[kAhead];
 #pragma unroll
     for (int e = 0; e < kAhead; ++e) c[e] = raw(e);
@@ -526,21 +523,17 @@ __device__ __forceinline__ void add_values(Softmax<N> (&soft)[CT], F raw, bool m
     }
     multiply(f, c);
     if (__any((bad[0] | bad[1] | bad[2] | bad[3]) != 0)) {
+      f32x4 n = {0, 0, 0, 0};
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        f32x4 n = {0, 0, 0, 0};
+      for (int k = 0; k < 2; ++k) {
+        f16x8 sees;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          f16x8 sees;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) sees[e] = (_Float16)(8 * k + e <= limit[ct] ? 1.0f : 0.0f);
-          // 0x38: e4m3's 1.
-          n = mfma_16x16x32_f16(codes_f16(bad[2 * k] * 0x38u, bad[2 * k + 1] * 0x38u), sees, n);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          soft[ct].o[f][i] = n[i] > 0.0f ? __builtin_nanf("") : soft[ct].o[f][i];
+        for (int e = 0; e < 8; ++e) sees[e] = (_Float16)(8 * k + e <= limit ? 1.0f : 0.0f);
+        // 0x38: e4m3's 1.
+        n = mfma_16x16x32_f16(codes_f16(bad[2 * k] * 0x38u, bad[2 * k + 1] * 0x38u), sees, n);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) soft.o[f][i] = n[i] > 0.0f ? __builtin_nanf("") : soft.o[f][i];
     }
   }
 }

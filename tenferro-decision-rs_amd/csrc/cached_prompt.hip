@@ -31,14 +31,13 @@ struct ValueStage {
   }
 };
 
-template <int W, int CT, int NW>
+template <int W, int NW>
 struct PromptLds {
-  static constexpr int kCols = 16 * CT * NW;
+  static constexpr int kCols = 16 * NW;
   union {
     struct {
       KeyStage<W> keys[2];
       ValueStage<W> values[2];
-      _Float16 low[CT > 1 ? kCols : 1][64 * W + 8];  // the queries' lower pieces
     };
     float x[kCols][64 * W + 4];     // queries before they are split
     float o[1][kCols][64 * W + 4];  // outputs
@@ -52,11 +51,10 @@ struct PromptLds {
   Deal::Lanes lanes;
 };
 
-// NW waves of CT tiles of 16 columns.
-template <typename T, int W, int CT, int NW>
-__device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W, CT, NW> &sh) {
-  constexpr int WIDE = 64 * W, kCols = 16 * CT * NW, kThreads = 64 * NW;
-  constexpr bool kLowInLds = CT > 1;
+// NW waves of 16 columns each.
+template <typename T, int W, int NW>
+__device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W, NW> &sh) {
+  constexpr int WIDE = 64 * W, kCols = 16 * NW, kThreads = 64 * NW;
   const CachedArgs &a = args_again();
   const CacheView &cv = a.cache;
   int lane = threadIdx.x;
@@ -86,18 +84,16 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W, CT
         }
       });
   __syncthreads();
-  const int used = tile.used, w0 = 16 * CT * wave;  // the wave's first column
-  // Operand of step (j, k): features 64 j + 16 grp + 8 k .. + 7 of the lane's columns (the lower
-  // pieces go to LDS: with them in registers, those of two tiles do not fit), and the last
-  // key that they see (columns past the last: what it sees).
-  f16x8 q[CT][2 * W], low[CT][2 * W];
-  float c1[CT];
-  int mine[CT];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const int c = w0 + 16 * ct + col;
+  const int used = tile.used, w0 = 16 * wave;  // the wave's first column
+  // Operand 2 j + k: features 64 j + 16 grp + 8 k .. + 7 of the lane's column; and the last
+  // key that it sees (columns past the last: what that one sees).
+  f16x8 high[2 * W], low[2 * W];
+  float c1;
+  int mine;
+  {
+    const int c = w0 + col;
     float *x = sh.x[c];
-    mine[ct] = first + (tile.c0 + min(c, used - 1)) / group;
+    mine = first + (tile.c0 + min(c, used - 1)) / group;
     f32x4 y[4 * W];
     if (a.q_norm) {
       // Each of the column's four lanes has a quarter of the features.
@@ -125,7 +121,7 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W, CT
     for (int i = grp; i < a.plan.pairs; i += 4) {
       const int fa = pair_first(a.plan, i), fb = pair_second(a.plan, i);
       float s, k;
-      sincospif(2.0f * (float)turn_of((double)mine[ct], a.plan.turns[i]), &s, &k);
+      sincospif(2.0f * (float)turn_of((double)mine, a.plan.turns[i]), &s, &k);
       s *= a.plan.magnitude;
       k *= a.plan.magnitude;
       const float p = x[fa], r = x[fb];
@@ -146,7 +142,7 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W, CT
     int e = 0;
     if (most > 0.0f && most <= 3.402823466e38f) (void)frexpf(most, &e);
     e = 14 - max(-100, e);
-    c1[ct] = ldexpf(a.c1, -e);
+    c1 = ldexpf(a.c1, -e);
 #pragma unroll
     for (int n = 0; n < 2 * W; ++n) {
       F16x2 s[2];
@@ -157,12 +153,12 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W, CT
         for (int i = 0; i < 4; ++i) v[i] = ldexpf(v[i], e);
         s[k] = split_f16x2(v);
       }
-      q[ct][n] = join_f16(s[0].hi, s[1].hi);
-      low[ct][n] = join_f16(s[0].lo, s[1].lo);
+      high[n] = join_f16(s[0].hi, s[1].hi);
+      low[n] = join_f16(s[0].lo, s[1].lo);
     }
   }
   // The wave's columns see keys up to here, all of them up to the first's.
-  const int wave_sees = first + (tile.c0 + min(w0 + 16 * CT - 1, used - 1)) / group;
+  const int wave_sees = first + (tile.c0 + min(w0 + 15, used - 1)) / group;
   const int seen_by_all = first + (tile.c0 + min(w0, used - 1)) / group;
 
   // A wave brings a quarter of a block. The loads are waited for by hand: by all before
@@ -188,18 +184,9 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W, CT
     k = place < 0 ? __builtin_nanf("") : scalar_read(cv.key_scales, place);
     v = place < 0 ? 1.0f : scalar_read(cv.value_scales, place);
   };
-  Softmax<4 * W> soft[CT];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) soft[ct].clear();
+  Softmax<4 * W> soft;
+  soft.clear();
   __syncthreads();  // the queries' place is the blocks'
-  if constexpr (kLowInLds) {
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-      for (int n = 0; n < 2 * W; ++n)
-        *reinterpret_cast<f16x8 *>(
-            &sh.low[w0 + 16 * ct + col][64 * (n >> 1) + 16 * grp + 8 * (n & 1)]) = low[ct][n];
-  }
   float next_ks = 0.0f, next_vs = 1.0f;
   if (b0 < b1) {
     look_up(b0);
@@ -235,88 +222,61 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W, CT
     const int row = here & 15, quarter = (here >> 4) & 3;
     const KeyStage<W> &keys = sh.keys[at];
     const ValueStage<W> &values = sh.values[at];
-    f32x4 s[CT][4];
+    f32x4 s[4];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
+    for (int t = 0; t < 4; ++t) s[t] = f32x4{0, 0, 0, 0};
+    // Operands ahead of the products, as the values' (add_values).
+    u32x4 c[4], next[4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) s[ct][t] = f32x4{0, 0, 0, 0};
-    constexpr int kAhead = 4 / CT;
-    u32x4 c[kAhead], next[kAhead];
-#pragma unroll
-    for (int e = 0; e < kAhead; ++e) c[e] = keys.get(e, 0, row, quarter);
+    for (int t = 0; t < 4; ++t) c[t] = keys.get(t, 0, row, quarter);
 #pragma unroll
     for (int j = 0; j < W; ++j) {
-      f16x8 lo[CT][2];
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
+      for (int t = 0; t < 4; ++t)
+        if (j + 1 < W) next[t] = keys.get(t, j + 1, row, quarter);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-          lo[ct][k] = kLowInLds ? *reinterpret_cast<const f16x8 *>(
-                                      &sh.low[w0 + 16 * ct + row][64 * j + 16 * quarter + 8 * k])
-                                : low[ct][2 * j + k];
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int t = 0; t < 4; t += kAhead) {
-#pragma unroll
-        for (int e = 0; e < kAhead; ++e) {
-          const int n = 4 * j + t + kAhead + e;
-          if (n < 4 * W) next[e] = keys.get(n & 3, n >> 2, row, quarter);
+        for (int k = 0; k < 2; ++k) {
+          const f16x8 key = codes_f16(c[t][2 * k], c[t][2 * k + 1]);
+          s[t] = mfma_16x16x32_f16(key, low[2 * j + k], s[t]);
+          s[t] = mfma_16x16x32_f16(key, high[2 * j + k], s[t]);
         }
-        __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int e = 0; e < kAhead; ++e)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const f16x8 key = codes_f16(c[e][2 * k], c[e][2 * k + 1]);
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct)
-              s[ct][t + e] = mfma_16x16x32_f16(key, lo[ct][k], s[ct][t + e]);
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct)
-              s[ct][t + e] = mfma_16x16x32_f16(key, q[ct][2 * j + k], s[ct][t + e]);
-          }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int e = 0; e < kAhead; ++e) c[e] = next[e];
-      }
+      for (int t = 0; t < 4; ++t) c[t] = next[t];
     }
     ahead();
     const bool masked = b * 64 + 63 > seen_by_all;
-    int limit[CT];
-    f16x8 p[CT][2][2];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      limit[ct] = mine[ct] - b * 64 - 16 * quarter;
-      soft[ct].step(s[ct], ks * c1[ct], masked, limit[ct], vs, p[ct]);
-    }
-    add_values<4 * W, CT>(soft, [&](int f) { return values.get(f, row, quarter); }, masked, limit,
-                          p);
+    const int limit = mine - b * 64 - 16 * quarter;
+    f16x8 p[2][2];
+    soft.step(s, ks * c1, masked, limit, vs, p);
+    add_values(soft, [&](int f) { return values.get(f, row, quarter); }, masked, limit, p);
   }
   __syncthreads();  // the blocks' place is the outputs'
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const int c = w0 + 16 * ct + col;
-    const float l = pair_sum(pair16_sum(soft[ct].l));
-    if (grp == 0) {
-      sh.m[0][c] = soft[ct].m;
-      sh.l[0][c] = l;
-      sh.unit[0][c] = soft[ct].unit * 0x1p-15f;
-    }
-#pragma unroll
-    for (int f = 0; f < 4 * W; ++f)
-      *reinterpret_cast<f32x4 *>(&sh.o[0][c][16 * f + 4 * grp]) = soft[ct].o[f];
+  const int c = w0 + col;
+  const float l = pair_sum(pair16_sum(soft.l));
+  if (grp == 0) {
+    sh.m[0][c] = soft.m;
+    sh.l[0][c] = l;
+    sh.unit[0][c] = soft.unit * 0x1p-15f;
   }
+#pragma unroll
+  for (int f = 0; f < 4 * W; ++f)
+    *reinterpret_cast<f32x4 *>(&sh.o[0][c][16 * f + 4 * grp]) = soft.o[f];
   __syncthreads();
   finish_share<T, W, kCols, 1, kThreads>(share, tile, sh);
 }
 
-template <typename T, int W, int CT, int NW>
-__global__ __launch_bounds__(64 * NW, 3 - CT) void cached_prompt_kernel(CachedArgs a) {
-  __shared__ PromptLds<W, CT, NW> sh;
+template <typename T, int W, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void cached_prompt_kernel(CachedArgs a) {
+  __shared__ PromptLds<W, NW> sh;
   Deal deal;
   deal.make(a, sh.lanes);
   Share share;
   for (uint32_t w = blockIdx.x; deal.find(args_again(), sh.lanes, w, share); w += gridDim.x) {
-    prompt_share<T, W, CT, NW>(share, sh);
+    prompt_share<T, W, NW>(share, sh);
     __syncthreads();
   }
 }
@@ -324,10 +284,10 @@ __global__ __launch_bounds__(64 * NW, 3 - CT) void cached_prompt_kernel(CachedAr
 template <typename T, int W>
 hipError_t launch_wide(const CachedArgs &a, hipStream_t stream, const KernelEvents &ev) {
   if (a.columns == 128)
-    hipExtLaunchKernelGGL((cached_prompt_kernel<T, W, 1, 8>), dim3((unsigned)a.grid), dim3(512),
+    hipExtLaunchKernelGGL((cached_prompt_kernel<T, W, 8>), dim3((unsigned)a.grid), dim3(512),
                           0, stream, ev.start, ev.stop, 0, a);
   else
-    hipExtLaunchKernelGGL((cached_prompt_kernel<T, W, 1, 4>), dim3((unsigned)a.grid), dim3(256),
+    hipExtLaunchKernelGGL((cached_prompt_kernel<T, W, 4>), dim3((unsigned)a.grid), dim3(256),
                           0, stream, ev.start, ev.stop, 0, a);
   return hipGetLastError();
 }

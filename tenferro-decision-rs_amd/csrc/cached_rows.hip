@@ -169,8 +169,8 @@ __device__ __forceinline__ void rows_share(const Share &share, RowsLds<W> &sh) {
   const int mine = first + min(c0 + col, last) / group;
   const int seen_by_all = first + tile.u0;
 
-  Softmax<4 * W> soft[1];
-  soft[0].clear();
+  Softmax<4 * W> soft;
+  soft.clear();
   // A wave's last block apart: the loads of another one without a branch, so that the waits
   // for the values count the next keys behind them (with it 64 ragged rows 43 us and 128 x 8192
   // 190, without 38 and 172). No other block holds a key that some column does not see:
@@ -210,10 +210,10 @@ __device__ __forceinline__ void rows_share(const Share &share, RowsLds<W> &sh) {
     if constexpr (!kLast) load_keys(next);
     __builtin_amdgcn_sched_barrier(0);
     const bool masked = kLast && b * 64 + 63 > seen_by_all;
-    const int limit[1] = {mine - b * 64 - 16 * grp};  // of the lane's 16 keys: those <= limit
-    f16x8 p[1][2][2];
-    soft[0].step(s, factor, masked, limit[0], vs, p[0]);
-    add_values<4 * W, 1>(soft, [&](int f) { return vr[f]; }, masked, limit, p);
+    const int limit = mine - b * 64 - 16 * grp;  // of the lane's 16 keys: those <= limit
+    f16x8 p[2][2];
+    soft.step(s, factor, masked, limit, vs, p);
+    add_values(soft, [&](int f) { return vr[f]; }, masked, limit, p);
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (!kLast) {
       load_values(next);
@@ -224,18 +224,18 @@ __device__ __forceinline__ void rows_share(const Share &share, RowsLds<W> &sh) {
   if (b + kWaves < b1) next = shared_block(cv, r, h, b + kWaves);
   for (; b + kWaves < b1; b += kWaves) block(b, std::false_type{});
   if (b < b1) block(b, std::true_type{});
-  const float l = pair_sum(pair16_sum(soft[0].l));
+  const float l = pair_sum(pair16_sum(soft.l));
   __syncthreads();  // the keys' place is the outputs'
   // The waves' sums, joined by all of them, in units of 1 and 2^-15 probabilities.
   if (grp == 0) {
-    sh.m[wave][col] = soft[0].m;
+    sh.m[wave][col] = soft.m;
     sh.l[wave][col] = l;
-    sh.unit[wave][col] = soft[0].unit * 0x1p-15f;
+    sh.unit[wave][col] = soft.unit * 0x1p-15f;
   }
 #pragma unroll
   for (int f = 0; f < 4 * W; ++f)
     if (col < tile.used)
-      *reinterpret_cast<f32x4 *>(&sh.o[wave][col][16 * f + 4 * grp]) = soft[0].o[f];
+      *reinterpret_cast<f32x4 *>(&sh.o[wave][col][16 * f + 4 * grp]) = soft.o[f];
   __syncthreads();
   finish_share<T, W, kCols, kWaves, kThreads>(share, tile, sh);
 }
