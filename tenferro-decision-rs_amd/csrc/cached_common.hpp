@@ -180,8 +180,10 @@ struct Share {
 // blocks. Every wave finds that out by itself, each lane for `each` rows in a row.
 // An even share for every workgroup is `all` / workgroups. If parts of up to 5/16 more are no
 // more than the workgroups (ragged lengths leave parts that are not full), that is it:
-// the work then takes as long as one part. Otherwise an even share goes in a.finer pieces, one
-// after another: one piece more than even at the end.
+// the work then takes as long as one part. Otherwise parts are even shares, and some workgroups
+// have one more: finer ones cost more in their beginnings and ends than a shorter last one
+// saves (200 rows of 1500 tokens, 2 kv heads: 39 us, in halves 60, in quarters 70; 300 rows
+// of 4096: 74, 76, 88).
 struct Deal {
   int each, most;
   // By lane, in LDS between the shares: parts of the lanes up to this one, and of this one;
@@ -217,7 +219,7 @@ struct Deal {
       for (int j = 1; j < each; ++j) n += parts(a, r0 + j, blocks(a, r0 + j));
       fits = (long long)all_sum_of(n) * per <= room;
     }
-    if (!fits) most = max(a.least, even / a.finer + 1);
+    if (!fits) most = max(a.least, even);
     uint32_t own = 0, split_own = 0;
     for (int j = 0; j < each; ++j) {
       const uint32_t n = (uint32_t)parts(a, r0 + j, j ? blocks(a, r0 + j) : nb) * per;

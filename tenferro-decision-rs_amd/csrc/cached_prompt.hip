@@ -9,6 +9,9 @@
 namespace tfd {
 namespace {
 
+constexpr int kWaves = 8;  // of 16 columns each
+constexpr int kThreads = 64 * kWaves;
+constexpr int kCols = 16 * kWaves;
 constexpr int kPromptCap = 256;
 
 // Values as keys (KeyStage): feature f's 64 tokens are four pieces, at places that f / 4 turns.
@@ -31,9 +34,8 @@ struct ValueStage {
   }
 };
 
-template <int W, int NW>
+template <int W>
 struct PromptLds {
-  static constexpr int kCols = 16 * NW;
   union {
     struct {
       KeyStage<W> keys[2];
@@ -51,10 +53,9 @@ struct PromptLds {
   Deal::Lanes lanes;
 };
 
-// NW waves of 16 columns each.
-template <typename T, int W, int NW>
-__device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W, NW> &sh) {
-  constexpr int WIDE = 64 * W, kCols = 16 * NW, kThreads = 64 * NW;
+template <typename T, int W>
+__device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W> &sh) {
+  constexpr int WIDE = 64 * W;
   const CachedArgs &a = args_again();
   const CacheView &cv = a.cache;
   int lane = threadIdx.x;
@@ -161,7 +162,7 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W, NW
   const int wave_sees = first + (tile.c0 + min(w0 + 15, used - 1)) / group;
   const int seen_by_all = first + (tile.c0 + min(w0, used - 1)) / group;
 
-  // A wave brings a quarter of a block. The loads are waited for by hand: by all before
+  // The waves bring a block together, 1 KB a load. The loads are waited for by hand: by all before
   // the barrier behind which they are read.
   float ks = 0.0f, vs = 1.0f;  // of the block that is on its way, then of the one that is read
   long long place = 0;         // of the next block to load
@@ -171,9 +172,9 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W, NW
     const u32x4r keys = rsrc_words(cv.keys + at, 64 * WIDE);
     const u32x4r values = rsrc_words(cv.values + at, 64 * WIDE);
 #pragma unroll
-    for (int n = 0; n < (4 * W + NW - 1) / NW; ++n) {
-      const int i = wave + NW * n;
-      if (4 * W % NW && i >= 4 * W) break;
+    for (int n = 0; n < (4 * W + kWaves - 1) / kWaves; ++n) {
+      const int i = wave + kWaves * n;
+      if (4 * W % kWaves && i >= 4 * W) break;
       load_lds16(keys, KeyStage<W>::source(i, lane), 1024 * i,
                  reinterpret_cast<unsigned char *>(&sh.keys[to].piece[64 * i]));
       load_lds16(values, ValueStage<W>::source(lane), 1024 * i,
@@ -269,26 +270,22 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W, NW
   finish_share<T, W, kCols, 1, kThreads>(share, tile, sh);
 }
 
-template <typename T, int W, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void cached_prompt_kernel(CachedArgs a) {
-  __shared__ PromptLds<W, NW> sh;
+template <typename T, int W>
+__global__ __launch_bounds__(kThreads, 2) void cached_prompt_kernel(CachedArgs a) {
+  __shared__ PromptLds<W> sh;
   Deal deal;
   deal.make(a, sh.lanes);
   Share share;
   for (uint32_t w = blockIdx.x; deal.find(args_again(), sh.lanes, w, share); w += gridDim.x) {
-    prompt_share<T, W, NW>(share, sh);
+    prompt_share<T, W>(share, sh);
     __syncthreads();
   }
 }
 
 template <typename T, int W>
 hipError_t launch_wide(const CachedArgs &a, hipStream_t stream, const KernelEvents &ev) {
-  if (a.columns == 128)
-    hipExtLaunchKernelGGL((cached_prompt_kernel<T, W, 8>), dim3((unsigned)a.grid), dim3(512),
-                          0, stream, ev.start, ev.stop, 0, a);
-  else
-    hipExtLaunchKernelGGL((cached_prompt_kernel<T, W, 4>), dim3((unsigned)a.grid), dim3(256),
-                          0, stream, ev.start, ev.stop, 0, a);
+  hipExtLaunchKernelGGL((cached_prompt_kernel<T, W>), dim3((unsigned)a.grid), dim3(kThreads), 0,
+                        stream, ev.start, ev.stop, 0, a);
   return hipGetLastError();
 }
 

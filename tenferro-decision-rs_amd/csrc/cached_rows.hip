@@ -271,21 +271,29 @@ hipError_t launch_typed(const CachedArgs &a, hipStream_t stream, const KernelEve
 
 }  // namespace
 
+// The rows kernel reads a row's blocks once for each tile of 16 columns, and gives every tile
+// workgroups of its own; the prompt kernel takes 128 columns at once. The first is faster up to
+// two tiles, and where there are few tiles in all (us, rows kernel and prompt kernel; heads of
+// 128, groups of 8, tokens seen: 4096 by 32 rows and kv heads of 32 columns 23 and 34, of 40 44
+// and 36, of 256 93 and 69; by 1 of 256 columns 300 15 and 27, 2048 16 and 32, 16384 19 and 48; by
+// 2 of 1024 columns 2048 18 and 37, 16384 52 and 74; by 16 of 64 columns 16384 45 and
+// 54). It loses where long rows are many: by 32 of 64 columns 2048 21 and 27, 16384 94 and
+// 76. How long they are is in device memory.
 void cached_plan(CachedArgs &a) {
-  const long long columns = (long long)a.group * a.cache.L;
-  a.prompt = columns > kCachedPromptColumns;
-  a.columns = !a.prompt ? 16 : columns > 64 ? 128 : 64;
+  const long long columns = (long long)a.group * a.cache.L, tiles = (columns + 15) / 16;
+  a.prompt = tiles > 2 && tiles * a.rows * a.cache.kv_heads > a.cus / 2;
+  a.columns = a.prompt ? 128 : 16;
   a.tiles = (int)((columns + a.columns - 1) / a.columns);
-  // What the CUs hold at once: one workgroup of eight waves or of four with 128 columns, two of
-  // four with 64.
-  const int cus = a.cus < 256 ? a.cus : 256;
-  a.grid = a.columns == 64 ? 2 * cus : cus;
+  // One workgroup of eight waves for a CU is what it holds of either kernel at once.
+  a.grid = a.cus < 256 ? a.cus : 256;
+  // A part of fewer blocks costs more in its beginning and end than it saves: a block for each
+  // wave (1 row of 65536 tokens: 16.3 us, from 4 blocks 18.6, from 16 19.1), or 4 that all
+  // read (128 tokens of 2 kv heads at 1024: 31.7 us, from 2 blocks 32.7, from 8 38.8).
   a.least = a.prompt ? 4 : kWaves;
-  a.finer = a.prompt ? 2 : 4;
   a.cap = a.prompt ? 256 : kRowsCap;
   // Parts of tiles in several: a tile in n > 1 parts has more than (n - 1) most blocks, and
-  // finer grid most is at least all blocks.
-  a.slots = 2 * a.finer * a.grid;
+  // grid most is at least all blocks.
+  a.slots = 2 * a.grid;
 }
 
 CachedSpace cached_space(const CachedArgs &a) {

@@ -500,18 +500,15 @@ struct CachedArgs {
   int cus;
   int rows;
   // Set by cached_plan: the kernel, columns of a tile, tiles per (row, kv head), workgroups,
-  // the least blocks that make a part, pieces of an even share, most parts of a tile, places
-  // for partial results.
+  // the least blocks that make a part, most parts of a tile, places for partial results.
   bool prompt;
-  int columns, tiles, grid, least, finer, cap, slots;
+  int columns, tiles, grid, least, cap, slots;
   unsigned *part_done;  // zeroed once, and left at zero by every launch
   float *part_stats, *part_out;
   RotaryPlan plan;
 };
-// Up to this many (token, query head of a group) columns of a row take the rows kernel.
-constexpr int kCachedPromptColumns = 32;
 // Most places for partial results; two counters each.
-constexpr size_t kCachedSlots = 2048;
+constexpr size_t kCachedSlots = 512;
 struct CachedSpace {
   size_t done, stats, out;  // bytes of the workspace's parts
 };
