@@ -116,7 +116,7 @@ __device__ __forceinline__ int need_exponent32(uint32_t size) {
   return min(127, max(kCacheLowest, (int)(size >> 24) - 135 + ((size & 0xffffff) > 0xc00000)));
 }
 
-// One block of one (row, kv head): its keys, or (blockIdx.z behind the rows) its values. Thread tid holds the E slots E (tid % QUADS) .. + E - 1 of the feature pairs
+// One block of one (row, kv head): its keys, or (blockIdx.y behind the heads) its values. Thread tid holds the E slots E (tid % QUADS) .. + E - 1 of the feature pairs
 // tid / QUADS + n * THREADS / QUADS, n < NP. QUADS 16, E 4: whole blocks; 1, 1: one token a row.
 template <typename T, int QUADS, int THREADS, int NP>
 __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
@@ -128,9 +128,9 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
   // Codes by token, 256 features; rows four bytes apart, so that 16 quads are in 16 banks.
   __shared__ uint32_t rows_s[QUADS == 16 ? 64 * 65 : 1];
   const CacheView &cv = a.cache;
-  const bool keys = blockIdx.z < gridDim.z / 2;
-  const int r = keys ? blockIdx.z : blockIdx.z - gridDim.z / 2, h = blockIdx.y;
-  const int L = cv.L, hd = cv.hd;
+  const int r = blockIdx.z, L = cv.L, hd = cv.hd;
+  const bool keys = blockIdx.y < (unsigned)cv.kv_heads;
+  const int h = keys ? blockIdx.y : blockIdx.y - cv.kv_heads;
   int first, count;
   if (!cache_row(cv, r, first, count) || count == 0) return;
   const int b = (first >> 6) + blockIdx.x;
@@ -370,7 +370,7 @@ hipError_t launch_append(const AppendArgs &a, int rows, hipStream_t stream, cons
   const int L = a.cache.L, half = a.cache.wide / 2;
   // Blocks that L tokens from any slot on may touch.
   const unsigned blocks = (unsigned)((L + 62) / 64 + 1);
-  const dim3 grid(blocks, (unsigned)a.cache.kv_heads, (unsigned)rows * 2);
+  const dim3 grid(blocks, (unsigned)a.cache.kv_heads * 2, (unsigned)rows);
 #define TFD_APPEND(Q, N, P)                                                                     \
   hipExtLaunchKernelGGL((append_kernel<T, Q, N, P>), grid, dim3(N), 0, stream, ev.start, ev.stop, 0, a)
   // For single tokens a thread for each pair of features; for runs 8 pairs and slots a

@@ -451,7 +451,7 @@ struct Softmax {
     float turn = alpha;
     if (vs > unit || vs < unit * 0x1p-4f) {
       top = fmaxf(top, vs);
-      const float to = fmaxf(vs, top * 0x1p-90f);
+      const float to = fmaxf(fmaxf(vs, top * 0x1p-90f), 0x1p-126f);  // not 0, for a scale of 0
       turn = alpha * (unit / to);
       unit = to;
     }
