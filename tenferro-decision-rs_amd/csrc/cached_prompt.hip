@@ -1,19 +1,21 @@
 // The attention over a paged 8-bit cache for many columns (cached_common.hpp): prompts behind
 // what is cached.
 //
-// Bound: the matrix unit. Per (column, key) 8 hd operations are done for 4 hd that the formula
-// has, as f32 operands go in two fp16 pieces; what a tile reads of the cache stays in L2.
+// Bound: the SIMDs' issue. Per (column, key) 8 hd operations are done for the 4 hd of the formula,
+// as f32 operands go in two fp16 pieces, and a code is converted by every wave that
+// multiplies it; what a tile reads of the cache stays in L2.
 //
 // A workgroup of eight waves takes 128 columns, 16 a wave, whose queries' pieces and outputs
 // stay in registers; all waves read each block from LDS, where it arrives as it is in memory
 // while the one before is multiplied (two places). A code becomes fp16 on its way from LDS to
-// the matrix unit: four conversions for two products, hidden behind the other wave of the SIMD.
+// the matrix unit: four conversions for two products, while the SIMD's other wave has products under way.
 // Blocks that no column of a wave sees are not multiplied.
 //
 // Measured: 2 rows of 900 to 1024 tokens behind 8000 to 8192, 2 kv heads of 256 features in groups of 4
-// (135 Gflop of the formula, 270 done): 327 us when sustained, 410 Tflop/s of the formula, 820 of the
-// matrix unit (whose rate here, at the clock that this load leaves, is 1.2 Pflop/s in a plain
-// product of 8192 cubed). Before: the rows kernel's order 450 us; four waves of 16 columns 360;
+// (135 Gflop of the formula, 270 done): 304 to 345 us by the clock that the load leaves, 0.8 to 0.9
+// Pflop/s of products, where a plain one of 8192 cubed reaches 1.2. The matrix unit is busy
+// for 33% of the cycles, vector instructions are issued in 46% (4.5 for each product: 2
+// conversions, softmax, pieces). Before: the rows kernel's order 450 us; four waves of 16 columns 360;
 // 32 columns a wave, whose registers leave one wave a SIMD, 503.
 #include <hip/hip_ext.h>
 
