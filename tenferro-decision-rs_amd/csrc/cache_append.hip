@@ -15,13 +15,16 @@
 // A workgroup has one block of one head, as all of it decides the scale: loads are runs of
 // tokens of a feature, a key's codes change to a token's features side by side in LDS.
 // Measured: 4 rows of 8192 bf16 tokens, 4 heads of 128 features (66 MB read, 33 MB written):
-// 70 us, 1.4 TB/s. Of it the values are 21 us and the keys 50, whose loads alone
-// take 26 (runs of 128 bytes, 16 KB apart), sines 15, norms, codes and stores the rest. 512
-// threads with 8 pairs of features each (88 registers): 70 us; 1024 with 4: 93; 256 with
-// 16: 73; held to 64 registers, which spills: 88; a workgroup for all heads of a block,
-// which takes sines once but holds them (over 126 registers): 91 to 117. For over 128
-// features 1024 threads and 512 measured the same (16 rows of up to 256 tokens: 14 us, a chain of
-// waits). A single token of 64 rows: 5 us, of which 3.5 are an empty launch's.
+// 67 us, 1.5 TB/s. Of it the values are 21 us and the keys the rest, whose loads alone take 26
+// (runs of 128 bytes, 16 KB apart, that begin anywhere: lines shared with the next block's are
+// read twice; neighbours on one XCD, which read them once, take 1 to 4 us more all the same),
+// sines 15, norms, codes and stores the rest. 512 threads with 8 pairs of features each, held to
+// 80 registers, three workgroups a CU, of which 6 spill: 67 us; in the 88 that they would take, two
+// workgroups: 70; in 64: 88; 1024 threads with 4 pairs 71 to 93; 256 with 16: 73; sines
+// before the norm, behind the loads: 74; a workgroup for all heads of a block, which takes sines once but
+// holds them (over 126 registers): 91 to 117. For over 128 features 1024 threads and 512 measured
+// the same (16 rows of up to 256 tokens: 14 us, a chain of waits). A single token of 64 rows:
+// 5 us.
 #include <hip/hip_ext.h>
 #include <string.h>
 
@@ -119,7 +122,7 @@ __device__ __forceinline__ int need_exponent32(uint32_t size) {
 // One block of one (row, kv head): its keys, or (blockIdx.y behind the heads) its values. Thread tid holds the E slots E (tid % QUADS) .. + E - 1 of the feature pairs
 // tid / QUADS + n * THREADS / QUADS, n < NP. QUADS 16, E 4: whole blocks; 1, 1: one token a row.
 template <typename T, int QUADS, int THREADS, int NP>
-__global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
+__global__ __launch_bounds__(THREADS, THREADS == 512 ? 6 : 4) void append_kernel(AppendArgs a) {
   constexpr int LANES = THREADS / QUADS;  // feature pairs side by side
   constexpr int WAVES = THREADS / 64;
   constexpr int E = QUADS == 1 ? 1 : 4;

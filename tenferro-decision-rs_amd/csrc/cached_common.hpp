@@ -210,7 +210,10 @@ struct Deal {
     float mine = (float)nb;
     for (int j = 1; j < each; ++j) mine += (float)blocks(a, r0 + j);
     const int room = (int)gridDim.x;
-    const int even = (int)(all_sum(mine) * (float)per / (float)room) + 1;
+    // At least an even share, whatever f32 rounds, as the places for partial results are counted
+    // by it; rows' blocks are at most 2^25.
+    int even = (int)fminf(all_sum(mine) * (float)per / (float)room, 0x1p26f) + 1;
+    even += even >> 16;
     most = max(a.least, even);
     bool fits = false;
     for (int step = 0; step < 6 && !fits && (size_t)a.rows * per <= (size_t)room; ++step) {
