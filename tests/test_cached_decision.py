@@ -151,6 +151,9 @@ def shapes():
     yield 300, 4, 2, 64, 1, tuple(7 * r % 2000 for r in range(300))  # more tiles than workgroups
     yield 3, 6, 1, 40, 150, (0, 5000, 63)  # 900 columns
     yield 140, 3, 1, 72, 11, tuple(r for r in range(140))  # 33 columns: over two tiles
+    yield 1, 8, 1, 64, 3000, (500,)  # 24000 columns
+    yield 5, 3, 3, 1, 4, (0, 63, 64, 300, 1)  # one feature
+    yield 40, 16, 1, 2, 9, tuple(3 * r for r in range(40))
 
 
 @pytest.mark.gpu
@@ -319,3 +322,68 @@ def test_many_rows_append(gpu_ctx):
     assert (keys[:, 0] == cuda(ref.keys[0, 0, 0])).all() and not keys[:, 1:].any()
     assert (values[:, :hd, 0] == cuda(ref.values[0, 0, 0, :hd, 0])).all() and not values[:, :, 1:].any()
     assert (cache[2] == float(ref.ks[0, 0, 0])).all() and (cache[3] == float(ref.vs[0, 0, 0])).all()
+
+
+@pytest.mark.gpu
+def test_captured_prompts():
+    """Many columns in parts, captured; eager calls of other kinds between the replays."""
+    import torch
+
+    stream = torch.cuda.Stream()
+    with te.Context(0, stream=stream.cuda_stream) as ctx, torch.cuda.stream(stream):
+        ready = calls(ctx)
+        want = [host(one()) for one in ready]
+        graphs, got = [], []
+        with te.asynchronous():
+            for n in (1, 4):
+                graphs.append(torch.cuda.CUDAGraph())
+                stream.synchronize()
+                with torch.cuda.graph(graphs[-1], stream=stream):
+                    got.append(ready[n]())
+        for i in range(4):
+            for x in got:
+                x.fill_(7.0)
+            for g in graphs:
+                g.replay()
+            stream.synchronize()
+            assert np.array_equal(host(got[0]), want[1]) and np.array_equal(host(got[1]), want[4])
+            for n in (i, 5):
+                assert np.array_equal(host(ready[n]()), want[n])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("L", [1, 70])
+def test_without_lengths_and_counts(gpu_ctx, L):
+    """None: no token before the call, all of its tokens new."""
+    R, H, HK, hd = 3, 4, 2, 64
+    k, v = normal(5, R, HK, hd, L), normal(6, R, HK, hd, L)
+    q, gate = problem(R, H, hd, L, False)
+    ref = Cache(R, HK, hd, 64, 2)
+    cache, table = ref.paged(cuda), cuda(ref.table.reshape(-1))
+    flat = lambda x: cuda(x.reshape(-1))
+    ref.append(k, v, None, None, np.full(R, L))
+    te.jeff_cache_append(flat(k), flat(v), None, cache, table, None, None, R, L, HK, hd, None, EPS,
+                         ctx=gpu_ctx)
+    assert ref.same(cache) == [True] * 4
+    out = cuda(np.full(q.size, np.nan, np.float32))
+    got = te.jeff_cached_attention(flat(q), flat(gate), None, cache, table, None, None, R, L, H, HK, hd,
+                                   None, EPS, ctx=gpu_ctx, out=out)
+    assert got is out
+    check(out, *reference(ref, q, gate, None, None, np.zeros(R, np.int64), np.full(R, L)))
+
+
+def test_nothing_to_do():
+    """No rows or no tokens: nothing is read, written or launched."""
+    none = np.zeros(0, np.float32)
+    cache = te.paged_cache(2, 2, 64)
+    i32 = lambda n: np.zeros(n, np.int32)
+    with te.Context(0) as ctx:
+        for R, L in ((0, 3), (2, 0)):
+            te.jeff_cache_append(none, none, None, cache, i32(R), i32(R), i32(R), R, L, 2, 64, None, EPS,
+                                 ctx=ctx)
+            out = te.jeff_cached_attention(none, none, None, cache, i32(R), i32(R), i32(R), R, L, 4, 2, 64,
+                                           None, EPS, ctx=ctx)
+            assert out.size == 0
+            rotary = te.Rotary(te.rotary_frequencies(32, 1e4))
+            assert te.rotary_rows(none, None, R, L, 2, 64, rotary, ctx=ctx).size == 0
+    assert not cache.keys.any()
