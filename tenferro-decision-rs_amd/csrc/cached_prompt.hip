@@ -212,7 +212,8 @@ __device__ __forceinline__ void prompt_share(const Share &share, PromptLds<W> &s
   }
   int at = 0;
   for (int b = b0; b < b1; ++b, at ^= 1) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // The block is there, and its reads of the place that the next one goes to are over.
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     if (b > b0) {
