@@ -12,7 +12,7 @@
 // Blocks that no column of a wave sees are not multiplied.
 //
 // Measured: 2 rows of 900 to 1024 tokens behind 8000 to 8192, 2 kv heads of 256 features in groups of 4
-// (135 Gflop of the formula, 270 done): 304 to 345 us by the clock that the load leaves, 0.8 to 0.9
+// (135 Gflop of the formula, 270 done): 301 to 345 us by the clock that the load leaves, 0.8 to 0.9
 // Pflop/s of products, where a plain one of 8192 cubed reaches 1.2. The matrix unit is busy
 // for 33% of the cycles, vector instructions are issued in 46% (4.5 for each product: 2
 // conversions, softmax, pieces). Before: the rows kernel's order 450 us; four waves of 16 columns 360;
