@@ -119,7 +119,8 @@ __device__ __forceinline__ int need_exponent32(uint32_t size) {
   return min(127, max(kCacheLowest, (int)(size >> 24) - 135 + ((size & 0xffffff) > 0xc00000)));
 }
 
-// One block of one (row, kv head): its keys, or (blockIdx.y behind the heads) its values. Thread tid holds the E slots E (tid % QUADS) .. + E - 1 of the feature pairs
+// One block of one (row, kv head): its keys, or (blockIdx.y behind the heads) its values.
+// Thread tid holds the E slots E (tid % QUADS) .. + E - 1 of the feature pairs
 // tid / QUADS + n * THREADS / QUADS, n < NP. QUADS 16, E 4: whole blocks; 1, 1: one token a row.
 template <typename T, int QUADS, int THREADS, int NP>
 __global__ __launch_bounds__(THREADS, THREADS == 512 ? 6 : 4) void append_kernel(AppendArgs a) {

@@ -372,6 +372,25 @@ def test_without_lengths_and_counts(gpu_ctx, L):
     check(out, *reference(ref, q, gate, None, None, np.zeros(R, np.int64), np.full(R, L)))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("weight", [3e38, 1e-30])
+@pytest.mark.parametrize("L", [1, 67])
+def test_norm_weights_of_any_size(gpu_ctx, L, weight):
+    """Keys past f32's range, whose scales are up to 2^122, and scales that go with small ones."""
+    R, HK, hd = 2, 1, 96
+    k, v = normal(5, R, HK, hd, L), normal(6, R, HK, hd, L)
+    norm = np.where(np.arange(hd) % 3 == 0, np.float32(weight), np.float32(weight / 3 - 1)).astype(
+        np.float32)
+    rotary = te.Rotary(te.rotary_frequencies(64, 1e4), True)
+    ref = Cache(R, HK, hd, 64, 2)
+    cache = ref.paged(cuda)
+    i32 = lambda x: cuda(np.asarray(x, np.int32).reshape(-1))
+    ref.append(k, v, norm, rotary, np.full(R, L))
+    te.jeff_cache_append(cuda(k.reshape(-1)), cuda(v.reshape(-1)), cuda(norm), cache, i32(ref.table), None,
+                         None, R, L, HK, hd, rotary, EPS, ctx=gpu_ctx)
+    assert ref.same(cache) == [True] * 4
+
+
 def test_nothing_to_do():
     """No rows or no tokens: nothing is read, written or launched."""
     none = np.zeros(0, np.float32)
