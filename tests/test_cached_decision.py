@@ -153,6 +153,9 @@ def shapes():
     yield 140, 3, 1, 72, 11, tuple(r for r in range(140))  # 33 columns: over two tiles
     yield 1, 8, 1, 64, 3000, (500,)  # 24000 columns
     yield 5, 3, 3, 1, 4, (0, 63, 64, 300, 1)  # one feature
+    yield 2, 200, 1, 64, 2, (70, 600)  # a token's heads over several tiles
+    yield 30, 200, 1, 64, 2, tuple(40 * r for r in range(30))
+    yield 12, 300, 2, 130, 1, tuple(90 * r for r in range(12))
     yield 40, 16, 1, 2, 9, tuple(3 * r for r in range(40))
 
 
