@@ -450,10 +450,11 @@ struct Softmax {
     m = mn;
     // The outputs' unit is a value scale that blocks have had: a block's own up to 16 times
     // smaller is made up for in the probabilities; another one becomes the unit, unless it is
-    // so far below the largest that the outputs could leave f32's range in it.
+    // so far below the largest that the outputs could leave f32's range in it. The largest is that
+    // of all blocks, also of those that did not become the unit (the first ones within 1 to 1/16).
     float turn = alpha;
+    top = fmaxf(top, vs);
     if (vs > unit || vs < unit * 0x1p-4f) {
-      top = fmaxf(top, vs);
       const float to = fmaxf(fmaxf(vs, top * 0x1p-90f), 0x1p-126f);  // not 0, for a scale of 0
       turn = alpha * (unit / to);
       unit = to;
