@@ -460,7 +460,7 @@ int tfd_jeff_cache_append_bf16(tfd_ctx *ctx, size_t rows, size_t length, size_t 
  *                 It may not overlap the inputs.
  * Every sum is f32. Queries (against their head's largest feature) and probabilities enter
  * the products with 22 significant bits, probabilities to within 2^-36 of the largest;
- * values more than 2^90 below the largest scale of a row's values are lost beside it. A NaN
+ * values more than 2^60 below the largest scale of a row's values are lost beside it. A NaN
  * that a key or value holds reaches the outputs that see its token, and no other.
  */
 int tfd_jeff_cached_attention_f32(tfd_ctx *ctx, size_t rows, size_t length, size_t heads,

@@ -452,10 +452,11 @@ struct Softmax {
     // smaller is made up for in the probabilities; another one becomes the unit, unless it is
     // so far below the largest that the outputs could leave f32's range in it. The largest is that
     // of all blocks, also of those that did not become the unit (the first ones within 1 to 1/16).
+    // N <= 2^31 tokens add up to 2^15 448 N of it, below 2^55: 2^60 times that is in range.
     float turn = alpha;
     top = fmaxf(top, vs);
     if (vs > unit || vs < unit * 0x1p-4f) {
-      const float to = fmaxf(fmaxf(vs, top * 0x1p-90f), 0x1p-126f);  // not 0, for a scale of 0
+      const float to = fmaxf(fmaxf(vs, top * 0x1p-60f), 0x1p-126f);  // not 0, for a scale of 0
       turn = alpha * (unit / to);
       unit = to;
     }

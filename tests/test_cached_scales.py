@@ -69,3 +69,14 @@ def test_only_large_values_and_zeros(gpu_ctx, shape, first, bf16):
     R, H, HK, L = shape
     ref, total = blocks_of([first] * 8 + [ZERO] * 8, [0x7E] * 8 + [0] * 8, R, HK)
     attend(gpu_ctx, ref, total, shape, bf16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape,large,zeros", [((256, 1, 1, 1), 2600, 8), (PROMPT, 330, 2)],
+                         ids=["single", "prompt"])
+def test_long_rows_of_large_values_and_zeros(gpu_ctx, shape, large, zeros, bf16):
+    """A wave sums up 20800 values of 896: 2^15 times that is 2^39 units of 2."""
+    R, H, HK, L = shape
+    ref, total = blocks_of([2.0] * large + [ZERO] * zeros, [0x7E] * large + [0] * zeros, R, HK)
+    attend(gpu_ctx, ref, total, shape, bf16)
