@@ -458,8 +458,10 @@ int tfd_jeff_cache_append_bf16(tfd_ctx *ctx, size_t rows, size_t length, size_t 
  *                 (see the append) has NaN for every out; a page outside the cache gives
  *                 NaN to the tokens that see it. With host operands both are TFD_EINVAL.
  *                 It may not overlap the inputs.
- * Every sum is f32. Queries (against their head's largest feature) and probabilities enter
- * the products with 22 significant bits, probabilities to within 2^-36 of the largest;
+ * Every sum is f32, so the squares of a query's features (where it is normalized) and a
+ * row's values times its tokens have to be in f32's range. Queries (against their head's
+ * largest feature) and probabilities enter the products with 22 significant bits,
+ * probabilities to within 2^-36 of the largest;
  * values more than 2^60 below the largest scale of a row's values are lost beside it. A NaN
  * that a key or value holds reaches the outputs that see its token, and no other.
  */
