@@ -67,6 +67,7 @@ struct tfd_ctx {
   DevBuf linear;      // chunk operands of the linear attention
   DevBuf readout;     // partial statistics of the token log probabilities
   DevBuf cached;      // partial outputs of the attention over a cache
+  bool cached_zeroed = false;  // its counters
   // Workspaces that a captured graph may still use, outgrown since.
   std::vector<void *> retired;
   size_t retired_bytes = 0;
@@ -1989,11 +1990,16 @@ int cached_run(tfd_ctx *c, bool bf16, CacheCall m, size_t heads, size_t rotary_d
   // The counters at the workspace's start are zero between calls, whatever sizes a call has.
   const tfd::CachedSpace space = tfd::cached_space(a);
   const size_t bytes = space.done + space.stats + space.out;
-  const bool grows = bytes > c->cached.cap;
+  if (bytes > c->cached.cap && !capturing) c->cached_zeroed = false;
   if ((rc = reserve_capturable(c, op, c->cached, bytes, capturing))) return rc;
-  if (grows)
+  if (!c->cached_zeroed) {
+    if (capturing)
+      return fail(c, TFD_EUNSUPPORTED,
+                  "%s: the workspace is not ready; make one call before capturing", op);
     TFD_HIP(c, tfd::launch_fill_zero(static_cast<float *>(c->cached.ptr),
                                      space.done / sizeof(float), c->stream), "fill_zero launch");
+    c->cached_zeroed = true;
+  }
   a.part_done = static_cast<unsigned *>(c->cached.ptr);
   a.part_stats = reinterpret_cast<float *>(a.part_done + space.done / sizeof(unsigned));
   a.part_out = a.part_stats + space.stats / sizeof(float);
