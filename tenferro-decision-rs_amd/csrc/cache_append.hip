@@ -372,8 +372,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 512 ? 6 : 4) void append_kernel
 template <typename T>
 hipError_t launch_append(const AppendArgs &a, int rows, hipStream_t stream, const KernelEvents &ev) {
   const int L = a.cache.L, half = a.cache.wide / 2;
-  // Blocks that L tokens from any slot on may touch.
-  const unsigned blocks = (unsigned)((L + 62) / 64 + 1);
+  const unsigned blocks = (unsigned)append_blocks(a);
   const dim3 grid(blocks, (unsigned)a.cache.kv_heads * 2, (unsigned)rows);
 #define TFD_APPEND(Q, N, P)                                                                     \
   hipExtLaunchKernelGGL((append_kernel<T, Q, N, P>), grid, dim3(N), 0, stream, ev.start, ev.stop, 0, a)

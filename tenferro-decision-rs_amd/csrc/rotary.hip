@@ -110,11 +110,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
 }  // namespace
 
 hipError_t launch_rotary(RotaryArgs a, int rows, hipStream_t stream, const KernelEvents &ev) {
-  // Eight tokens of 16 bits or four of 32 are one 16-byte access.
-  const int v = a.L == 1 ? 1 : a.bf16 ? 8 : 4;
+  const int v = rotary_vec(a);
   a.steps = (a.L + v - 1) / v;
   a.groups = (a.hd + 1) / 2;
-  const size_t blocks = ((size_t)a.steps * a.groups + 255) / 256;
+  const size_t blocks = rotary_blocks(a);
   // Heads over several workgroups until the grid has eight a CU.
   const size_t wanted = (size_t)8 * a.cus;
   size_t shares = (wanted + blocks * rows - 1) / (blocks * rows);

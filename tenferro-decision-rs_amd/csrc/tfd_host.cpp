@@ -1728,8 +1728,13 @@ int rotary_plan(tfd_ctx *c, const char *op, size_t head_dim, size_t rotary_dim,
   return TFD_OK;
 }
 
-// Workgroups of a launch of 512 threads each at most; a grid may have 2^32 threads.
-constexpr size_t kGridBlocks = (size_t)1 << 22;
+// Rows of a launch whose rows have `threads` each: rows are independent, more go in several.
+size_t rows_at_once(size_t threads, size_t rows) {
+  return std::min({rows, tfd::kGridRows, tfd::kGridThreads / threads});
+}
+const void *from(const void *p, size_t bytes) {
+  return p ? static_cast<const char *>(p) + bytes : nullptr;
+}
 
 int rotary_run(tfd_ctx *c, bool bf16, size_t rows, size_t length, size_t heads, size_t head_dim,
                size_t rotary_dim, const void *x, const int32_t *positions,
@@ -1747,9 +1752,12 @@ int rotary_run(tfd_ctx *c, bool bf16, size_t rows, size_t length, size_t heads, 
   if ((rc = rotary_plan(c, op, head_dim, rotary_dim, frequencies, magnitude_bits, flags, &a.plan)))
     return rc;
   if (n == 0) return TFD_OK;
-  if (length > (size_t)1 << 28 || head_dim > (size_t)1 << 20 || heads > 65535 || rows > 65535 ||
-      ((length + 3) / 4 * ((head_dim + 1) / 2) / 256 + 1) * rows > kGridBlocks)
-    return fail(c, TFD_EUNSUPPORTED, "%s: length/head_dim/heads/rows exceed the launch grid", op);
+  a.L = (int)std::min(length, (size_t)INT32_MAX);
+  a.hd = (int)std::min(head_dim, (size_t)INT32_MAX);
+  a.bf16 = bf16;
+  if (length > (size_t)1 << 28 || head_dim > (size_t)1 << 20 || heads > (size_t)1 << 28 ||
+      tfd::rotary_blocks(a) * 256 > tfd::kGridThreads)
+    return fail(c, TFD_EUNSUPPORTED, "%s: length/head_dim/heads exceed the launch grid", op);
   if (!x || !out) return invalid(c, op, "inputs", "null buffer");
   if ((rc = ensure_ready(c))) return rc;
   bool capturing = false;
@@ -1760,18 +1768,23 @@ int rotary_run(tfd_ctx *c, bool bf16, size_t rows, size_t length, size_t heads, 
   if ((rc = operand(c, flags, 1, x, es * n, &x_d))) return rc;
   if (positions && (rc = operand(c, flags, 2, positions, sizeof(int32_t) * mn, &p_d))) return rc;
   if ((rc = output(c, flags, 0, out, es * n, &out_d))) return rc;
-  a.x = x_d;
-  a.positions = static_cast<const int32_t *>(p_d);
-  a.out = out_d;
-  a.L = (int)length;
   a.heads = (int)heads;
-  a.hd = (int)head_dim;
   a.inverse = (flags & TFD_INVERSE) ? 1 : 0;
-  a.bf16 = bf16;
   a.cus = c->cus;
   tfd::KernelEvents ev;
   if (!capturing && (rc = timing_events(c, &ev))) return rc;
-  TFD_HIP(c, tfd::launch_rotary(a, (int)rows, c->stream, ev), "rotary launch");
+  const size_t at_once = rows_at_once(tfd::rotary_blocks(a) * 256, rows), row = heads * head_dim * length;
+  for (size_t r0 = 0; r0 < rows; r0 += at_once) {
+    const size_t run = std::min(at_once, rows - r0);
+    a.x = from(x_d, es * row * r0);
+    a.positions = static_cast<const int32_t *>(from(p_d, sizeof(int32_t) * length * r0));
+    a.out = static_cast<char *>(out_d) + es * row * r0;
+    TFD_HIP(c,
+            tfd::launch_rotary(a, (int)run, c->stream,
+                               tfd::KernelEvents{r0 ? nullptr : ev.start,
+                                                 r0 + run < rows ? nullptr : ev.stop}),
+            "rotary launch");
+  }
   return finish(c, flags, out, out_d, es * n);
 }
 
@@ -1891,8 +1904,11 @@ int append_run(tfd_ctx *c, bool bf16, CacheCall m, size_t rotary_dim, const void
     return rc;
   if ((rc = check_cache(c, op, m, flags))) return rc;
   if (n == 0) return TFD_OK;
-  if ((m.length / 64 + 2) * m.kv_heads * 2 * m.rows > kGridBlocks)
-    return fail(c, TFD_EUNSUPPORTED, "%s: length/kv_heads/rows exceed the launch grid", op);
+  a.cache.L = (int)m.length;
+  a.cache.wide = (int)m.wide;
+  const size_t threads = tfd::append_blocks(a) * m.kv_heads * 2 * tfd::append_threads(a);
+  if (threads > tfd::kGridThreads)
+    return fail(c, TFD_EUNSUPPORTED, "%s: length/kv_heads exceed the launch grid", op);
   if (!k || !v) return invalid(c, op, "inputs", "null buffer");
   if (!(flags & TFD_DEVICE_PTRS)) {
     // Two rows that append to one page would each scale it by itself.
@@ -1921,14 +1937,26 @@ int append_run(tfd_ctx *c, bool bf16, CacheCall m, size_t rotary_dim, const void
   if ((rc = operand(c, flags, 2, v, es * n, &v_d))) return rc;
   if (k_norm && (rc = operand(c, flags, 3, k_norm, sizeof(float) * m.head_dim, &n_d))) return rc;
   if ((rc = cache_view(c, m, flags, &a.cache))) return rc;
-  a.k = k_d;
-  a.v = v_d;
   a.k_norm = static_cast<const float *>(n_d);
   a.eps = bits_to_f32(eps_bits);
   a.bf16 = bf16;
   tfd::KernelEvents ev;
   if (!capturing && (rc = timing_events(c, &ev))) return rc;
-  TFD_HIP(c, tfd::launch_cache_append(a, (int)m.rows, c->stream, ev), "cache_append launch");
+  const size_t at_once = rows_at_once(threads, m.rows), row = m.kv_heads * m.head_dim * m.length;
+  const tfd::CacheView all = a.cache;
+  for (size_t r0 = 0; r0 < m.rows; r0 += at_once) {
+    const size_t run = std::min(at_once, m.rows - r0);
+    a.k = from(k_d, es * row * r0);
+    a.v = from(v_d, es * row * r0);
+    a.cache.table = all.table + m.per_row * r0;
+    a.cache.lengths = all.lengths ? all.lengths + r0 : nullptr;
+    a.cache.counts = all.counts ? all.counts + r0 : nullptr;
+    TFD_HIP(c,
+            tfd::launch_cache_append(a, (int)run, c->stream,
+                                     tfd::KernelEvents{r0 ? nullptr : ev.start,
+                                                       r0 + run < m.rows ? nullptr : ev.stop}),
+            "cache_append launch");
+  }
   if (!(flags & TFD_DEVICE_PTRS)) {
     const struct { void *host, *dev; size_t bytes; } back[3] = {
         {m.cache->values, a.cache.values, m.code_bytes},
@@ -1961,8 +1989,12 @@ int cached_run(tfd_ctx *c, bool bf16, CacheCall m, size_t heads, size_t rotary_d
     return rc;
   if ((rc = check_cache(c, op, m, flags))) return rc;
   if (n == 0) return TFD_OK;
-  if (heads > 65535 || (m.length * (heads / m.kv_heads) / 16 + 1) * m.kv_heads * m.rows > kGridBlocks)
-    return fail(c, TFD_EUNSUPPORTED, "%s: length/heads/rows exceed the launch grid", op);
+  // The kernels count a row's columns (tokens times heads of a group) and all tiles of them in
+  // 32 bits; their grid is one workgroup a CU.
+  const size_t columns = m.length * (heads / m.kv_heads);
+  if (heads > 65535 || columns > (size_t)1 << 30 ||
+      (columns / 16 + 1) * m.kv_heads * m.rows > (size_t)1 << 30)
+    return fail(c, TFD_EUNSUPPORTED, "%s: length/heads/rows exceed 32-bit counts", op);
   if (!q || !out) return invalid(c, op, "inputs", "null buffer");
   if ((rc = ensure_ready(c))) return rc;
   bool capturing = false;

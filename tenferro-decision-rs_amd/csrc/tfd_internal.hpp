@@ -415,6 +415,9 @@ struct LogProbArgs {
 void log_probs_plan(LogProbArgs &a, int cus);
 hipError_t launch_log_probs(const LogProbArgs &a, hipStream_t stream, const KernelEvents &ev);
 
+// Rows of a launch that has them in one dimension, and the threads that it may have.
+constexpr size_t kGridRows = 65535, kGridThreads = ((size_t)1 << 32) - 1;
+
 // ------------------------------------------------ rotary positions
 
 // Pairs of features that may be turned.
@@ -436,6 +439,14 @@ struct RotaryArgs {
   int steps, groups;
   RotaryPlan plan;
 };
+// Tokens of a pair that a thread takes: eight of 16 bits or four of 32 are one 16-byte access.
+inline int rotary_vec(const RotaryArgs &a) { return a.L == 1 ? 1 : a.bf16 ? 8 : 4; }
+// Workgroups of 256 threads for a row (its heads side by side where there are few).
+inline size_t rotary_blocks(const RotaryArgs &a) {
+  const size_t steps = ((size_t)a.L + rotary_vec(a) - 1) / rotary_vec(a);
+  return (steps * (((size_t)a.hd + 1) / 2) + 255) / 256;
+}
+// rows: at most kGridRows, their threads below kGridThreads.
 hipError_t launch_rotary(RotaryArgs a, int rows, hipStream_t stream, const KernelEvents &ev);
 
 // ------------------------------------------------ paged 8-bit cache
@@ -486,6 +497,13 @@ struct AppendArgs {
   bool bf16;
   RotaryPlan plan;
 };
+// Threads of a workgroup, which has a block of a head: one token's, or up to 64's.
+inline int append_threads(const AppendArgs &a) {
+  return a.cache.L == 1 ? 128 : a.cache.wide <= 128 ? 512 : 1024;
+}
+// Blocks that L tokens from any slot on may touch.
+inline size_t append_blocks(const AppendArgs &a) { return ((size_t)a.cache.L + 62) / 64 + 1; }
+// rows: at most kGridRows, their threads below kGridThreads.
 hipError_t launch_cache_append(const AppendArgs &a, int rows, hipStream_t stream,
                                const KernelEvents &ev);
 
