@@ -297,6 +297,25 @@ _TORCH_DTYPES = {
 _accepted: set = set()  # (torch dtype, host dtype) pairs that passed the check by name
 
 
+def _host_array(x, dtype, name) -> np.ndarray:
+    """x as a contiguous array of the type. Codes are bytes, and whole numbers have to fit: neither
+    is converted to what it does not stand for."""
+    if dtype == "e4m3":
+        given = np.asarray(x)
+        if given.dtype != np.uint8:
+            raise InvalidArgument(
+                TFD_EINVAL, f"{name}: expected a contiguous uint8 array, got {given.dtype}")
+        return np.ascontiguousarray(given)
+    if dtype is np.int32:
+        given = np.asarray(x)
+        with np.errstate(invalid="ignore"):
+            arr = np.ascontiguousarray(given, dtype=dtype)
+        if given.dtype != dtype and not np.array_equal(arr, given.reshape(arr.shape)):
+            raise InvalidArgument(TFD_EINVAL, f"{name}: not all numbers are 32-bit integers")
+        return arr
+    return np.ascontiguousarray(x, dtype=dtype)
+
+
 class _Arg:
     """A flat buffer argument: host numpy array or torch tensor (CUDA: device
     pointer; CPU: host pointer).
@@ -328,7 +347,7 @@ class _Arg:
             self.n = x.numel()
             self.device = x.is_cuda
         else:
-            arr = np.ascontiguousarray(x, dtype=np.uint8 if dtype == "e4m3" else dtype)
+            arr = _host_array(x, dtype, name)
             self.obj = arr
             self.ptr = arr.ctypes.data
             self.n = arr.size
