@@ -370,8 +370,8 @@ int tfd_token_log_probs_bf16(tfd_ctx *ctx, const uint16_t *logits, size_t vocab,
  *                likes); read before the call returns. rotary_dim is even and at most 256
  *                (else TFD_EUNSUPPORTED).
  *   magnitude_bits: f32 bits of the factor on the turned features.
- * TFD_EUNSUPPORTED: length or heads past 2^28, head_dim past 2^20, length * head_dim of
- * 2^34 and more.
+ * TFD_EUNSUPPORTED: length or heads past 2^28, head_dim past 2^20, or a row's features past
+ * what a launch holds (length * head_dim below 2^34 always fits). Any number of rows.
  * flags may carry TFD_INTERLEAVED and TFD_INVERSE (turns by -u; with the same magnitude
  * the gradient of the forward call).
  * This and the two cache entries may run under stream capture (with TFD_ASYNC); the
@@ -428,9 +428,9 @@ typedef struct tfd_paged_cache {
  * and the codes of its earlier tokens are rounded again under the new scale. Codes are
  * rounded to nearest even from 64-bit keys; NaN and inf become the code of NaN.
  * TFD_EUNSUPPORTED: head_dim past 256, rows past 65535, kv_heads past 32767, length past
- * 2^24, (length / 64 + 2) * kv_heads of 2^21 and more. A row whose length or count is negative, whose
- * count exceeds length, or that its pages cannot hold, and pages outside the
- * cache: with host operands TFD_EINVAL; with device operands, which the host does not
+ * 2^24, or a row's blocks past what a launch holds ((length / 64 + 2) * kv_heads below 2^21
+ * always fits). A row whose length or count is negative, whose count exceeds length, or that
+ * its pages cannot hold, and pages outside the cache: with host operands TFD_EINVAL; with device operands, which the host does not
  * read, nothing is written for that row or page.
  */
 int tfd_jeff_cache_append_f32(tfd_ctx *ctx, size_t rows, size_t length, size_t kv_heads,
@@ -461,7 +461,7 @@ int tfd_jeff_cache_append_bf16(tfd_ctx *ctx, size_t rows, size_t length, size_t 
  *                 (see the append) has NaN for every out; a page outside the cache gives
  *                 NaN to the tokens that see it. With host operands both are TFD_EINVAL.
  *                 It may not overlap the inputs.
- * TFD_EUNSUPPORTED: as the append but for its product; heads past 65535, and, with columns =
+ * TFD_EUNSUPPORTED: as the append, without its last limit; heads past 65535, and, with columns =
  * length * heads / kv_heads, columns or rows * kv_heads * (columns / 16 + 1) past 2^30.
  * Every sum is f32, so the squares of a query's features (where it is normalized) and a
  * row's values times its tokens have to be in f32's range. Queries (against their head's

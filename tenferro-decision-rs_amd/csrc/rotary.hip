@@ -8,8 +8,9 @@
 //
 // Bound: memory, x once in and out once. Lanes go along the tokens, 16 bytes each of the
 // pair's two features; the sines, a function of token and pair, are taken once for all
-// heads that a workgroup walks. Measured: 2 rows of 8192 f32 tokens, 16 heads of 128 (268 MB) 45 us,
-// 5.9 TB/s; 3 rows of 1003 bf16 tokens, 5 heads of 96 6.5 us; single tokens of 64 rows 3.0 us, where an
+// heads that a workgroup walks. Measured: 2 rows of 8192 f32 tokens, 16 heads of 128 (268 MB) 45 us
+// (46 to 51 from call to call), 5.9 TB/s; 8 such rows of bf16 tokens (537 MB) 104 us a call,
+// 5.1 TB/s; 3 rows of 1003 bf16 tokens, 5 heads of 96 6.5 us; single tokens of 64 rows 3.0 us, where an
 // empty launch takes 3.5 from one call to the next.
 #include <hip/hip_ext.h>
 #include <string.h>
